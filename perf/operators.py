@@ -211,7 +211,7 @@ def _prepare_attend(case, g, state):
         starts.append(starts[-1] + c)
     first = [max(0, length - c + 1 - case["window"]) if case["window"] else 0 for c, length in zip(counts, lens)]
     state.update(q=q.to(DTYPES[case["dtype"]]), lens=torch.tensor(lens, dtype=torch.int32, device="cuda"),
-                 starts=torch.tensor(starts, dtype=torch.int32, device="cuda"), max_q=max(counts), max_len=max_seq,
+                 starts=torch.tensor(starts, dtype=torch.int32, device="cuda"), max_q=max(counts),
                  first=torch.tensor(first, device="cuda"), span=max(a - b for a, b in zip(lens, first)),
                  single=all(c == 1 for c in counts), scale=head_dim ** -0.5)
     _cache(state, n, -(-max_seq // size) * size, kv_heads, head_dim, case["page"], k_rows, v_rows, table)
@@ -258,7 +258,7 @@ def _run_own(s):
         return {"q": q, "k": k, "v": v}
     if s["op"] == "attend":
         return s["cache"].attention(s["q"], s["lens"], q_start=None if s["single"] else s["starts"], max_q=s["max_q"],
-                                    max_len=s["max_len"], window=s["window"], sinks=s["sinks"], scale=s["scale"])
+                                    window=s["window"], sinks=s["sinks"], scale=s["scale"])
     token, logprob = bt.sample_batch(s["logits"], s["u"], s["temperature"], s["top_k"], s["top_p"], s["min_p"])
     return {"token": token, "logprob": logprob}
 
