@@ -21,6 +21,7 @@ __all__ = [
     "ModelConfig", "TransformerEngine", "KVCache", "CudaBackendError", "BT_KV_FP16", "BT_KV_FP32",
     "quantize_q8_0", "dequantize_q8_0", "matvec_q8_0", "repack_q8_0", "gemv_q8",
     "rmsnorm", "rope", "softmax", "silu", "argmax", "launch_count", "model_config",
+    "KV4Cache", "qk_norm_rope", "rope_table", "sample_batch",
 ]
 
 Q8_BLOCK = 32
@@ -31,6 +32,15 @@ def model_config(vocab_size, dim, hidden_dim, num_layers, num_heads, num_kv_head
                  max_seq_len, rms_norm_eps=1e-5) -> ModelConfig:
     return ModelConfig(vocab_size, dim, hidden_dim, num_layers, num_heads, num_kv_heads, head_dim,
                        max_seq_len, rms_norm_eps)
+
+
+def __getattr__(name):
+    # the serving operators work on torch tensors throughout; the rest of the package does not need torch to import
+    if name in ("KV4Cache", "qk_norm_rope", "rope_table", "sample_batch"):
+        from . import serving
+        value = globals()[name] = getattr(serving, name)
+        return value
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")
 
 
 def launch_count() -> int:

@@ -23,6 +23,13 @@ BT_ERR_DEVICE_TIMEOUT = -7
 BT_KV_FP32 = 0
 BT_KV_FP16 = 1
 
+BT_F32 = 0
+BT_F16 = 1
+BT_BF16 = 2
+
+BT_KV4_RANGE = 1
+BT_KV4_TIMEOUT = 2
+
 
 class CudaBackendError(RuntimeError):
     """A CUDA runtime failure inside the backend (BT_ERR_CUDA / BT_ERR_DEVICE_TIMEOUT)."""
@@ -68,6 +75,45 @@ class TensorView(C.Structure):
 
 _vp, _u32, _u64, _i32, _f32 = C.c_void_p, C.c_uint32, C.c_uint64, C.c_int, C.c_float
 
+
+def _heads_fields(name):
+    """The three members of a bt_heads (all 8 bytes wide, so laid out as the nested struct is)."""
+    return [(name, C.c_void_p), (name + "_token_stride", C.c_int64), (name + "_head_stride", C.c_int64)]
+
+
+class KV4(C.Structure):
+    """bt_kv4: a 4-bit cache of one layer."""
+
+    _fields_ = [("k_rows", _vp), ("v_rows", _vp), ("page_table", _vp), ("status", _vp), ("n_seq", _u32), ("max_seq", _u32),
+                ("kv_heads", _u32), ("head_dim", _u32), ("page_tokens", _u32), ("n_pages", _u32), ("max_pages", _u32),
+                ("reserved", _u32)]
+
+
+class QkArgs(C.Structure):
+    """bt_qk_args."""
+
+    _fields_ = [f for n in ("q", "k", "v", "q_out", "k_out") for f in _heads_fields(n)] + [
+        ("q_weight", _vp), ("k_weight", _vp), ("positions", _vp), ("slots", _vp), ("rope", _vp), ("rope_positions", _u32),
+        ("rot_dim", _u32), ("tokens", _u32), ("heads", _u32), ("kv_heads", _u32), ("head_dim", _u32), ("dtype", C.c_int32),
+        ("eps", _f32)]
+
+
+class KV4AttnArgs(C.Structure):
+    """bt_kv4_attn_args."""
+
+    _fields_ = _heads_fields("q") + _heads_fields("out") + [
+        ("kv_len", _vp), ("q_start", _vp), ("slots", _vp), ("n", _u32), ("tokens", _u32), ("heads", _u32), ("max_q", _u32),
+        ("window", _u32), ("sinks", _u32), ("dtype", C.c_int32), ("scale", _f32)]
+
+
+class SampleArgs(C.Structure):
+    """bt_sample_args."""
+
+    _fields_ = [("logits", _vp), ("row_stride", C.c_int64), ("u", _vp), ("temperature", _vp), ("top_k", _vp), ("top_p", _vp),
+                ("min_p", _vp), ("token", _vp), ("logprob", _vp), ("rows", _u32), ("vocab", _u32), ("dtype", C.c_int32),
+                ("reserved", _u32)]
+
+
 # name -> (restype, argtypes); must match include/bt_cuda.h
 SIGNATURES = {
     "bt_cuda_abi_version": (_i32, []),
@@ -99,6 +145,13 @@ SIGNATURES = {
     "bt_cuda_silu": (_i32, [_vp, _vp, _u32, _vp]),
     "bt_cuda_argmax": (_i32, [_vp, _u32, _vp, _vp]),
     "bt_cuda_sample_top_p_top_k": (_i32, [_vp, _u32, _f32, _f32, _u32, _u64, _vp, _vp]),
+    "bt_kv4_row_bytes": (_u32, [_u32]),
+    "bt_cuda_qk_norm_rope": (_i32, [_vp, _vp]),
+    "bt_cuda_kv4_append": (_i32, [_vp, _vp, _vp]),
+    "bt_cuda_kv4_read": (_i32, [_vp, _vp, _vp, _u32, C.c_int32, _vp, _vp, _vp]),
+    "bt_cuda_kv4_attention": (_i32, [_vp, _vp, _vp, _u64, _vp]),
+    "bt_cuda_kv4_attention_workspace": (_u64, [_u32]),
+    "bt_cuda_sample_batch": (_i32, [_vp, _vp]),
     "bt_engine_create": (_i32, [_i32, C.POINTER(ModelConfig), C.POINTER(EngineOptions), C.POINTER(_vp)]),
     "bt_engine_destroy": (_i32, [_vp]),
     "bt_engine_load": (_i32, [_vp, C.POINTER(TensorView), _u32, _i32]),

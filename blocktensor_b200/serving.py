@@ -1,0 +1,303 @@
+"""Serving operators on torch CUDA tensors: head norms with rotation, 4-bit K/V caches with the
+attention over them, batched sampling (bt_cuda_qk_norm_rope, bt_cuda_kv4_*, bt_cuda_sample_batch in
+include/bt_cuda.h, which states their mathematics).
+
+Activations are fp32, fp16 or bf16 tensors whose last dimension is contiguous; every call checks its
+arguments (ValueError), launches on ``stream`` or torch's current stream, and does not synchronise.
+Index tensors (positions, slots, lengths) are int32 on the device; values out of range are never
+followed and show in :meth:`KV4Cache.check`.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import native
+from .native import BT_BF16, BT_F16, BT_F32, KV4, KV4AttnArgs, QkArgs, SampleArgs
+
+__all__ = ["KV4Cache", "qk_norm_rope", "rope_table", "sample_batch"]
+
+_DTYPES = {torch.float32: BT_F32, torch.float16: BT_F16, torch.bfloat16: BT_BF16}
+_NO_HEADS = (None, 0, 0)
+
+
+def _dtype(t) -> int:
+    d = _DTYPES.get(t.dtype)
+    if d is None:
+        raise ValueError(f"expected a float32, float16 or bfloat16 tensor, got {t.dtype}")
+    return d
+
+
+def _heads(t, name, like=None, heads=None):
+    """(pointer, token stride, head stride) of a [tokens, heads, head_dim] tensor."""
+    if t.dim() != 3 or not t.is_cuda:
+        raise ValueError(f"{name}: expected a [tokens, heads, head_dim] CUDA tensor")
+    s = t.stride()
+    if s[2] != 1 and t.shape[2] > 1:
+        raise ValueError(f"{name}: the elements of a head must be contiguous")
+    if like is not None and (t.shape[0] != like.shape[0] or t.shape[2] != like.shape[2] or t.dtype != like.dtype
+                             or t.device != like.device or (heads is not None and t.shape[1] != heads)):
+        raise ValueError(f"{name}: tokens, heads, head_dim, dtype or device do not match")
+    return t.data_ptr(), s[0], s[1]
+
+
+def _vector(t, name, n, dtype, device):
+    if t.dtype != dtype or t.device != device or t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"{name}: expected {n} contiguous {dtype} values on {device}")
+    return t.data_ptr()
+
+
+def _launch(name, device, stream, outs, *args):
+    """The C call on the tensors' device; ``outs``: tensors allocated here for the call."""
+    fn = getattr(native.load(), name)
+    if stream is None:
+        s = torch.cuda.current_stream(device).cuda_stream
+    else:
+        s = stream.cuda_stream
+        for t in outs:
+            t.record_stream(stream)
+    if device.index == torch.cuda.current_device():
+        rc = fn(*args, s)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, s)
+    if rc:
+        native.check(rc, name)
+
+
+def rope_table(positions: int, rot_dim: int, theta: float = 10000.0, device="cuda"):
+    """cos and sin of cpu_ref::rope's angles (cpu_ref.hpp:38-41) for positions 0 .. positions - 1, taken
+    in double precision: [positions, rot_dim / 2, 2] fp32."""
+    if rot_dim <= 0 or rot_dim % 16:
+        raise ValueError("rope_table: rot_dim must be a positive multiple of 16")
+    freq = theta ** (-torch.arange(0, rot_dim, 2, dtype=torch.float64) / rot_dim)
+    angle = torch.arange(positions, dtype=torch.float64)[:, None] * freq
+    return torch.stack([angle.cos(), angle.sin()], -1).float().to(device)
+
+
+def _rope(table, device):
+    if table is None:
+        return None, 0, 0
+    if table.dim() != 3 or table.shape[2] != 2 or table.dtype != torch.float32 or table.device != device or not table.is_contiguous():
+        raise ValueError("table: expected a contiguous [positions, rot_dim / 2, 2] float32 tensor on the queries' device")
+    return table.data_ptr(), table.shape[0], 2 * table.shape[1]
+
+
+def qk_norm_rope(q, k, q_weight, k_weight, positions, table, eps: float = 1e-5, q_out=None, k_out=None, stream=None):
+    """Norms of each head of q [T, H, hd] and k [T, KVH, hd] and their rotation, one pass over both
+    (bt_cuda_qk_norm_rope).  q_weight / k_weight: [hd] float32, or None for no norm; table: rope_table(),
+    or None for no rotation; positions: [T] int32.  q_out / k_out may be q and k.  k may be None."""
+    hd = q.shape[-1]
+    qh = _heads(q, "q")
+    dev, tokens = q.device, q.shape[0]
+    q_out = torch.empty_like(q, memory_format=torch.contiguous_format) if q_out is None else q_out
+    outs = [q_out]
+    kh = koh = _NO_HEADS
+    kv_heads = 0
+    if k is not None:
+        kh = _heads(k, "k", q)
+        kv_heads = k.shape[1]
+        k_out = torch.empty_like(k, memory_format=torch.contiguous_format) if k_out is None else k_out
+        koh = _heads(k_out, "k_out", q, kv_heads)
+        outs.append(k_out)
+    rp, rn, rot = _rope(table, dev)
+    a = QkArgs(*qh, *kh, *_NO_HEADS, *_heads(q_out, "q_out", q, q.shape[1]), *koh,
+               None if q_weight is None else _vector(q_weight, "q_weight", hd, torch.float32, dev),
+               None if k_weight is None else _vector(k_weight, "k_weight", hd, torch.float32, dev),
+               _vector(positions, "positions", tokens, torch.int32, dev), None,
+               rp, rn, rot, tokens, q.shape[1], kv_heads, hd, _dtype(q), eps)
+    _launch("bt_cuda_qk_norm_rope", dev, stream, outs, C.byref(a))
+    return q_out, k_out
+
+
+class KV4Cache:
+    """A 4-bit cache of one layer (bt_kv4): ``n_seq`` slots of up to ``max_seq`` positions.
+
+    Contiguous by default.  With ``page_tokens`` the rows live in a pool of ``n_pages`` pages;
+    :meth:`reserve` and :meth:`release` hand them out (of several layers, the first one's ``page_table``
+    given to the others serves all), or a ``page_table`` the caller keeps is read as it is.  ``k_rows`` /
+    ``v_rows``: existing uint8 storage [pages, kv_heads, page_tokens, row bytes]."""
+
+    def __init__(self, n_seq: int, max_seq: int, kv_heads: int, head_dim: int, page_tokens: int = 0, n_pages: int = 0,
+                 page_table=None, k_rows=None, v_rows=None, device=None):
+        self.row_bytes = native.load().bt_kv4_row_bytes(head_dim)
+        if not self.row_bytes:
+            raise ValueError("KV4Cache: head_dim must be 64, 128 or 256")
+        if min(n_seq, max_seq, kv_heads) <= 0:
+            raise ValueError("KV4Cache: n_seq, max_seq and kv_heads must be positive")
+        self.n_seq, self.max_seq, self.kv_heads, self.head_dim = n_seq, max_seq, kv_heads, head_dim
+        self.paged = page_tokens > 0
+        if (k_rows is None) != (v_rows is None):
+            raise ValueError("KV4Cache: give both k_rows and v_rows, or neither")
+        device = k_rows.device if k_rows is not None else torch.device("cuda" if device is None else device)
+        if device.type == "cuda" and device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        self.device = device
+        self.page_tokens = page_tokens if self.paged else (max_seq + 15) // 16 * 16
+        if k_rows is not None:
+            self.n_pages = k_rows.shape[0]
+        else:
+            self.n_pages = n_pages if self.paged else n_seq
+        shape = (self.n_pages, kv_heads, self.page_tokens, self.row_bytes)
+        if k_rows is None:
+            k_rows, v_rows = (torch.zeros(shape, dtype=torch.uint8, device=device) for _ in range(2))
+        for name, t in (("k_rows", k_rows), ("v_rows", v_rows)):
+            if t.dtype != torch.uint8 or tuple(t.shape) != shape or not t.is_contiguous() or t.device != device:
+                raise ValueError(f"KV4Cache: {name} must be contiguous uint8 {shape} on {device}")
+        self.k_rows, self.v_rows = k_rows, v_rows
+        self.max_pages = -(-max_seq // self.page_tokens)
+        self._free = self._held = None
+        if self.paged:
+            if page_table is None:
+                page_table = torch.full((n_seq, self.max_pages), -1, dtype=torch.int32, device=device)
+                self._free = list(range(self.n_pages - 1, -1, -1))
+                self._held = [[] for _ in range(n_seq)]
+            if (page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.shape[0] != n_seq
+                    or page_table.shape[1] < self.max_pages or not page_table.is_contiguous() or page_table.device != device):
+                raise ValueError(f"KV4Cache: page_table must be contiguous int32 [{n_seq}, >= {self.max_pages}] on {device}")
+            self.max_pages = page_table.shape[1]
+        elif page_table is not None:
+            raise ValueError("KV4Cache: a page_table needs page_tokens")
+        self.page_table = page_table
+        self.status = torch.zeros(1, dtype=torch.int32, device=device)
+        self._workspaces = {}
+        self._c = KV4(k_rows.data_ptr(), v_rows.data_ptr(), page_table.data_ptr() if self.paged else None,
+                      self.status.data_ptr(), n_seq, max_seq, kv_heads, head_dim, self.page_tokens, self.n_pages,
+                      self.max_pages, 0)
+        self._ref = C.byref(self._c)
+
+    # ------------------------------------------------------------ pages
+
+    def reserve(self, slot: int, positions: int):
+        """Pages for positions 0 .. positions - 1 of a slot; MemoryError (and none taken) when too few are free."""
+        if self._free is None:
+            raise ValueError("reserve: this cache does not hand out its pages")
+        if not 0 <= slot < self.n_seq or positions > self.max_seq:
+            raise IndexError("reserve: slot or positions out of range")
+        held = self._held[slot]
+        more = -(-positions // self.page_tokens) - len(held)
+        if more <= 0:
+            return
+        if more > len(self._free):
+            raise MemoryError(f"reserve: {more} pages needed, {len(self._free)} free")
+        new = [self._free.pop() for _ in range(more)]
+        self.page_table[slot, len(held):len(held) + more] = torch.tensor(new, dtype=torch.int32, device=self.device)
+        held += new
+
+    def release(self, slot: int):
+        """A slot's pages back to the pool.  Work that reads them has to be on the same stream, or done."""
+        if self._free is None:
+            raise ValueError("release: this cache does not hand out its pages")
+        self._free += reversed(self._held[slot])
+        self._held[slot] = []
+        self.page_table[slot] = -1
+
+    def pages(self):
+        """(free, total) pages of the pool."""
+        return (len(self._free) if self._free is not None else 0), self.n_pages
+
+    def check(self):
+        """Waits for the device and raises IndexError if a call met a slot, position, length or page out of
+        range since the last check, CudaBackendError if a device wait gave up."""
+        status = int(self.status.item())
+        self.status.zero_()
+        if status & native.BT_KV4_TIMEOUT:
+            raise native.CudaBackendError(native.BT_ERR_DEVICE_TIMEOUT, "KV4Cache: a device wait gave up")
+        if status & native.BT_KV4_RANGE:
+            raise IndexError("KV4Cache: a slot, position, length or page was out of range")
+
+    # ------------------------------------------------------------ rows
+
+    def append(self, k, v, slots, positions, stream=None):
+        """Stores k, v [T, KVH, hd] at (slots[t], positions[t]); slots < 0: padding."""
+        self._append(None, k, v, None, None, slots, positions, None, 0.0, None, stream)
+
+    def append_normed(self, q, k, v, q_weight, k_weight, slots, positions, table, eps: float = 1e-5, q_out=None, stream=None):
+        """qk_norm_rope of q and k with the keys and values stored, one launch (bt_cuda_kv4_append); returns
+        the queries."""
+        return self._append(q, k, v, q_weight, k_weight, slots, positions, table, eps, q_out, stream)
+
+    def _append(self, q, k, v, q_weight, k_weight, slots, positions, table, eps, q_out, stream):
+        kh = _heads(k, "k")
+        dev, tokens, hd = k.device, k.shape[0], k.shape[2]
+        if k.shape[1] != self.kv_heads or hd != self.head_dim or dev != self.device:
+            raise ValueError("append: k must have the cache's kv_heads, head_dim and device")
+        qh = qoh = _NO_HEADS
+        heads, outs = 0, ()
+        if q is not None:
+            qh, heads = _heads(q, "q", k), q.shape[1]
+            q_out = torch.empty_like(q, memory_format=torch.contiguous_format) if q_out is None else q_out
+            qoh, outs = _heads(q_out, "q_out", q, heads), (q_out,)
+        rp, rn, rot = _rope(table, dev)
+        a = QkArgs(*qh, *kh, *_heads(v, "v", k, self.kv_heads), *qoh, *_NO_HEADS,
+                   None if q_weight is None else _vector(q_weight, "q_weight", hd, torch.float32, dev),
+                   None if k_weight is None else _vector(k_weight, "k_weight", hd, torch.float32, dev),
+                   _vector(positions, "positions", tokens, torch.int32, dev), _vector(slots, "slots", tokens, torch.int32, dev),
+                   rp, rn, rot, tokens, heads, self.kv_heads, hd, _dtype(k), eps)
+        _launch("bt_cuda_kv4_append", dev, stream, outs, self._ref, C.byref(a))
+        return q_out
+
+    def read(self, slots, positions, dtype=torch.float16, stream=None):
+        """The values that the rows at (slots[t], positions[t]) stand for: k, v [T, KVH, hd]."""
+        dev, tokens = self.device, positions.numel()
+        if dtype not in _DTYPES:
+            raise ValueError("read: dtype must be float32, float16 or bfloat16")
+        k = torch.empty((tokens, self.kv_heads, self.head_dim), dtype=dtype, device=dev)
+        v = torch.empty_like(k)
+        _launch("bt_cuda_kv4_read", dev, stream, (k, v), self._ref, _vector(slots, "slots", tokens, torch.int32, dev),
+                _vector(positions, "positions", tokens, torch.int32, dev), tokens, _DTYPES[dtype], k.data_ptr(), v.data_ptr())
+        return k, v
+
+    # ------------------------------------------------------------ attention
+
+    def attention(self, q, kv_len, q_start=None, slots=None, max_q: int = 0, window: int = 0, sinks: int = 0,
+                  scale: float | None = None, out=None, stream=None):
+        """Causal attention of q [T, H, hd] over the cache (bt_cuda_kv4_attention), with an optional sliding
+        window whose first ``sinks`` positions stay visible.
+
+        kv_len [n] int32: cached positions of each sequence; its queries are the last ones.  q_start
+        [n + 1] int32: sequence i's queries are rows q_start[i] .. q_start[i + 1] - 1 of q; None: one each.
+        slots [n] int32: the sequences' slots; None: sequence i is slot i.  max_q: no sequence has more
+        queries (0: not known)."""
+        qh = _heads(q, "q")
+        dev, tokens, heads, n = q.device, q.shape[0], q.shape[1], kv_len.numel()
+        if q.shape[2] != self.head_dim or dev != self.device:
+            raise ValueError("attention: q must have the cache's head_dim and device")
+        if window < 0 or sinks < 0 or max_q < 0:
+            raise ValueError("attention: window, sinks and max_q must not be negative")
+        out = torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else out
+        a = KV4AttnArgs(*qh, *_heads(out, "out", q, heads), _vector(kv_len, "kv_len", n, torch.int32, dev),
+                        None if q_start is None else _vector(q_start, "q_start", n + 1, torch.int32, dev),
+                        None if slots is None else _vector(slots, "slots", n, torch.int32, dev),
+                        n, tokens, heads, max_q, window, sinks, _dtype(q), self.head_dim ** -0.5 if scale is None else scale)
+        s = (torch.cuda.current_stream(dev) if stream is None else stream).cuda_stream
+        ws = self._workspaces.get((s, n))
+        if ws is None:  # one for every stream that the calls come from
+            with torch.cuda.device(dev):
+                size = native.load().bt_cuda_kv4_attention_workspace(n)
+            with torch.cuda.stream(torch.cuda.current_stream(dev) if stream is None else stream):
+                ws = self._workspaces[(s, n)] = torch.zeros(size, dtype=torch.uint8, device=dev)
+        _launch("bt_cuda_kv4_attention", dev, stream, (out,), self._ref, C.byref(a), ws.data_ptr(), ws.numel())
+        return out
+
+
+def sample_batch(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, token=None, logprob=None, stream=None):
+    """A token for every row of logits [B, V] from the given random numbers u [B] in [0, 1)
+    (bt_cuda_sample_batch).  temperature, top_p, min_p [B] float32 and top_k [B] int32 on the device, or
+    None for none of that.  Returns (token [B] int32, logprob [B] float32)."""
+    if logits.dim() != 2 or not logits.is_cuda or (logits.stride(1) != 1 and logits.shape[1] > 1):
+        raise ValueError("sample_batch: expected a [rows, vocab] CUDA tensor with contiguous rows")
+    dev, (rows, vocab) = logits.device, logits.shape
+    f32, i32 = torch.float32, torch.int32
+    token = torch.empty(rows, dtype=i32, device=dev) if token is None else token
+    logprob = torch.empty(rows, dtype=f32, device=dev) if logprob is None else logprob
+    a = SampleArgs(logits.data_ptr(), logits.stride(0), _vector(u, "u", rows, f32, dev),
+                   None if temperature is None else _vector(temperature, "temperature", rows, f32, dev),
+                   None if top_k is None else _vector(top_k, "top_k", rows, i32, dev),
+                   None if top_p is None else _vector(top_p, "top_p", rows, f32, dev),
+                   None if min_p is None else _vector(min_p, "min_p", rows, f32, dev),
+                   _vector(token, "token", rows, i32, dev), _vector(logprob, "logprob", rows, f32, dev),
+                   rows, vocab, _dtype(logits), 0)
+    _launch("bt_cuda_sample_batch", dev, stream, (token, logprob), C.byref(a))
+    return token, logprob

@@ -456,6 +456,159 @@ BT_API int bt_batch_release(bt_batch* b, uint32_t s);
 /* Free and total pages of the pool (0 and 0 for a contiguous batch). */
 BT_API int bt_batch_pages(bt_batch* b, uint32_t* free_pages, uint32_t* total_pages);
 
+/* ------------------------------------------------------------------ */
+/* Serving operators: head norms with rotation, 4-bit K/V caches,       */
+/* batched sampling (no counterpart in the reference)                   */
+/* ------------------------------------------------------------------ */
+
+/* Element types of the activations these operators take and give.  All
+ * arithmetic is fp32 (or wider); results are rounded once, to the type. */
+#define BT_F32  0
+#define BT_F16  1
+#define BT_BF16 2
+
+/* A 4-bit cache of one layer: n_seq sequence slots of up to max_seq positions.
+ * Memory is the caller's; the struct itself is read on the host during a call.
+ *   k_rows, v_rows: [n_pages][kv_heads][page_tokens][row] bytes, 16-byte aligned.
+ *     A row of bt_kv4_row_bytes(head_dim) = head_dim / 2 + head_dim / 16 bytes
+ *     holds head_dim / 2 bytes of codes (element 2i in the low nibble of byte i),
+ *     then for every 64 elements a pair (scale, min) of fp16; code c stands for
+ *     scale * c + min.
+ *   page_table: device int32 [n_seq][max_pages], the page of positions
+ *     [i page_tokens, (i + 1) page_tokens) of a slot; page_tokens is then a power
+ *     of two >= 16.  NULL: slot s owns page s, n_pages = n_seq, and page_tokens
+ *     is max_seq rounded up to a multiple of 16.
+ *   status: device uint32 or NULL.  A slot, position, length or page id out of
+ *     range is never followed: what it names is neither stored nor seen, and
+ *     the word (if given) becomes BT_KV4_RANGE; BT_KV4_TIMEOUT when a device
+ *     wait gave up after 2 s (the results are then not valid).  Zero it once.
+ * head_dim is 64, 128 or 256. */
+typedef struct bt_kv4 {
+    void*          k_rows;
+    void*          v_rows;
+    const int32_t* page_table;
+    uint32_t*      status;
+    uint32_t       n_seq;
+    uint32_t       max_seq;
+    uint32_t       kv_heads;
+    uint32_t       head_dim;
+    uint32_t       page_tokens;
+    uint32_t       n_pages;
+    uint32_t       max_pages;
+    uint32_t       reserved;
+} bt_kv4;
+
+#define BT_KV4_RANGE   1u
+#define BT_KV4_TIMEOUT 2u
+
+/* Bytes of a cache row; 0 for a head_dim that is not supported. */
+BT_API uint32_t bt_kv4_row_bytes(uint32_t head_dim);
+
+/* A [tokens][heads][head_dim] device tensor: elements of a head contiguous,
+ * strides in elements.  Any alignment; 16-byte aligned data and strides (of 16
+ * bytes) take the wide loads. */
+typedef struct bt_heads {
+    void*   data;
+    int64_t token_stride;
+    int64_t head_stride;
+} bt_heads;
+
+typedef struct bt_qk_args {
+    bt_heads       q, k, v;        /* [tokens][heads | kv_heads][head_dim]; v: append only */
+    bt_heads       q_out, k_out;   /* may be q and k themselves; k_out: not for append */
+    const float*   q_weight;       /* [head_dim] fp32, or NULL: no norm (q and k as they are) */
+    const float*   k_weight;
+    const int32_t* positions;      /* [tokens] device */
+    const int32_t* slots;          /* [tokens] device: cache slot of each token; append only */
+    const float*   rope;           /* [rope_positions][rot_dim / 2][2] fp32 (cos, sin), or NULL: no rotation */
+    uint32_t       rope_positions;
+    uint32_t       rot_dim;        /* multiple of 16, <= head_dim; pairs (i, i + rot_dim / 2) */
+    uint32_t       tokens, heads, kv_heads, head_dim;
+    int32_t        dtype;          /* BT_F32, BT_F16 or BT_BF16: q, k, v and the outputs */
+    float          eps;
+} bt_qk_args;
+
+/* Norms of queries and keys for each head with the position rotation in the
+ * same pass: x * rsqrt(mean(x^2) + eps) * weight over every head's head_dim
+ * elements, then the first rot_dim of them rotated as cpu_ref::rope does
+ * (cpu_ref.hpp:30-53) by the row of `rope` that positions[token] names.  A token
+ * whose position is not in the table gives NaN rows.  head_dim 64, 128 or 256;
+ * tokens may be 0.  k.data NULL: queries only. */
+BT_API int bt_cuda_qk_norm_rope(const bt_qk_args* a, void* stream);
+
+/* The same with the keys and the (unchanged) values of token t stored in 4 bits
+ * at position positions[t] of slot slots[t] of the cache, one launch.  Values
+ * are held to +-57344 and NaN becomes 0 (four bits hold neither).  Per 64
+ * elements: min and scale = (max - min) / 15 are rounded to fp16, code =
+ * clamp(round((x - min) * (1 / scale)), 0, 15).  slots[t] < 0: the token is
+ * padding and stores nothing.  q.data NULL: keys and values only. */
+BT_API int bt_cuda_kv4_append(const bt_kv4* cache, const bt_qk_args* a, void* stream);
+
+/* The values that cached rows stand for: k, v [tokens][kv_heads][head_dim]
+ * (contiguous, `dtype`) of position positions[t] of slot slots[t]; rows that are
+ * out of range read as 0.  k or v may be NULL. */
+BT_API int bt_cuda_kv4_read(const bt_kv4* cache, const int32_t* slots, const int32_t* positions, uint32_t tokens,
+                            int32_t dtype, void* k, void* v, void* stream);
+
+typedef struct bt_kv4_attn_args {
+    bt_heads       q;         /* [tokens][heads][head_dim] */
+    bt_heads       out;       /* the same shape and type */
+    const int32_t* kv_len;    /* [n] device: cached positions of each sequence (0: its rows become 0) */
+    const int32_t* q_start;   /* [n + 1] device: sequence i's queries are rows q_start[i] .. q_start[i + 1] - 1;
+                                 NULL: one query per sequence (tokens = n) */
+    const int32_t* slots;     /* [n] device: cache slot of each sequence, or NULL: sequence i is slot i */
+    uint32_t       n;         /* sequences */
+    uint32_t       tokens;    /* rows of q and out */
+    uint32_t       heads;     /* a multiple of the cache's kv_heads */
+    uint32_t       max_q;     /* no sequence has more queries (0: not known) */
+    uint32_t       window;    /* 0: none; else a query at position p sees positions > p - window ... */
+    uint32_t       sinks;     /* ... and positions < sinks (with a window only) */
+    int32_t        dtype;     /* BT_F32, BT_F16 or BT_BF16: q and out */
+    float          scale;     /* of the scores, e.g. 1 / sqrt(head_dim) */
+} bt_kv4_attn_args;
+
+/* Causal attention over a 4-bit cache.  Sequence i's queries are its last
+ * positions: query j of c sits at position kv_len[i] - c + j and sees positions
+ * <= its own, within the window and the sinks.  heads / kv_heads query heads
+ * share a KV head, in order.  A row that sees nothing becomes 0.  Positions that
+ * no row of their sequence sees may hold anything, and their pages need not be
+ * in the table.  workspace: device memory of
+ * bt_cuda_kv4_attention_workspace() bytes, zeroed once before its first call
+ * (calls leave it ready for the next); calls that may overlap on the GPU need
+ * one each.  Deterministic: the same inputs give the same bits. */
+BT_API int bt_cuda_kv4_attention(const bt_kv4* cache, const bt_kv4_attn_args* a, void* workspace,
+                                 uint64_t workspace_bytes, void* stream);
+/* Bytes of workspace that a call with n sequences needs on the current device. */
+BT_API uint64_t bt_cuda_kv4_attention_workspace(uint32_t n);
+
+typedef struct bt_sample_args {
+    const void*    logits;       /* [rows][vocab], rows row_stride elements apart */
+    int64_t        row_stride;
+    const float*   u;            /* [rows] device: random numbers in [0, 1) */
+    const float*   temperature;  /* [rows] device, or NULL: 1; <= 0: greedy */
+    const int32_t* top_k;        /* [rows] device, or NULL; <= 0: no cut */
+    const float*   top_p;        /* [rows] device, or NULL; >= 1: no cut */
+    const float*   min_p;        /* [rows] device, or NULL; <= 0: no cut */
+    int32_t*       token;        /* [rows] device */
+    float*         logprob;      /* [rows] device, or NULL */
+    uint32_t       rows, vocab;  /* vocab <= 4194304 */
+    int32_t        dtype;        /* BT_F32, BT_F16 or BT_BF16 */
+    uint32_t       reserved;
+} bt_sample_args;
+
+/* A token for every row, each row with its own parameters and its own given
+ * random number: the batched form of bt_cuda_sample_top_p_top_k, over the whole
+ * vocabulary, with min-p.  With tokens ordered by decreasing logit (equal ones by
+ * id), the kept ones are the first top_k; of these the shortest prefix that holds
+ * top_p of their probability; of these the ones with at least min_p times the
+ * largest probability; always the first.  The token is the first, in order of
+ * ids, at which the kept probabilities' running sum passes u of their sum.
+ * Probabilities are whole multiples of 2^-40 of the largest one, so that sums
+ * are exact whatever their order.  -inf and NaN logits are never drawn; where a
+ * row has nothing else, its token is -1.  logprob: the token's log-probability
+ * among the kept ones (0 for greedy rows, -inf with token -1). */
+BT_API int bt_cuda_sample_batch(const bt_sample_args* a, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
