@@ -35,6 +35,12 @@ template <> struct Act<__nv_bfloat16> {
 
 inline uint32_t act_bytes(int dtype) { return dtype == BT_F32 ? 4u : 2u; }
 
+// Whether 16-byte accesses may be used on a tensor (also where it is absent).
+inline bool heads_wide(const bt_heads& h, int dtype) {
+    const int64_t b = act_bytes(dtype);
+    return !h.data || ((uintptr_t)h.data % 16 == 0 && (h.token_stride * b) % 16 == 0 && (h.head_stride * b) % 16 == 0);
+}
+
 // Eight consecutive elements as fp32.  `wide`: the address is 16-byte aligned.
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, bool wide, float (&x)[8]) {

@@ -1,116 +1,634 @@
-// bt_kv4_attn.cu -- causal attention over a 4-bit cache.
+// bt_kv4_attn.cu -- causal attention over a 4-bit cache (bt_cuda_kv4_attention).
+// The arithmetic of a tile and its formulas: bt_kv4_attn.cuh.
 //
-// Mathematics, per query row q of a head at position p:
-//   o = sum_j softmax_j(scale q.k_j) v_j over the positions j <= p that the window
-//   and the sinks leave, k_j and v_j the values the cached codes stand for.
-// One pass over the keys with the running maximum and sum.  A CTA takes one
-// (query row, head); a tile is one key a thread.
-#include "bt_kv4.cuh"
+// Dealing out the work.  An item is (sequence, KV head, block of 8 columns); its
+// units are 16-key tiles, and the units of all items in order are cut into equal
+// ranges, one per group of warps, so that ragged lengths need no tuning: a group
+// works on at most two items it shares with others (its first and its last).  Each
+// shared item's pieces go to the workspace, and the group that finds itself last (an
+// atomic ticket) adds them in the order of the keys, so results do not depend on
+// which that was.  The lengths are read on the device: no host copy, and a captured
+// graph may be replayed with other lengths.
+//
+// A group is a CTA's 16 (or 8) warps where items are long, 4 warps where they are
+// short (less than a tile for every warp), so that a CTA works on several short
+// items at a time.  A warp takes every 16th (8th, 4th) tile of its group's range
+// and streams them through its own ring of bulk copies, which runs on across the
+// ends of items; warps meet only to add up an item.
+#include "bt_kv4_attn.cuh"
 
 namespace bt {
 
-constexpr int kAttnThreads = 128;
+constexpr float kLazyMax = 8.0f;  // a column's reference maximum may be exceeded by 2^8 before it moves
 
-struct AttnParams {
-    const void* q;
-    void* out;
-    int64_t q_ts, q_hs, o_ts, o_hs;
-    const int32_t *kv_len, *q_start, *slots;
-    uint32_t n, heads, window, sinks;
-    float scale;
-    Kv4Map map;
+template <int HD, int TERMS>
+struct AttnCfg {
+    static constexpr int NG = HD / 64;                       // 64-element groups of a row
+    static constexpr uint32_t RB = kv4_row_bytes(HD), TILE = 16 * RB;
+    static constexpr int NW = (HD == 256 || TERMS == 2) ? 8 : 16;  // 128 or 255 registers a thread
+    static constexpr int GROUPS = NW / 4;                    // groups of a CTA, at most
+    static constexpr uint32_t SLOT = 8 * HD;                 // floats of a warp's sums
+    static constexpr uint32_t FIT = (212u * 1024u - NW * SLOT * 4u) / (NW * 2u * TILE);
+    static constexpr uint32_t STAGES = FIT > 8 ? 8 : FIT;
+    static constexpr uint32_t SMEM = NW * (STAGES * 2u * TILE + SLOT * 4u);
 };
 
-template <typename T, int HD>
-__global__ void __launch_bounds__(kAttnThreads) kv4_attn_simple(AttnParams p) {
-    __shared__ float qs[HD], ps[kAttnThreads], red[32];
-    __shared__ int64_t rowid[kAttnThreads];
-    const uint32_t row = blockIdx.x, head = blockIdx.y, tid = threadIdx.x;
-    // the row's sequence: the last i with q_start[i] <= row
-    uint32_t i = row, first = row, count = 1;
-    if (p.q_start) {
-        uint32_t lo = 0, hi = p.n;
-        while (lo + 1 < hi) {
-            const uint32_t mid = (lo + hi) / 2;
-            if ((uint32_t)p.q_start[mid] <= row) lo = mid; else hi = mid;
-        }
-        i = lo;
-        first = p.q_start[i];
-        count = p.q_start[i + 1] - first;
+constexpr int kMaxGroups = 4;                        // of a CTA
+constexpr uint32_t kPieceFloats = 8 * 256 + 16;      // sums, maxima and sums of probabilities of 8 columns
+
+struct AttnShared {
+    uint64_t bar[16][8];
+    uint32_t tile_ok[16][8];
+    float m[16][8], l[16][8];
+    uint64_t warp_units[16];
+    uint32_t warp_items[16];
+    uint64_t total, start_unit[kMaxGroups];
+    uint32_t items, start_seq[kMaxGroups], last[kMaxGroups];
+};
+
+// Walks a warp's tiles in order: every `step`-th unit from a first one on.
+struct TileWalk {
+    uint32_t seq;     // current sequence (n: past the end)
+    uint32_t item, tile;
+    uint64_t unit;    // units from the first one on
+    SeqWork w;
+    int32_t pos_min, pos_max;  // positions of the block's columns
+
+    __device__ __forceinline__ void enter_item(const AttnParams& p) {
+        const uint32_t c0 = (item % w.blocks) * 8, c1 = min(c0 + 8, (uint32_t)w.count * p.group) - 1;
+        pos_min = w.len - w.count + (int32_t)(c0 / p.group);
+        pos_max = w.len - w.count + (int32_t)(c1 / p.group);
     }
-    T* out = (T*)p.out + (int64_t)row * p.o_ts + (int64_t)head * p.o_hs;
-    const int32_t len = min(max(p.kv_len[i], 0), (int32_t)p.map.max_seq);
-    if (tid == 0 && p.kv_len[i] != len) p.map.flag(BT_KV4_RANGE);
-    const int32_t slot = p.slots ? p.slots[i] : (int32_t)i;
-    const int32_t pos = len - (int32_t)count + (int32_t)(row - first);
-    const uint32_t kvh = head / (p.heads / p.map.kv_heads);
-    for (uint32_t d = tid; d < HD; d += kAttnThreads)
-        qs[d] = Act<T>::to_f(((const T*)p.q + (int64_t)row * p.q_ts + (int64_t)head * p.q_hs)[d]) * p.scale;
-    constexpr int PER = (HD + kAttnThreads - 1) / kAttnThreads;
-    float m = -INFINITY, l = 0.0f, o[PER] = {};
-    const int32_t lo = p.window ? max(0, pos - (int32_t)min(p.window, 0x7fffffffu) + 1) : 0;
-    const int32_t sinks = p.window ? min((int32_t)min(p.sinks, 0x7fffffffu), lo) : 0;
-    const int32_t total = pos < 0 ? 0 : sinks + pos - lo + 1;
-    for (int32_t t0 = 0; t0 < total; t0 += kAttnThreads) {
-        __syncthreads();
-        const int32_t at = t0 + (int32_t)tid, j = at < sinks ? at : lo + at - sinks;
-        float s = -INFINITY;
-        int64_t r = -1;
-        if (at < total) {
-            r = p.map.row(slot, kvh, j);
-            if (r < 0) {
-                p.map.flag(BT_KV4_RANGE);
-            } else {
-                const uint8_t* src = p.map.k + (size_t)r * kv4_row_bytes(HD);
-                s = 0.0f;
-                for (int g = 0; g < HD / 64; ++g) {
-                    const __half2 sm = reinterpret_cast<const __half2*>(src + HD / 2)[g];
-                    float a = 0.0f, b = 0.0f;
-                    for (int w = 0; w < 8; ++w) {
-                        const uint32_t c = reinterpret_cast<const uint32_t*>(src)[g * 8 + w];
+    __device__ __forceinline__ void enter_seq(const AttnParams& p) {
+        for (; seq < p.n; ++seq) {
+            w = seq_work(p, seq, false);
+            if (w.blocks) break;
+        }
+    }
+    // Some column of the block sees some key of the tile.
+    __device__ __forceinline__ bool live(const AttnParams& p) const {
+        const int32_t k0 = w.key0(tile);
+        return k0 <= pos_max && (!p.window || k0 + 15 > pos_min - (int64_t)p.window || (uint32_t)k0 < p.sinks);
+    }
+    __device__ __forceinline__ void advance(const AttnParams& p, uint32_t by) {
+        unit += by;
+        tile += by;
+        if (tile < w.tiles) return;
+        do {
+            tile -= w.tiles;
+            if (++item == w.blocks * p.map.kv_heads) {
+                item = 0;
+                ++seq;
+                enter_seq(p);
+                if (seq >= p.n) return;
+            }
+        } while (tile >= w.tiles);
+        enter_item(p);
+    }
+    __device__ __forceinline__ void begin(const AttnParams& p, uint32_t s, uint64_t seq_unit, uint64_t u) {
+        seq = s;
+        w = seq_work(p, s, false);
+        item = (uint32_t)((u - seq_unit) / w.tiles);
+        tile = (uint32_t)((u - seq_unit) % w.tiles);
+        unit = u;
+        enter_item(p);
+    }
+};
+
+__device__ __forceinline__ void group_sync(uint32_t group, uint32_t threads) {
+    asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(threads) : "memory");
+}
+
+template <typename T, int HD, int TERMS>
+__global__ void __launch_bounds__(AttnCfg<HD, TERMS>::NW * 32, 1) kv4_attn_kernel(AttnParams p) {
+    using C = AttnCfg<HD, TERMS>;
+    constexpr int NG = C::NG, NW = C::NW, S = C::STAGES;
+    extern __shared__ __align__(128) uint8_t dyn[];
+    __shared__ AttnShared sh;
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+    uint8_t* ring = dyn + warp * (S * 2u * C::TILE);
+    float* slots = reinterpret_cast<float*>(dyn + NW * (S * 2u * C::TILE));
+
+    // ---- how much work there is, and where this CTA's groups begin
+    if (lane == 0) {
+        for (int i = 0; i < S; ++i) mbar_init(&sh.bar[warp][i], 1);
+        fence_mbar_init();
+    }
+    uint64_t units = 0;
+    uint32_t items = 0;
+    uint64_t own = 0;  // of the sequence this thread looked at last
+    for (uint32_t i = tid; i < p.n; i += NW * 32) {
+        const SeqWork w = seq_work(p, i, blockIdx.x == 0);
+        const uint32_t it = w.blocks * p.map.kv_heads;
+        own = (uint64_t)it * w.tiles;
+        units += own;
+        items += it;
+    }
+    uint64_t su = units;
+    uint32_t si = items;
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const float x = qs[g * 64 + w * 8 + e];
-                            a = fmaf((float)((c >> (4 * e)) & 15u), x, a);
-                            b += x;
+    for (int o = 16; o > 0; o >>= 1) {
+        su += __shfl_xor_sync(0xffffffffu, su, o);
+        si += __shfl_xor_sync(0xffffffffu, si, o);
+    }
+    if (lane == 0) { sh.warp_units[warp] = su; sh.warp_items[warp] = si; }
+    __syncthreads();
+    uint64_t total = 0;
+    items = 0;
+    for (int i = 0; i < NW; ++i) { total += sh.warp_units[i]; items += sh.warp_items[i]; }
+    if (total == 0) return;
+    const uint32_t WG = total >= (uint64_t)items * NW ? NW : 4;  // warps of a group
+    const uint32_t per_cta = NW / WG, group = warp / WG, gw = warp % WG;
+    const uint64_t all = (uint64_t)gridDim.x * per_cta, want = total / (WG / 2 ? WG / 2 : 1);
+    const uint64_t ranges = want < 1 ? 1 : want < all ? want : all;
+    const uint64_t range = (uint64_t)group * gridDim.x + blockIdx.x;  // this group's
+    const uint64_t u0 = range < ranges ? total * range / ranges : 0, u1 = range < ranges ? total * (range + 1) / ranges : 0;
+    {
+        // the sequence that holds each group's first unit
+        uint64_t base = 0;
+        for (uint32_t i0 = 0; i0 < p.n; i0 += NW * 32) {
+            const uint32_t i = i0 + tid;
+            if (p.n > NW * 32) {
+                own = 0;
+                if (i < p.n) {
+                    const SeqWork w = seq_work(p, i, false);
+                    own = (uint64_t)w.blocks * p.map.kv_heads * w.tiles;
+                }
+            }
+            uint64_t inc = own;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint64_t v = __shfl_up_sync(0xffffffffu, inc, o);
+                if (lane >= (uint32_t)o) inc += v;
+            }
+            __syncthreads();
+            if (lane == 31) sh.warp_units[warp] = inc;
+            __syncthreads();
+            uint64_t at = base + inc - own;
+            for (int k = 0; k < NW; ++k) {
+                if (k < (int)warp) at += sh.warp_units[k];
+                base += sh.warp_units[k];
+            }
+            for (uint32_t k = 0; k < per_cta; ++k) {
+                const uint64_t r = (uint64_t)k * gridDim.x + blockIdx.x;
+                if (r >= ranges) break;
+                const uint64_t u = total * r / ranges;
+                if (u >= at && u < at + own) { sh.start_seq[k] = i; sh.start_unit[k] = at; }
+            }
+        }
+        __syncthreads();
+    }
+    if (u0 >= u1) return;
+
+    // ---- the ring of this warp
+    TileWalk next;  // the next tile to copy
+    next.begin(p, sh.start_seq[group], sh.start_unit[group], u0);
+    if (gw) next.advance(p, gw);
+    uint32_t put = 0, put_phase = 0, got = 0, got_phase = 0, in_flight = 0;
+    bool dead = false;  // a wait gave up
+    auto skip_dead = [&] {
+        while (next.unit < u1 && !next.live(p)) next.advance(p, WG);
+    };
+    int64_t next_row = -1;
+    auto look = [&] {  // the row of the next tile; its page is on its way while other tiles are worked on
+        skip_dead();
+        if (next.unit < u1) next_row = p.map.row(next.w.slot, next.item / next.w.blocks, next.w.key0(next.tile));
+    };
+    auto issue = [&] {
+        if (next.unit >= u1) return;
+        if (lane == 0) {
+            uint64_t* bar = &sh.bar[warp][put];
+            if (next_row >= 0) {
+                uint8_t* dst = ring + put * 2u * C::TILE;
+                mbar_expect_tx(bar, 2u * C::TILE);
+                bulk_g2s(dst, p.map.k + (size_t)next_row * C::RB, C::TILE, bar);
+                bulk_g2s(dst + C::TILE, p.map.v + (size_t)next_row * C::RB, C::TILE, bar);
+            } else {
+                p.map.flag(BT_KV4_RANGE);
+                mbar_arrive(bar);
+            }
+            sh.tile_ok[warp][put] = next_row >= 0;
+        }
+        if (++put == S) { put = 0; put_phase ^= 1; }
+        ++in_flight;
+        next.advance(p, WG);
+        look();
+    };
+    look();
+    for (int i = 0; i < S; ++i) issue();
+    __syncwarp();
+
+    // ---- items
+    TileWalk cur;
+    cur.begin(p, sh.start_seq[group], sh.start_unit[group], u0);
+    while (cur.unit < u1) {
+        const SeqWork& w = cur.w;
+        const uint32_t left = w.tiles - cur.tile, seg = (uint32_t)(u1 - cur.unit < left ? u1 - cur.unit : left);
+        const uint32_t kvh = cur.item / w.blocks, c0 = (cur.item % w.blocks) * 8, columns = (uint32_t)w.count * p.group;
+        const bool whole = seg == w.tiles;
+        const uint32_t offset = (gw + WG - (uint32_t)((cur.unit - u0) % WG)) % WG;  // this warp's first tile of the segment
+        const bool active = offset < seg;
+
+        // q of column g as B fragments, scaled so that its largest element is in [2^13, 2^14)
+        uint32_t qf[NG * 4][2], ql[TERMS == 2 ? NG * 4 : 1][2];
+        float qsum[NG][2], factor[2];
+        int32_t pos[2];
+        if (active) {
+            const uint32_t c = c0 + g, row = (uint32_t)w.first + c / p.group;
+            const bool there = c < columns;
+            const T* src = (const T*)p.q + (there ? (int64_t)row * p.q_ts + (int64_t)(kvh * p.group + c % p.group) * p.q_hs : 0);
+            float big = 0.0f;
+            float x[NG][16];
+#pragma unroll
+            for (int j = 0; j < NG; ++j) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float y[8] = {};
+                    if (there) load8(src + 64 * j + 16 * t + 8 * h, p.wide, y);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) {
+                        x[j][8 * h + e] = y[e];
+                        big = fmaxf(big, fabsf(y[e]));
+                    }
+                }
+            }
+            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+            // 2^up brings the largest element to [2^13, 2^14); zero, infinite and subnormal columns stay as they are
+            const int be = (int)(__float_as_uint(big) >> 23);
+            const int up = be > 0 && be < 255 ? min(13 - (be - 127), 126) : 0;
+            const float f = __int_as_float((127 + up) << 23);
+#pragma unroll
+            for (int j = 0; j < NG; ++j) {
+                float s = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) { x[j][e] *= f; s += x[j][e]; }
+                s += __shfl_xor_sync(0xffffffffu, s, 1);
+                s += __shfl_xor_sync(0xffffffffu, s, 2);
+                s *= 0x1p-24f;
+                qsum[j][0] = __shfl_sync(0xffffffffu, s, 8 * t);
+                qsum[j][1] = __shfl_sync(0xffffffffu, s, 8 * t + 4);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {  // elements (a, a + 4) at code weight 1, (a + 1, a + 5) at 16
+                    const int a = 8 * (k >> 1) + 2 * (k & 1);
+                    const float v[4] = {x[j][a], x[j][a + 4], x[j][a + 1] * 0.0625f, x[j][a + 5] * 0.0625f};
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        qf[4 * j + k][h] = pack_half2(v[2 * h], v[2 * h + 1]);
+                        if (TERMS == 2) {
+                            const float2 r = unpack_half2(qf[4 * j + k][h]);
+                            ql[4 * j + k][h] = pack_half2(v[2 * h] - r.x, v[2 * h + 1] - r.y);
                         }
                     }
-                    s += __low2float(sm) * a + __high2float(sm) * b;
+                }
+            }
+            // scores come in units of 2^-24 2^up
+            const float own_f = p.scale_log2 * __int_as_float((127 - up) << 23) * 0x1p24f;
+            factor[0] = __shfl_sync(0xffffffffu, own_f, 8 * t);
+            factor[1] = __shfl_sync(0xffffffffu, own_f, 8 * t + 4);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const uint32_t col = min(c0 + 2 * t + h, columns - 1);
+                pos[h] = w.len - w.count + (int32_t)(col / p.group);
+            }
+        }
+
+        float o[NG * 4][4] = {}, mo[NG][2] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {};
+        uint32_t v_bound = 0;       // no V scale so far is larger (as fp16 bits)
+        int v_exp = 0;              // p s is multiplied by 2^v_exp
+        float v_mul = 1.0f;
+
+        auto tile = [&](auto masked_c, int32_t key0, const uint8_t* kt) {
+            constexpr bool MASKED = decltype(masked_c)::value;
+            const uint8_t* vt = kt + C::TILE;
+            const uint32_t r0 = key_of(g), r1 = r0 + 2;  // MMA rows g and g + 8
+            bool vis[4] = {true, true, true, true};
+            uint32_t ok0 = 0xffffffffu, ok1 = 0xffffffffu;
+            if (MASKED) {
+                const int32_t k0 = key0 + (int32_t)r0, k1 = k0 + 2;
+                auto sees = [&](int32_t at, int32_t key) {
+                    return key <= at && (!p.window || key > at - (int64_t)p.window || (uint32_t)key < p.sinks);
+                };
+                vis[0] = sees(pos[0], k0); vis[1] = sees(pos[1], k0); vis[2] = sees(pos[0], k1); vis[3] = sees(pos[1], k1);
+                // keys that no column of the block sees may hold anything
+                auto held = [&](int32_t key) {
+                    return key <= cur.pos_max && (!p.window || key > cur.pos_min - (int64_t)p.window || (uint32_t)key < p.sinks);
+                };
+                ok0 = held(k0) ? 0xffffffffu : 0u;
+                ok1 = held(k1) ? 0xffffffffu : 0u;
+            }
+            // scores
+            float s[4] = {};
+#pragma unroll
+            for (int j = 0; j < NG; ++j) {
+                uint32_t a[2], b[2];  // the lane's 16 codes of rows g and g + 8
+                const uint8_t *pa = kt + r0 * C::RB + 32 * j + 8 * t, *pb = kt + r1 * C::RB + 32 * j + 8 * t;
+                if (HD == 64) {  // rows of 36 bytes
+                    a[0] = reinterpret_cast<const uint32_t*>(pa)[0]; a[1] = reinterpret_cast<const uint32_t*>(pa)[1];
+                    b[0] = reinterpret_cast<const uint32_t*>(pb)[0]; b[1] = reinterpret_cast<const uint32_t*>(pb)[1];
+                } else {
+                    const uint2 va = *reinterpret_cast<const uint2*>(pa), vb = *reinterpret_cast<const uint2*>(pb);
+                    a[0] = va.x; a[1] = va.y; b[0] = vb.x; b[1] = vb.y;
+                }
+                float c[4] = {};
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t a8 = a[h] >> 8, b8 = b[h] >> 8;
+                    const uint32_t f0[4] = {a[h] & 0x000f000fu, b[h] & 0x000f000fu, a[h] & 0x00f000f0u, b[h] & 0x00f000f0u};
+                    const uint32_t f1[4] = {a8 & 0x000f000fu, b8 & 0x000f000fu, a8 & 0x00f000f0u, b8 & 0x00f000f0u};
+                    const int k = 4 * j + 2 * h;
+                    mma_f16(c, f0[0], f0[1], f0[2], f0[3], qf[k][0], qf[k][1]);
+                    mma_f16(c, f1[0], f1[1], f1[2], f1[3], qf[k + 1][0], qf[k + 1][1]);
+                    if (TERMS == 2) {
+                        mma_f16(c, f0[0], f0[1], f0[2], f0[3], ql[k][0], ql[k][1]);
+                        mma_f16(c, f1[0], f1[1], f1[2], f1[3], ql[k + 1][0], ql[k + 1][1]);
+                    }
+                }
+                const float2 e0 = unpack_half2(reinterpret_cast<const uint32_t*>(kt + r0 * C::RB + HD / 2)[j] & ok0);
+                const float2 e1 = unpack_half2(reinterpret_cast<const uint32_t*>(kt + r1 * C::RB + HD / 2)[j] & ok1);
+                s[0] = fmaf(e0.x, c[0], fmaf(e0.y, qsum[j][0], s[0]));
+                s[1] = fmaf(e0.x, c[1], fmaf(e0.y, qsum[j][1], s[1]));
+                s[2] = fmaf(e1.x, c[2], fmaf(e1.y, qsum[j][0], s[2]));
+                s[3] = fmaf(e1.x, c[3], fmaf(e1.y, qsum[j][1], s[3]));
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[i] = vis[i] ? s[i] * factor[i & 1] : -INFINITY;
+
+            // the pairs of V, and whether a maximum or the largest V scale moves
+            uint32_t e0[NG], e1[NG], big = 0;
+#pragma unroll
+            for (int j = 0; j < NG; ++j) {
+                e0[j] = reinterpret_cast<const uint32_t*>(vt + r0 * C::RB + HD / 2)[j] & ok0;
+                e1[j] = reinterpret_cast<const uint32_t*>(vt + r1 * C::RB + HD / 2)[j] & ok1;
+                big = max(big, max(e0[j] & 0xffffu, e1[j] & 0xffffu));
+            }
+            const float top0 = fmaxf(s[0], s[2]), top1 = fmaxf(s[1], s[3]);
+            if (__any_sync(0xffffffffu, top0 > m[0] + kLazyMax || top1 > m[1] + kLazyMax || big > v_bound)) {
+                float a = top0, b = top1;
+#pragma unroll
+                for (int x = 4; x < 32; x <<= 1) {
+                    a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, x));
+                    b = fmaxf(b, __shfl_xor_sync(0xffffffffu, b, x));
+                }
+                a = fmaxf(a, m[0]);
+                b = fmaxf(b, m[1]);
+                const float fa = a == m[0] ? 1.0f : exp2_fast(m[0] - a), fb = b == m[1] ? 1.0f : exp2_fast(m[1] - b);
+                m[0] = a;
+                m[1] = b;
+                big = __reduce_max_sync(0xffffffffu, big);
+                float fv = 1.0f;
+                if (big > v_bound) {
+                    // s < 2^(x + 1): p s 2^v_exp stays below 2^15 with p <= 2^8
+                    const int x = max((int)(big >> 10), 1) - 15, e = 6 - x;
+                    fv = v_bound ? __int_as_float((127 + e - v_exp) << 23) : 0.0f;
+                    v_exp = e;
+                    v_mul = __int_as_float((127 + e) << 23);
+                    v_bound = big | 0x3ffu;
+                }
+                l[0] *= fa;
+                l[1] *= fb;
+#pragma unroll
+                for (int j = 0; j < NG; ++j) { mo[j][0] *= fa; mo[j][1] *= fb; }
+#pragma unroll
+                for (int i = 0; i < NG * 4; ++i) {
+                    o[i][0] *= fa * fv; o[i][1] *= fb * fv; o[i][2] *= fa * fv; o[i][3] *= fb * fv;
+                }
+            }
+            float pr[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                pr[i] = exp2_fast(s[i] - m[i & 1]);
+                if (MASKED && !vis[i]) pr[i] = 0.0f;
+            }
+            l[0] += pr[0] + pr[2];
+            l[1] += pr[1] + pr[3];
+
+            // values: rows 2t, 2t + 1, 2t + 8, 2t + 9 of the tile are this lane's keys of V
+            const uint32_t ra = key_of(2 * t), rb = key_of(2 * t + 1);
+#pragma unroll
+            for (int j = 0; j < NG; ++j) {
+                const float2 x0 = unpack_half2(e0[j]), x1 = unpack_half2(e1[j]);
+                mo[j][0] = fmaf(pr[0], x0.y, fmaf(pr[2], x1.y, mo[j][0]));
+                mo[j][1] = fmaf(pr[1], x0.y, fmaf(pr[3], x1.y, mo[j][1]));
+                const float s0 = x0.x * v_mul, s1 = x1.x * v_mul;
+                const uint32_t h0 = pack_half2(pr[0] * s0, pr[1] * s0), h1 = pack_half2(pr[2] * s1, pr[3] * s1);
+                const uint32_t b0 = transpose8(h0), b1 = transpose8(h1);
+                uint32_t b2 = 0, b3 = 0;
+                if (TERMS == 2) {
+                    const float2 y0 = unpack_half2(h0), y1 = unpack_half2(h1);
+                    b2 = transpose8(pack_half2(fmaf(pr[0], s0, -y0.x), fmaf(pr[1], s0, -y0.y)));
+                    b3 = transpose8(pack_half2(fmaf(pr[2], s1, -y1.x), fmaf(pr[3], s1, -y1.y)));
+                }
+                const uint8_t* q0 = vt + 32 * j + 4 * g;
+                const uint32_t va = *reinterpret_cast<const uint32_t*>(q0 + ra * C::RB), vb = *reinterpret_cast<const uint32_t*>(q0 + rb * C::RB);
+                const uint32_t vc = *reinterpret_cast<const uint32_t*>(q0 + (ra + 2) * C::RB), vd = *reinterpret_cast<const uint32_t*>(q0 + (rb + 2) * C::RB);
+                uint32_t f[4] = {__byte_perm(va, vb, 0x5410), __byte_perm(va, vb, 0x7632), __byte_perm(vc, vd, 0x5410), __byte_perm(vc, vd, 0x7632)};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {  // dims 8g + i (rows g) and 8g + i + 4 (rows g + 8) of the group
+                    const uint32_t mask = i & 1 ? 0x00f000f0u : 0x000f000fu;
+                    if (i == 2) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) f[k] >>= 8;
+                    }
+                    mma_f16(o[4 * j + i], f[0] & mask, f[1] & mask, f[2] & mask, f[3] & mask, b0, b1);
+                    if (TERMS == 2) mma_f16(o[4 * j + i], f[0] & mask, f[1] & mask, f[2] & mask, f[3] & mask, b2, b3);
+                }
+            }
+        };
+
+        for (uint32_t x = offset; x < seg; x += WG) {
+            const int32_t key0 = w.key0(cur.tile + x);
+            if (!(key0 <= cur.pos_max && (!p.window || key0 + 15 > cur.pos_min - (int64_t)p.window || (uint32_t)key0 < p.sinks))) continue;
+            if (!dead && !mbar_wait(&sh.bar[warp][got], got_phase, nullptr)) {
+                dead = true;
+                if (lane == 0) p.map.flag(BT_KV4_TIMEOUT);
+            }
+            dead = __any_sync(0xffffffffu, dead);
+            const uint8_t* kt = ring + got * 2u * C::TILE;
+            if (!dead && sh.tile_ok[warp][got]) {
+                const bool all_seen = key0 + 15 <= cur.pos_min &&
+                                      (!p.window || key0 > cur.pos_max - (int64_t)p.window || (uint32_t)key0 + 15 < p.sinks);
+                if (all_seen) tile(std::false_type(), key0, kt);
+                else tile(std::true_type(), key0, kt);
+            }
+            __syncwarp();  // every lane is done with the stage
+            if (++got == S) { got = 0; got_phase ^= 1; }
+            --in_flight;
+            if (!dead) issue();
+            __syncwarp();
+        }
+
+        // ---- add up the warps' sums
+        float* slot = slots + warp * C::SLOT;
+        if (active) {
+#pragma unroll
+            for (int x = 4; x < 32; x <<= 1) {
+                l[0] += __shfl_xor_sync(0xffffffffu, l[0], x);
+                l[1] += __shfl_xor_sync(0xffffffffu, l[1], x);
+#pragma unroll
+                for (int j = 0; j < NG; ++j) {
+                    mo[j][0] += __shfl_xor_sync(0xffffffffu, mo[j][0], x);
+                    mo[j][1] += __shfl_xor_sync(0xffffffffu, mo[j][1], x);
+                }
+            }
+            if (g == 0) {
+                sh.m[warp][2 * t] = m[0]; sh.m[warp][2 * t + 1] = m[1];
+            }
+        } else if (g == 0) {
+            sh.m[warp][2 * t] = sh.m[warp][2 * t + 1] = -INFINITY;
+        }
+        group_sync(group, WG * 32);
+        if (active) {
+            float f[2], k0[2], k1[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float top = -INFINITY;
+                for (uint32_t i = 0; i < WG; ++i) top = fmaxf(top, sh.m[group * WG + i][2 * t + h]);
+                f[h] = m[h] == -INFINITY ? 0.0f : exp2_fast(m[h] - top);
+                if (!(l[h] == l[h])) f[h] = NAN;  // a column with NaN scores has no maximum
+                k0[h] = f[h] * __int_as_float((127 + 24 - v_exp) << 23);  // codes at weight 2^-24
+                k1[h] = k0[h] * 0.0625f;                                   // and at 2^-20
+                if (g == 0) sh.l[warp][2 * t + h] = l[h] * f[h];
+            }
+#pragma unroll
+            for (int j = 0; j < NG; ++j) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float base = mo[j][h] * f[h];
+                    float4* dst = reinterpret_cast<float4*>(slot + (2 * t + h) * HD + 64 * j + 8 * g);
+                    dst[0] = make_float4(fmaf(o[4 * j][h], k0[h], base), fmaf(o[4 * j + 1][h], k1[h], base),
+                                         fmaf(o[4 * j + 2][h], k0[h], base), fmaf(o[4 * j + 3][h], k1[h], base));
+                    dst[1] = make_float4(fmaf(o[4 * j][h + 2], k0[h], base), fmaf(o[4 * j + 1][h + 2], k1[h], base),
+                                         fmaf(o[4 * j + 2][h + 2], k0[h], base), fmaf(o[4 * j + 3][h + 2], k1[h], base));
                 }
             }
         }
-        const float m_new = fmaxf(m, block_max(s, red));
-        const float prob = r >= 0 ? expf(s - m_new) : 0.0f, fix = m == -INFINITY ? 0.0f : expf(m - m_new);
-        ps[tid] = prob;
-        rowid[tid] = r;
-        l = l * fix + block_sum(prob, red);
-        m = m_new;
+        group_sync(group, WG * 32);
+
+        const uint32_t gt = gw * 32 + lane, threads = WG * 32;
+        // the warps that had tiles, in order of their first tile
+        const uint32_t used = min(seg, WG), first_warp = (uint32_t)((cur.unit - u0) % WG);
+        auto sum4 = [&](uint32_t i) {  // floats 4 i .. 4 i + 3 of the item's sums
+            float4 a = make_float4(0, 0, 0, 0);
+            for (uint32_t k = 0; k < used; ++k) {
+                const float4 b = reinterpret_cast<const float4*>(slots + (group * WG + (first_warp + k) % WG) * C::SLOT)[i];
+                a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
+            }
+            return a;
+        };
+        auto sum_l = [&](uint32_t c) {
+            float a = 0.0f;
+            for (uint32_t k = 0; k < used; ++k) a += sh.l[group * WG + (first_warp + k) % WG][c];
+            return a;
+        };
+        auto store4 = [&](uint32_t c, uint32_t d, float4 v, float sum) {  // column c of the block
+            const uint32_t col = c0 + c;
+            if (col >= columns) return;
+            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+            T* dst = (T*)p.out + (int64_t)((uint32_t)w.first + col / p.group) * p.o_ts +
+                     (int64_t)(kvh * p.group + col % p.group) * p.o_hs + d;
+            union { uint2 u[sizeof(T) / 2]; T x[4]; } r;
+            r.x[0] = Act<T>::from_f(v.x * inv); r.x[1] = Act<T>::from_f(v.y * inv);
+            r.x[2] = Act<T>::from_f(v.z * inv); r.x[3] = Act<T>::from_f(v.w * inv);
+            if (p.wide) {
 #pragma unroll
-        for (int k = 0; k < PER; ++k) {
-            const uint32_t d = tid + k * kAttnThreads;
-            o[k] *= fix;
-            if (d < HD) {
-                for (int32_t t = 0; t < min(kAttnThreads, total - t0); ++t) {
-                    if (rowid[t] < 0) continue;
-                    const uint8_t* src = p.map.v + (size_t)rowid[t] * kv4_row_bytes(HD);
-                    const __half2 sm = reinterpret_cast<const __half2*>(src + HD / 2)[d / 64];
-                    o[k] = fmaf(ps[t], (float)((src[d / 2] >> (4 * (d & 1))) & 15u) * __low2float(sm) + __high2float(sm), o[k]);
+                for (int i = 0; i < (int)(sizeof(T) / 2); ++i) reinterpret_cast<uint2*>(dst)[i] = r.u[i];
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) dst[i] = r.x[i];
+            }
+        };
+        if (whole) {
+            for (uint32_t i = gt; i < C::SLOT / 4; i += threads) store4(i / (HD / 4), i % (HD / 4) * 4, sum4(i), sum_l(i / (HD / 4)));
+        } else {
+            // this group's piece: slot 0 of its range if the item began before it, else slot 1
+            float* mine = p.partial + (range * 2 + (cur.tile ? 0 : 1)) * kPieceFloats;
+            for (uint32_t i = gt; i < C::SLOT / 4; i += threads) __stcg(reinterpret_cast<float4*>(mine + 16) + i, sum4(i));
+            if (gt < 8) {
+                float top = -INFINITY;
+                for (uint32_t i = 0; i < WG; ++i) top = fmaxf(top, sh.m[group * WG + i][gt]);
+                __stcg(mine + gt, top);
+                __stcg(mine + 8 + gt, sum_l(gt));
+            }
+            // the item's units and the ranges that share it
+            const uint64_t i0 = cur.unit - cur.tile, i1 = i0 + w.tiles - 1;
+            const uint64_t ra = ((i0 + 1) * ranges - 1) / total, rb = ((i1 + 1) * ranges - 1) / total;
+            __threadfence();
+            group_sync(group, threads);
+            if (gt == 0) {
+                const uint32_t before = atomicAdd(p.tickets + ra, 1u);
+                sh.last[group] = before == (uint32_t)(rb - ra);
+                if (sh.last[group]) p.tickets[ra] = 0;  // ready for the next call
+                __threadfence();
+            }
+            group_sync(group, threads);
+            if (sh.last[group]) {
+                for (uint32_t i = gt; i < C::SLOT / 4; i += threads) {
+                    const uint32_t c = i / (HD / 4);
+                    float top = -INFINITY;
+                    for (uint64_t r = ra; r <= rb; ++r) top = fmaxf(top, __ldcg(p.partial + (r * 2 + (r == ra ? 1 : 0)) * kPieceFloats + c));
+                    float4 a = make_float4(0, 0, 0, 0);
+                    float sum = 0.0f;
+                    for (uint64_t r = ra; r <= rb; ++r) {
+                        const float* piece = p.partial + (r * 2 + (r == ra ? 1 : 0)) * kPieceFloats;
+                        const float pm = __ldcg(piece + c), pl = __ldcg(piece + 8 + c);
+                        const float f = pl != pl ? NAN : pm == -INFINITY ? 0.0f : exp2_fast(pm - top);
+                        const float4 b = __ldcg(reinterpret_cast<const float4*>(piece + 16) + i);
+                        a.x = fmaf(b.x, f, a.x); a.y = fmaf(b.y, f, a.y); a.z = fmaf(b.z, f, a.z); a.w = fmaf(b.w, f, a.w);
+                        sum = fmaf(pl, f, sum);
+                    }
+                    store4(c, i % (HD / 4) * 4, a, sum);
                 }
             }
         }
+        group_sync(group, threads);  // the slots are free again
+        cur.advance(p, seg);
     }
-#pragma unroll
-    for (int k = 0; k < PER; ++k) {
-        const uint32_t d = tid + k * kAttnThreads;
-        if (d < HD) out[d] = Act<T>::from_f(l > 0.0f ? o[k] / l : 0.0f);
+    // after an expired wait copies may still be on their way to this CTA's shared memory
+    for (; dead && in_flight > 0; --in_flight) {
+        mbar_wait(&sh.bar[warp][got], got_phase, nullptr);
+        if (++got == S) { got = 0; got_phase ^= 1; }
     }
+}
+
+static int device_sms() {
+    static std::atomic<int> known[64];
+    int dev = 0, sms = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+    if (dev < 64 && (sms = known[dev].load(std::memory_order_relaxed)) > 0) return sms;
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+    if (dev < 64) known[dev].store(sms, std::memory_order_relaxed);
+    return sms;
+}
+
+template <typename T, int HD, int TERMS>
+static cudaError_t attn_launch(const AttnParams& p, int sms, cudaStream_t s) {
+    using C = AttnCfg<HD, TERMS>;
+    static std::atomic<uint64_t> ready{0};  // devices whose attribute is set
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev >= 64 || !(ready.load(std::memory_order_relaxed) >> dev & 1)) {
+        e = cudaFuncSetAttribute(kv4_attn_kernel<T, HD, TERMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+        if (e != cudaSuccess) return e;
+        if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
+    }
+    g_launches.fetch_add(1, std::memory_order_relaxed);
+    kv4_attn_kernel<T, HD, TERMS><<<sms, C::NW * 32, C::SMEM, s>>>(p);
+    return cudaGetLastError();
 }
 
 }  // namespace bt
 
 using namespace bt;
 
-extern "C" uint64_t bt_cuda_kv4_attention_workspace(uint32_t n) { return 256 + (uint64_t)n * 0; }
+// tickets of every range, then two pieces for each
+static uint64_t ticket_bytes(int sms) { return ((uint64_t)sms * kMaxGroups * 4 + 255) / 256 * 256; }
+
+extern "C" uint64_t bt_cuda_kv4_attention_workspace(void) {
+    const int sms = device_sms();
+    return sms > 0 ? ticket_bytes(sms) + (uint64_t)sms * kMaxGroups * 2 * kPieceFloats * 4 : 0;
+}
 
 extern "C" int bt_cuda_kv4_attention(const bt_kv4* cache, const bt_kv4_attn_args* a, void* workspace,
                                      uint64_t workspace_bytes, void* stream) {
@@ -120,29 +638,33 @@ extern "C" int bt_cuda_kv4_attention(const bt_kv4* cache, const bt_kv4_attn_args
     BT_CHECK_ARG(a, "kv4_attention: null arguments");
     BT_CHECK_ARG(a->dtype == BT_F32 || a->dtype == BT_F16 || a->dtype == BT_BF16, "kv4_attention: unknown dtype");
     BT_CHECK_ARG(a->heads > 0 && a->heads <= 65535 && a->heads % cache->kv_heads == 0, "kv4_attention: heads must be a multiple of kv_heads");
-    BT_CHECK_ARG(a->tokens <= 0x7fffffffu && a->n <= 0x7fffffffu, "kv4_attention: too many tokens or sequences");
+    BT_CHECK_ARG((uint64_t)a->tokens * a->heads <= 0x7fffffffu && a->n <= 0x7fffffffu, "kv4_attention: too many rows or sequences");
     BT_CHECK_ARG(a->q_start || a->tokens == a->n, "kv4_attention: without q_start there is one query per sequence");
     BT_CHECK_ARG(a->slots || a->n <= cache->n_seq, "kv4_attention: more sequences than slots");
     if (a->tokens == 0 || a->n == 0) return BT_OK;
     BT_CHECK_ARG(a->q.data && a->out.data && a->kv_len, "kv4_attention: null q, out or kv_len");
     BT_CHECK_ARG(((uintptr_t)a->q.data | (uintptr_t)a->out.data) % act_bytes(a->dtype) == 0, "kv4_attention: a tensor is not aligned to its elements");
-    BT_CHECK_ARG(workspace && (uintptr_t)workspace % 256 == 0 && workspace_bytes >= bt_cuda_kv4_attention_workspace(a->n),
+    const int sms = device_sms();
+    if (sms <= 0) return fail(BT_ERR_CUDA, "kv4_attention: no device");
+    BT_CHECK_ARG(workspace && (uintptr_t)workspace % 256 == 0 && workspace_bytes >= bt_cuda_kv4_attention_workspace(),
                  "kv4_attention: the workspace is null, not 256-byte aligned or too small");
     p.q = a->q.data; p.out = a->out.data; p.q_ts = a->q.token_stride; p.q_hs = a->q.head_stride;
     p.o_ts = a->out.token_stride; p.o_hs = a->out.head_stride; p.kv_len = a->kv_len; p.q_start = a->q_start; p.slots = a->slots;
-    p.n = a->n; p.heads = a->heads; p.window = a->window; p.sinks = a->window ? a->sinks : 0; p.scale = a->scale;
-    const dim3 grid(a->tokens, a->heads);
+    p.n = a->n; p.tokens = a->tokens; p.heads = a->heads; p.group = a->heads / cache->kv_heads;
+    p.window = a->window; p.sinks = a->window ? a->sinks : 0; p.scale_log2 = a->scale * 1.4426950408889634f;
+    p.wide = heads_wide(a->q, a->dtype) && heads_wide(a->out, a->dtype);
+    p.tickets = (uint32_t*)workspace;
+    p.partial = (float*)((uint8_t*)workspace + ticket_bytes(sms));
     const cudaStream_t s = as_stream(stream);
-    g_launches.fetch_add(1, std::memory_order_relaxed);
-    auto by_hd = [&](auto type) {
+    auto by_hd = [&](auto type, auto terms) {
         using T = decltype(type);
-        if (cache->head_dim == 64) kv4_attn_simple<T, 64><<<grid, kAttnThreads, 0, s>>>(p);
-        else if (cache->head_dim == 128) kv4_attn_simple<T, 128><<<grid, kAttnThreads, 0, s>>>(p);
-        else kv4_attn_simple<T, 256><<<grid, kAttnThreads, 0, s>>>(p);
+        constexpr int N = decltype(terms)::value;
+        if (cache->head_dim == 64) return attn_launch<T, 64, N>(p, sms, s);
+        if (cache->head_dim == 128) return attn_launch<T, 128, N>(p, sms, s);
+        return attn_launch<T, 256, N>(p, sms, s);
     };
-    if (a->dtype == BT_F32) by_hd(float());
-    else if (a->dtype == BT_F16) by_hd(__half());
-    else by_hd(__nv_bfloat16());
-    BT_CUDA_CHECK(cudaGetLastError());
+    if (a->dtype == BT_F32) BT_CUDA_CHECK(by_hd(float(), std::integral_constant<int, 2>()));
+    else if (a->dtype == BT_F16) BT_CUDA_CHECK(by_hd(__half(), std::integral_constant<int, 1>()));
+    else BT_CUDA_CHECK(by_hd(__nv_bfloat16(), std::integral_constant<int, 1>()));
     return BT_OK;
 }

@@ -1,0 +1,117 @@
+// bt_kv4_attn.cuh -- attention of a few query rows over a 4-bit cache: the key
+// loop of one warp on tensor cores, and how a call's work is dealt out.
+//
+// Mathematics.  Eight (query, head) columns that share a KV head go over 16-key
+// tiles.  With codes c, and (s, m) the pair of a key's 64-element group j,
+//   score[key][col] = sum_j s_j (sum_{i in j} c_i q_i) + m_j (sum_{i in j} q_i)
+//   out[col][d]     = sum_key (p s_j) c_d + sum_key p m_j,     d in group j
+// so the tensor cores only ever see codes, which are exact in fp16: a code's four
+// bits masked into the low mantissa bits of a half are the subnormal c 2^-24 (or
+// c 2^-20 from the next nibble up), one logical operation for two codes and no
+// conversion.  s and m stay in fp32.  The queries (scaled by a power of two per
+// column so that both terms stay normal) are exact for fp16 and bf16 inputs and two
+// fp16 terms (22 bits) for fp32; p s_j likewise is one or two terms.
+//
+// mma.sync m16n8k16: scores have the 16 keys as M, the 8 columns as N; out has 16
+// dims as M and the tile's 16 keys as K.  tcgen05 has no use here: M is the cache's
+// side at 16 rows a warp, the operands come from registers after unpacking, and
+// at 4.5 bits an element the kernel is bound by memory and by the unpacking's
+// issue slots (about 200 a 16-key tile of head_dim 128, 2304 bytes).
+#pragma once
+
+#include "bt_kv4.cuh"
+#include "bt_ptx.cuh"
+
+namespace bt {
+
+struct AttnParams {
+    const void* q;
+    void* out;
+    int64_t q_ts, q_hs, o_ts, o_hs;  // elements
+    const int32_t *kv_len, *q_start, *slots;
+    uint32_t n, tokens, heads, group;  // group: query heads of a KV head
+    uint32_t window, sinks;
+    float scale_log2;                  // scale * log2(e)
+    bool wide;
+    Kv4Map map;
+    float* partial;                    // workspace: partial results and their tickets
+    uint32_t* tickets;
+};
+
+// ---------------------------------------------------------------- mma helpers
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// 8x8 transpose of halves over the warp: lane (g, t) gives row g, columns 2t, 2t+1
+// and gets row g, columns 2t, 2t+1 of the transposed matrix.
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 unpack_half2(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// The row of a 16-key tile that MMA row r reads: a 4x4 transpose of the keys, so
+// that the rows a warp reads together lie in different shared-memory banks.
+__device__ __forceinline__ uint32_t key_of(uint32_t r) { return 4 * (r & 3) + (r >> 2); }
+
+// ---------------------------------------------------------------- work
+
+// One sequence's share of the work: `blocks` blocks of 8 columns per KV head, each
+// over `tiles` 16-key tiles; the first sink_tiles start at key 0, the rest at key lo.
+struct SeqWork {
+    int32_t first, count, len, slot;  // rows of q, cached positions
+    uint32_t blocks, tiles, sink_tiles;
+    int32_t lo;
+    __device__ __forceinline__ int32_t key0(uint32_t tile) const {
+        return tile < sink_tiles ? (int32_t)tile * 16 : lo + (int32_t)(tile - sink_tiles) * 16;
+    }
+};
+
+__device__ __forceinline__ SeqWork seq_work(const AttnParams& p, uint32_t i, bool report) {
+    SeqWork w;
+    w.first = (int32_t)i;
+    w.count = 1;
+    if (p.q_start) {
+        const int32_t a = p.q_start[i], b = p.q_start[i + 1];
+        w.first = a;
+        w.count = b - a;
+        if (a < 0 || b < a || (uint32_t)b > p.tokens) {
+            w.count = 0;
+            if (report) p.map.flag(BT_KV4_RANGE);
+        }
+    }
+    const int32_t given = p.kv_len[i];
+    w.slot = p.slots ? p.slots[i] : (int32_t)i;
+    w.len = min(max(given, 0), (int32_t)p.map.max_seq);
+    const bool slot_ok = (uint32_t)w.slot < p.map.n_seq;
+    if (report && (w.len != given || !slot_ok)) p.map.flag(BT_KV4_RANGE);
+    if (!slot_ok) w.len = 0;
+    const int32_t lowest = w.len - w.count;  // the first query's position
+    int32_t lo = 0;
+    if (p.window && lowest >= 0 && (uint32_t)lowest >= p.window) lo = lowest - (int32_t)p.window + 1;
+    w.lo = lo & ~15;
+    w.sink_tiles = p.window ? min((min(p.sinks, 0x7ffffff0u) + 15) / 16, (uint32_t)w.lo / 16) : 0;
+    w.blocks = ((uint32_t)w.count * p.group + 7) / 8;
+    // at least one tile, so that the rows of an empty sequence are written
+    w.tiles = max(1u, w.sink_tiles + (uint32_t)(max(w.len - w.lo, 0) + 15) / 16);
+    return w;
+}
+
+}  // namespace bt

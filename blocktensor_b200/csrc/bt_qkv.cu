@@ -186,11 +186,6 @@ __global__ void __launch_bounds__(kQkvThreads) kv4_read_kernel(Kv4Map map, const
     }
 }
 
-static bool wide_ok(const bt_heads& h, int dtype) {
-    const int64_t b = act_bytes(dtype);
-    return !h.data || (((uintptr_t)h.data % 16 == 0) && (h.token_stride * b) % 16 == 0 && (h.head_stride * b) % 16 == 0);
-}
-
 int kv4_map(const bt_kv4* c, const char* who, Kv4Map* m) {
     const std::string w(who);
     BT_CHECK_ARG(c, w + ": null cache");
@@ -255,8 +250,8 @@ static int qkv_launch(const bt_qk_args* a, const bt_kv4* cache, const char* who,
     p.qw = a->q_weight; p.kw = a->k_weight; p.positions = a->positions; p.slots = a->slots;
     p.rope = reinterpret_cast<const float2*>(a->rope); p.rope_positions = a->rope_positions; p.rot = a->rope ? a->rot_dim : 0;
     p.heads = a->heads; p.kv_heads = a->kv_heads; p.eps = a->eps;
-    p.wide = wide_ok(a->q, a->dtype) && wide_ok(a->k, a->dtype) && wide_ok(a->q_out, a->dtype) &&
-             (append ? wide_ok(a->v, a->dtype) : wide_ok(a->k_out, a->dtype));
+    p.wide = heads_wide(a->q, a->dtype) && heads_wide(a->k, a->dtype) && heads_wide(a->q_out, a->dtype) &&
+             (append ? heads_wide(a->v, a->dtype) : heads_wide(a->k_out, a->dtype));
     const uint32_t rows = (p.q ? p.heads : 0) + (p.k ? p.kv_heads : 0) + (append ? p.kv_heads : 0);
     const uint32_t per = kQkvThreads / (a->head_dim / 8), passes = (rows + per - 1) / per;
     // about four CTAs per SM before a CTA takes more than one set of rows

@@ -272,12 +272,12 @@ class KV4Cache:
                         None if slots is None else _vector(slots, "slots", n, torch.int32, dev),
                         n, tokens, heads, max_q, window, sinks, _dtype(q), self.head_dim ** -0.5 if scale is None else scale)
         s = (torch.cuda.current_stream(dev) if stream is None else stream).cuda_stream
-        ws = self._workspaces.get((s, n))
+        ws = self._workspaces.get(s)
         if ws is None:  # one for every stream that the calls come from
             with torch.cuda.device(dev):
-                size = native.load().bt_cuda_kv4_attention_workspace(n)
+                size = native.load().bt_cuda_kv4_attention_workspace()
             with torch.cuda.stream(torch.cuda.current_stream(dev) if stream is None else stream):
-                ws = self._workspaces[(s, n)] = torch.zeros(size, dtype=torch.uint8, device=dev)
+                ws = self._workspaces[s] = torch.zeros(size, dtype=torch.uint8, device=dev)
         _launch("bt_cuda_kv4_attention", dev, stream, (out,), self._ref, C.byref(a), ws.data_ptr(), ws.numel())
         return out
 

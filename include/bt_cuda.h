@@ -578,8 +578,8 @@ typedef struct bt_kv4_attn_args {
  * one each.  Deterministic: the same inputs give the same bits. */
 BT_API int bt_cuda_kv4_attention(const bt_kv4* cache, const bt_kv4_attn_args* a, void* workspace,
                                  uint64_t workspace_bytes, void* stream);
-/* Bytes of workspace that a call with n sequences needs on the current device. */
-BT_API uint64_t bt_cuda_kv4_attention_workspace(uint32_t n);
+/* Bytes of workspace that a call needs on the current device, whatever its sizes. */
+BT_API uint64_t bt_cuda_kv4_attention_workspace(void);
 
 typedef struct bt_sample_args {
     const void*    logits;       /* [rows][vocab], rows row_stride elements apart */
