@@ -2,7 +2,7 @@
 // The arithmetic of a tile and its formulas: bt_kv4_attn.cuh.
 //
 // Dealing out the work.  An item is (sequence, KV head, block of 8 columns); its
-// units are 16-key tiles, and the units of all items in order are cut into equal
+// units are 32 keys, and the units of all items in order are cut into equal
 // ranges, one per group of warps, so that ragged lengths need no tuning: a group
 // works on at most two items it shares with others (its first and its last).  Each
 // shared item's pieces go to the workspace, and the group that finds itself last (an
@@ -11,88 +11,80 @@
 // graph may be replayed with other lengths.
 //
 // A group is a CTA's 16 (or 8) warps where items are long, 4 warps where they are
-// short (less than a tile for every warp), so that a CTA works on several short
-// items at a time.  A warp takes every 16th (8th, 4th) tile of its group's range
+// short (less than a unit for every warp), so that a CTA works on several short
+// items at a time.  A warp takes every 16th (8th, 4th) unit of its group's range
 // and streams them through its own ring of bulk copies, which runs on across the
 // ends of items; warps meet only to add up an item.
 #include "bt_kv4_attn.cuh"
 
 namespace bt {
 
-constexpr float kLazyMax = 8.0f;  // a column's reference maximum may be exceeded by 2^8 before it moves
+constexpr float kLazyMax = 8.0f;     // a column's reference maximum may be exceeded by 2^8 before it moves
+constexpr float kNothing = -1e30f;   // a column's maximum before it sees a key (finite: differences stay defined)
 
 template <int HD, int TERMS>
 struct AttnCfg {
     static constexpr int NG = HD / 64;                       // 64-element groups of a row
-    static constexpr uint32_t RB = kv4_row_bytes(HD), TILE = 16 * RB;
+    static constexpr uint32_t RB = kv4_row_bytes(HD), SIDE = kUnit * RB, STAGE = 2 * SIDE;  // K rows, then V rows
     static constexpr int NW = (HD == 256 || TERMS == 2) ? 8 : 16;  // 128 or 255 registers a thread
-    static constexpr int GROUPS = NW / 4;                    // groups of a CTA, at most
     static constexpr uint32_t SLOT = 8 * HD;                 // floats of a warp's sums
-    static constexpr uint32_t FIT = (212u * 1024u - NW * SLOT * 4u) / (NW * 2u * TILE);
-    static constexpr uint32_t STAGES = FIT > 8 ? 8 : FIT;
-    static constexpr uint32_t SMEM = NW * (STAGES * 2u * TILE + SLOT * 4u);
+    static constexpr uint32_t FIT = (212u * 1024u - NW * SLOT * 4u) / (NW * STAGE);
+    static constexpr uint32_t STAGES = FIT > 4 ? 4 : FIT;
+    static constexpr uint32_t SMEM = NW * (STAGES * STAGE + SLOT * 4u);
+    static_assert(STAGES >= 2, "a warp copies one stage while it works on another");
 };
 
 constexpr int kMaxGroups = 4;                        // of a CTA
 constexpr uint32_t kPieceFloats = 8 * 256 + 16;      // sums, maxima and sums of probabilities of 8 columns
 
-struct AttnShared {
-    uint64_t bar[16][8];
-    uint32_t tile_ok[16][8];
-    float m[16][8], l[16][8];
-    uint64_t warp_units[16];
-    uint32_t warp_items[16];
-    uint64_t total, start_unit[kMaxGroups];
-    uint32_t items, start_seq[kMaxGroups], last[kMaxGroups];
-};
-
-// Walks a warp's tiles in order: every `step`-th unit from a first one on.
-struct TileWalk {
-    uint32_t seq;     // current sequence (n: past the end)
-    uint32_t item, tile;
-    uint64_t unit;    // units from the first one on
+// What a warp copies next; lane 0's.
+struct CopyWalk {
     SeqWork w;
-    int32_t pos_min, pos_max;  // positions of the block's columns
+    Seen seen;
+    uint32_t seq, item, tile, head;
+    uint64_t unit;
 
-    __device__ __forceinline__ void enter_item(const AttnParams& p) {
-        const uint32_t c0 = (item % w.blocks) * 8, c1 = min(c0 + 8, (uint32_t)w.count * p.group) - 1;
-        pos_min = w.len - w.count + (int32_t)(c0 / p.group);
-        pos_max = w.len - w.count + (int32_t)(c1 / p.group);
-    }
-    __device__ __forceinline__ void enter_seq(const AttnParams& p) {
-        for (; seq < p.n; ++seq) {
-            w = seq_work(p, seq, false);
-            if (w.blocks) break;
-        }
-    }
-    // Some column of the block sees some key of the tile.
-    __device__ __forceinline__ bool live(const AttnParams& p) const {
-        const int32_t k0 = w.key0(tile);
-        return k0 <= pos_max && (!p.window || k0 + 15 > pos_min - (int64_t)p.window || (uint32_t)k0 < p.sinks);
-    }
-    __device__ __forceinline__ void advance(const AttnParams& p, uint32_t by) {
-        unit += by;
-        tile += by;
-        if (tile < w.tiles) return;
-        do {
-            tile -= w.tiles;
-            if (++item == w.blocks * p.map.kv_heads) {
-                item = 0;
-                ++seq;
-                enter_seq(p);
-                if (seq >= p.n) return;
-            }
-        } while (tile >= w.tiles);
-        enter_item(p);
-    }
-    __device__ __forceinline__ void begin(const AttnParams& p, uint32_t s, uint64_t seq_unit, uint64_t u) {
+    __device__ void begin(const AttnParams& p, uint32_t s, uint64_t seq_unit, uint64_t u) {
         seq = s;
         w = seq_work(p, s, false);
         item = (uint32_t)((u - seq_unit) / w.tiles);
         tile = (uint32_t)((u - seq_unit) % w.tiles);
         unit = u;
-        enter_item(p);
+        head = item / w.blocks;
+        seen.set(p, w, item % w.blocks);
     }
+    // Steps past the current item's last unit.
+    __device__ __noinline__ void next_item(const AttnParams& p) {
+        do {
+            tile -= w.tiles;
+            if (++item == w.blocks * p.map.kv_heads) {
+                item = 0;
+                for (++seq;; ++seq) {
+                    if (seq >= p.n) return;  // past the last unit
+                    w = seq_work(p, seq, false);
+                    if (w.blocks) break;
+                }
+            }
+        } while (tile >= w.tiles);
+        head = item / w.blocks;
+        seen.set(p, w, item % w.blocks);
+    }
+    __device__ __forceinline__ void advance(const AttnParams& p, uint32_t by) {
+        unit += by;
+        tile += by;
+        if (tile >= w.tiles) next_item(p);
+    }
+};
+
+struct AttnShared {
+    uint64_t bar[16][4];
+    uint32_t halves[16][4];  // which 16-key halves of a stage hold keys
+    float m[16][8], l[16][8];
+    uint64_t warp_units[16];
+    uint32_t warp_items[16];
+    uint64_t start_unit[kMaxGroups];
+    uint32_t start_seq[kMaxGroups], last[kMaxGroups];
+    CopyWalk walk[16];
 };
 
 __device__ __forceinline__ void group_sync(uint32_t group, uint32_t threads) {
@@ -100,14 +92,14 @@ __device__ __forceinline__ void group_sync(uint32_t group, uint32_t threads) {
 }
 
 template <typename T, int HD, int TERMS>
-__global__ void __launch_bounds__(AttnCfg<HD, TERMS>::NW * 32, 1) kv4_attn_kernel(AttnParams p) {
+__global__ void __launch_bounds__(AttnCfg<HD, TERMS>::NW * 32, 1) kv4_attn_kernel(const __grid_constant__ AttnParams p) {
     using C = AttnCfg<HD, TERMS>;
     constexpr int NG = C::NG, NW = C::NW, S = C::STAGES;
     extern __shared__ __align__(128) uint8_t dyn[];
     __shared__ AttnShared sh;
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    uint8_t* ring = dyn + warp * (S * 2u * C::TILE);
-    float* slots = reinterpret_cast<float*>(dyn + NW * (S * 2u * C::TILE));
+    uint8_t* ring = dyn + warp * (S * C::STAGE);
+    float* slots = reinterpret_cast<float*>(dyn + NW * (S * C::STAGE));
 
     // ---- how much work there is, and where this CTA's groups begin
     if (lane == 0) {
@@ -139,7 +131,7 @@ __global__ void __launch_bounds__(AttnCfg<HD, TERMS>::NW * 32, 1) kv4_attn_kerne
     if (total == 0) return;
     const uint32_t WG = total >= (uint64_t)items * NW ? NW : 4;  // warps of a group
     const uint32_t per_cta = NW / WG, group = warp / WG, gw = warp % WG;
-    const uint64_t all = (uint64_t)gridDim.x * per_cta, want = total / (WG / 2 ? WG / 2 : 1);
+    const uint64_t all = (uint64_t)gridDim.x * per_cta, want = total / (WG / 2);
     const uint64_t ranges = want < 1 ? 1 : want < all ? want : all;
     const uint64_t range = (uint64_t)group * gridDim.x + blockIdx.x;  // this group's
     const uint64_t u0 = range < ranges ? total * range / ranges : 0, u1 = range < ranges ? total * (range + 1) / ranges : 0;
@@ -180,59 +172,75 @@ __global__ void __launch_bounds__(AttnCfg<HD, TERMS>::NW * 32, 1) kv4_attn_kerne
     }
     if (u0 >= u1) return;
 
-    // ---- the ring of this warp
-    TileWalk next;  // the next tile to copy
-    next.begin(p, sh.start_seq[group], sh.start_unit[group], u0);
-    if (gw) next.advance(p, gw);
-    uint32_t put = 0, put_phase = 0, got = 0, got_phase = 0, in_flight = 0;
-    bool dead = false;  // a wait gave up
-    auto skip_dead = [&] {
-        while (next.unit < u1 && !next.live(p)) next.advance(p, WG);
-    };
-    int64_t next_row = -1;
-    auto look = [&] {  // the row of the next tile; its page is on its way while other tiles are worked on
-        skip_dead();
-        if (next.unit < u1) next_row = p.map.row(next.w.slot, next.item / next.w.blocks, next.w.key0(next.tile));
-    };
-    auto issue = [&] {
-        if (next.unit >= u1) return;
+    // ---- the ring of this warp: lane 0 walks ahead and copies
+    CopyWalk& next = sh.walk[warp];
+    uint32_t put = 0, got = 0, got_phase = 0, ahead = 0;  // stages: next to fill, next to read, filled and not read
+    bool dead = false;                                     // a wait gave up
+    auto issue = [&] {  // copies the next unit that some column sees, if there is one
         if (lane == 0) {
-            uint64_t* bar = &sh.bar[warp][put];
-            if (next_row >= 0) {
-                uint8_t* dst = ring + put * 2u * C::TILE;
-                mbar_expect_tx(bar, 2u * C::TILE);
-                bulk_g2s(dst, p.map.k + (size_t)next_row * C::RB, C::TILE, bar);
-                bulk_g2s(dst + C::TILE, p.map.v + (size_t)next_row * C::RB, C::TILE, bar);
-            } else {
-                p.map.flag(BT_KV4_RANGE);
-                mbar_arrive(bar);
+            while (next.unit < u1 && !next.seen.any(next.w.key0(next.tile), kUnit, p.sinks)) next.advance(p, WG);
+            if (next.unit < u1) {
+                const int32_t k = next.w.key0(next.tile);
+                uint64_t* bar = &sh.bar[warp][put];
+                uint8_t* dst = ring + put * C::STAGE;
+                // two 16-key halves, each in one page: one copy a side where they lie together
+                const bool two = next.seen.any(k + 16, 16, p.sinks), one = next.seen.any(k, 16, p.sinks);
+                const int64_t row = p.map.row(next.w.slot, next.head, k);
+                uint32_t halves = (one ? 1u : 0u) | (two ? 2u : 0u);
+                if (halves == 3 && row >= 0 && p.map.shift > 4) {
+                    mbar_expect_tx(bar, C::STAGE);
+                    const size_t at = (size_t)row * C::RB;
+                    bulk_g2s(dst, p.map.k + at, C::SIDE, bar);
+                    bulk_g2s(dst + C::SIDE, p.map.v + at, C::SIDE, bar);
+                } else {
+                    const int64_t row2 = p.map.row(next.w.slot, next.head, k + 16);
+                    if ((one && row < 0) || (two && row2 < 0)) p.map.flag(BT_KV4_RANGE);
+                    halves &= (row >= 0 ? 1u : 0u) | (row2 >= 0 ? 2u : 0u);
+                    mbar_expect_tx(bar, C::STAGE / 2 * (halves == 3 ? 2 : halves ? 1 : 0));
+#pragma unroll 1
+                    for (int i = 0; i < 2; ++i) {
+                        if (!(halves >> i & 1)) continue;
+                        const size_t at = (size_t)(i ? row2 : row) * C::RB;
+                        bulk_g2s(dst + i * C::SIDE / 2, p.map.k + at, C::SIDE / 2, bar);
+                        bulk_g2s(dst + C::SIDE + i * C::SIDE / 2, p.map.v + at, C::SIDE / 2, bar);
+                    }
+                }
+                sh.halves[warp][put] = halves;
+                put = put + 1 == S ? 0 : put + 1;
+                ++ahead;
+                next.advance(p, WG);
             }
-            sh.tile_ok[warp][put] = next_row >= 0;
         }
-        if (++put == S) { put = 0; put_phase ^= 1; }
-        ++in_flight;
-        next.advance(p, WG);
-        look();
     };
-    look();
+    if (lane == 0) {
+        next.begin(p, sh.start_seq[group], sh.start_unit[group], u0);
+        if (gw) next.advance(p, gw);
+    }
+    __syncwarp();
+#pragma unroll 1
     for (int i = 0; i < S; ++i) issue();
     __syncwarp();
 
     // ---- items
-    TileWalk cur;
-    cur.begin(p, sh.start_seq[group], sh.start_unit[group], u0);
-    while (cur.unit < u1) {
-        const SeqWork& w = cur.w;
-        const uint32_t left = w.tiles - cur.tile, seg = (uint32_t)(u1 - cur.unit < left ? u1 - cur.unit : left);
-        const uint32_t kvh = cur.item / w.blocks, c0 = (cur.item % w.blocks) * 8, columns = (uint32_t)w.count * p.group;
+    uint32_t seq = sh.start_seq[group], item, tile0;
+    uint64_t unit = u0;
+    SeqWork w = seq_work(p, seq, false);
+    item = (uint32_t)((u0 - sh.start_unit[group]) / w.tiles);
+    tile0 = (uint32_t)((u0 - sh.start_unit[group]) % w.tiles);
+    while (unit < u1) {
+        const uint32_t left = w.tiles - tile0, seg = (uint32_t)(u1 - unit < left ? u1 - unit : left);
+        const uint32_t kvh = item / w.blocks, c0 = (item % w.blocks) * 8, columns = (uint32_t)w.count * p.group;
         const bool whole = seg == w.tiles;
-        const uint32_t offset = (gw + WG - (uint32_t)((cur.unit - u0) % WG)) % WG;  // this warp's first tile of the segment
+        const uint32_t first_warp = (uint32_t)(unit - u0) & (WG - 1);     // has the segment's first unit
+        const uint32_t offset = (gw - first_warp) & (WG - 1);             // this warp's first unit of the segment
         const bool active = offset < seg;
+        Seen seen;
+        seen.set(p, w, item % w.blocks);
 
         // q of column g as B fragments, scaled so that its largest element is in [2^13, 2^14)
         uint32_t qf[NG * 4][2], ql[TERMS == 2 ? NG * 4 : 1][2];
         float qsum[NG][2], factor[2];
-        int32_t pos[2];
+        int32_t pos[2], above[2];
         if (active) {
             const uint32_t c = c0 + g, row = (uint32_t)w.first + c / p.group;
             const bool there = c < columns;
@@ -290,40 +298,45 @@ __global__ void __launch_bounds__(AttnCfg<HD, TERMS>::NW * 32, 1) kv4_attn_kerne
             for (int h = 0; h < 2; ++h) {
                 const uint32_t col = min(c0 + 2 * t + h, columns - 1);
                 pos[h] = w.len - w.count + (int32_t)(col / p.group);
+                above[h] = p.window && pos[h] >= 0 && (uint32_t)pos[h] >= p.window ? pos[h] - (int32_t)p.window : -1;
             }
         }
 
-        float o[NG * 4][4] = {}, mo[NG][2] = {}, m[2] = {-INFINITY, -INFINITY}, l[2] = {};
+        float o[NG * 4][4] = {}, mo[NG][2] = {}, m[2] = {kNothing, kNothing}, l[2] = {};
         uint32_t v_bound = 0;       // no V scale so far is larger (as fp16 bits)
         int v_exp = 0;              // p s is multiplied by 2^v_exp
         float v_mul = 1.0f;
 
-        auto tile = [&](auto masked_c, int32_t key0, const uint8_t* kt) {
-            constexpr bool MASKED = decltype(masked_c)::value;
-            const uint8_t* vt = kt + C::TILE;
-            const uint32_t r0 = key_of(g), r1 = r0 + 2;  // MMA rows g and g + 8
-            bool vis[4] = {true, true, true, true};
-            uint32_t ok0 = 0xffffffffu, ok1 = 0xffffffffu;
-            if (MASKED) {
-                const int32_t k0 = key0 + (int32_t)r0, k1 = k0 + 2;
-                auto sees = [&](int32_t at, int32_t key) {
-                    return key <= at && (!p.window || key > at - (int64_t)p.window || (uint32_t)key < p.sinks);
-                };
-                vis[0] = sees(pos[0], k0); vis[1] = sees(pos[1], k0); vis[2] = sees(pos[0], k1); vis[3] = sees(pos[1], k1);
-                // keys that no column of the block sees may hold anything
-                auto held = [&](int32_t key) {
-                    return key <= cur.pos_max && (!p.window || key > cur.pos_min - (int64_t)p.window || (uint32_t)key < p.sinks);
-                };
-                ok0 = held(k0) ? 0xffffffffu : 0u;
-                ok1 = held(k1) ? 0xffffffffu : 0u;
+        const uint32_t r0 = key_of(g), r1 = r0 + 2;                          // keys of MMA rows g and g + 8
+        const uint32_t ra = key_of(2 * t), rb = key_of(2 * t + 1);           // and of rows 2t, 2t + 1 (+ 8: + 2)
+        const uint32_t k_at = r0 * C::RB + 8 * t, e_at = r0 * C::RB + HD / 2;
+        const uint32_t va_at = C::SIDE + ra * C::RB + 4 * g, vb_at = C::SIDE + rb * C::RB + 4 * g;
+
+        // 16 keys at kt (K; V a side further)
+        auto tile_of = [&](int32_t key0, uint8_t* kt) {
+            const bool masked = !seen.all(key0, 16, p.sinks);
+            if (masked) {
+                // keys that no column sees may hold anything: their pairs become zero
+                if (lane < 16) {
+                    const int32_t key = key0 + (int32_t)lane;
+                    if (key > seen.top || (key <= seen.above && (uint32_t)key >= p.sinks)) {
+#pragma unroll
+                        for (int j = 0; j < NG; ++j) {
+                            reinterpret_cast<uint32_t*>(kt + lane * C::RB + HD / 2)[j] = 0;
+                            reinterpret_cast<uint32_t*>(kt + C::SIDE + lane * C::RB + HD / 2)[j] = 0;
+                        }
+                        fence_proxy_async();  // before the next copy into the stage
+                    }
+                }
+                __syncwarp();
             }
-            // scores
+            // scores of keys r0 (columns 2t, 2t + 1) and r1
             float s[4] = {};
 #pragma unroll
             for (int j = 0; j < NG; ++j) {
                 uint32_t a[2], b[2];  // the lane's 16 codes of rows g and g + 8
-                const uint8_t *pa = kt + r0 * C::RB + 32 * j + 8 * t, *pb = kt + r1 * C::RB + 32 * j + 8 * t;
-                if (HD == 64) {  // rows of 36 bytes
+                const uint8_t *pa = kt + k_at + 32 * j, *pb = pa + 2 * C::RB;
+                if (HD == 64) {       // rows of 36 bytes
                     a[0] = reinterpret_cast<const uint32_t*>(pa)[0]; a[1] = reinterpret_cast<const uint32_t*>(pa)[1];
                     b[0] = reinterpret_cast<const uint32_t*>(pb)[0]; b[1] = reinterpret_cast<const uint32_t*>(pb)[1];
                 } else {
@@ -344,24 +357,32 @@ __global__ void __launch_bounds__(AttnCfg<HD, TERMS>::NW * 32, 1) kv4_attn_kerne
                         mma_f16(c, f1[0], f1[1], f1[2], f1[3], ql[k + 1][0], ql[k + 1][1]);
                     }
                 }
-                const float2 e0 = unpack_half2(reinterpret_cast<const uint32_t*>(kt + r0 * C::RB + HD / 2)[j] & ok0);
-                const float2 e1 = unpack_half2(reinterpret_cast<const uint32_t*>(kt + r1 * C::RB + HD / 2)[j] & ok1);
+                const float2 e0 = unpack_half2(*reinterpret_cast<const uint32_t*>(kt + e_at + 4 * j));
+                const float2 e1 = unpack_half2(*reinterpret_cast<const uint32_t*>(kt + e_at + 2 * C::RB + 4 * j));
                 s[0] = fmaf(e0.x, c[0], fmaf(e0.y, qsum[j][0], s[0]));
                 s[1] = fmaf(e0.x, c[1], fmaf(e0.y, qsum[j][1], s[1]));
                 s[2] = fmaf(e1.x, c[2], fmaf(e1.y, qsum[j][0], s[2]));
                 s[3] = fmaf(e1.x, c[3], fmaf(e1.y, qsum[j][1], s[3]));
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[i] = vis[i] ? s[i] * factor[i & 1] : -INFINITY;
+            for (int i = 0; i < 4; ++i) s[i] *= factor[i & 1];
+            if (masked) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int32_t key = key0 + (int32_t)(i < 2 ? r0 : r1);
+                    if (key > pos[i & 1] || (key <= above[i & 1] && (uint32_t)key >= p.sinks)) s[i] = -INFINITY;
+                }
+            }
 
             // the pairs of V, and whether a maximum or the largest V scale moves
-            uint32_t e0[NG], e1[NG], big = 0;
+            uint32_t ev[2][NG], big2 = 0;
 #pragma unroll
             for (int j = 0; j < NG; ++j) {
-                e0[j] = reinterpret_cast<const uint32_t*>(vt + r0 * C::RB + HD / 2)[j] & ok0;
-                e1[j] = reinterpret_cast<const uint32_t*>(vt + r1 * C::RB + HD / 2)[j] & ok1;
-                big = max(big, max(e0[j] & 0xffffu, e1[j] & 0xffffu));
+                ev[0][j] = *reinterpret_cast<const uint32_t*>(kt + C::SIDE + e_at + 4 * j);
+                ev[1][j] = *reinterpret_cast<const uint32_t*>(kt + C::SIDE + e_at + 2 * C::RB + 4 * j);
+                big2 = __vmaxu2(big2, __vmaxu2(ev[0][j], ev[1][j]));
             }
+            uint32_t big = big2 & 0xffffu;
             const float top0 = fmaxf(s[0], s[2]), top1 = fmaxf(s[1], s[3]);
             if (__any_sync(0xffffffffu, top0 > m[0] + kLazyMax || top1 > m[1] + kLazyMax || big > v_bound)) {
                 float a = top0, b = top1;
@@ -372,7 +393,7 @@ __global__ void __launch_bounds__(AttnCfg<HD, TERMS>::NW * 32, 1) kv4_attn_kerne
                 }
                 a = fmaxf(a, m[0]);
                 b = fmaxf(b, m[1]);
-                const float fa = a == m[0] ? 1.0f : exp2_fast(m[0] - a), fb = b == m[1] ? 1.0f : exp2_fast(m[1] - b);
+                const float fa = exp2_fast(m[0] - a), fb = exp2_fast(m[1] - b);
                 m[0] = a;
                 m[1] = b;
                 big = __reduce_max_sync(0xffffffffu, big);
@@ -389,39 +410,32 @@ __global__ void __launch_bounds__(AttnCfg<HD, TERMS>::NW * 32, 1) kv4_attn_kerne
                 l[1] *= fb;
 #pragma unroll
                 for (int j = 0; j < NG; ++j) { mo[j][0] *= fa; mo[j][1] *= fb; }
+                const float ga = fa * fv, gb = fb * fv;
 #pragma unroll
-                for (int i = 0; i < NG * 4; ++i) {
-                    o[i][0] *= fa * fv; o[i][1] *= fb * fv; o[i][2] *= fa * fv; o[i][3] *= fb * fv;
-                }
+                for (int i = 0; i < NG * 4; ++i) { o[i][0] *= ga; o[i][1] *= gb; o[i][2] *= ga; o[i][3] *= gb; }
             }
-            float pr[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                pr[i] = exp2_fast(s[i] - m[i & 1]);
-                if (MASKED && !vis[i]) pr[i] = 0.0f;
-            }
-            l[0] += pr[0] + pr[2];
-            l[1] += pr[1] + pr[3];
+            for (int i = 0; i < 4; ++i) s[i] = exp2_fast(s[i] - m[i & 1]);
+            l[0] += s[0] + s[2];
+            l[1] += s[1] + s[3];
 
-            // values: rows 2t, 2t + 1, 2t + 8, 2t + 9 of the tile are this lane's keys of V
-            const uint32_t ra = key_of(2 * t), rb = key_of(2 * t + 1);
+            // values
 #pragma unroll
             for (int j = 0; j < NG; ++j) {
-                const float2 x0 = unpack_half2(e0[j]), x1 = unpack_half2(e1[j]);
-                mo[j][0] = fmaf(pr[0], x0.y, fmaf(pr[2], x1.y, mo[j][0]));
-                mo[j][1] = fmaf(pr[1], x0.y, fmaf(pr[3], x1.y, mo[j][1]));
+                const float2 x0 = unpack_half2(ev[0][j]), x1 = unpack_half2(ev[1][j]);
+                mo[j][0] = fmaf(s[0], x0.y, fmaf(s[2], x1.y, mo[j][0]));
+                mo[j][1] = fmaf(s[1], x0.y, fmaf(s[3], x1.y, mo[j][1]));
                 const float s0 = x0.x * v_mul, s1 = x1.x * v_mul;
-                const uint32_t h0 = pack_half2(pr[0] * s0, pr[1] * s0), h1 = pack_half2(pr[2] * s1, pr[3] * s1);
+                const uint32_t h0 = pack_half2(s[0] * s0, s[1] * s0), h1 = pack_half2(s[2] * s1, s[3] * s1);
                 const uint32_t b0 = transpose8(h0), b1 = transpose8(h1);
                 uint32_t b2 = 0, b3 = 0;
                 if (TERMS == 2) {
                     const float2 y0 = unpack_half2(h0), y1 = unpack_half2(h1);
-                    b2 = transpose8(pack_half2(fmaf(pr[0], s0, -y0.x), fmaf(pr[1], s0, -y0.y)));
-                    b3 = transpose8(pack_half2(fmaf(pr[2], s1, -y1.x), fmaf(pr[3], s1, -y1.y)));
+                    b2 = transpose8(pack_half2(fmaf(s[0], s0, -y0.x), fmaf(s[1], s0, -y0.y)));
+                    b3 = transpose8(pack_half2(fmaf(s[2], s1, -y1.x), fmaf(s[3], s1, -y1.y)));
                 }
-                const uint8_t* q0 = vt + 32 * j + 4 * g;
-                const uint32_t va = *reinterpret_cast<const uint32_t*>(q0 + ra * C::RB), vb = *reinterpret_cast<const uint32_t*>(q0 + rb * C::RB);
-                const uint32_t vc = *reinterpret_cast<const uint32_t*>(q0 + (ra + 2) * C::RB), vd = *reinterpret_cast<const uint32_t*>(q0 + (rb + 2) * C::RB);
+                const uint32_t va = *reinterpret_cast<const uint32_t*>(kt + va_at + 32 * j), vb = *reinterpret_cast<const uint32_t*>(kt + vb_at + 32 * j);
+                const uint32_t vc = *reinterpret_cast<const uint32_t*>(kt + va_at + 32 * j + 2 * C::RB), vd = *reinterpret_cast<const uint32_t*>(kt + vb_at + 32 * j + 2 * C::RB);
                 uint32_t f[4] = {__byte_perm(va, vb, 0x5410), __byte_perm(va, vb, 0x7632), __byte_perm(vc, vd, 0x5410), __byte_perm(vc, vd, 0x7632)};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {  // dims 8g + i (rows g) and 8g + i + 4 (rows g + 8) of the group
@@ -436,26 +450,31 @@ __global__ void __launch_bounds__(AttnCfg<HD, TERMS>::NW * 32, 1) kv4_attn_kerne
             }
         };
 
+#pragma unroll 1
         for (uint32_t x = offset; x < seg; x += WG) {
-            const int32_t key0 = w.key0(cur.tile + x);
-            if (!(key0 <= cur.pos_max && (!p.window || key0 + 15 > cur.pos_min - (int64_t)p.window || (uint32_t)key0 < p.sinks))) continue;
-            if (!dead && !mbar_wait(&sh.bar[warp][got], got_phase, nullptr)) {
-                dead = true;
-                if (lane == 0) p.map.flag(BT_KV4_TIMEOUT);
+            const int32_t key0 = w.key0(tile0 + x);
+            if (!seen.any(key0, kUnit, p.sinks)) continue;
+            if (!dead) {
+                const bool in_time = mbar_wait(&sh.bar[warp][got], got_phase, nullptr);
+                if (!__all_sync(0xffffffffu, in_time)) {
+                    dead = true;
+                    if (lane == 0) p.map.flag(BT_KV4_TIMEOUT);
+                }
             }
-            dead = __any_sync(0xffffffffu, dead);
-            const uint8_t* kt = ring + got * 2u * C::TILE;
-            if (!dead && sh.tile_ok[warp][got]) {
-                const bool all_seen = key0 + 15 <= cur.pos_min &&
-                                      (!p.window || key0 > cur.pos_max - (int64_t)p.window || (uint32_t)key0 + 15 < p.sinks);
-                if (all_seen) tile(std::false_type(), key0, kt);
-                else tile(std::true_type(), key0, kt);
+            if (!dead) {
+                uint8_t* kt = ring + got * C::STAGE;
+                const uint32_t halves = sh.halves[warp][got];
+#pragma unroll 1
+                for (int u = 0; u < 2; ++u) {
+                    if (halves >> u & 1) tile_of(key0 + 16 * u, kt + u * (C::SIDE / 2));
+                }
+                __syncwarp();  // every lane is done with the stage
+                got_phase ^= got + 1 == S ? 1u : 0u;
+                got = got + 1 == S ? 0 : got + 1;
+                --ahead;
+                issue();
+                __syncwarp();
             }
-            __syncwarp();  // every lane is done with the stage
-            if (++got == S) { got = 0; got_phase ^= 1; }
-            --in_flight;
-            if (!dead) issue();
-            __syncwarp();
         }
 
         // ---- add up the warps' sums
@@ -475,17 +494,16 @@ __global__ void __launch_bounds__(AttnCfg<HD, TERMS>::NW * 32, 1) kv4_attn_kerne
                 sh.m[warp][2 * t] = m[0]; sh.m[warp][2 * t + 1] = m[1];
             }
         } else if (g == 0) {
-            sh.m[warp][2 * t] = sh.m[warp][2 * t + 1] = -INFINITY;
+            sh.m[warp][2 * t] = sh.m[warp][2 * t + 1] = kNothing;
         }
         group_sync(group, WG * 32);
         if (active) {
             float f[2], k0[2], k1[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                float top = -INFINITY;
+                float top = kNothing;
                 for (uint32_t i = 0; i < WG; ++i) top = fmaxf(top, sh.m[group * WG + i][2 * t + h]);
-                f[h] = m[h] == -INFINITY ? 0.0f : exp2_fast(m[h] - top);
-                if (!(l[h] == l[h])) f[h] = NAN;  // a column with NaN scores has no maximum
+                f[h] = l[h] == l[h] ? exp2_fast(m[h] - top) : NAN;  // a column with NaN scores stays NaN
                 k0[h] = f[h] * __int_as_float((127 + 24 - v_exp) << 23);  // codes at weight 2^-24
                 k1[h] = k0[h] * 0.0625f;                                   // and at 2^-20
                 if (g == 0) sh.l[warp][2 * t + h] = l[h] * f[h];
@@ -506,19 +524,19 @@ __global__ void __launch_bounds__(AttnCfg<HD, TERMS>::NW * 32, 1) kv4_attn_kerne
         group_sync(group, WG * 32);
 
         const uint32_t gt = gw * 32 + lane, threads = WG * 32;
-        // the warps that had tiles, in order of their first tile
-        const uint32_t used = min(seg, WG), first_warp = (uint32_t)((cur.unit - u0) % WG);
+        // the warps that had units, in order of their first one
+        const uint32_t used = min(seg, WG);
         auto sum4 = [&](uint32_t i) {  // floats 4 i .. 4 i + 3 of the item's sums
             float4 a = make_float4(0, 0, 0, 0);
             for (uint32_t k = 0; k < used; ++k) {
-                const float4 b = reinterpret_cast<const float4*>(slots + (group * WG + (first_warp + k) % WG) * C::SLOT)[i];
+                const float4 b = reinterpret_cast<const float4*>(slots + (group * WG + ((first_warp + k) & (WG - 1))) * C::SLOT)[i];
                 a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
             }
             return a;
         };
         auto sum_l = [&](uint32_t c) {
             float a = 0.0f;
-            for (uint32_t k = 0; k < used; ++k) a += sh.l[group * WG + (first_warp + k) % WG][c];
+            for (uint32_t k = 0; k < used; ++k) a += sh.l[group * WG + ((first_warp + k) & (WG - 1))][c];
             return a;
         };
         auto store4 = [&](uint32_t c, uint32_t d, float4 v, float sum) {  // column c of the block
@@ -542,16 +560,16 @@ __global__ void __launch_bounds__(AttnCfg<HD, TERMS>::NW * 32, 1) kv4_attn_kerne
             for (uint32_t i = gt; i < C::SLOT / 4; i += threads) store4(i / (HD / 4), i % (HD / 4) * 4, sum4(i), sum_l(i / (HD / 4)));
         } else {
             // this group's piece: slot 0 of its range if the item began before it, else slot 1
-            float* mine = p.partial + (range * 2 + (cur.tile ? 0 : 1)) * kPieceFloats;
+            float* mine = p.partial + (range * 2 + (tile0 ? 0 : 1)) * kPieceFloats;
             for (uint32_t i = gt; i < C::SLOT / 4; i += threads) __stcg(reinterpret_cast<float4*>(mine + 16) + i, sum4(i));
             if (gt < 8) {
-                float top = -INFINITY;
+                float top = kNothing;
                 for (uint32_t i = 0; i < WG; ++i) top = fmaxf(top, sh.m[group * WG + i][gt]);
                 __stcg(mine + gt, top);
                 __stcg(mine + 8 + gt, sum_l(gt));
             }
             // the item's units and the ranges that share it
-            const uint64_t i0 = cur.unit - cur.tile, i1 = i0 + w.tiles - 1;
+            const uint64_t i0 = unit - tile0, i1 = i0 + w.tiles - 1;
             const uint64_t ra = ((i0 + 1) * ranges - 1) / total, rb = ((i1 + 1) * ranges - 1) / total;
             __threadfence();
             group_sync(group, threads);
@@ -563,17 +581,27 @@ __global__ void __launch_bounds__(AttnCfg<HD, TERMS>::NW * 32, 1) kv4_attn_kerne
             }
             group_sync(group, threads);
             if (sh.last[group]) {
+                const uint32_t pieces = (uint32_t)(rb - ra) + 1;
+                const float* base = p.partial + ra * 2 * kPieceFloats;  // the first piece is its range's slot 1
+                auto piece = [&](uint32_t r) { return base + (size_t)(2 * r + (r == 0 ? 1 : 0)) * kPieceFloats; };
+                // the columns' maxima over the pieces
+                float top = kNothing;
+                for (uint32_t r = gt / 8; r < pieces; r += threads / 8) top = fmaxf(top, __ldcg(piece(r) + gt % 8));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                if (lane < 8) sh.m[warp][lane] = top;
+                group_sync(group, threads);
                 for (uint32_t i = gt; i < C::SLOT / 4; i += threads) {
                     const uint32_t c = i / (HD / 4);
-                    float top = -INFINITY;
-                    for (uint64_t r = ra; r <= rb; ++r) top = fmaxf(top, __ldcg(p.partial + (r * 2 + (r == ra ? 1 : 0)) * kPieceFloats + c));
+                    top = kNothing;
+                    for (uint32_t k = 0; k < WG; ++k) top = fmaxf(top, sh.m[group * WG + k][c]);
                     float4 a = make_float4(0, 0, 0, 0);
                     float sum = 0.0f;
-                    for (uint64_t r = ra; r <= rb; ++r) {
-                        const float* piece = p.partial + (r * 2 + (r == ra ? 1 : 0)) * kPieceFloats;
-                        const float pm = __ldcg(piece + c), pl = __ldcg(piece + 8 + c);
-                        const float f = pl != pl ? NAN : pm == -INFINITY ? 0.0f : exp2_fast(pm - top);
-                        const float4 b = __ldcg(reinterpret_cast<const float4*>(piece + 16) + i);
+#pragma unroll 8
+                    for (uint32_t r = 0; r < pieces; ++r) {
+                        const float pm = __ldcg(piece(r) + c), pl = __ldcg(piece(r) + 8 + c);
+                        const float4 b = __ldcg(reinterpret_cast<const float4*>(piece(r) + 16) + i);
+                        const float f = pl == pl ? exp2_fast(pm - top) : NAN;
                         a.x = fmaf(b.x, f, a.x); a.y = fmaf(b.y, f, a.y); a.z = fmaf(b.z, f, a.z); a.w = fmaf(b.w, f, a.w);
                         sum = fmaf(pl, f, sum);
                     }
@@ -582,12 +610,22 @@ __global__ void __launch_bounds__(AttnCfg<HD, TERMS>::NW * 32, 1) kv4_attn_kerne
             }
         }
         group_sync(group, threads);  // the slots are free again
-        cur.advance(p, seg);
+        unit += seg;
+        tile0 += seg;
+        if (tile0 == w.tiles && unit < u1) {
+            tile0 = 0;
+            if (++item == w.blocks * p.map.kv_heads) {
+                item = 0;
+                do w = seq_work(p, ++seq, false);
+                while (w.blocks == 0);
+            }
+        }
     }
     // after an expired wait copies may still be on their way to this CTA's shared memory
-    for (; dead && in_flight > 0; --in_flight) {
+    for (; dead && ahead > 0; --ahead) {
         mbar_wait(&sh.bar[warp][got], got_phase, nullptr);
-        if (++got == S) { got = 0; got_phase ^= 1; }
+        got_phase ^= got + 1 == S ? 1u : 0u;
+        got = got + 1 == S ? 0 : got + 1;
     }
 }
 

@@ -73,18 +73,22 @@ __device__ __forceinline__ uint32_t key_of(uint32_t r) { return 4 * (r & 3) + (r
 
 // ---------------------------------------------------------------- work
 
+// Keys of a unit of work: two MMA tiles, one stage of a warp's ring.
+constexpr int kUnit = 32;
+
 // One sequence's share of the work: `blocks` blocks of 8 columns per KV head, each
-// over `tiles` 16-key tiles; the first sink_tiles start at key 0, the rest at key lo.
+// over `tiles` units of keys; the first sink_tiles start at key 0, the rest at key lo.
 struct SeqWork {
     int32_t first, count, len, slot;  // rows of q, cached positions
     uint32_t blocks, tiles, sink_tiles;
     int32_t lo;
     __device__ __forceinline__ int32_t key0(uint32_t tile) const {
-        return tile < sink_tiles ? (int32_t)tile * 16 : lo + (int32_t)(tile - sink_tiles) * 16;
+        return (int32_t)tile * kUnit + (tile < sink_tiles ? 0 : lo - (int32_t)sink_tiles * kUnit);
     }
 };
 
-__device__ __forceinline__ SeqWork seq_work(const AttnParams& p, uint32_t i, bool report) {
+// (Not inlined: it is asked for in several places, and the kernel's code has to stay small.)
+static __device__ __noinline__ SeqWork seq_work(const AttnParams& p, uint32_t i, bool report) {
     SeqWork w;
     w.first = (int32_t)i;
     w.count = 1;
@@ -106,12 +110,34 @@ __device__ __forceinline__ SeqWork seq_work(const AttnParams& p, uint32_t i, boo
     const int32_t lowest = w.len - w.count;  // the first query's position
     int32_t lo = 0;
     if (p.window && lowest >= 0 && (uint32_t)lowest >= p.window) lo = lowest - (int32_t)p.window + 1;
-    w.lo = lo & ~15;
-    w.sink_tiles = p.window ? min((min(p.sinks, 0x7ffffff0u) + 15) / 16, (uint32_t)w.lo / 16) : 0;
+    w.lo = lo & ~(kUnit - 1);
+    w.sink_tiles = p.window ? min((min(p.sinks, 0x7fffff00u) + kUnit - 1) / kUnit, (uint32_t)w.lo / kUnit) : 0;
     w.blocks = ((uint32_t)w.count * p.group + 7) / 8;
-    // at least one tile, so that the rows of an empty sequence are written
-    w.tiles = max(1u, w.sink_tiles + (uint32_t)(max(w.len - w.lo, 0) + 15) / 16);
+    // at least one unit, so that the rows of an empty sequence are written
+    w.tiles = max(1u, w.sink_tiles + (uint32_t)(max(w.len - w.lo, 0) + kUnit - 1) / kUnit);
     return w;
 }
+
+// The keys that some column of a block sees: [0, sinks) and (above, top].
+struct Seen {
+    int32_t top, bottom;  // positions of the block's last and first column
+    int32_t above, above_top;  // window starts (exclusive) of the first and of the last column; -1: no window
+    __device__ __forceinline__ void set(const AttnParams& p, const SeqWork& w, uint32_t block) {
+        const uint32_t c0 = block * 8, c1 = min(c0 + 8, (uint32_t)w.count * p.group) - 1;
+        bottom = w.len - w.count + (int32_t)(c0 / p.group);
+        top = w.len - w.count + (int32_t)(c1 / p.group);
+        auto start = [&](int32_t pos) { return p.window && pos >= 0 && (uint32_t)pos >= p.window ? pos - (int32_t)p.window : -1; };
+        above = start(bottom);
+        above_top = start(top);
+    }
+    // some column sees some key of [k, k + n)
+    __device__ __forceinline__ bool any(int32_t k, int32_t n, uint32_t sinks) const {
+        return k <= top && (k + n - 1 > above || (uint32_t)k < sinks);
+    }
+    // every column sees every key of [k, k + n)
+    __device__ __forceinline__ bool all(int32_t k, int32_t n, uint32_t sinks) const {
+        return k + n - 1 <= bottom && (k > above_top || (uint32_t)(k + n) <= sinks);
+    }
+};
 
 }  // namespace bt
