@@ -1,20 +1,24 @@
 // bt_kv4_attn.cu -- causal attention over a 4-bit cache (bt_cuda_kv4_attention).
 // The arithmetic of a tile and its formulas: bt_kv4_attn.cuh.
 //
-// Dealing out the work.  An item is (sequence, KV head, block of 8 columns); its
-// units are 32 keys, and the units of all items in order are cut into equal
-// ranges, one per group of warps, so that ragged lengths need no tuning: a group
-// works on at most two items it shares with others (its first and its last).  Each
-// shared item's pieces go to the workspace, and the group that finds itself last (an
-// atomic ticket) adds them in the order of the keys, so results do not depend on
-// which that was.  The lengths are read on the device: no host copy, and a captured
-// graph may be replayed with other lengths.
+// Dealing out the work.  An item is (sequence, KV head, block of 8 columns); its units
+// are 32 keys.  A range of units goes to a group of warps:
+//   few items (no more than half the SMs): a group is a whole CTA, and every item is cut
+//     into pieces of its own, of about equal length over all items, so that a CTA has
+//     one piece of one item;
+//   many items: a group is 4 warps, and the units of all items in order (kItemCost more
+//     for an item's own cost) are cut into equal ranges, so that a group works on whole
+//     items but for its first and its last.
+// Either way ragged lengths need no tuning, and the lengths are read on the device: no
+// host copy, and a captured graph may be replayed with other lengths.  The pieces of an
+// item go to the workspace; the group that finds itself last (an atomic ticket) adds
+// them in the order of the keys, so results do not depend on which that was.
 //
-// A group is a CTA's 16 (or 8) warps where items are long, 4 warps where they are
-// short (less than a unit for every warp), so that a CTA works on several short
-// items at a time.  A warp takes every 16th (8th, 4th) unit of its group's range
-// and streams them through its own ring of bulk copies, which runs on across the
-// ends of items; warps meet only to add up an item.
+// A warp takes every 16th (8th, 4th) unit of its group's range and streams them
+// through its own ring of bulk copies, which runs on across the ends of items; warps
+// meet only at an item's ends.
+// Code that is not in the key loop is kept small (rolled loops, one copy of each
+// step): a call on short caches spends its time fetching it.
 #include "bt_kv4_attn.cuh"
 
 namespace bt {
@@ -28,7 +32,7 @@ struct AttnCfg {
     static constexpr uint32_t RB = kv4_row_bytes(HD), SIDE = kUnit * RB, STAGE = 2 * SIDE;  // K rows, then V rows
     static constexpr int NW = (HD == 256 || TERMS == 2) ? 8 : 16;  // 128 or 255 registers a thread
     static constexpr uint32_t SLOT = 8 * HD;                 // floats of a warp's sums
-    static constexpr uint32_t FIT = (212u * 1024u - NW * SLOT * 4u) / (NW * STAGE);
+    static constexpr uint32_t FIT = (216u * 1024u - NW * SLOT * 4u) / (NW * STAGE);
     static constexpr uint32_t STAGES = FIT > 4 ? 4 : FIT;
     static constexpr uint32_t SMEM = NW * (STAGES * STAGE + SLOT * 4u);
     static_assert(STAGES >= 2, "a warp copies one stage while it works on another");
@@ -37,42 +41,77 @@ struct AttnCfg {
 constexpr int kMaxGroups = 4;                        // of a CTA
 constexpr uint32_t kPieceFloats = 8 * 256 + 16;      // sums, maxima and sums of probabilities of 8 columns
 
-// What a warp copies next; lane 0's.
-struct CopyWalk {
+constexpr uint32_t kItemCost = 4;
+
+// floor(a / b); 32 bits wide wherever that does (64-bit divisions are long)
+__device__ __forceinline__ uint64_t div64(uint64_t a, uint32_t b) {
+    return a >> 32 ? a / b : (uint64_t)((uint32_t)a / b);
+}
+
+// Walks the items of a range.  [tile, end): the current item's units in the range.
+struct Walk {
     SeqWork w;
     Seen seen;
-    uint32_t seq, item, tile, head;
-    uint64_t unit;
+    uint32_t seq, item, head, tile, end, done;
+    uint64_t at, until;  // where the current item and the range's end lie among all units
+    uint32_t first_range, ranges;  // that share the item
 
-    __device__ void begin(const AttnParams& p, uint32_t s, uint64_t seq_unit, uint64_t u) {
+    __device__ __forceinline__ void enter(const AttnParams& p, uint64_t step) {
+        const uint64_t left = until - at;
+        end = left <= kItemCost ? 0 : left - kItemCost < w.tiles ? (uint32_t)(left - kItemCost) : w.tiles;
+        head = item / w.blocks;
+        seen.set(p, w, item - head * w.blocks);
+        const uint64_t a = at + kItemCost, b = a + w.tiles - 1;
+        first_range = (uint32_t)(step >> 32 ? a / step : div64(a, (uint32_t)step));
+        ranges = (uint32_t)(step >> 32 ? b / step : div64(b, (uint32_t)step)) - first_range + 1;
+    }
+    // The range [from, to) of units cut every `step`, in a sequence whose units start at seq_at.
+    __device__ __forceinline__ void begin(const AttnParams& p, uint32_t s, uint64_t seq_at, uint64_t from, uint64_t to, uint64_t step) {
         seq = s;
         w = seq_work(p, s, false);
-        item = (uint32_t)((u - seq_unit) / w.tiles);
-        tile = (uint32_t)((u - seq_unit) % w.tiles);
-        unit = u;
-        head = item / w.blocks;
-        seen.set(p, w, item % w.blocks);
+        const uint32_t units = w.tiles + kItemCost;
+        item = (uint32_t)div64(from - seq_at, units);
+        at = seq_at + (uint64_t)item * units;
+        const uint32_t in = (uint32_t)(from - at);
+        tile = in < kItemCost ? 0 : in - kItemCost;
+        until = to;
+        done = 0;
+        enter(p, step);
     }
-    // Steps past the current item's last unit.
-    __device__ __noinline__ void next_item(const AttnParams& p) {
-        do {
-            tile -= w.tiles;
-            if (++item == w.blocks * p.map.kv_heads) {
-                item = 0;
-                for (++seq;; ++seq) {
-                    if (seq >= p.n) return;  // past the last unit
-                    w = seq_work(p, seq, false);
-                    if (w.blocks) break;
-                }
-            }
-        } while (tile >= w.tiles);
+    // Piece `range` of the pieces of at most `step` units, in a sequence whose pieces start at seq_at.
+    __device__ __forceinline__ void begin_piece(const AttnParams& p, uint32_t s, uint32_t seq_at, uint32_t range, uint32_t step) {
+        seq = s;
+        w = seq_work(p, s, false);
+        ranges = (w.tiles + step - 1) / step;
+        item = (range - seq_at) / ranges;
+        first_range = seq_at + item * ranges;
+        const uint32_t i = range - first_range;
+        tile = (uint32_t)div64((uint64_t)w.tiles * i, ranges);
+        end = (uint32_t)div64((uint64_t)w.tiles * (i + 1), ranges);
+        at = until = 0;  // no other item follows
+        done = 0;
         head = item / w.blocks;
-        seen.set(p, w, item % w.blocks);
+        seen.set(p, w, item - head * w.blocks);
     }
-    __device__ __forceinline__ void advance(const AttnParams& p, uint32_t by) {
-        unit += by;
+    __device__ __noinline__ void next_item(const AttnParams& p, uint64_t step) {
+        at += w.tiles + kItemCost;
+        tile = end = 0;
+        if (at >= until) { done = 1; return; }
+        if (++item == w.blocks * p.map.kv_heads) {
+            item = 0;
+            do w = seq_work(p, ++seq, false);  // (there is one: units are left)
+            while (w.blocks == 0);
+        }
+        enter(p, step);
+    }
+    // `by` units further, across items; done past the range's last one
+    __device__ __forceinline__ void advance(const AttnParams& p, uint32_t by, uint64_t step) {
         tile += by;
-        if (tile >= w.tiles) next_item(p);
+        while (tile >= end && !done) {
+            const uint32_t over = tile - end;
+            next_item(p, step);
+            tile = over;
+        }
     }
 };
 
@@ -82,9 +121,10 @@ struct AttnShared {
     float m[16][8], l[16][8];
     uint64_t warp_units[16];
     uint32_t warp_items[16];
-    uint64_t start_unit[kMaxGroups];
+    uint64_t start_at[kMaxGroups];
     uint32_t start_seq[kMaxGroups], last[kMaxGroups];
-    CopyWalk walk[16];
+    float qsum[kMaxGroups][8][4], factor[kMaxGroups][8];
+    Walk copy[16], work[16];  // of every warp, lane 0's: what to copy next, what to work on
 };
 
 __device__ __forceinline__ void group_sync(uint32_t group, uint32_t threads) {
@@ -101,85 +141,91 @@ __global__ void __launch_bounds__(AttnCfg<HD, TERMS>::NW * 32, 1) kv4_attn_kerne
     uint8_t* ring = dyn + warp * (S * C::STAGE);
     float* slots = reinterpret_cast<float*>(dyn + NW * (S * C::STAGE));
 
-    // ---- how much work there is, and where this CTA's groups begin
-    if (lane == 0) {
-        for (int i = 0; i < S; ++i) mbar_init(&sh.bar[warp][i], 1);
-        fence_mbar_init();
-    }
-    uint64_t units = 0;
+    // ---- how much work there is
+    if (lane < S) mbar_init(&sh.bar[warp][lane], 1);
+    fence_mbar_init();
+    uint64_t total = 0;
     uint32_t items = 0;
-    uint64_t own = 0;  // of the sequence this thread looked at last
+    SeqWork mine = {};  // the sequence this thread looked at last
     for (uint32_t i = tid; i < p.n; i += NW * 32) {
-        const SeqWork w = seq_work(p, i, blockIdx.x == 0);
-        const uint32_t it = w.blocks * p.map.kv_heads;
-        own = (uint64_t)it * w.tiles;
-        units += own;
+        mine = seq_work(p, i, blockIdx.x == 0);
+        const uint32_t it = mine.blocks * p.map.kv_heads;
+        total += (uint64_t)it * mine.tiles;
         items += it;
     }
-    uint64_t su = units;
-    uint32_t si = items;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-        su += __shfl_xor_sync(0xffffffffu, su, o);
-        si += __shfl_xor_sync(0xffffffffu, si, o);
+        total += __shfl_xor_sync(0xffffffffu, total, o);
+        items += __shfl_xor_sync(0xffffffffu, items, o);
     }
-    if (lane == 0) { sh.warp_units[warp] = su; sh.warp_items[warp] = si; }
+    if (lane == 0) { sh.warp_units[warp] = total; sh.warp_items[warp] = items; }
     __syncthreads();
-    uint64_t total = 0;
-    items = 0;
-    for (int i = 0; i < NW; ++i) { total += sh.warp_units[i]; items += sh.warp_items[i]; }
-    if (total == 0) return;
-    const uint32_t WG = total >= (uint64_t)items * NW ? NW : 4;  // warps of a group
-    const uint32_t per_cta = NW / WG, group = warp / WG, gw = warp % WG;
-    const uint64_t all = (uint64_t)gridDim.x * per_cta, want = total / (WG / 2);
-    const uint64_t ranges = want < 1 ? 1 : want < all ? want : all;
-    const uint64_t range = (uint64_t)group * gridDim.x + blockIdx.x;  // this group's
-    const uint64_t u0 = range < ranges ? total * range / ranges : 0, u1 = range < ranges ? total * (range + 1) / ranges : 0;
-    {
-        // the sequence that holds each group's first unit
-        uint64_t base = 0;
-        for (uint32_t i0 = 0; i0 < p.n; i0 += NW * 32) {
-            const uint32_t i = i0 + tid;
-            if (p.n > NW * 32) {
-                own = 0;
-                if (i < p.n) {
-                    const SeqWork w = seq_work(p, i, false);
-                    own = (uint64_t)w.blocks * p.map.kv_heads * w.tiles;
-                }
-            }
-            uint64_t inc = own;
+    total = sh.warp_units[lane % NW];
+    items = sh.warp_items[lane % NW];
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const uint64_t v = __shfl_up_sync(0xffffffffu, inc, o);
-                if (lane >= (uint32_t)o) inc += v;
-            }
+    for (int o = NW / 2; o > 0; o >>= 1) {
+        total += __shfl_xor_sync(0xffffffffu, total, o);
+        items += __shfl_xor_sync(0xffffffffu, items, o);
+    }
+    if (total == 0) return;
+    const bool few = items <= gridDim.x / 2;
+    const uint32_t WG = few ? NW : 4;  // warps of a group
+    const uint32_t per_cta = NW / WG, group = warp / WG, gw = warp % WG;
+    const uint32_t range = group * gridDim.x + blockIdx.x;  // this group's
+    // units of a range.  Few items: as sum ceil(t / step) <= total / step + items, no more
+    // pieces than CTAs; and half a unit at least for each warp.
+    uint64_t step;
+    if (few) {
+        step = max(div64(total + gridDim.x - items - 1, gridDim.x - items), (uint64_t)(NW / 2));
+    } else {
+        total += (uint64_t)items * kItemCost;
+        step = div64(total + gridDim.x * per_cta - 1, gridDim.x * per_cta);
+    }
+
+    // ---- the sequence that holds each group's range
+    uint64_t base = 0;
+    if (tid < kMaxGroups) sh.start_seq[tid] = 0xffffffffu;
+    __syncthreads();
+    for (uint32_t i0 = 0; i0 < p.n; i0 += NW * 32) {
+        const uint32_t i = i0 + tid;
+        if (p.n > NW * 32) {
+            mine.blocks = 0;
+            if (i < p.n) mine = seq_work(p, i, false);
+        }
+        // its ranges (few items) or units (many)
+        const uint64_t own = (uint64_t)mine.blocks * p.map.kv_heads * (few ? (uint32_t)div64(mine.tiles + step - 1, (uint32_t)step) : mine.tiles + kItemCost);
+        uint64_t inc = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint64_t v = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= (uint32_t)o) inc += v;
+        }
+        uint64_t at = base + inc - own;
+        if (p.n > 32) {  // the warps before this one
             __syncthreads();
             if (lane == 31) sh.warp_units[warp] = inc;
             __syncthreads();
-            uint64_t at = base + inc - own;
             for (int k = 0; k < NW; ++k) {
                 if (k < (int)warp) at += sh.warp_units[k];
                 base += sh.warp_units[k];
             }
-            for (uint32_t k = 0; k < per_cta; ++k) {
-                const uint64_t r = (uint64_t)k * gridDim.x + blockIdx.x;
-                if (r >= ranges) break;
-                const uint64_t u = total * r / ranges;
-                if (u >= at && u < at + own) { sh.start_seq[k] = i; sh.start_unit[k] = at; }
-            }
         }
-        __syncthreads();
+        for (uint32_t k = 0; k < per_cta; ++k) {
+            const uint64_t u = (uint64_t)(k * gridDim.x + blockIdx.x) * (few ? 1 : step);
+            if (u >= at && u < at + own) { sh.start_seq[k] = i; sh.start_at[k] = at; }
+        }
     }
-    if (u0 >= u1) return;
+    __syncthreads();
+    if (sh.start_seq[group] == 0xffffffffu) return;  // nothing left for this group
 
     // ---- the ring of this warp: lane 0 walks ahead and copies
-    CopyWalk& next = sh.walk[warp];
+    Walk& next = sh.copy[warp];
     uint32_t put = 0, got = 0, got_phase = 0, ahead = 0;  // stages: next to fill, next to read, filled and not read
     bool dead = false;                                     // a wait gave up
     auto issue = [&] {  // copies the next unit that some column sees, if there is one
         if (lane == 0) {
-            while (next.unit < u1 && !next.seen.any(next.w.key0(next.tile), kUnit, p.sinks)) next.advance(p, WG);
-            if (next.unit < u1) {
+            while (!next.done && !next.seen.any(next.w.key0(next.tile), kUnit, p.sinks)) next.advance(p, WG, step);
+            if (!next.done) {
                 const int32_t k = next.w.key0(next.tile);
                 uint64_t* bar = &sh.bar[warp][put];
                 uint8_t* dst = ring + put * C::STAGE;
@@ -208,98 +254,101 @@ __global__ void __launch_bounds__(AttnCfg<HD, TERMS>::NW * 32, 1) kv4_attn_kerne
                 sh.halves[warp][put] = halves;
                 put = put + 1 == S ? 0 : put + 1;
                 ++ahead;
-                next.advance(p, WG);
+                next.advance(p, WG, step);
             }
         }
     };
+    Walk& cur = sh.work[warp];
     if (lane == 0) {
-        next.begin(p, sh.start_seq[group], sh.start_unit[group], u0);
-        if (gw) next.advance(p, gw);
+        if (few) next.begin_piece(p, sh.start_seq[group], (uint32_t)sh.start_at[group], range, (uint32_t)step);
+        else next.begin(p, sh.start_seq[group], sh.start_at[group], range * step, min((range + 1) * step, total), step);
+        cur = next;
+        next.advance(p, gw, step);
     }
-    __syncwarp();
 #pragma unroll 1
     for (int i = 0; i < S; ++i) issue();
     __syncwarp();
 
     // ---- items
-    uint32_t seq = sh.start_seq[group], item, tile0;
-    uint64_t unit = u0;
-    SeqWork w = seq_work(p, seq, false);
-    item = (uint32_t)((u0 - sh.start_unit[group]) / w.tiles);
-    tile0 = (uint32_t)((u0 - sh.start_unit[group]) % w.tiles);
-    while (unit < u1) {
-        const uint32_t left = w.tiles - tile0, seg = (uint32_t)(u1 - unit < left ? u1 - unit : left);
-        const uint32_t kvh = item / w.blocks, c0 = (item % w.blocks) * 8, columns = (uint32_t)w.count * p.group;
+    // the queries as fragments, in the group's slots: read before the slots are written
+    uint8_t* qfrag = reinterpret_cast<uint8_t*>(slots + group * WG * C::SLOT);
+    uint32_t before = 0;  // units of the range before the item, modulo WG
+#pragma unroll 1
+    for (;; ) {
+        if (cur.done) break;
+        const SeqWork w = cur.w;
+        const Seen seen = cur.seen;
+        const uint32_t tile0 = cur.tile, seg = cur.end > tile0 ? cur.end - tile0 : 0;
+        const uint32_t kvh = cur.head, c0 = (cur.item - kvh * w.blocks) * 8, columns = (uint32_t)w.count * p.group;
+        const uint32_t pieces = cur.ranges, first_range = cur.first_range;
+        __syncwarp();
+        if (lane == 0) cur.next_item(p, step);
+        __syncwarp();
+        if (seg == 0) continue;  // only the item's own cost lies in the range
         const bool whole = seg == w.tiles;
-        const uint32_t first_warp = (uint32_t)(unit - u0) & (WG - 1);     // has the segment's first unit
-        const uint32_t offset = (gw - first_warp) & (WG - 1);             // this warp's first unit of the segment
+        const uint32_t first_warp = before;                    // has the segment's first unit
+        const uint32_t offset = (gw - first_warp) & (WG - 1);  // this warp's first unit of the segment
         const bool active = offset < seg;
-        Seen seen;
-        seen.set(p, w, item % w.blocks);
+        before = (before + seg) & (WG - 1);
 
-        // q of column g as B fragments, scaled so that its largest element is in [2^13, 2^14)
-        uint32_t qf[NG * 4][2], ql[TERMS == 2 ? NG * 4 : 1][2];
-        float qsum[NG][2], factor[2];
-        int32_t pos[2], above[2];
-        if (active) {
-            const uint32_t c = c0 + g, row = (uint32_t)w.first + c / p.group;
-            const bool there = c < columns;
-            const T* src = (const T*)p.q + (there ? (int64_t)row * p.q_ts + (int64_t)(kvh * p.group + c % p.group) * p.q_hs : 0);
-            float big = 0.0f;
-            float x[NG][16];
+        // ---- the queries as B fragments, scaled so that a column's largest element is in
+        // [2^13, 2^14): a warp takes a column, a lane HD / 32 elements
+#pragma unroll 1
+        for (uint32_t c = gw; c < 8; c += WG) {
+            constexpr int E = HD / 32;
+            const uint32_t col = c0 + c, row = (uint32_t)w.first + col / p.group;
+            float x[E], big = 0.0f, sum = 0.0f;
+            const T* src = (const T*)p.q + (int64_t)row * p.q_ts + (int64_t)(kvh * p.group + col % p.group) * p.q_hs + lane * E;
 #pragma unroll
-            for (int j = 0; j < NG; ++j) {
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    float y[8] = {};
-                    if (there) load8(src + 64 * j + 16 * t + 8 * h, p.wide, y);
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        x[j][8 * h + e] = y[e];
-                        big = fmaxf(big, fabsf(y[e]));
-                    }
-                }
+            for (int e = 0; e < E; ++e) {
+                x[e] = col < columns ? Act<T>::to_f(src[e]) : 0.0f;
+                big = fmaxf(big, fabsf(x[e]));
             }
-            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
-            big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-            // 2^up brings the largest element to [2^13, 2^14); zero, infinite and subnormal columns stay as they are
+            big = warp_max(big);
+            // 2^up brings the largest element there; zero, infinite and subnormal columns stay as they are
             const int be = (int)(__float_as_uint(big) >> 23);
             const int up = be > 0 && be < 255 ? min(13 - (be - 127), 126) : 0;
             const float f = __int_as_float((127 + up) << 23);
 #pragma unroll
-            for (int j = 0; j < NG; ++j) {
-                float s = 0.0f;
-#pragma unroll
-                for (int e = 0; e < 16; ++e) { x[j][e] *= f; s += x[j][e]; }
-                s += __shfl_xor_sync(0xffffffffu, s, 1);
-                s += __shfl_xor_sync(0xffffffffu, s, 2);
-                s *= 0x1p-24f;
-                qsum[j][0] = __shfl_sync(0xffffffffu, s, 8 * t);
-                qsum[j][1] = __shfl_sync(0xffffffffu, s, 8 * t + 4);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {  // elements (a, a + 4) at code weight 1, (a + 1, a + 5) at 16
-                    const int a = 8 * (k >> 1) + 2 * (k & 1);
-                    const float v[4] = {x[j][a], x[j][a + 4], x[j][a + 1] * 0.0625f, x[j][a + 5] * 0.0625f};
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        qf[4 * j + k][h] = pack_half2(v[2 * h], v[2 * h + 1]);
-                        if (TERMS == 2) {
-                            const float2 r = unpack_half2(qf[4 * j + k][h]);
-                            ql[4 * j + k][h] = pack_half2(v[2 * h] - r.x, v[2 * h + 1] - r.y);
-                        }
-                    }
-                }
+            for (int e = 0; e < E; ++e) {
+                x[e] *= f;
+                sum += x[e];
+                // element d of the row: code (d % 8) of a word, MMA step, register and half it lands in
+                const uint32_t d = lane * E + e, n = d % 8;
+                const uint32_t step_k = d / 64 * 4 + d / 8 % 2 * 2 + (n >> 1 & 1);
+                const uint32_t to = ((step_k * 32 + c * 4 + d / 16 % 4) * 2 + (n & 1)) * 4 + (n >> 2) * 2;
+                const float v = n & 1 ? x[e] * 0.0625f : x[e];  // codes of odd places weigh 16 times as much
+                const __half hi = __float2half_rn(v);
+                *reinterpret_cast<__half*>(qfrag + to) = hi;
+                if (TERMS == 2) *reinterpret_cast<__half*>(qfrag + NG * 4 * 256 + to) = __float2half_rn(v - __half2float(hi));
             }
+#pragma unroll
+            for (int o = 1; o < 64 / E; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+            if (lane % (64 / E) == 0) sh.qsum[group][c][lane / (64 / E)] = sum * 0x1p-24f;
             // scores come in units of 2^-24 2^up
-            const float own_f = p.scale_log2 * __int_as_float((127 - up) << 23) * 0x1p24f;
-            factor[0] = __shfl_sync(0xffffffffu, own_f, 8 * t);
-            factor[1] = __shfl_sync(0xffffffffu, own_f, 8 * t + 4);
+            if (lane == 0) sh.factor[group][c] = p.scale_log2 * __int_as_float((127 - up) << 23) * 0x1p24f;
+        }
+        group_sync(group, WG * 32);
+        uint32_t qf[NG * 4][2], ql[TERMS == 2 ? NG * 4 : 1][2];
+        float qsum[NG][2], factor[2];
+        int32_t pos[2], above[2];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const uint32_t col = min(c0 + 2 * t + h, columns - 1);
-                pos[h] = w.len - w.count + (int32_t)(col / p.group);
-                above[h] = p.window && pos[h] >= 0 && (uint32_t)pos[h] >= p.window ? pos[h] - (int32_t)p.window : -1;
+        for (int k = 0; k < NG * 4; ++k) {
+            const uint2 v = reinterpret_cast<const uint2*>(qfrag)[k * 32 + lane];
+            qf[k][0] = v.x; qf[k][1] = v.y;
+            if (TERMS == 2) {
+                const uint2 r = reinterpret_cast<const uint2*>(qfrag + NG * 4 * 256)[k * 32 + lane];
+                ql[k][0] = r.x; ql[k][1] = r.y;
             }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int j = 0; j < NG; ++j) qsum[j][h] = sh.qsum[group][2 * t + h][j];
+            factor[h] = sh.factor[group][2 * t + h];
+            const uint32_t col = min(c0 + 2 * t + h, columns - 1);
+            pos[h] = w.len - w.count + (int32_t)(col / p.group);
+            above[h] = p.window && pos[h] >= 0 && (uint32_t)pos[h] >= p.window ? pos[h] - (int32_t)p.window : -1;
         }
 
         float o[NG * 4][4] = {}, mo[NG][2] = {}, m[2] = {kNothing, kNothing}, l[2] = {};
@@ -307,8 +356,8 @@ __global__ void __launch_bounds__(AttnCfg<HD, TERMS>::NW * 32, 1) kv4_attn_kerne
         int v_exp = 0;              // p s is multiplied by 2^v_exp
         float v_mul = 1.0f;
 
-        const uint32_t r0 = key_of(g), r1 = r0 + 2;                          // keys of MMA rows g and g + 8
-        const uint32_t ra = key_of(2 * t), rb = key_of(2 * t + 1);           // and of rows 2t, 2t + 1 (+ 8: + 2)
+        const uint32_t r0 = key_of(g), r1 = r0 + 2;                  // keys of MMA rows g and g + 8
+        const uint32_t ra = key_of(2 * t), rb = key_of(2 * t + 1);   // and of rows 2t, 2t + 1 (+ 8: + 2)
         const uint32_t k_at = r0 * C::RB + 8 * t, e_at = r0 * C::RB + HD / 2;
         const uint32_t va_at = C::SIDE + ra * C::RB + 4 * g, vb_at = C::SIDE + rb * C::RB + 4 * g;
 
@@ -528,6 +577,7 @@ __global__ void __launch_bounds__(AttnCfg<HD, TERMS>::NW * 32, 1) kv4_attn_kerne
         const uint32_t used = min(seg, WG);
         auto sum4 = [&](uint32_t i) {  // floats 4 i .. 4 i + 3 of the item's sums
             float4 a = make_float4(0, 0, 0, 0);
+#pragma unroll 4
             for (uint32_t k = 0; k < used; ++k) {
                 const float4 b = reinterpret_cast<const float4*>(slots + (group * WG + ((first_warp + k) & (WG - 1))) * C::SLOT)[i];
                 a.x += b.x; a.y += b.y; a.z += b.z; a.w += b.w;
@@ -536,54 +586,38 @@ __global__ void __launch_bounds__(AttnCfg<HD, TERMS>::NW * 32, 1) kv4_attn_kerne
         };
         auto sum_l = [&](uint32_t c) {
             float a = 0.0f;
+#pragma unroll 4
             for (uint32_t k = 0; k < used; ++k) a += sh.l[group * WG + ((first_warp + k) & (WG - 1))][c];
             return a;
         };
-        auto store4 = [&](uint32_t c, uint32_t d, float4 v, float sum) {  // column c of the block
-            const uint32_t col = c0 + c;
-            if (col >= columns) return;
-            const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-            T* dst = (T*)p.out + (int64_t)((uint32_t)w.first + col / p.group) * p.o_ts +
-                     (int64_t)(kvh * p.group + col % p.group) * p.o_hs + d;
-            union { uint2 u[sizeof(T) / 2]; T x[4]; } r;
-            r.x[0] = Act<T>::from_f(v.x * inv); r.x[1] = Act<T>::from_f(v.y * inv);
-            r.x[2] = Act<T>::from_f(v.z * inv); r.x[3] = Act<T>::from_f(v.w * inv);
-            if (p.wide) {
-#pragma unroll
-                for (int i = 0; i < (int)(sizeof(T) / 2); ++i) reinterpret_cast<uint2*>(dst)[i] = r.u[i];
-            } else {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) dst[i] = r.x[i];
-            }
+        auto top_of = [&](uint32_t c) {
+            float a = kNothing;
+#pragma unroll 4
+            for (uint32_t k = 0; k < WG; ++k) a = fmaxf(a, sh.m[group * WG + k][c]);
+            return a;
         };
-        if (whole) {
-            for (uint32_t i = gt; i < C::SLOT / 4; i += threads) store4(i / (HD / 4), i % (HD / 4) * 4, sum4(i), sum_l(i / (HD / 4)));
-        } else {
-            // this group's piece: slot 0 of its range if the item began before it, else slot 1
-            float* mine = p.partial + (range * 2 + (tile0 ? 0 : 1)) * kPieceFloats;
+        bool finish = whole;
+        // an item's first piece is in slot 1 of its range (it begins in it), the others in slot 0
+        const float* first_piece = p.partial + (size_t)first_range * 2 * kPieceFloats;
+        auto piece = [&](uint32_t r) { return first_piece + (size_t)(2 * r + (r == 0 ? 1 : 0)) * kPieceFloats; };
+        if (!whole) {
+            float* mine = p.partial + ((size_t)range * 2 + (tile0 ? 0 : 1)) * kPieceFloats;
             for (uint32_t i = gt; i < C::SLOT / 4; i += threads) __stcg(reinterpret_cast<float4*>(mine + 16) + i, sum4(i));
             if (gt < 8) {
-                float top = kNothing;
-                for (uint32_t i = 0; i < WG; ++i) top = fmaxf(top, sh.m[group * WG + i][gt]);
-                __stcg(mine + gt, top);
+                __stcg(mine + gt, top_of(gt));
                 __stcg(mine + 8 + gt, sum_l(gt));
             }
-            // the item's units and the ranges that share it
-            const uint64_t i0 = unit - tile0, i1 = i0 + w.tiles - 1;
-            const uint64_t ra = ((i0 + 1) * ranges - 1) / total, rb = ((i1 + 1) * ranges - 1) / total;
-            __threadfence();
             group_sync(group, threads);
             if (gt == 0) {
-                const uint32_t before = atomicAdd(p.tickets + ra, 1u);
-                sh.last[group] = before == (uint32_t)(rb - ra);
-                if (sh.last[group]) p.tickets[ra] = 0;  // ready for the next call
+                __threadfence();
+                const uint32_t others = atomicAdd(p.tickets + first_range, 1u);
+                sh.last[group] = others == pieces - 1;
+                if (sh.last[group]) p.tickets[first_range] = 0;  // ready for the next call
                 __threadfence();
             }
             group_sync(group, threads);
-            if (sh.last[group]) {
-                const uint32_t pieces = (uint32_t)(rb - ra) + 1;
-                const float* base = p.partial + ra * 2 * kPieceFloats;  // the first piece is its range's slot 1
-                auto piece = [&](uint32_t r) { return base + (size_t)(2 * r + (r == 0 ? 1 : 0)) * kPieceFloats; };
+            finish = sh.last[group];
+            if (finish) {
                 // the columns' maxima over the pieces
                 float top = kNothing;
                 for (uint32_t r = gt / 8; r < pieces; r += threads / 8) top = fmaxf(top, __ldcg(piece(r) + gt % 8));
@@ -591,12 +625,22 @@ __global__ void __launch_bounds__(AttnCfg<HD, TERMS>::NW * 32, 1) kv4_attn_kerne
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
                 if (lane < 8) sh.m[warp][lane] = top;
                 group_sync(group, threads);
-                for (uint32_t i = gt; i < C::SLOT / 4; i += threads) {
-                    const uint32_t c = i / (HD / 4);
-                    top = kNothing;
-                    for (uint32_t k = 0; k < WG; ++k) top = fmaxf(top, sh.m[group * WG + k][c]);
-                    float4 a = make_float4(0, 0, 0, 0);
-                    float sum = 0.0f;
+            }
+        }
+        if (finish) {
+#pragma unroll 1
+            for (uint32_t i = gt; i < C::SLOT / 4; i += threads) {
+                const uint32_t c = i / (HD / 4), d = i % (HD / 4) * 4, col = c0 + c;
+                if (col >= columns) break;
+                float4 a;
+                float sum;
+                if (whole) {
+                    a = sum4(i);
+                    sum = sum_l(c);
+                } else {
+                    const float top = top_of(c);
+                    a = make_float4(0, 0, 0, 0);
+                    sum = 0.0f;
 #pragma unroll 8
                     for (uint32_t r = 0; r < pieces; ++r) {
                         const float pm = __ldcg(piece(r) + c), pl = __ldcg(piece(r) + 8 + c);
@@ -605,21 +649,23 @@ __global__ void __launch_bounds__(AttnCfg<HD, TERMS>::NW * 32, 1) kv4_attn_kerne
                         a.x = fmaf(b.x, f, a.x); a.y = fmaf(b.y, f, a.y); a.z = fmaf(b.z, f, a.z); a.w = fmaf(b.w, f, a.w);
                         sum = fmaf(pl, f, sum);
                     }
-                    store4(c, i % (HD / 4) * 4, a, sum);
+                }
+                const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                T* dst = (T*)p.out + (int64_t)((uint32_t)w.first + col / p.group) * p.o_ts +
+                         (int64_t)(kvh * p.group + col % p.group) * p.o_hs + d;
+                union { uint2 u[sizeof(T) / 2]; T x[4]; } r;
+                r.x[0] = Act<T>::from_f(a.x * inv); r.x[1] = Act<T>::from_f(a.y * inv);
+                r.x[2] = Act<T>::from_f(a.z * inv); r.x[3] = Act<T>::from_f(a.w * inv);
+                if (p.wide) {
+#pragma unroll
+                    for (int k = 0; k < (int)(sizeof(T) / 2); ++k) reinterpret_cast<uint2*>(dst)[k] = r.u[k];
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) dst[k] = r.x[k];
                 }
             }
         }
-        group_sync(group, threads);  // the slots are free again
-        unit += seg;
-        tile0 += seg;
-        if (tile0 == w.tiles && unit < u1) {
-            tile0 = 0;
-            if (++item == w.blocks * p.map.kv_heads) {
-                item = 0;
-                do w = seq_work(p, ++seq, false);
-                while (w.blocks == 0);
-            }
-        }
+        group_sync(group, threads);  // the slots and the queries' place are free again
     }
     // after an expired wait copies may still be on their way to this CTA's shared memory
     for (; dead && ahead > 0; --ahead) {

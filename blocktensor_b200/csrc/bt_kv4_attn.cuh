@@ -87,8 +87,7 @@ struct SeqWork {
     }
 };
 
-// (Not inlined: it is asked for in several places, and the kernel's code has to stay small.)
-static __device__ __noinline__ SeqWork seq_work(const AttnParams& p, uint32_t i, bool report) {
+__device__ __forceinline__ SeqWork seq_work(const AttnParams& p, uint32_t i, bool report) {
     SeqWork w;
     w.first = (int32_t)i;
     w.count = 1;
