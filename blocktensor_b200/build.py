@@ -17,7 +17,7 @@ CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "libbt_cuda.so")
 
 SOURCES = ["bt_quant.cu", "bt_prims.cu", "bt_engine.cu", "bt_noalloc.cu", "bt_prefill.cu", "bt_batch.cu", "bt_q4.cu", "bt_sample.cu",
-           "bt_qkv.cu", "bt_kv4_attn.cu", "bt_sample_batch.cu"]
+           "bt_qkv.cu", "bt_kv4_attn.cu", "bt_kv4_prefill.cu", "bt_sample_batch.cu"]
 HEADERS = ["bt_attn_mma.cuh", "bt_common.cuh", "bt_gemv.cuh", "bt_gemv_mma.cuh", "bt_ptx.cuh", "bt_attention.cuh", "bt_step.cuh",
            "bt_gemm.cuh", "bt_engine_impl.h", "bt_internal.h", "bt_kv4.cuh", "bt_kv4_attn.cuh"]
 

@@ -23,9 +23,6 @@
 
 namespace bt {
 
-constexpr float kLazyMax = 8.0f;     // a column's reference maximum may be exceeded by 2^8 before it moves
-constexpr float kNothing = -1e30f;   // a column's maximum before it sees a key (finite: differences stay defined)
-
 template <int HD, int TERMS>
 struct AttnCfg {
     static constexpr int NG = HD / 64;                       // 64-element groups of a row
@@ -48,6 +45,13 @@ __device__ __forceinline__ uint64_t div64(uint64_t a, uint32_t b) {
     return a >> 32 ? a / b : (uint64_t)((uint32_t)a / b);
 }
 
+// The few-row kernel's share: sequences with more rows are the prefill kernel's.
+__device__ __forceinline__ SeqWork few_row_work(const AttnParams& p, uint32_t i, bool report) {
+    SeqWork w = seq_work(p, i, report);
+    if ((uint32_t)w.count * p.group > p.few_rows) w.blocks = 0;
+    return w;
+}
+
 // Walks the items of a range.  [tile, end): the current item's units in the range.
 struct Walk {
     SeqWork w;
@@ -68,7 +72,7 @@ struct Walk {
     // The range [from, to) of units cut every `step`, in a sequence whose units start at seq_at.
     __device__ __forceinline__ void begin(const AttnParams& p, uint32_t s, uint64_t seq_at, uint64_t from, uint64_t to, uint64_t step) {
         seq = s;
-        w = seq_work(p, s, false);
+        w = few_row_work(p, s, false);
         const uint32_t units = w.tiles + kItemCost;
         item = (uint32_t)div64(from - seq_at, units);
         at = seq_at + (uint64_t)item * units;
@@ -81,7 +85,7 @@ struct Walk {
     // Piece `range` of the pieces of at most `step` units, in a sequence whose pieces start at seq_at.
     __device__ __forceinline__ void begin_piece(const AttnParams& p, uint32_t s, uint32_t seq_at, uint32_t range, uint32_t step) {
         seq = s;
-        w = seq_work(p, s, false);
+        w = few_row_work(p, s, false);
         ranges = (w.tiles + step - 1) / step;
         item = (range - seq_at) / ranges;
         first_range = seq_at + item * ranges;
@@ -99,7 +103,7 @@ struct Walk {
         if (at >= until) { done = 1; return; }
         if (++item == w.blocks * p.map.kv_heads) {
             item = 0;
-            do w = seq_work(p, ++seq, false);  // (there is one: units are left)
+            do w = few_row_work(p, ++seq, false);  // (there is one: units are left)
             while (w.blocks == 0);
         }
         enter(p, step);
@@ -148,7 +152,7 @@ __global__ void __launch_bounds__(AttnCfg<HD, TERMS>::NW * 32, 1) kv4_attn_kerne
     uint32_t items = 0;
     SeqWork mine = {};  // the sequence this thread looked at last
     for (uint32_t i = tid; i < p.n; i += NW * 32) {
-        mine = seq_work(p, i, blockIdx.x == 0);
+        mine = few_row_work(p, i, blockIdx.x == 0);
         const uint32_t it = mine.blocks * p.map.kv_heads;
         total += (uint64_t)it * mine.tiles;
         items += it;
@@ -190,7 +194,7 @@ __global__ void __launch_bounds__(AttnCfg<HD, TERMS>::NW * 32, 1) kv4_attn_kerne
         const uint32_t i = i0 + tid;
         if (p.n > NW * 32) {
             mine.blocks = 0;
-            if (i < p.n) mine = seq_work(p, i, false);
+            if (i < p.n) mine = few_row_work(p, i, false);
         }
         // its ranges (few items) or units (many)
         const uint64_t own = (uint64_t)mine.blocks * p.map.kv_heads * (few ? (uint32_t)div64(mine.tiles + step - 1, (uint32_t)step) : mine.tiles + kItemCost);
@@ -740,6 +744,13 @@ extern "C" int bt_cuda_kv4_attention(const bt_kv4* cache, const bt_kv4_attn_args
     p.tickets = (uint32_t*)workspace;
     p.partial = (float*)((uint8_t*)workspace + ticket_bytes(sms));
     const cudaStream_t s = as_stream(stream);
+    // Sequences with many rows go to the tcgen05 kernel, which unpacks a tile once for 256 rows
+    // instead of once for 8 but takes a whole tile's time for any number of them.
+    const uint64_t most = (uint64_t)(!a->q_start ? 1 : a->max_q ? a->max_q : a->tokens) * p.group;
+    const bool many = prefill_takes(a->dtype, cache->head_dim) && most > kFewRows;
+    p.few_rows = !many ? 0xffffffffu : a->n == 1 ? 0 : kFewRows;
+    if (many) BT_CUDA_CHECK(launch_kv4_prefill(p, a->dtype, cache->head_dim, sms, s));
+    if (p.few_rows == 0) return BT_OK;
     auto by_hd = [&](auto type, auto terms) {
         using T = decltype(type);
         constexpr int N = decltype(terms)::value;

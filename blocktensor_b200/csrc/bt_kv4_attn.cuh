@@ -32,11 +32,21 @@ struct AttnParams {
     uint32_t n, tokens, heads, group;  // group: query heads of a KV head
     uint32_t window, sinks;
     float scale_log2;                  // scale * log2(e)
+    uint32_t few_rows;                 // sequences with more (query, head) rows a KV head go to the prefill kernel
     bool wide;
     Kv4Map map;
     float* partial;                    // workspace: partial results and their tickets
     uint32_t* tickets;
 };
+
+// The many-row kernel (bt_kv4_prefill.cu): whether it takes a type and head_dim, and its
+// launch over the sequences with more than few_rows rows.
+bool prefill_takes(int dtype, uint32_t head_dim);
+cudaError_t launch_kv4_prefill(const AttnParams& p, int dtype, uint32_t head_dim, int sms, cudaStream_t s);
+
+constexpr uint32_t kFewRows = 64;     // see bt_cuda_kv4_attention
+constexpr float kLazyMax = 8.0f;     // a row's reference maximum may be exceeded by 2^8 before it moves
+constexpr float kNothing = -1e30f;   // a row's maximum before it sees a key (finite: differences stay defined)
 
 // ---------------------------------------------------------------- mma helpers
 

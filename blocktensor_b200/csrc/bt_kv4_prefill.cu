@@ -1,0 +1,561 @@
+// bt_kv4_prefill.cu -- causal attention of many query rows over a 4-bit cache
+// (the chunks of bt_cuda_kv4_attention) on tcgen05 tensor cores.
+//
+// Mathematics.  256 (query, head) rows that share a KV head go over 128-key tiles
+// with the running maximum and sum of a softmax:
+//   S = Q K^T,  P = exp2(f S - m),  O += P V,  l += sum P,  out = O / l.
+// A tile's keys and values are unpacked once into fp16 operands in shared memory
+// (scale * code + min, one rounding of 2^-12 rms) and serve both 128-row halves.
+// Queries enter scaled by a power of two per row, exact for bf16 and fp16; P is
+// rounded to fp16 (2^-12 rms); sums, maxima and O are fp32.
+//
+// Bound: at head_dim 128 a tile is 2048 tensor cycles (4 MMA blocks of 128 x 128 x
+// 128), 2048 cycles of the exponential unit (256 x 128) and about 1500 issue slots
+// a scheduler for softmax and unpacking, so the three run side by side in warps of
+// their own:
+//   warps 0-3, 4-7  softmax of a row half each, a thread a row: S from tensor memory,
+//                   P back into the same columns (half as wide, behind the reader)
+//   warps 8-11      unpack K and V tiles into two stages each
+//   warp 12         bulk copies of the packed rows
+//   warp 13         issues the MMAs: S of the next tile and one half's P V run while the
+//                   other half's softmax does
+// Tensor memory: S (or P) of the halves in columns 0 and 128, O in 256 and 384.
+//
+// A CTA is resident on an SM and takes blocks of rows in turn, those with the
+// longest keys first.  V's rows (the N of P V) are stored in the order e, chunk of
+// d = 8 chunk + e, so that the unpackers' 16-byte stores of neighbouring lanes are
+// contiguous; K's and Q's elements of 8 are in the order 0 4 1 5 2 6 3 7, in which a
+// word's codes come out two at a time.
+#include "bt_kv4_attn.cuh"
+
+namespace bt {
+
+constexpr int kPfKeys = 128;     // keys of a tile
+constexpr int kPfThreads = 14 * 32;
+constexpr uint32_t kPfRaw = 3;   // packed K or V tiles in flight
+
+template <int HD>
+struct PfCfg {
+    static constexpr uint32_t RB = kv4_row_bytes(HD), RAW = kPfKeys * RB;
+    static constexpr uint32_t Q = 128 * HD * 2, KV = kPfKeys * HD * 2;  // bytes of an operand tile
+    static constexpr uint32_t SMEM = 2 * Q + 4 * KV + kPfRaw * RAW;
+    static constexpr uint32_t IDESC_S = (1u << 4) | ((kPfKeys >> 3) << 17) | ((128u >> 4) << 24);  // f16 x f16 -> f32
+    static constexpr uint32_t IDESC_O = (1u << 4) | ((HD >> 3) << 17) | ((128u >> 4) << 24);
+};
+
+struct PfShared {
+    uint64_t raw_full[kPfRaw], raw_empty[kPfRaw];
+    uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
+    uint64_t q_full[2], s_full[2], p_full[2], o_full[2], drain;
+    uint32_t pieces[8];  // of a tile: which of its 16-key pieces hold keys
+    uint32_t tmem;
+    volatile uint32_t dead;  // a wait gave up: everybody leaves
+};
+
+// tcgen05.mma with A in tensor memory
+__device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&v)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
+        "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+        "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_ld8(uint32_t addr, uint32_t (&d)[8]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3]), "=r"(d[4]), "=r"(d[5]), "=r"(d[6]), "=r"(d[7])
+                 : "r"(addr)
+                 : "memory");
+}
+
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("{\n .reg .b64 x, y, z, w;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n"
+        " fma.rn.f32x2 w, x, y, z;\n mov.b64 {%0, %1}, w;\n}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 r;
+    asm("{\n .reg .b64 x, y, w;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 w, x, y;\n mov.b64 {%0, %1}, w;\n}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+
+// A block of rows of one sequence and KV head, and its tiles.
+struct PfItem {
+    SeqWork w;
+    uint32_t head, row0, rows;  // rows row0 .. of the sequence's count * group
+    int32_t top, above;         // positions seen: (above, top] and [0, sinks)
+    uint32_t tiles, sink_tiles;
+    int32_t lo;
+    __device__ __forceinline__ int32_t key0(uint32_t t) const {
+        return (int32_t)t * kPfKeys + (t < sink_tiles ? 0 : lo - (int32_t)sink_tiles * kPfKeys);
+    }
+    __device__ __forceinline__ bool any(int32_t k, int32_t n, uint32_t sinks) const {
+        return k <= top && (k + n - 1 > above || (uint32_t)k < sinks);
+    }
+};
+
+__device__ __forceinline__ int32_t window_start(const AttnParams& p, int32_t pos) {
+    return p.window && pos >= 0 && (uint32_t)pos >= p.window ? pos - (int32_t)p.window : -1;
+}
+
+// Walks all blocks in order; every lane of a warp calls it alike.
+struct PfWalk {
+    uint32_t s0;     // first sequence of the 32 that the lanes look at
+    uint64_t base;   // blocks before them
+    __device__ __forceinline__ bool find(const AttnParams& p, uint64_t b, uint32_t lane, PfItem* it) {
+        for (; s0 < p.n; s0 += 32) {
+            uint32_t own = 0;
+            if (s0 + lane < p.n) {
+                const SeqWork w = seq_work(p, s0 + lane, false);
+                const uint32_t rows = (uint32_t)w.count * p.group;
+                own = rows > p.few_rows ? (rows + 255) / 256 * p.map.kv_heads : 0;
+            }
+            uint64_t inc = own;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint64_t v = __shfl_up_sync(0xffffffffu, inc, o);
+                if (lane >= (uint32_t)o) inc += v;
+            }
+            const uint64_t all = __shfl_sync(0xffffffffu, inc, 31);
+            if (b < base + all) {
+                const uint32_t hit = __ffs(__ballot_sync(0xffffffffu, b < base + inc)) - 1;
+                const uint32_t at = (uint32_t)(b - base - __shfl_sync(0xffffffffu, inc - own, hit));
+                it->w = seq_work(p, s0 + hit, false);
+                const uint32_t total = (uint32_t)it->w.count * p.group, blocks = (total + 255) / 256;
+                const uint32_t block = blocks - 1 - at / p.map.kv_heads;  // longest first
+                it->head = at % p.map.kv_heads;
+                it->row0 = block * 256;
+                it->rows = min(256u, total - it->row0);
+                const int32_t first = it->w.len - it->w.count;
+                it->top = first + (int32_t)((it->row0 + it->rows - 1) / p.group);
+                it->above = window_start(p, first + (int32_t)(it->row0 / p.group));
+                it->lo = (it->above + 1) & ~(kPfKeys - 1);
+                it->sink_tiles = p.window ? min((min(p.sinks, 0x7fffff00u) + kPfKeys - 1) / kPfKeys, (uint32_t)it->lo / kPfKeys) : 0;
+                it->tiles = it->top < 0 ? 0 : it->sink_tiles + (uint32_t)(it->top - it->lo) / kPfKeys + 1;
+                return true;
+            }
+            base += all;
+        }
+        return false;
+    }
+};
+
+// code pairs of a word as exact fp16 integers: (w >> 4 i) & 15 in the low half, 4 codes further in the high half
+__device__ __forceinline__ __half2 code_pair(uint32_t w, int i) {
+    const uint32_t x = i & 2 ? w >> 8 : w;
+    if (i & 1) {  // 1024 + 16 c
+        const uint32_t v = (x & 0x00f000f0u) | 0x64006400u;
+        return __hfma2(*reinterpret_cast<const __half2*>(&v), __float2half2_rn(0.0625f), __float2half2_rn(-64.0f));
+    }
+    const uint32_t v = (x & 0x000f000fu) | 0x64006400u;
+    return __hadd2(*reinterpret_cast<const __half2*>(&v), __float2half2_rn(-1024.0f));
+}
+__device__ __forceinline__ uint32_t as_u32(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
+__device__ __forceinline__ __half2 as_half2(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
+
+template <typename T, int HD>
+__global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid_constant__ AttnParams p) {
+    using C = PfCfg<HD>;
+    constexpr int CH = HD / 8;  // chunks of 8 elements
+    extern __shared__ __align__(128) uint8_t dyn[];
+    __shared__ PfShared sh;
+    const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    uint8_t* qs = dyn;
+    uint8_t* ks = dyn + 2 * C::Q;
+    uint8_t* vs = ks + 2 * C::KV;
+    uint8_t* raw = vs + 2 * C::KV;
+
+    if (warp == 13) {
+        tmem_alloc(&sh.tmem, 512);
+        tmem_relinquish();
+    }
+    if (tid == 0) {
+        for (uint32_t i = 0; i < kPfRaw; ++i) { mbar_init(&sh.raw_full[i], 1); mbar_init(&sh.raw_empty[i], 4); }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&sh.k_full[i], 4); mbar_init(&sh.k_empty[i], 1); mbar_init(&sh.v_full[i], 4); mbar_init(&sh.v_empty[i], 1);
+            mbar_init(&sh.q_full[i], 4); mbar_init(&sh.s_full[i], 1); mbar_init(&sh.p_full[i], 4); mbar_init(&sh.o_full[i], 1);
+        }
+        mbar_init(&sh.drain, 1);
+        sh.dead = 0;
+        fence_mbar_init();
+    }
+    tcgen05_fence_before();
+    __syncthreads();
+    tcgen05_fence_after();
+    const uint32_t tmem = sh.tmem;
+
+    // A bounded wait; false: it, or another warp's, gave up.
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+        if (mbar_try_wait(bar, parity)) return true;
+        const uint64_t t0 = global_ns();
+        while (!sh.dead) {
+            if (mbar_try_wait_sleep(bar, parity, 20000u)) return true;
+            if (global_ns() - t0 > kWaitNs) {
+                sh.dead = 1;
+                p.map.flag(BT_KV4_TIMEOUT);
+            }
+        }
+        return false;
+    };
+    auto warp_wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
+
+    PfItem it;
+    PfWalk walk = {0, 0};
+    uint32_t tile_no = 0;  // tiles before the item, over all of this CTA's items
+
+    if (warp < 8) {
+        // ------------------------------------------------ softmax: a thread a row
+        const uint32_t r = warp >> 2, row = (warp & 3) * 32 + lane;
+        const uint32_t lanes = tmem + ((warp & 3) * 32u << 16), s_at = lanes + r * 128, o_at = lanes + 256 + r * 128;
+        const float sign = p.scale_log2 < 0.0f ? -1.0f : 1.0f;
+        uint32_t s_phase = 0, o_phase = 0;
+        for (uint64_t b = blockIdx.x; walk.find(p, b, lane, &it); b += gridDim.x) {
+            if (it.rows <= r * 128) { tile_no += it.tiles; continue; }
+            const bool there = r * 128 + row < it.rows;
+            const uint32_t c = it.row0 + r * 128 + (there ? row : 0);
+            const int64_t token = (int64_t)((uint32_t)it.w.first + c / p.group), head = it.head * p.group + c % p.group;
+            const int32_t pos = it.w.len - it.w.count + (int32_t)(c / p.group), above = window_start(p, pos);
+            T* out = (T*)p.out + token * p.o_ts + head * p.o_hs;
+            float f = 0.0f, m = kNothing, l = 0.0f;
+            if (it.tiles) {
+                // the row as fp16, scaled so that its largest element is in [2^13, 2^14)
+                const T* src = (const T*)p.q + token * p.q_ts + head * p.q_hs;
+                float big = 0.0f;
+#pragma unroll 4
+                for (int k = 0; k < CH; ++k) {
+                    float x[8];
+                    load8(src + 8 * k, p.wide, x);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(x[e]));
+                }
+                const int be = (int)(__float_as_uint(big) >> 23);
+                const int up = be > 0 && be < 255 ? min(13 - (be - 127), 126) : 0;
+                const bool flat = p.scale_log2 == 0.0f;  // all scores equal: f stays positive
+                const float mul = there && !flat ? sign * __int_as_float((127 + up) << 23) : 0.0f;
+                f = flat ? 1.0f : fabsf(p.scale_log2) * __int_as_float((127 - up) << 23);
+#pragma unroll 4
+                for (int k = 0; k < CH; ++k) {
+                    float x[8];
+                    load8(src + 8 * k, p.wide, x);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] = there ? x[e] * mul : 0.0f;
+                    uint4 v;
+                    v.x = pack_half2(x[0], x[4]); v.y = pack_half2(x[1], x[5]); v.z = pack_half2(x[2], x[6]); v.w = pack_half2(x[3], x[7]);
+                    *reinterpret_cast<uint4*>(qs + r * C::Q + (k * 128 + row) * 16) = v;
+                }
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.q_full[r]);
+            }
+            bool ok = true;
+            for (uint32_t i = 0; i < it.tiles; ++i) {
+                const int32_t k0 = it.key0(i);
+                if (!(ok = warp_wait(&sh.s_full[r], s_phase))) break;
+                s_phase ^= 1;
+                tcgen05_fence_after();
+                const uint32_t pieces = sh.pieces[(tile_no + i) & 7];
+                // every row of the warp sees the whole tile
+                const bool plain = __all_sync(0xffffffffu, k0 + kPfKeys - 1 <= pos && (k0 > above || (uint32_t)(k0 + kPfKeys) <= p.sinks)) && pieces == 0xffu;
+                auto bar_unseen = [&](float (&s)[32], int32_t k) {
+                    if (plain) return;
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        const int32_t key = k + e;
+                        const bool in = key <= pos && (key > above || (uint32_t)key < p.sinks) && (pieces >> ((key - k0) >> 4) & 1);
+                        s[e] = in ? s[e] : -INFINITY;
+                    }
+                };
+                float top = -INFINITY;
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {
+                    float s[32];
+                    tmem_ld32(s_at + 32 * h, reinterpret_cast<uint32_t(&)[32]>(s));
+                    tmem_wait_ld();
+                    bar_unseen(s, k0 + 32 * h);
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) top = fmaxf(top, fmaxf(s[e], s[e + 1]));
+                }
+                top *= f;
+                if (__any_sync(0xffffffffu, top > m + kLazyMax)) {
+                    const float now = fmaxf(m, top), fix = exp2_fast(m - now);
+                    m = now;
+                    l *= fix;
+                    if (i > 0) {  // the products of the tiles so far are complete: this tile's S came after them
+#pragma unroll 1
+                        for (int h = 0; h < HD / 16; ++h) {
+                            uint32_t o[16];
+                            tmem_ld16(o_at + 16 * h, o);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * fix);
+                            tmem_st16(o_at + 16 * h, o);
+                        }
+                    }
+                }
+                float2 sum = make_float2(0.0f, 0.0f);
+                const float2 ff = make_float2(f, f), mm = make_float2(-m, -m);
+#pragma unroll
+                for (int h = 0; h < 4; ++h) {
+                    float s[32];
+                    tmem_ld32(s_at + 32 * h, reinterpret_cast<uint32_t(&)[32]>(s));
+                    tmem_wait_ld();
+                    bar_unseen(s, k0 + 32 * h);
+                    uint32_t v[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        float2 x = fma2(make_float2(s[2 * e], s[2 * e + 1]), ff, mm);
+                        x.x = exp2_fast(x.x);
+                        x.y = exp2_fast(x.y);
+                        sum = add2(sum, x);
+                        v[e] = pack_half2(x.x, x.y);
+                    }
+                    tmem_st16(s_at + 16 * h, v);  // behind the columns still to be read
+                }
+                l += sum.x + sum.y;
+                tmem_wait_st();
+                tcgen05_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.p_full[r]);
+            }
+            if (!ok) break;
+            tile_no += it.tiles;
+            if (it.tiles) {
+                if (!warp_wait(&sh.o_full[r], o_phase)) break;
+                o_phase ^= 1;
+                tcgen05_fence_after();
+            }
+            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll 1
+            for (int h = 0; h < CH / 8; ++h) {  // column e CH + chunk is element 8 chunk + e
+                uint32_t o[8][8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) tmem_ld8(o_at + e * CH + 8 * h, o[e]);
+                tmem_wait_ld();
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    float x[8];
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) x[e] = it.tiles ? __uint_as_float(o[e][k]) * inv : 0.0f;
+                    if (there) store8(out + 8 * (8 * h + k), p.wide, x);
+                }
+            }
+            tcgen05_fence_before();
+        }
+    } else if (warp < 12) {
+        // ------------------------------------------------ unpacking
+        const uint32_t u = tid - 256;  // 0 .. 127
+        uint32_t raw_at = 0, raw_phase = 0, st = 0, st_phase = 1;
+        for (uint64_t b = blockIdx.x; walk.find(p, b, lane, &it); b += gridDim.x) {
+            bool ok = true;
+            for (uint32_t i = 0; i < it.tiles && ok; ++i) {
+                const int32_t k0 = it.key0(i);
+                // K: a thread a key
+                if (!(ok = warp_wait(&sh.raw_full[raw_at], raw_phase) && warp_wait(&sh.k_empty[st], st_phase))) break;
+                {
+                    const uint8_t* src = raw + raw_at * C::RAW + u * C::RB;
+                    uint8_t* dst = ks + st * C::KV + u * 16;
+#pragma unroll
+                    for (int j = 0; j < HD / 64; ++j) {
+                        const __half2 e = as_half2(reinterpret_cast<const uint32_t*>(src + HD / 2)[j]);
+                        const __half2 s = __low2half2(e), m = __high2half2(e);
+#pragma unroll
+                        for (int k = 8 * j; k < 8 * j + 8; ++k) {
+                            const uint32_t w = reinterpret_cast<const uint32_t*>(src)[k];
+                            uint4 v;
+                            v.x = as_u32(__hfma2(code_pair(w, 0), s, m)); v.y = as_u32(__hfma2(code_pair(w, 1), s, m));
+                            v.z = as_u32(__hfma2(code_pair(w, 2), s, m)); v.w = as_u32(__hfma2(code_pair(w, 3), s, m));
+                            *reinterpret_cast<uint4*>(dst + k * (kPfKeys * 16)) = v;
+                        }
+                    }
+                }
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) { mbar_arrive(&sh.k_full[st]); mbar_arrive(&sh.raw_empty[raw_at]); }
+                if (++raw_at == kPfRaw) { raw_at = 0; raw_phase ^= 1; }
+                // V: a thread 8 keys x 8 elements at a time
+                if (!(ok = warp_wait(&sh.raw_full[raw_at], raw_phase) && warp_wait(&sh.v_empty[st], st_phase))) break;
+                {
+                    const uint32_t pieces = sh.pieces[(tile_no + i) & 7];
+#pragma unroll 1
+                    for (uint32_t x = u; x < 16 * CH; x += 128) {
+                        const uint32_t oct = x / CH, chunk = x % CH;
+                        const uint8_t* src = raw + raw_at * C::RAW + oct * 8 * C::RB;
+                        uint8_t* dst = vs + st * C::KV + oct * (HD * 16) + chunk * 16;
+                        uint32_t o[8][4];
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {  // keys 2q, 2q + 1 of the eight
+                            const uint8_t *a = src + 2 * q * C::RB, *c = a + C::RB;
+                            const uint32_t wa = reinterpret_cast<const uint32_t*>(a)[chunk], wc = reinterpret_cast<const uint32_t*>(c)[chunk];
+                            const int32_t key = k0 + (int32_t)(oct * 8) + 2 * q;
+                            const bool got = pieces >> (oct >> 1) & 1;
+                            // what no row sees may hold anything: its values become zero
+                            const uint32_t ea = got && it.any(key, 1, p.sinks) ? reinterpret_cast<const uint32_t*>(a + HD / 2)[chunk / 8] : 0u;
+                            const uint32_t ec = got && it.any(key + 1, 1, p.sinks) ? reinterpret_cast<const uint32_t*>(c + HD / 2)[chunk / 8] : 0u;
+                            const __half2 s = as_half2(__byte_perm(ea, ec, 0x5410)), m = as_half2(__byte_perm(ea, ec, 0x7632));
+                            const uint32_t lo = __byte_perm(wa, wc, 0x5410), hi = __byte_perm(wa, wc, 0x7632);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                o[e][q] = as_u32(__hfma2(code_pair(lo, e), s, m));
+                                o[e + 4][q] = as_u32(__hfma2(code_pair(hi, e), s, m));
+                            }
+                        }
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) *reinterpret_cast<uint4*>(dst + e * (CH * 16)) = make_uint4(o[e][0], o[e][1], o[e][2], o[e][3]);
+                    }
+                }
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) { mbar_arrive(&sh.v_full[st]); mbar_arrive(&sh.raw_empty[raw_at]); }
+                if (++raw_at == kPfRaw) { raw_at = 0; raw_phase ^= 1; }
+                st ^= 1;
+                st_phase ^= st == 0;
+            }
+            if (!ok) break;
+            tile_no += it.tiles;
+        }
+    } else if (warp == 12) {
+        // ------------------------------------------------ packed rows
+        uint32_t at = 0, phase = 1, sent = 0;
+        if (blockIdx.x == 0) {
+            for (uint32_t i = lane; i < p.n; i += 32) seq_work(p, i, true);  // reports what is out of range
+        }
+        for (uint64_t b = blockIdx.x; walk.find(p, b, lane, &it); b += gridDim.x) {
+            bool ok = true;
+            for (uint32_t i = 0; i < it.tiles && ok; ++i) {
+                const int32_t k0 = it.key0(i), key = k0 + 16 * (int32_t)lane;
+                const bool live = lane < 8 && it.any(key, 16, p.sinks);
+                const int64_t row = live ? p.map.row(it.w.slot, it.head, key) : -1;
+                if (live && row < 0) p.map.flag(BT_KV4_RANGE);
+                const uint32_t pieces = __ballot_sync(0xffffffffu, row >= 0);
+                // one copy where the whole tile lies together
+                const bool joined = pieces == 0xffu && p.map.shift >= 7;
+                for (int side = 0; side < 2 && ok; ++side) {
+                    if (!(ok = warp_wait(&sh.raw_empty[at], phase))) break;
+                    if (lane == 0) {
+                        if (side == 0) sh.pieces[(tile_no + i) & 7] = pieces;
+                        mbar_expect_tx(&sh.raw_full[at], __popc(pieces) * 16 * C::RB);
+                    }
+                    __syncwarp();
+                    const uint8_t* src = side ? p.map.v : p.map.k;
+                    uint8_t* dst = raw + at * C::RAW;
+                    if (joined) {
+                        if (lane == 0) bulk_g2s(dst, src + (size_t)row * C::RB, C::RAW, &sh.raw_full[at]);
+                    } else if (row >= 0) {
+                        bulk_g2s(dst + lane * 16 * C::RB, src + (size_t)row * C::RB, 16 * C::RB, &sh.raw_full[at]);
+                    }
+                    ++sent;
+                    if (++at == kPfRaw) { at = 0; phase ^= 1; }
+                }
+            }
+            if (!ok) break;
+            tile_no += it.tiles;
+        }
+        // every copy has arrived before the CTA may end (a wait may have given up on one)
+        for (uint32_t k = sent > kPfRaw ? sent - kPfRaw : 0; k < sent; ++k) mbar_wait(&sh.raw_full[k % kPfRaw], (k / kPfRaw) & 1, nullptr);
+    } else {
+        // ------------------------------------------------ MMAs (one thread issues; the warp walks along)
+        uint32_t kst = 0, kph = 0, vst = 0, vph = 0, qph[2] = {0, 0}, pph[2] = {0, 0};
+        auto scores = [&](uint32_t r) {
+            if (lane == 0) {
+                const uint64_t a = umma_desc(smem_u32(qs + r * C::Q), 128 * 16, 128), kb = umma_desc(smem_u32(ks + kst * C::KV), kPfKeys * 16, 128);
+#pragma unroll
+                for (int k = 0; k < HD / 16; ++k) umma_f16(tmem + r * 128, a + k * 256, kb + k * (2 * kPfKeys), C::IDESC_S, k > 0);
+                umma_commit(&sh.s_full[r]);
+            }
+        };
+        for (uint64_t b = blockIdx.x; walk.find(p, b, lane, &it); b += gridDim.x) {
+            if (it.tiles == 0) continue;
+            const uint32_t halves = it.rows > 128 ? 2 : 1;
+            bool ok = true;
+            for (uint32_t r = 0; r < halves && ok; ++r) { ok = warp_wait(&sh.q_full[r], qph[r]); qph[r] ^= 1; }
+            if (!ok || !warp_wait(&sh.k_full[kst], kph)) break;
+            tcgen05_fence_after();
+            for (uint32_t r = 0; r < halves; ++r) scores(r);
+            if (lane == 0) umma_commit(&sh.k_empty[kst]);
+            kst ^= 1;
+            kph ^= kst == 0;
+            for (uint32_t i = 0; i < it.tiles && ok; ++i) {
+                const bool more = i + 1 < it.tiles;
+                if (!(ok = warp_wait(&sh.v_full[vst], vph))) break;
+                for (uint32_t r = 0; r < halves && ok; ++r) {
+                    if (!(ok = warp_wait(&sh.p_full[r], pph[r]))) break;
+                    pph[r] ^= 1;
+                    tcgen05_fence_after();
+                    if (lane == 0) {
+                        const uint64_t vb = umma_desc(smem_u32(vs + vst * C::KV), HD * 16, 128);
+#pragma unroll
+                        for (int k = 0; k < kPfKeys / 16; ++k)
+                            umma_f16_ts(tmem + 256 + r * 128, tmem + r * 128 + 8 * k, vb + k * (2 * HD), C::IDESC_O, i > 0 || k > 0);
+                        if (r + 1 == halves) umma_commit(&sh.v_empty[vst]);
+                        if (!more) umma_commit(&sh.o_full[r]);
+                    }
+                    if (more) {
+                        if (r == 0) {
+                            if (!(ok = warp_wait(&sh.k_full[kst], kph))) break;
+                            tcgen05_fence_after();
+                        }
+                        scores(r);
+                    }
+                }
+                if (!ok) break;
+                vst ^= 1;
+                vph ^= vst == 0;
+                if (more) {
+                    if (lane == 0) umma_commit(&sh.k_empty[kst]);
+                    kst ^= 1;
+                    kph ^= kst == 0;
+                }
+            }
+            if (!ok) break;
+        }
+        // all MMAs are complete before the tensor memory is given back
+        if (lane == 0) {
+            umma_commit(&sh.drain);
+            mbar_wait(&sh.drain, 0, nullptr);
+        }
+        __syncwarp();
+    }
+    tcgen05_fence_before();
+    __syncthreads();
+    tcgen05_fence_after();
+    if (warp == 13) tmem_dealloc(tmem, 512);
+}
+
+template <typename T, int HD>
+static cudaError_t prefill_go(const AttnParams& p, int sms, cudaStream_t s) {
+    static std::atomic<uint64_t> ready{0};  // devices whose attribute is set
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev >= 64 || !(ready.load(std::memory_order_relaxed) >> dev & 1)) {
+        e = cudaFuncSetAttribute(kv4_prefill_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, PfCfg<HD>::SMEM);
+        if (e != cudaSuccess) return e;
+        if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
+    }
+    g_launches.fetch_add(1, std::memory_order_relaxed);
+    kv4_prefill_kernel<T, HD><<<sms, kPfThreads, PfCfg<HD>::SMEM, s>>>(p);
+    return cudaGetLastError();
+}
+
+bool prefill_takes(int dtype, uint32_t head_dim) { return dtype != BT_F32 && head_dim <= 128; }
+
+cudaError_t launch_kv4_prefill(const AttnParams& p, int dtype, uint32_t head_dim, int sms, cudaStream_t s) {
+    if (dtype == BT_F16) return head_dim == 64 ? prefill_go<__half, 64>(p, sms, s) : prefill_go<__half, 128>(p, sms, s);
+    return head_dim == 64 ? prefill_go<__nv_bfloat16, 64>(p, sms, s) : prefill_go<__nv_bfloat16, 128>(p, sms, s);
+}
+
+}  // namespace bt
