@@ -17,8 +17,10 @@
 //                   P back into the same columns (half as wide, behind the reader)
 //   warps 8-11      unpack K and V tiles into two stages each
 //   warp 12         bulk copies of the packed rows
-//   warp 13         issues the MMAs: S of the next tile and one half's P V run while the
-//                   other half's softmax does
+//   warps 13, 14    issue the MMAs of a half each: S of the next tile and P V run while the
+//                   other half's softmax does (an issuing thread manages one MMA in about
+//                   150 cycles, so one thread for both halves would be the limit)
+// The warpgroups trade registers (setmaxnreg).
 // Tensor memory: S (or P) of the halves in columns 0 and 128, O in 256 and 384.
 //
 // A CTA is resident on an SM and takes blocks of rows in turn, those with the
@@ -31,7 +33,10 @@
 namespace bt {
 
 constexpr int kPfKeys = 128;     // keys of a tile
-constexpr int kPfThreads = 14 * 32;
+constexpr int kPfThreads = 4 * 128;  // softmax, softmax, unpacking, copies and MMAs
+// Registers a thread of each warpgroup: a softmax thread holds its whole row of S.
+constexpr int kPfSoftmax = 184, kPfUnpack = 88, kPfRest = 56;
+static_assert(2 * kPfSoftmax + kPfUnpack + kPfRest <= 4 * 128, "no more than the block is launched with");
 constexpr uint32_t kPfRaw = 3;   // packed K or V tiles in flight
 
 template <int HD>
@@ -46,18 +51,32 @@ struct PfCfg {
 struct PfShared {
     uint64_t raw_full[kPfRaw], raw_empty[kPfRaw];
     uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
-    uint64_t q_full[2], s_full[2], p_full[2], o_full[2], drain;
+    uint64_t q_full[2], s_full[2], p_full[2], o_full[2], drain[2];
     uint32_t pieces[8];  // of a tile: which of its 16-key pieces hold keys
     uint32_t tmem;
     volatile uint32_t dead;  // a wait gave up: everybody leaves
 };
 
-// tcgen05.mma with A in tensor memory
+// MMAs issued by one elected lane of a converged warp: A and B in shared memory, or A in
+// tensor memory.
+__device__ __forceinline__ void umma_f16_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n elect.sync _|q, 0xffffffff;\n"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
 __device__ __forceinline__ void umma_f16_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+        "{\n .reg .pred p, q;\n setp.ne.b32 p, %4, 0;\n elect.sync _|q, 0xffffffff;\n"
+        " @q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
         "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void umma_commit_one(uint64_t* bar) {
+    asm volatile(
+        "{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n"
+        " @q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(smem_u32(bar))
         : "memory");
 }
 
@@ -154,6 +173,16 @@ struct PfWalk {
     }
 };
 
+template <int N> __device__ __forceinline__ void take_registers() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void give_registers() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// Bits lo .. hi - 1 (clamped to 0 .. 32) of a word.
+__device__ __forceinline__ uint32_t bits_between(int32_t lo, int32_t hi) {
+    const uint32_t below_hi = hi <= 0 ? 0u : hi >= 32 ? 0xffffffffu : (1u << hi) - 1u;
+    const uint32_t below_lo = lo <= 0 ? 0u : lo >= 32 ? 0xffffffffu : (1u << lo) - 1u;
+    return below_hi & ~below_lo;
+}
+
 // code pairs of a word as exact fp16 integers: (w >> 4 i) & 15 in the low half, 4 codes further in the high half
 __device__ __forceinline__ __half2 code_pair(uint32_t w, int i) {
     const uint32_t x = i & 2 ? w >> 8 : w;
@@ -186,10 +215,9 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
     if (tid == 0) {
         for (uint32_t i = 0; i < kPfRaw; ++i) { mbar_init(&sh.raw_full[i], 1); mbar_init(&sh.raw_empty[i], 4); }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&sh.k_full[i], 4); mbar_init(&sh.k_empty[i], 1); mbar_init(&sh.v_full[i], 4); mbar_init(&sh.v_empty[i], 1);
-            mbar_init(&sh.q_full[i], 4); mbar_init(&sh.s_full[i], 1); mbar_init(&sh.p_full[i], 4); mbar_init(&sh.o_full[i], 1);
+            mbar_init(&sh.k_full[i], 4); mbar_init(&sh.k_empty[i], 2); mbar_init(&sh.v_full[i], 4); mbar_init(&sh.v_empty[i], 2);
+            mbar_init(&sh.q_full[i], 4); mbar_init(&sh.s_full[i], 1); mbar_init(&sh.p_full[i], 4); mbar_init(&sh.o_full[i], 1); mbar_init(&sh.drain[i], 1);
         }
-        mbar_init(&sh.drain, 1);
         sh.dead = 0;
         fence_mbar_init();
     }
@@ -219,6 +247,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
 
     if (warp < 8) {
         // ------------------------------------------------ softmax: a thread a row
+        take_registers<kPfSoftmax>();
         const uint32_t r = warp >> 2, row = (warp & 3) * 32 + lane;
         const uint32_t lanes = tmem + ((warp & 3) * 32u << 16), s_at = lanes + r * 128, o_at = lanes + 256 + r * 128;
         const float sign = p.scale_log2 < 0.0f ? -1.0f : 1.0f;
@@ -268,28 +297,30 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
                 s_phase ^= 1;
                 tcgen05_fence_after();
                 const uint32_t pieces = sh.pieces[(tile_no + i) & 7];
+                float s[128];
+                tmem_ld64(s_at, reinterpret_cast<uint32_t(&)[64]>(s[0]));
+                tmem_ld64(s_at + 64, reinterpret_cast<uint32_t(&)[64]>(s[64]));
                 // every row of the warp sees the whole tile
                 const bool plain = __all_sync(0xffffffffu, k0 + kPfKeys - 1 <= pos && (k0 > above || (uint32_t)(k0 + kPfKeys) <= p.sinks)) && pieces == 0xffu;
-                auto bar_unseen = [&](float (&s)[32], int32_t k) {
-                    if (plain) return;
+                tmem_wait_ld();
+                if (!plain) {
+                    const int32_t end = pos - k0 + 1, begin = above - k0 + 1;
+                    const int32_t sink_end = min(end, (int32_t)min(p.sinks, 0x7fffff00u) - k0);
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        const int32_t key = k + e;
-                        const bool in = key <= pos && (key > above || (uint32_t)key < p.sinks) && (pieces >> ((key - k0) >> 4) & 1);
-                        s[e] = in ? s[e] : -INFINITY;
+                    for (int h = 0; h < 4; ++h) {
+                        uint32_t in = bits_between(begin - 32 * h, end - 32 * h) | bits_between(0, sink_end - 32 * h);
+                        in &= (pieces >> (2 * h) & 1 ? 0xffffu : 0u) | (pieces >> (2 * h + 1) & 1 ? 0xffff0000u : 0u);
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) s[32 * h + e] = in >> e & 1 ? s[32 * h + e] : -INFINITY;
                     }
-                };
-                float top = -INFINITY;
-#pragma unroll
-                for (int h = 0; h < 4; ++h) {
-                    float s[32];
-                    tmem_ld32(s_at + 32 * h, reinterpret_cast<uint32_t(&)[32]>(s));
-                    tmem_wait_ld();
-                    bar_unseen(s, k0 + 32 * h);
-#pragma unroll
-                    for (int e = 0; e < 32; e += 2) top = fmaxf(top, fmaxf(s[e], s[e + 1]));
                 }
-                top *= f;
+                float top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int e = 0; e < 128; e += 8) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) top4[k] = fmaxf(top4[k], fmaxf(s[e + 2 * k], s[e + 2 * k + 1]));
+                }
+                const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * f;
                 if (__any_sync(0xffffffffu, top > m + kLazyMax)) {
                     const float now = fmaxf(m, top), fix = exp2_fast(m - now);
                     m = now;
@@ -306,26 +337,22 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
                         }
                     }
                 }
-                float2 sum = make_float2(0.0f, 0.0f);
+                float2 sum[2] = {};
                 const float2 ff = make_float2(f, f), mm = make_float2(-m, -m);
 #pragma unroll
                 for (int h = 0; h < 4; ++h) {
-                    float s[32];
-                    tmem_ld32(s_at + 32 * h, reinterpret_cast<uint32_t(&)[32]>(s));
-                    tmem_wait_ld();
-                    bar_unseen(s, k0 + 32 * h);
                     uint32_t v[16];
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
-                        float2 x = fma2(make_float2(s[2 * e], s[2 * e + 1]), ff, mm);
+                        float2 x = fma2(make_float2(s[32 * h + 2 * e], s[32 * h + 2 * e + 1]), ff, mm);
                         x.x = exp2_fast(x.x);
                         x.y = exp2_fast(x.y);
-                        sum = add2(sum, x);
+                        sum[e & 1] = add2(sum[e & 1], x);
                         v[e] = pack_half2(x.x, x.y);
                     }
-                    tmem_st16(s_at + 16 * h, v);  // behind the columns still to be read
+                    tmem_st16(s_at + 16 * h, v);
                 }
-                l += sum.x + sum.y;
+                l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                 tmem_wait_st();
                 tcgen05_fence_before();
                 __syncwarp();
@@ -357,6 +384,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
         }
     } else if (warp < 12) {
         // ------------------------------------------------ unpacking
+        give_registers<kPfUnpack>();
         const uint32_t u = tid - 256;  // 0 .. 127
         uint32_t raw_at = 0, raw_phase = 0, st = 0, st_phase = 1;
         for (uint64_t b = blockIdx.x; walk.find(p, b, lane, &it); b += gridDim.x) {
@@ -366,20 +394,20 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
                 // K: a thread a key
                 if (!(ok = warp_wait(&sh.raw_full[raw_at], raw_phase) && warp_wait(&sh.k_empty[st], st_phase))) break;
                 {
-                    const uint8_t* src = raw + raw_at * C::RAW + u * C::RB;
+                    const uint32_t* src = reinterpret_cast<const uint32_t*>(raw + raw_at * C::RAW + u * C::RB);
                     uint8_t* dst = ks + st * C::KV + u * 16;
+                    uint32_t w[CH], e[HD / 64];  // all loads before the stores
 #pragma unroll
-                    for (int j = 0; j < HD / 64; ++j) {
-                        const __half2 e = as_half2(reinterpret_cast<const uint32_t*>(src + HD / 2)[j]);
-                        const __half2 s = __low2half2(e), m = __high2half2(e);
+                    for (int k = 0; k < CH; ++k) w[k] = src[k];
 #pragma unroll
-                        for (int k = 8 * j; k < 8 * j + 8; ++k) {
-                            const uint32_t w = reinterpret_cast<const uint32_t*>(src)[k];
-                            uint4 v;
-                            v.x = as_u32(__hfma2(code_pair(w, 0), s, m)); v.y = as_u32(__hfma2(code_pair(w, 1), s, m));
-                            v.z = as_u32(__hfma2(code_pair(w, 2), s, m)); v.w = as_u32(__hfma2(code_pair(w, 3), s, m));
-                            *reinterpret_cast<uint4*>(dst + k * (kPfKeys * 16)) = v;
-                        }
+                    for (int j = 0; j < HD / 64; ++j) e[j] = src[CH + j];
+#pragma unroll
+                    for (int k = 0; k < CH; ++k) {
+                        const __half2 s = __low2half2(as_half2(e[k / 8])), m = __high2half2(as_half2(e[k / 8]));
+                        uint4 v;
+                        v.x = as_u32(__hfma2(code_pair(w[k], 0), s, m)); v.y = as_u32(__hfma2(code_pair(w[k], 1), s, m));
+                        v.z = as_u32(__hfma2(code_pair(w[k], 2), s, m)); v.w = as_u32(__hfma2(code_pair(w[k], 3), s, m));
+                        *reinterpret_cast<uint4*>(dst + k * (kPfKeys * 16)) = v;
                     }
                 }
                 fence_proxy_async();
@@ -389,7 +417,16 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
                 // V: a thread 8 keys x 8 elements at a time
                 if (!(ok = warp_wait(&sh.raw_full[raw_at], raw_phase) && warp_wait(&sh.v_empty[st], st_phase))) break;
                 {
+                    // what no row sees may hold anything: its pairs become zero
                     const uint32_t pieces = sh.pieces[(tile_no + i) & 7];
+                    if (pieces != 0xffu || k0 + kPfKeys - 1 > it.top || (k0 <= it.above && (uint32_t)(k0 + kPfKeys) > p.sinks)) {
+                        if (!(pieces >> (u >> 4) & 1) || !it.any(k0 + (int32_t)u, 1, p.sinks)) {
+                            uint32_t* e = reinterpret_cast<uint32_t*>(raw + raw_at * C::RAW + u * C::RB + HD / 2);
+#pragma unroll
+                            for (int j = 0; j < HD / 64; ++j) e[j] = 0;
+                        }
+                        asm volatile("bar.sync 1, 128;" ::: "memory");
+                    }
 #pragma unroll 1
                     for (uint32_t x = u; x < 16 * CH; x += 128) {
                         const uint32_t oct = x / CH, chunk = x % CH;
@@ -400,11 +437,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
                         for (int q = 0; q < 4; ++q) {  // keys 2q, 2q + 1 of the eight
                             const uint8_t *a = src + 2 * q * C::RB, *c = a + C::RB;
                             const uint32_t wa = reinterpret_cast<const uint32_t*>(a)[chunk], wc = reinterpret_cast<const uint32_t*>(c)[chunk];
-                            const int32_t key = k0 + (int32_t)(oct * 8) + 2 * q;
-                            const bool got = pieces >> (oct >> 1) & 1;
-                            // what no row sees may hold anything: its values become zero
-                            const uint32_t ea = got && it.any(key, 1, p.sinks) ? reinterpret_cast<const uint32_t*>(a + HD / 2)[chunk / 8] : 0u;
-                            const uint32_t ec = got && it.any(key + 1, 1, p.sinks) ? reinterpret_cast<const uint32_t*>(c + HD / 2)[chunk / 8] : 0u;
+                            const uint32_t ea = reinterpret_cast<const uint32_t*>(a + HD / 2)[chunk / 8], ec = reinterpret_cast<const uint32_t*>(c + HD / 2)[chunk / 8];
                             const __half2 s = as_half2(__byte_perm(ea, ec, 0x5410)), m = as_half2(__byte_perm(ea, ec, 0x7632));
                             const uint32_t lo = __byte_perm(wa, wc, 0x5410), hi = __byte_perm(wa, wc, 0x7632);
 #pragma unroll
@@ -427,7 +460,9 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
             if (!ok) break;
             tile_no += it.tiles;
         }
-    } else if (warp == 12) {
+    } else {
+    give_registers<kPfRest>();
+    if (warp == 12) {
         // ------------------------------------------------ packed rows
         uint32_t at = 0, phase = 1, sent = 0;
         if (blockIdx.x == 0) {
@@ -466,68 +501,69 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
         }
         // every copy has arrived before the CTA may end (a wait may have given up on one)
         for (uint32_t k = sent > kPfRaw ? sent - kPfRaw : 0; k < sent; ++k) mbar_wait(&sh.raw_full[k % kPfRaw], (k / kPfRaw) & 1, nullptr);
-    } else {
-        // ------------------------------------------------ MMAs (one thread issues; the warp walks along)
-        uint32_t kst = 0, kph = 0, vst = 0, vph = 0, qph[2] = {0, 0}, pph[2] = {0, 0};
-        auto scores = [&](uint32_t r) {
-            if (lane == 0) {
-                const uint64_t a = umma_desc(smem_u32(qs + r * C::Q), 128 * 16, 128), kb = umma_desc(smem_u32(ks + kst * C::KV), kPfKeys * 16, 128);
+    } else if (warp < 15) {
+        // ------------------------------------------------ MMAs of a half
+        const uint32_t r = warp - 13;
+        uint32_t kst = 0, kph = 0, vst = 0, vph = 0, qph = 0, pph = 0;
+        const uint64_t qa = umma_desc(smem_u32(qs + r * C::Q), 128 * 16, 128);
+        const uint64_t ka = umma_desc(smem_u32(ks), kPfKeys * 16, 128), va = umma_desc(smem_u32(vs), HD * 16, 128);
+        auto scores = [&] {  // S of the next tile; its keys may then go, as far as this half is concerned
+            const uint64_t kb = ka + kst * (C::KV / 16);
 #pragma unroll
-                for (int k = 0; k < HD / 16; ++k) umma_f16(tmem + r * 128, a + k * 256, kb + k * (2 * kPfKeys), C::IDESC_S, k > 0);
-                umma_commit(&sh.s_full[r]);
-            }
-        };
-        for (uint64_t b = blockIdx.x; walk.find(p, b, lane, &it); b += gridDim.x) {
-            if (it.tiles == 0) continue;
-            const uint32_t halves = it.rows > 128 ? 2 : 1;
-            bool ok = true;
-            for (uint32_t r = 0; r < halves && ok; ++r) { ok = warp_wait(&sh.q_full[r], qph[r]); qph[r] ^= 1; }
-            if (!ok || !warp_wait(&sh.k_full[kst], kph)) break;
-            tcgen05_fence_after();
-            for (uint32_t r = 0; r < halves; ++r) scores(r);
-            if (lane == 0) umma_commit(&sh.k_empty[kst]);
+            for (int k = 0; k < HD / 16; ++k) umma_f16_ss(tmem + r * 128, qa + k * 256, kb + k * (2 * kPfKeys), C::IDESC_S, k > 0);
+            umma_commit_one(&sh.s_full[r]);
+            umma_commit_one(&sh.k_empty[kst]);
             kst ^= 1;
             kph ^= kst == 0;
-            for (uint32_t i = 0; i < it.tiles && ok; ++i) {
-                const bool more = i + 1 < it.tiles;
-                if (!(ok = warp_wait(&sh.v_full[vst], vph))) break;
-                for (uint32_t r = 0; r < halves && ok; ++r) {
-                    if (!(ok = warp_wait(&sh.p_full[r], pph[r]))) break;
-                    pph[r] ^= 1;
-                    tcgen05_fence_after();
-                    if (lane == 0) {
-                        const uint64_t vb = umma_desc(smem_u32(vs + vst * C::KV), HD * 16, 128);
-#pragma unroll
-                        for (int k = 0; k < kPfKeys / 16; ++k)
-                            umma_f16_ts(tmem + 256 + r * 128, tmem + r * 128 + 8 * k, vb + k * (2 * HD), C::IDESC_O, i > 0 || k > 0);
-                        if (r + 1 == halves) umma_commit(&sh.v_empty[vst]);
-                        if (!more) umma_commit(&sh.o_full[r]);
-                    }
-                    if (more) {
-                        if (r == 0) {
-                            if (!(ok = warp_wait(&sh.k_full[kst], kph))) break;
-                            tcgen05_fence_after();
-                        }
-                        scores(r);
-                    }
-                }
-                if (!ok) break;
-                vst ^= 1;
-                vph ^= vst == 0;
-                if (more) {
-                    if (lane == 0) umma_commit(&sh.k_empty[kst]);
+        };
+        for (uint64_t b = blockIdx.x; walk.find(p, b, lane, &it); b += gridDim.x) {
+            bool ok = true;
+            if (it.rows <= r * 128) {  // nothing in this half: the tiles pass by
+                for (uint32_t i = 0; i < it.tiles && ok; ++i) {
+                    if (!(ok = warp_wait(&sh.k_full[kst], kph))) break;
+                    if (lane == 0) mbar_arrive(&sh.k_empty[kst]);
                     kst ^= 1;
                     kph ^= kst == 0;
+                    if (!(ok = warp_wait(&sh.v_full[vst], vph))) break;
+                    if (lane == 0) mbar_arrive(&sh.v_empty[vst]);
+                    vst ^= 1;
+                    vph ^= vst == 0;
+                }
+                if (!ok) break;
+                continue;
+            }
+            if (it.tiles == 0) continue;
+            if (!warp_wait(&sh.q_full[r], qph) || !warp_wait(&sh.k_full[kst], kph)) break;
+            qph ^= 1;
+            tcgen05_fence_after();
+            scores();
+            for (uint32_t i = 0; i < it.tiles; ++i) {
+                const bool more = i + 1 < it.tiles;
+                if (!(ok = warp_wait(&sh.v_full[vst], vph) && warp_wait(&sh.p_full[r], pph))) break;
+                pph ^= 1;
+                tcgen05_fence_after();
+                const uint64_t vb = va + vst * (C::KV / 16);
+#pragma unroll
+                for (int k = 0; k < kPfKeys / 16; ++k)
+                    umma_f16_ts(tmem + 256 + r * 128, tmem + r * 128 + 8 * k, vb + k * (2 * HD), C::IDESC_O, i > 0 || k > 0);
+                umma_commit_one(&sh.v_empty[vst]);
+                vst ^= 1;
+                vph ^= vst == 0;
+                if (more) {  // (in order after P V: S may overwrite P)
+                    if (!(ok = warp_wait(&sh.k_full[kst], kph))) break;
+                    tcgen05_fence_after();
+                    scores();
+                } else {
+                    umma_commit_one(&sh.o_full[r]);
                 }
             }
             if (!ok) break;
         }
         // all MMAs are complete before the tensor memory is given back
-        if (lane == 0) {
-            umma_commit(&sh.drain);
-            mbar_wait(&sh.drain, 0, nullptr);
-        }
+        umma_commit_one(&sh.drain[r]);
+        mbar_wait(&sh.drain[r], 0, nullptr);
         __syncwarp();
+    }
     }
     tcgen05_fence_before();
     __syncthreads();
