@@ -1,27 +1,27 @@
 // bt_kv4_prefill.cu -- causal attention of many query rows over a 4-bit cache
 // (the chunks of bt_cuda_kv4_attention) on tcgen05 tensor cores.
 //
-// Mathematics.  256 (query, head) rows that share a KV head go over 128-key tiles
-// with the running maximum and sum of a softmax:
+// Mathematics.  256 (query, head) rows that share a KV head go over 64-key tiles with
+// the running maximum and sum of a softmax:
 //   S = Q K^T,  P = exp2(f S - m),  O += P V,  l += sum P,  out = O / l.
 // A tile's keys and values are unpacked once into fp16 operands in shared memory
 // (scale * code + min, one rounding of 2^-12 rms) and serve both 128-row halves.
 // Queries enter scaled by a power of two per row, exact for bf16 and fp16; P is
 // rounded to fp16 (2^-12 rms); sums, maxima and O are fp32.
 //
-// Bound: at head_dim 128 a tile is 2048 tensor cycles (4 MMA blocks of 128 x 128 x
-// 128), 2048 cycles of the exponential unit (256 x 128) and about 1500 issue slots
-// a scheduler for softmax and unpacking, so the three run side by side in warps of
-// their own:
-//   warps 0-3, 4-7  softmax of a row half each, a thread a row: S from tensor memory,
-//                   P back into the same columns (half as wide, behind the reader)
-//   warps 8-11      unpack K and V tiles into two stages each
-//   warp 12         bulk copies of the packed rows
-//   warps 13, 14    issue the MMAs of a half each: S of the next tile and P V run while the
-//                   other half's softmax does (an issuing thread manages one MMA in about
-//                   150 cycles, so one thread for both halves would be the limit)
-// The warpgroups trade registers (setmaxnreg).
-// Tensor memory: S (or P) of the halves in columns 0 and 128, O in 256 and 384.
+// Bound: at head_dim 128, 128 keys are 2048 tensor cycles (both halves' S and P V),
+// 2048 cycles of the exponential unit (256 x 128) and about 1500 issue slots a scheduler
+// for softmax and unpacking, so the three run side by side in warpgroups of their own,
+// which trade registers (setmaxnreg):
+//   0, 1   softmax of a row half each, a thread a row: S from tensor memory, P back into
+//          the same columns (half as wide, behind the reader)
+//   2, 3   unpack the K and the V tiles, into four stages each
+//   4      warp 0: bulk copies of the packed rows; warps 1, 2: issue the MMAs of a half
+//          each (an issuing thread manages one MMA in about 100 cycles, so one thread
+//          for both halves would be the limit)
+// Each half has two S buffers, so its softmax works on a tile while the tensor cores
+// make the next one's S and add the previous one's P V.  Tensor memory: the S (or P)
+// buffers of the halves in columns 0 and 128, O in 256 and 384.
 //
 // A CTA is resident on an SM and takes blocks of rows in turn, those with the
 // longest keys first.  V's rows (the N of P V) are stored in the order e, chunk of
@@ -32,27 +32,28 @@
 
 namespace bt {
 
-constexpr int kPfKeys = 128;     // keys of a tile
-constexpr int kPfThreads = 4 * 128;  // softmax, softmax, unpacking, copies and MMAs
-// Registers a thread of each warpgroup: a softmax thread holds its whole row of S.
-constexpr int kPfSoftmax = 184, kPfUnpack = 88, kPfRest = 56;
-static_assert(2 * kPfSoftmax + kPfUnpack + kPfRest <= 4 * 128, "no more than the block is launched with");
-constexpr uint32_t kPfRaw = 3;   // packed K or V tiles in flight
+constexpr int kPfKeys = 64;      // keys of a tile
+constexpr int kPfThreads = 5 * 128;
+// Registers a thread of each warpgroup, of the 96 at launch.
+constexpr int kPfSoftmax = 128, kPfUnpack = 80, kPfRest = 56;
+static_assert(2 * kPfSoftmax + 2 * kPfUnpack + kPfRest <= 5 * 96, "no more than the block is launched with");
+constexpr uint32_t kPfRaw = 3;     // packed K (and V) tiles in flight
+constexpr uint32_t kPfStages = 4;  // unpacked K (and V) tiles
 
 template <int HD>
 struct PfCfg {
     static constexpr uint32_t RB = kv4_row_bytes(HD), RAW = kPfKeys * RB;
     static constexpr uint32_t Q = 128 * HD * 2, KV = kPfKeys * HD * 2;  // bytes of an operand tile
-    static constexpr uint32_t SMEM = 2 * Q + 4 * KV + kPfRaw * RAW;
+    static constexpr uint32_t SMEM = 2 * Q + 2 * kPfStages * KV + 2 * kPfRaw * RAW;
     static constexpr uint32_t IDESC_S = (1u << 4) | ((kPfKeys >> 3) << 17) | ((128u >> 4) << 24);  // f16 x f16 -> f32
     static constexpr uint32_t IDESC_O = (1u << 4) | ((HD >> 3) << 17) | ((128u >> 4) << 24);
 };
 
 struct PfShared {
-    uint64_t raw_full[kPfRaw], raw_empty[kPfRaw];
-    uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
-    uint64_t q_full[2], s_full[2], p_full[2], o_full[2], drain[2];
-    uint32_t pieces[8];  // of a tile: which of its 16-key pieces hold keys
+    uint64_t raw_full[2][kPfRaw], raw_empty[2][kPfRaw];        // of K, of V
+    uint64_t full[2][kPfStages], empty[2][kPfStages];
+    uint64_t q_full[2], s_full[2][2], p_full[2][2], pv_done[2], o_full[2], drain[2];  // of the halves
+    uint32_t pieces[16];  // of a tile: which of its 16-key pieces hold keys
     uint32_t tmem;
     volatile uint32_t dead;  // a wait gave up: everybody leaves
 };
@@ -204,19 +205,19 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
     __shared__ PfShared sh;
     const uint32_t tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     uint8_t* qs = dyn;
-    uint8_t* ks = dyn + 2 * C::Q;
-    uint8_t* vs = ks + 2 * C::KV;
-    uint8_t* raw = vs + 2 * C::KV;
+    uint8_t* kvs = dyn + 2 * C::Q;                       // stages of K, then of V
+    uint8_t* raws = kvs + 2 * kPfStages * C::KV;
 
-    if (warp == 13) {
+    if (warp == 16) {
         tmem_alloc(&sh.tmem, 512);
         tmem_relinquish();
     }
     if (tid == 0) {
-        for (uint32_t i = 0; i < kPfRaw; ++i) { mbar_init(&sh.raw_full[i], 1); mbar_init(&sh.raw_empty[i], 4); }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&sh.k_full[i], 4); mbar_init(&sh.k_empty[i], 2); mbar_init(&sh.v_full[i], 4); mbar_init(&sh.v_empty[i], 2);
-            mbar_init(&sh.q_full[i], 4); mbar_init(&sh.s_full[i], 1); mbar_init(&sh.p_full[i], 4); mbar_init(&sh.o_full[i], 1); mbar_init(&sh.drain[i], 1);
+            for (uint32_t k = 0; k < kPfRaw; ++k) { mbar_init(&sh.raw_full[i][k], 1); mbar_init(&sh.raw_empty[i][k], 4); }
+            for (uint32_t k = 0; k < kPfStages; ++k) { mbar_init(&sh.full[i][k], 4); mbar_init(&sh.empty[i][k], 2); }
+            for (int k = 0; k < 2; ++k) { mbar_init(&sh.s_full[i][k], 1); mbar_init(&sh.p_full[i][k], 4); }
+            mbar_init(&sh.q_full[i], 4); mbar_init(&sh.pv_done[i], 1); mbar_init(&sh.o_full[i], 1); mbar_init(&sh.drain[i], 1);
         }
         sh.dead = 0;
         fence_mbar_init();
@@ -249,9 +250,9 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
         // ------------------------------------------------ softmax: a thread a row
         take_registers<kPfSoftmax>();
         const uint32_t r = warp >> 2, row = (warp & 3) * 32 + lane;
-        const uint32_t lanes = tmem + ((warp & 3) * 32u << 16), s_at = lanes + r * 128, o_at = lanes + 256 + r * 128;
+        const uint32_t lanes = tmem + ((warp & 3) * 32u << 16), o_at = lanes + 256 + r * 128;
         const float sign = p.scale_log2 < 0.0f ? -1.0f : 1.0f;
-        uint32_t s_phase = 0, o_phase = 0;
+        uint32_t done = 0, o_phase = 0;  // tiles this half has done
         for (uint64_t b = blockIdx.x; walk.find(p, b, lane, &it); b += gridDim.x) {
             if (it.rows <= r * 128) { tile_no += it.tiles; continue; }
             const bool there = r * 128 + row < it.rows;
@@ -293,21 +294,20 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
             bool ok = true;
             for (uint32_t i = 0; i < it.tiles; ++i) {
                 const int32_t k0 = it.key0(i);
-                if (!(ok = warp_wait(&sh.s_full[r], s_phase))) break;
-                s_phase ^= 1;
+                const uint32_t buf = done & 1, s_at = lanes + r * 128 + buf * 64;
+                if (!(ok = warp_wait(&sh.s_full[r][buf], done >> 1 & 1))) break;
                 tcgen05_fence_after();
-                const uint32_t pieces = sh.pieces[(tile_no + i) & 7];
-                float s[128];
-                tmem_ld64(s_at, reinterpret_cast<uint32_t(&)[64]>(s[0]));
-                tmem_ld64(s_at + 64, reinterpret_cast<uint32_t(&)[64]>(s[64]));
+                const uint32_t pieces = sh.pieces[(tile_no + i) & 15];
+                float s[64];
+                tmem_ld64(s_at, reinterpret_cast<uint32_t(&)[64]>(s));
                 // every row of the warp sees the whole tile
-                const bool plain = __all_sync(0xffffffffu, k0 + kPfKeys - 1 <= pos && (k0 > above || (uint32_t)(k0 + kPfKeys) <= p.sinks)) && pieces == 0xffu;
+                const bool plain = __all_sync(0xffffffffu, k0 + kPfKeys - 1 <= pos && (k0 > above || (uint32_t)(k0 + kPfKeys) <= p.sinks)) && pieces == 0xfu;
                 tmem_wait_ld();
                 if (!plain) {
                     const int32_t end = pos - k0 + 1, begin = above - k0 + 1;
                     const int32_t sink_end = min(end, (int32_t)min(p.sinks, 0x7fffff00u) - k0);
 #pragma unroll
-                    for (int h = 0; h < 4; ++h) {
+                    for (int h = 0; h < 2; ++h) {
                         uint32_t in = bits_between(begin - 32 * h, end - 32 * h) | bits_between(0, sink_end - 32 * h);
                         in &= (pieces >> (2 * h) & 1 ? 0xffffu : 0u) | (pieces >> (2 * h + 1) & 1 ? 0xffff0000u : 0u);
 #pragma unroll
@@ -316,7 +316,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
                 }
                 float top4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                for (int e = 0; e < 128; e += 8) {
+                for (int e = 0; e < 64; e += 8) {
 #pragma unroll
                     for (int k = 0; k < 4; ++k) top4[k] = fmaxf(top4[k], fmaxf(s[e + 2 * k], s[e + 2 * k + 1]));
                 }
@@ -325,7 +325,9 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
                     const float now = fmaxf(m, top), fix = exp2_fast(m - now);
                     m = now;
                     l *= fix;
-                    if (i > 0) {  // the products of the tiles so far are complete: this tile's S came after them
+                    if (i > 0) {  // once the products of the tiles so far are complete
+                        if (!(ok = warp_wait(&sh.pv_done[r], (done - 1) & 1))) break;
+                        tcgen05_fence_after();
 #pragma unroll 1
                         for (int h = 0; h < HD / 16; ++h) {
                             uint32_t o[16];
@@ -340,7 +342,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
                 float2 sum[2] = {};
                 const float2 ff = make_float2(f, f), mm = make_float2(-m, -m);
 #pragma unroll
-                for (int h = 0; h < 4; ++h) {
+                for (int h = 0; h < 2; ++h) {
                     uint32_t v[16];
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
@@ -356,7 +358,8 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
                 tmem_wait_st();
                 tcgen05_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&sh.p_full[r]);
+                if (lane == 0) mbar_arrive(&sh.p_full[r][buf]);
+                ++done;
             }
             if (!ok) break;
             tile_no += it.tiles;
@@ -382,56 +385,51 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
             }
             tcgen05_fence_before();
         }
-    } else if (warp < 12) {
-        // ------------------------------------------------ unpacking
+    } else if (warp < 16) {
+        // ------------------------------------------------ unpacking, of K or of V
         give_registers<kPfUnpack>();
-        const uint32_t u = tid - 256;  // 0 .. 127
+        const uint32_t u = tid & 127, side = warp < 12 ? 0 : 1;
+        uint8_t* raw = raws + side * kPfRaw * C::RAW;
+        uint8_t* to = kvs + side * kPfStages * C::KV;
         uint32_t raw_at = 0, raw_phase = 0, st = 0, st_phase = 1;
         for (uint64_t b = blockIdx.x; walk.find(p, b, lane, &it); b += gridDim.x) {
             bool ok = true;
-            for (uint32_t i = 0; i < it.tiles && ok; ++i) {
-                const int32_t k0 = it.key0(i);
-                // K: a thread a key
-                if (!(ok = warp_wait(&sh.raw_full[raw_at], raw_phase) && warp_wait(&sh.k_empty[st], st_phase))) break;
-                {
-                    const uint32_t* src = reinterpret_cast<const uint32_t*>(raw + raw_at * C::RAW + u * C::RB);
-                    uint8_t* dst = ks + st * C::KV + u * 16;
-                    uint32_t w[CH], e[HD / 64];  // all loads before the stores
+            for (uint32_t i = 0; i < it.tiles; ++i) {
+                if (!(ok = warp_wait(&sh.raw_full[side][raw_at], raw_phase) && warp_wait(&sh.empty[side][st], st_phase))) break;
+                if (side == 0) {
+                    // a thread half a key
+                    const uint32_t key = u & 63, k0 = (u >> 6) * (CH / 2);
+                    const uint32_t* src = reinterpret_cast<const uint32_t*>(raw + raw_at * C::RAW + key * C::RB);
+                    uint8_t* dst = to + st * C::KV + key * 16 + k0 * (kPfKeys * 16);
+                    uint32_t w[CH / 2];  // all loads before the stores
 #pragma unroll
-                    for (int k = 0; k < CH; ++k) w[k] = src[k];
+                    for (int k = 0; k < CH / 2; ++k) w[k] = src[k0 + k];
+                    const __half2 e = as_half2(src[CH + (HD == 128 ? u >> 6 : 0)]);  // (half a key: one group at most)
+                    const __half2 s = __low2half2(e), m = __high2half2(e);
 #pragma unroll
-                    for (int j = 0; j < HD / 64; ++j) e[j] = src[CH + j];
-#pragma unroll
-                    for (int k = 0; k < CH; ++k) {
-                        const __half2 s = __low2half2(as_half2(e[k / 8])), m = __high2half2(as_half2(e[k / 8]));
+                    for (int k = 0; k < CH / 2; ++k) {
                         uint4 v;
                         v.x = as_u32(__hfma2(code_pair(w[k], 0), s, m)); v.y = as_u32(__hfma2(code_pair(w[k], 1), s, m));
                         v.z = as_u32(__hfma2(code_pair(w[k], 2), s, m)); v.w = as_u32(__hfma2(code_pair(w[k], 3), s, m));
                         *reinterpret_cast<uint4*>(dst + k * (kPfKeys * 16)) = v;
                     }
-                }
-                fence_proxy_async();
-                __syncwarp();
-                if (lane == 0) { mbar_arrive(&sh.k_full[st]); mbar_arrive(&sh.raw_empty[raw_at]); }
-                if (++raw_at == kPfRaw) { raw_at = 0; raw_phase ^= 1; }
-                // V: a thread 8 keys x 8 elements at a time
-                if (!(ok = warp_wait(&sh.raw_full[raw_at], raw_phase) && warp_wait(&sh.v_empty[st], st_phase))) break;
-                {
+                } else {
                     // what no row sees may hold anything: its pairs become zero
-                    const uint32_t pieces = sh.pieces[(tile_no + i) & 7];
-                    if (pieces != 0xffu || k0 + kPfKeys - 1 > it.top || (k0 <= it.above && (uint32_t)(k0 + kPfKeys) > p.sinks)) {
-                        if (!(pieces >> (u >> 4) & 1) || !it.any(k0 + (int32_t)u, 1, p.sinks)) {
+                    const int32_t k0 = it.key0(i);
+                    const uint32_t pieces = sh.pieces[(tile_no + i) & 15];
+                    if (pieces != 0xfu || k0 + kPfKeys - 1 > it.top || (k0 <= it.above && (uint32_t)(k0 + kPfKeys) > p.sinks)) {
+                        if (u < kPfKeys && (!(pieces >> (u >> 4) & 1) || !it.any(k0 + (int32_t)u, 1, p.sinks))) {
                             uint32_t* e = reinterpret_cast<uint32_t*>(raw + raw_at * C::RAW + u * C::RB + HD / 2);
 #pragma unroll
                             for (int j = 0; j < HD / 64; ++j) e[j] = 0;
                         }
                         asm volatile("bar.sync 1, 128;" ::: "memory");
                     }
-#pragma unroll 1
-                    for (uint32_t x = u; x < 16 * CH; x += 128) {
-                        const uint32_t oct = x / CH, chunk = x % CH;
+                    // a thread 8 keys x 8 elements
+                    const uint32_t oct = u / CH, chunk = u % CH;
+                    if (oct < kPfKeys / 8) {
                         const uint8_t* src = raw + raw_at * C::RAW + oct * 8 * C::RB;
-                        uint8_t* dst = vs + st * C::KV + oct * (HD * 16) + chunk * 16;
+                        uint8_t* dst = to + st * C::KV + oct * (HD * 16) + chunk * 16;
                         uint32_t o[8][4];
 #pragma unroll
                         for (int q = 0; q < 4; ++q) {  // keys 2q, 2q + 1 of the eight
@@ -452,17 +450,16 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
                 }
                 fence_proxy_async();
                 __syncwarp();
-                if (lane == 0) { mbar_arrive(&sh.v_full[st]); mbar_arrive(&sh.raw_empty[raw_at]); }
+                if (lane == 0) { mbar_arrive(&sh.full[side][st]); mbar_arrive(&sh.raw_empty[side][raw_at]); }
                 if (++raw_at == kPfRaw) { raw_at = 0; raw_phase ^= 1; }
-                st ^= 1;
-                st_phase ^= st == 0;
+                if (++st == kPfStages) { st = 0; st_phase ^= 1; }
             }
             if (!ok) break;
             tile_no += it.tiles;
         }
     } else {
     give_registers<kPfRest>();
-    if (warp == 12) {
+    if (warp == 16) {
         // ------------------------------------------------ packed rows
         uint32_t at = 0, phase = 1, sent = 0;
         if (blockIdx.x == 0) {
@@ -470,92 +467,92 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
         }
         for (uint64_t b = blockIdx.x; walk.find(p, b, lane, &it); b += gridDim.x) {
             bool ok = true;
-            for (uint32_t i = 0; i < it.tiles && ok; ++i) {
-                const int32_t k0 = it.key0(i), key = k0 + 16 * (int32_t)lane;
-                const bool live = lane < 8 && it.any(key, 16, p.sinks);
+            for (uint32_t i = 0; i < it.tiles; ++i) {
+                const int32_t key = it.key0(i) + 16 * (int32_t)lane;
+                const bool live = lane < kPfKeys / 16 && it.any(key, 16, p.sinks);
                 const int64_t row = live ? p.map.row(it.w.slot, it.head, key) : -1;
                 if (live && row < 0) p.map.flag(BT_KV4_RANGE);
                 const uint32_t pieces = __ballot_sync(0xffffffffu, row >= 0);
                 // one copy where the whole tile lies together
-                const bool joined = pieces == 0xffu && p.map.shift >= 7;
-                for (int side = 0; side < 2 && ok; ++side) {
-                    if (!(ok = warp_wait(&sh.raw_empty[at], phase))) break;
-                    if (lane == 0) {
-                        if (side == 0) sh.pieces[(tile_no + i) & 7] = pieces;
-                        mbar_expect_tx(&sh.raw_full[at], __popc(pieces) * 16 * C::RB);
-                    }
-                    __syncwarp();
-                    const uint8_t* src = side ? p.map.v : p.map.k;
-                    uint8_t* dst = raw + at * C::RAW;
-                    if (joined) {
-                        if (lane == 0) bulk_g2s(dst, src + (size_t)row * C::RB, C::RAW, &sh.raw_full[at]);
-                    } else if (row >= 0) {
-                        bulk_g2s(dst + lane * 16 * C::RB, src + (size_t)row * C::RB, 16 * C::RB, &sh.raw_full[at]);
-                    }
-                    ++sent;
-                    if (++at == kPfRaw) { at = 0; phase ^= 1; }
+                const bool joined = pieces == 0xfu && p.map.shift >= 6;
+                if (!(ok = warp_wait(&sh.raw_empty[0][at], phase) && warp_wait(&sh.raw_empty[1][at], phase))) break;
+                if (lane == 0) {
+                    sh.pieces[(tile_no + i) & 15] = pieces;
+                    mbar_expect_tx(&sh.raw_full[0][at], __popc(pieces) * 16 * C::RB);
+                    mbar_expect_tx(&sh.raw_full[1][at], __popc(pieces) * 16 * C::RB);
                 }
+                __syncwarp();
+                if (row >= 0 && (lane == 0 || !joined)) {
+                    const uint32_t bytes = joined ? C::RAW : 16 * C::RB;
+                    uint8_t* dst = raws + at * C::RAW + lane * 16 * C::RB;
+                    bulk_g2s(dst, p.map.k + (size_t)row * C::RB, bytes, &sh.raw_full[0][at]);
+                    bulk_g2s(dst + kPfRaw * C::RAW, p.map.v + (size_t)row * C::RB, bytes, &sh.raw_full[1][at]);
+                }
+                ++sent;
+                if (++at == kPfRaw) { at = 0; phase ^= 1; }
             }
             if (!ok) break;
             tile_no += it.tiles;
         }
         // every copy has arrived before the CTA may end (a wait may have given up on one)
-        for (uint32_t k = sent > kPfRaw ? sent - kPfRaw : 0; k < sent; ++k) mbar_wait(&sh.raw_full[k % kPfRaw], (k / kPfRaw) & 1, nullptr);
-    } else if (warp < 15) {
+        for (uint32_t k = sent > kPfRaw ? sent - kPfRaw : 0; k < sent; ++k) {
+            mbar_wait(&sh.raw_full[0][k % kPfRaw], k / kPfRaw & 1, nullptr);
+            mbar_wait(&sh.raw_full[1][k % kPfRaw], k / kPfRaw & 1, nullptr);
+        }
+    } else if (warp < 19) {
         // ------------------------------------------------ MMAs of a half
-        const uint32_t r = warp - 13;
-        uint32_t kst = 0, kph = 0, vst = 0, vph = 0, qph = 0, pph = 0;
+        const uint32_t r = warp - 17;
+        uint32_t kst = 0, kph = 0, vst = 0, vph = 0, qph = 0, made = 0, done = 0;  // tiles with S, with P V
+        auto next_k = [&] { if (++kst == kPfStages) { kst = 0; kph ^= 1; } };
+        auto next_v = [&] { if (++vst == kPfStages) { vst = 0; vph ^= 1; } };
         const uint64_t qa = umma_desc(smem_u32(qs + r * C::Q), 128 * 16, 128);
-        const uint64_t ka = umma_desc(smem_u32(ks), kPfKeys * 16, 128), va = umma_desc(smem_u32(vs), HD * 16, 128);
+        const uint64_t ka = umma_desc(smem_u32(kvs), kPfKeys * 16, 128), va = umma_desc(smem_u32(kvs + kPfStages * C::KV), HD * 16, 128);
         auto scores = [&] {  // S of the next tile; its keys may then go, as far as this half is concerned
+            if (!warp_wait(&sh.full[0][kst], kph)) return false;
+            tcgen05_fence_after();
             const uint64_t kb = ka + kst * (C::KV / 16);
 #pragma unroll
-            for (int k = 0; k < HD / 16; ++k) umma_f16_ss(tmem + r * 128, qa + k * 256, kb + k * (2 * kPfKeys), C::IDESC_S, k > 0);
-            umma_commit_one(&sh.s_full[r]);
-            umma_commit_one(&sh.k_empty[kst]);
-            kst ^= 1;
-            kph ^= kst == 0;
+            for (int k = 0; k < HD / 16; ++k)
+                umma_f16_ss(tmem + r * 128 + (made & 1) * 64, qa + k * 256, kb + k * (2 * kPfKeys), C::IDESC_S, k > 0);
+            umma_commit_one(&sh.s_full[r][made & 1]);
+            umma_commit_one(&sh.empty[0][kst]);
+            next_k();
+            ++made;
+            return true;
         };
         for (uint64_t b = blockIdx.x; walk.find(p, b, lane, &it); b += gridDim.x) {
             bool ok = true;
             if (it.rows <= r * 128) {  // nothing in this half: the tiles pass by
-                for (uint32_t i = 0; i < it.tiles && ok; ++i) {
-                    if (!(ok = warp_wait(&sh.k_full[kst], kph))) break;
-                    if (lane == 0) mbar_arrive(&sh.k_empty[kst]);
-                    kst ^= 1;
-                    kph ^= kst == 0;
-                    if (!(ok = warp_wait(&sh.v_full[vst], vph))) break;
-                    if (lane == 0) mbar_arrive(&sh.v_empty[vst]);
-                    vst ^= 1;
-                    vph ^= vst == 0;
+                for (uint32_t i = 0; i < it.tiles; ++i) {
+                    if (!(ok = warp_wait(&sh.full[0][kst], kph))) break;
+                    if (lane == 0) mbar_arrive(&sh.empty[0][kst]);
+                    next_k();
+                    if (!(ok = warp_wait(&sh.full[1][vst], vph))) break;
+                    if (lane == 0) mbar_arrive(&sh.empty[1][vst]);
+                    next_v();
                 }
                 if (!ok) break;
                 continue;
             }
             if (it.tiles == 0) continue;
-            if (!warp_wait(&sh.q_full[r], qph) || !warp_wait(&sh.k_full[kst], kph)) break;
+            if (!warp_wait(&sh.q_full[r], qph)) break;
             qph ^= 1;
-            tcgen05_fence_after();
-            scores();
+            if (!scores() || (it.tiles > 1 && !scores())) break;
             for (uint32_t i = 0; i < it.tiles; ++i) {
-                const bool more = i + 1 < it.tiles;
-                if (!(ok = warp_wait(&sh.v_full[vst], vph) && warp_wait(&sh.p_full[r], pph))) break;
-                pph ^= 1;
+                const uint32_t buf = done & 1;
+                if (!(ok = warp_wait(&sh.full[1][vst], vph) && warp_wait(&sh.p_full[r][buf], done >> 1 & 1))) break;
                 tcgen05_fence_after();
                 const uint64_t vb = va + vst * (C::KV / 16);
 #pragma unroll
                 for (int k = 0; k < kPfKeys / 16; ++k)
-                    umma_f16_ts(tmem + 256 + r * 128, tmem + r * 128 + 8 * k, vb + k * (2 * HD), C::IDESC_O, i > 0 || k > 0);
-                umma_commit_one(&sh.v_empty[vst]);
-                vst ^= 1;
-                vph ^= vst == 0;
-                if (more) {  // (in order after P V: S may overwrite P)
-                    if (!(ok = warp_wait(&sh.k_full[kst], kph))) break;
-                    tcgen05_fence_after();
-                    scores();
-                } else {
-                    umma_commit_one(&sh.o_full[r]);
-                }
+                    umma_f16_ts(tmem + 256 + r * 128, tmem + r * 128 + buf * 64 + 8 * k, vb + k * (2 * HD), C::IDESC_O, i > 0 || k > 0);
+                umma_commit_one(&sh.empty[1][vst]);
+                umma_commit_one(&sh.pv_done[r]);
+                next_v();
+                ++done;
+                if (i + 1 == it.tiles) umma_commit_one(&sh.o_full[r]);
+                // the tile after next, into the buffer that P V has just read (MMAs run in order)
+                if (i + 2 < it.tiles && !(ok = scores())) break;
             }
             if (!ok) break;
         }
@@ -568,7 +565,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
     tcgen05_fence_before();
     __syncthreads();
     tcgen05_fence_after();
-    if (warp == 13) tmem_dealloc(tmem, 512);
+    if (warp == 16) tmem_dealloc(tmem, 512);
 }
 
 template <typename T, int HD>
