@@ -113,6 +113,12 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     return r;
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
 // A block of rows of one sequence and KV head, and its tiles.
 struct PfItem {
     SeqWork w;
@@ -242,6 +248,10 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
     };
     auto warp_wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, wait(bar, parity)) != 0; };
 
+    // Blocks are dealt out there and back, so that no CTA has the longer end every time.
+    auto block_of = [&](uint32_t turn) {
+        return (uint64_t)turn * gridDim.x + (turn & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+    };
     PfItem it;
     PfWalk walk = {0, 0};
     uint32_t tile_no = 0;  // tiles before the item, over all of this CTA's items
@@ -253,12 +263,13 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
         const uint32_t lanes = tmem + ((warp & 3) * 32u << 16), o_at = lanes + 256 + r * 128;
         const float sign = p.scale_log2 < 0.0f ? -1.0f : 1.0f;
         uint32_t done = 0, o_phase = 0;  // tiles this half has done
-        for (uint64_t b = blockIdx.x; walk.find(p, b, lane, &it); b += gridDim.x) {
+        for (uint32_t turn = 0; walk.find(p, block_of(turn), lane, &it); ++turn) {
             if (it.rows <= r * 128) { tile_no += it.tiles; continue; }
             const bool there = r * 128 + row < it.rows;
             const uint32_t c = it.row0 + r * 128 + (there ? row : 0);
             const int64_t token = (int64_t)((uint32_t)it.w.first + c / p.group), head = it.head * p.group + c % p.group;
             const int32_t pos = it.w.len - it.w.count + (int32_t)(c / p.group), above = window_start(p, pos);
+            const int32_t warp_pos = __reduce_min_sync(0xffffffffu, pos), warp_above = __reduce_max_sync(0xffffffffu, above);
             T* out = (T*)p.out + token * p.o_ts + head * p.o_hs;
             float f = 0.0f, m = kNothing, l = 0.0f;
             if (it.tiles) {
@@ -301,7 +312,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
                 float s[64];
                 tmem_ld64(s_at, reinterpret_cast<uint32_t(&)[64]>(s));
                 // every row of the warp sees the whole tile
-                const bool plain = __all_sync(0xffffffffu, k0 + kPfKeys - 1 <= pos && (k0 > above || (uint32_t)(k0 + kPfKeys) <= p.sinks)) && pieces == 0xfu;
+                const bool plain = k0 + kPfKeys - 1 <= warp_pos && (k0 > warp_above || (uint32_t)(k0 + kPfKeys) <= p.sinks) && pieces == 0xfu;
                 tmem_wait_ld();
                 if (!plain) {
                     const int32_t end = pos - k0 + 1, begin = above - k0 + 1;
@@ -318,9 +329,9 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
 #pragma unroll
                 for (int e = 0; e < 64; e += 8) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) top4[k] = fmaxf(top4[k], fmaxf(s[e + 2 * k], s[e + 2 * k + 1]));
+                    for (int k = 0; k < 4; ++k) top4[k] = max3(top4[k], s[e + 2 * k], s[e + 2 * k + 1]);
                 }
-                const float top = fmaxf(fmaxf(top4[0], top4[1]), fmaxf(top4[2], top4[3])) * f;
+                const float top = max3(fmaxf(top4[0], top4[1]), top4[2], top4[3]) * f;
                 if (__any_sync(0xffffffffu, top > m + kLazyMax)) {
                     const float now = fmaxf(m, top), fix = exp2_fast(m - now);
                     m = now;
@@ -392,7 +403,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
         uint8_t* raw = raws + side * kPfRaw * C::RAW;
         uint8_t* to = kvs + side * kPfStages * C::KV;
         uint32_t raw_at = 0, raw_phase = 0, st = 0, st_phase = 1;
-        for (uint64_t b = blockIdx.x; walk.find(p, b, lane, &it); b += gridDim.x) {
+        for (uint32_t turn = 0; walk.find(p, block_of(turn), lane, &it); ++turn) {
             bool ok = true;
             for (uint32_t i = 0; i < it.tiles; ++i) {
                 if (!(ok = warp_wait(&sh.raw_full[side][raw_at], raw_phase) && warp_wait(&sh.empty[side][st], st_phase))) break;
@@ -465,7 +476,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
         if (blockIdx.x == 0) {
             for (uint32_t i = lane; i < p.n; i += 32) seq_work(p, i, true);  // reports what is out of range
         }
-        for (uint64_t b = blockIdx.x; walk.find(p, b, lane, &it); b += gridDim.x) {
+        for (uint32_t turn = 0; walk.find(p, block_of(turn), lane, &it); ++turn) {
             bool ok = true;
             for (uint32_t i = 0; i < it.tiles; ++i) {
                 const int32_t key = it.key0(i) + 16 * (int32_t)lane;
@@ -520,7 +531,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
             ++made;
             return true;
         };
-        for (uint64_t b = blockIdx.x; walk.find(p, b, lane, &it); b += gridDim.x) {
+        for (uint32_t turn = 0; walk.find(p, block_of(turn), lane, &it); ++turn) {
             bool ok = true;
             if (it.rows <= r * 128) {  // nothing in this half: the tiles pass by
                 for (uint32_t i = 0; i < it.tiles; ++i) {
