@@ -11,12 +11,15 @@
 // floor(u * total).  Whole-number sums are exact in any order, so the result does
 // not depend on how the row is split or on the order of atomics.
 //
-// Layout.  A row is a cluster of up to 8 CTAs; each holds its share of the row in
-// registers (kItems values a thread), so the logits are read from memory once
-// whatever the row's parameters ask for.  Thresholds come from a radix search over
-// the order-preserving keys (11 bits a level from the largest key down; a level
-// is one histogram in shared memory, added up over the cluster).  A row that does
-// not fit the registers (more than 8 * 32768 logits) is read again at every pass.
+// Layout.  A row is a cluster of up to 8 CTAs; each holds its share of the row in shared
+// memory, so the logits are read from memory once whatever the row's parameters ask for.
+// (Held in registers, 32 values a thread, every pass is unrolled 32 times and spills.)
+// A threshold is found in two steps: one histogram of the tokens (and weights) over
+// 1023 equal steps of (m - l) / T, added up over the cluster, gives the step it lies in; the tokens of that step, a few hundred, are
+// collected, sorted and counted through by the cluster's first CTA.  Where one step
+// holds more than kSbList tokens (many equal logits) a radix search over the
+// order-preserving keys, 10 bits a level, takes its place.  A row that does not fit
+// (more than 8 * kSbHeld logits) is read again at every pass.
 //
 // Bound: memory for large batches, the chain of cluster barriers for single rows.
 #include <cooperative_groups.h>
@@ -29,8 +32,12 @@ namespace bt {
 namespace cg = cooperative_groups;
 
 constexpr int kSbThreads = 512;
-constexpr int kSbBins = 2048;
+constexpr int kSbBits = 10, kSbBins = 1 << kSbBits;
+constexpr int kSbList = 1024;
+constexpr uint32_t kSbShare = 16384;  // logits of a CTA at two CTAs an SM
+constexpr uint32_t kSbHeld = 45056;   // and at one
 constexpr uint32_t kSbMaxCluster = 8;
+constexpr float kSbReach = 27.8f;  // exp(-27.8) < 2^-40: tokens further below the maximum weigh nothing
 constexpr float kSbUnit = 1099511627776.0f;  // 2^40
 
 struct SampleParams {
@@ -44,18 +51,21 @@ struct SampleParams {
     bool wide;
 };
 
-struct SbShared {
-    uint32_t cnt[kSbBins];             // histogram: tokens, and their weights as two 32-bit words
-    uint32_t lo[kSbBins], hi[kSbBins];
-    unsigned long long tot[kSbBins];   // rank 0: the cluster's sums
+struct __align__(16) SbShared {
+    uint32_t cnt[kSbBins], lo[kSbBins], hi[kSbBins];  // this CTA's histogram: tokens, and weights as two words
+    // rank 0's: the cluster's histogram, and the tokens of one step
+    unsigned long long tot[kSbBins];
+    uint32_t totc[kSbBins];
+    uint32_t list_key[kSbList], list_id[kSbList], listed;
     unsigned long long red64[32];
     unsigned long long part[kSbMaxCluster];  // one value from every CTA
-    float redf[32];
+    float redf[32], redm[32];
     uint32_t redi[32];
-    float fpart[kSbMaxCluster];
+    float fpart[kSbMaxCluster], mpart[kSbMaxCluster];
     uint32_t ipart[kSbMaxCluster];
-    uint32_t found_bin;
-    unsigned long long found_before;
+    // what rank 0 found, in every CTA
+    uint32_t found_bin, found_key, found_ties, found_all;
+    unsigned long long found_mass;
 };
 
 __device__ __forceinline__ uint32_t sb_key(float v) {
@@ -69,7 +79,7 @@ __device__ __forceinline__ unsigned long long warp_sum64(unsigned long long v) {
     return v;
 }
 
-template <typename T, int ITEMS, bool HELD>
+template <typename T, bool HELD>
 struct SampleRow {
     static constexpr int VEC = 8;
     cg::cluster_group cl;
@@ -77,10 +87,10 @@ struct SampleRow {
     const SampleParams& p;
     const T* row;
     uint32_t C, rank, base, end;  // this CTA's ids: [base, end)
-    float x[HELD ? ITEMS : 1];
-    float m, inv;                 // the row's maximum, 1 / temperature
+    float4* held;                  // the CTA's logits, two float4 rows of kSbThreads a round
+    float m, inv, steps;          // the row's maximum, 1 / temperature, histogram steps per unit
 
-    __device__ SampleRow(SbShared& s, const SampleParams& pp) : cl(cg::this_cluster()), sh(s), p(pp) {
+    __device__ SampleRow(SbShared& s, float4* h, const SampleParams& pp) : cl(cg::this_cluster()), sh(s), p(pp), held(h) {
         C = cl.num_blocks();
         rank = cl.block_rank();
         row = (const T*)p.logits + (int64_t)(blockIdx.x / C) * p.row_stride;
@@ -106,15 +116,25 @@ struct SampleRow {
     // f(the eight values of a round, the first one's id) for every round of this thread.
     template <typename F>
     __device__ __forceinline__ void each_round(F f) const {
-        if constexpr (HELD) {
-#pragma unroll
-            for (int j = 0; j < ITEMS / VEC; ++j) f(x + j * VEC, id_of(j));
-        } else {
-            for (uint32_t j = 0, n = (end - base + kSbThreads * VEC - 1) / (kSbThreads * VEC); j < n; ++j) {
-                float v[VEC];
+        for (uint32_t j = 0, n = (end - base + kSbThreads * VEC - 1) / (kSbThreads * VEC); j < n; ++j) {
+            float v[VEC];
+            if constexpr (HELD) {
+                reinterpret_cast<float4*>(v)[0] = held[2 * j * kSbThreads + threadIdx.x];
+                reinterpret_cast<float4*>(v)[1] = held[(2 * j + 1) * kSbThreads + threadIdx.x];
+            } else {
                 load(id_of(j), v);
-                f(v, id_of(j));
             }
+            f(v, id_of(j));
+        }
+    }
+    // Brings the CTA's logits into shared memory, each thread its own.
+    __device__ __forceinline__ void hold() {
+#pragma unroll 2
+        for (uint32_t j = 0, n = (end - base + kSbThreads * VEC - 1) / (kSbThreads * VEC); j < n; ++j) {
+            float v[VEC];
+            load(id_of(j), v);
+            held[2 * j * kSbThreads + threadIdx.x] = make_float4(v[0], v[1], v[2], v[3]);
+            held[(2 * j + 1) * kSbThreads + threadIdx.x] = make_float4(v[4], v[5], v[6], v[7]);
         }
     }
     // f(value, id) for every token of this thread, in order of ids.
@@ -159,34 +179,178 @@ struct SampleRow {
         return t;
     }
 
-    // The row's maximum and its lowest id.
-    __device__ void maximum(uint32_t* arg) {
-        float best = -INFINITY;
+    // The row's maximum, its lowest id, and the smallest logit above -inf.
+    __device__ void maximum(uint32_t* arg, float* least) {
+        float best = -INFINITY, low = INFINITY;
         uint32_t at = 0xffffffffu;
         each([&](float v, uint32_t id) {
             if (v > best) { best = v; at = id; }
+            low = fminf(low, v == -INFINITY ? INFINITY : v);
         });
         warp_argmax(best, at);
-        if (threadIdx.x % 32 == 0) { sh.redf[threadIdx.x / 32] = best; sh.redi[threadIdx.x / 32] = at; }
+        low = -warp_max(-low);
+        if (threadIdx.x % 32 == 0) { sh.redf[threadIdx.x / 32] = best; sh.redm[threadIdx.x / 32] = low; sh.redi[threadIdx.x / 32] = at; }
         __syncthreads();
         if (threadIdx.x < 32) {
-            best = threadIdx.x < kSbThreads / 32 ? sh.redf[threadIdx.x] : -INFINITY;
-            at = threadIdx.x < kSbThreads / 32 ? sh.redi[threadIdx.x] : 0xffffffffu;
+            const bool in = threadIdx.x < kSbThreads / 32;
+            best = in ? sh.redf[threadIdx.x] : -INFINITY;
+            low = -warp_max(in ? -sh.redm[threadIdx.x] : -INFINITY);
+            at = in ? sh.redi[threadIdx.x] : 0xffffffffu;
             warp_argmax(best, at);
             if (threadIdx.x < C) {
                 *cl.map_shared_rank(&sh.fpart[rank], threadIdx.x) = best;
+                *cl.map_shared_rank(&sh.mpart[rank], threadIdx.x) = low;
                 *cl.map_shared_rank(&sh.ipart[rank], threadIdx.x) = at;
             }
         }
         sync();
         best = -INFINITY;
+        low = INFINITY;
         at = 0xffffffffu;
         for (uint32_t c = 0; c < C; ++c) {
             if (better(sh.fpart[c], sh.ipart[c], best, at)) { best = sh.fpart[c]; at = sh.ipart[c]; }
+            low = fminf(low, sh.mpart[c]);
         }
         m = best;
         *arg = at;
+        *least = low;
         sync();
+    }
+
+    // ---- the two-step search
+
+    // The step of a logit: 0 .. kSbBins - 2 evenly over the row's range, kSbBins - 1 beyond kSbReach.
+    // Monotone in the logit, rounding included.
+    __device__ __forceinline__ uint32_t bin_of(float v) const {
+        return v == m ? 0u : (uint32_t)fminf((m - v) * inv * steps, (float)(kSbBins - 1));
+    }
+
+    // Adds up the cluster's histograms at rank 0.
+    __device__ void gather_bins(bool counts, bool weights) {
+        sync();
+        const uint32_t mine = kSbBins / C;  // C is a power of two
+        for (uint32_t i = rank * mine + threadIdx.x; i < (rank + 1) * mine; i += kSbThreads) {
+            unsigned long long w = 0;
+            uint32_t n = 0;
+            for (uint32_t c = 0; c < C; ++c) {
+                if (weights) w += ((unsigned long long)*cl.map_shared_rank(&sh.hi[i], c) << 32) + *cl.map_shared_rank(&sh.lo[i], c);
+                if (counts) n += *cl.map_shared_rank(&sh.cnt[i], c);
+            }
+            if (weights) *cl.map_shared_rank(&sh.tot[i], 0) = w;
+            if (counts) *cl.map_shared_rank(&sh.totc[i], 0) = n;
+        }
+        sync();
+    }
+
+    __device__ __forceinline__ void add_weight(uint32_t bin, unsigned long long w) {
+        const uint32_t w0 = (uint32_t)w, old = atomicAdd(&sh.lo[bin], w0);
+        const uint32_t up = (uint32_t)(w >> 32) + (old + w0 < old ? 1u : 0u);
+        if (up) atomicAdd(&sh.hi[bin], up);
+    }
+
+    __device__ void histogram(bool counts, bool weights) {
+        for (uint32_t i = threadIdx.x; i < kSbBins; i += kSbThreads) { sh.cnt[i] = 0; sh.lo[i] = 0; sh.hi[i] = 0; }
+        __syncthreads();
+        each([&](float v, uint32_t) {
+            if (v == -INFINITY) return;
+            const uint32_t bin = bin_of(v);
+            if (counts) atomicAdd(&sh.cnt[bin], 1u);
+            if (weights && bin < kSbBins - 1) add_weight(bin, weight(v));
+        });
+        gather_bins(counts, weights);
+    }
+
+    // Rank 0, all of its threads: value(i) summed over i < n in order; in the thread that
+    // holds the first i where the sum reaches `need`, hit(i, sum before i).
+    template <int PER, typename V, typename H>
+    __device__ void first_reach(uint32_t n, unsigned long long need, V value, H hit) {
+        unsigned long long v[PER], s = 0;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const uint32_t at = threadIdx.x * PER + i;
+            v[i] = at < n ? value(at) : 0ull;
+            s += v[i];
+        }
+        unsigned long long inc = s;
+        const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned long long t = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= o) inc += t;
+        }
+        __syncthreads();
+        if (lane == 31) sh.red64[warp] = inc;
+        __syncthreads();
+        unsigned long long run = inc - s;
+        for (uint32_t c = 0; c < warp; ++c) run += sh.red64[c];
+        if (run < need && run + s >= need) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                if (run < need && run + v[i] >= need) hit(threadIdx.x * PER + i, run);
+                run += v[i];
+            }
+        }
+        __syncthreads();
+    }
+
+    // Rank 0's findings to every CTA.
+    __device__ void tell() {
+        if (rank == 0 && threadIdx.x < C && threadIdx.x > 0) {
+            SbShared* to = cl.map_shared_rank(&sh, threadIdx.x);
+            to->found_bin = sh.found_bin; to->found_key = sh.found_key; to->found_ties = sh.found_ties;
+            to->found_all = sh.found_all; to->found_mass = sh.found_mass;
+        }
+        sync();
+    }
+
+    // The tokens of found_bin, sorted (largest first, equal ones by id), at rank 0; false: too many.
+    __device__ bool list_bin() {
+        const uint32_t bin = sh.found_bin;
+        if (rank == 0 && threadIdx.x == 0) sh.listed = 0;
+        sync();
+        uint32_t* keys = cl.map_shared_rank(sh.list_key, 0);
+        uint32_t* ids = cl.map_shared_rank(sh.list_id, 0);
+        uint32_t* count = cl.map_shared_rank(&sh.listed, 0);
+        each([&](float v, uint32_t id) {
+            if (v == -INFINITY || bin_of(v) != bin) return;
+            const uint32_t at = atomicAdd(count, 1u);
+            if (at < kSbList) { keys[at] = sb_key(v); ids[at] = id; }
+        });
+        sync();
+        const uint32_t n = *count;
+        if (n > kSbList) return false;
+        if (rank == 0) {
+            uint32_t size = 2;
+            while (size < n) size <<= 1;
+            for (uint32_t i = n + threadIdx.x; i < size; i += kSbThreads) { sh.list_key[i] = 0; sh.list_id[i] = 0xffffffffu; }
+            __syncthreads();
+            for (uint32_t k = 2; k <= size; k <<= 1) {
+                for (uint32_t j = k >> 1; j > 0; j >>= 1) {
+                    for (uint32_t i = threadIdx.x; i < size / 2; i += kSbThreads) {
+                        const uint32_t a = 2 * i - (i & (j - 1)), b = a + j;
+                        const uint32_t ka = sh.list_key[a], kb = sh.list_key[b], ia = sh.list_id[a], ib = sh.list_id[b];
+                        const bool a_first = ka > kb || (ka == kb && ia < ib);
+                        if (a_first != ((a & k) == 0)) {
+                            sh.list_key[a] = kb; sh.list_key[b] = ka;
+                            sh.list_id[a] = ib; sh.list_id[b] = ia;
+                        }
+                    }
+                    __syncthreads();
+                }
+            }
+        }
+        return true;
+    }
+
+    // Rank 0: the threshold is the list's entry i.
+    __device__ __forceinline__ void cut_at(uint32_t i) {
+        const uint32_t key = sh.list_key[i], n = sh.listed;
+        uint32_t first = i, last = i;
+        while (first > 0 && sh.list_key[first - 1] == key) --first;
+        while (last + 1 < n && sh.list_key[last + 1] == key) ++last;
+        sh.found_key = key;
+        sh.found_ties = i - first + 1;
+        sh.found_all = last - first + 1;
     }
 
     // Searches the keys from `top` (the largest) down for the one at which the running
@@ -200,7 +364,7 @@ struct SampleRow {
         unsigned long long ahead = 0;
         const uint32_t span = top - floor_key;
         const int bits = 32 - __clz(span | 1u);
-        int shift = bits > 11 ? bits - 11 : 0;
+        int shift = bits > kSbBits ? bits - kSbBits : 0;
         uint32_t range = span;  // largest distance below top - off
         for (;;) {
             for (uint32_t i = threadIdx.x; i < kSbBins; i += kSbThreads) {
@@ -211,68 +375,25 @@ struct SampleRow {
             each([&](float v, uint32_t) {
                 const uint32_t d = top - sb_key(v) - off;  // wraps (and so is far) for larger keys
                 if (d <= range) {
-                    if (MASS) {
-                        const unsigned long long w = weight(v);
-                        const uint32_t w0 = (uint32_t)w, old = atomicAdd(&sh.lo[d >> shift], w0);
-                        const uint32_t up = (uint32_t)(w >> 32) + (old + w0 < old ? 1u : 0u);
-                        if (up) atomicAdd(&sh.hi[d >> shift], up);
-                    } else {
-                        atomicAdd(&sh.cnt[d >> shift], 1u);
-                    }
+                    if (MASS) add_weight(d >> shift, weight(v));
+                    else atomicAdd(&sh.cnt[d >> shift], 1u);
                 }
             });
-            sync();
-            // the cluster's histogram at rank 0, every CTA adding up its share of the bins
-            const uint32_t each_bins = kSbBins / C + (kSbBins % C ? 1 : 0);
-            for (uint32_t i = rank * each_bins + threadIdx.x; i < min((uint32_t)kSbBins, (rank + 1) * each_bins); i += kSbThreads) {
-                unsigned long long s = 0;
-                for (uint32_t c = 0; c < C; ++c) {
-                    if (MASS) s += ((unsigned long long)*cl.map_shared_rank(&sh.hi[i], c) << 32) + *cl.map_shared_rank(&sh.lo[i], c);
-                    else s += *cl.map_shared_rank(&sh.cnt[i], c);
-                }
-                *cl.map_shared_rank(&sh.tot[i], 0) = s;
-            }
-            sync();
+            gather_bins(!MASS, MASS);
             if (rank == 0) {
-                // first bin whose running sum reaches need - ahead
-                constexpr int PER = kSbBins / kSbThreads;
-                unsigned long long v[PER], s = 0;
-#pragma unroll
-                for (int i = 0; i < PER; ++i) { v[i] = sh.tot[threadIdx.x * PER + i]; s += v[i]; }
-                unsigned long long inc = s;
-                const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const unsigned long long t = __shfl_up_sync(0xffffffffu, inc, o);
-                    if (lane >= o) inc += t;
-                }
-                if (lane == 31) sh.red64[warp] = inc;
                 if (threadIdx.x == 0) sh.found_bin = 0xffffffffu;
-                __syncthreads();
-                unsigned long long run = ahead + inc - s;
-                for (uint32_t c = 0; c < warp; ++c) run += sh.red64[c];
-                if (run < need && run + s >= need) {
-#pragma unroll
-                    for (int i = 0; i < PER; ++i) {
-                        if (run < need && run + v[i] >= need) { sh.found_bin = threadIdx.x * PER + i; sh.found_before = run; }
-                        run += v[i];
-                    }
-                }
-                __syncthreads();
-                if (threadIdx.x < C && threadIdx.x > 0) {
-                    *cl.map_shared_rank(&sh.found_bin, threadIdx.x) = sh.found_bin;
-                    *cl.map_shared_rank(&sh.found_before, threadIdx.x) = sh.found_before;
-                }
+                first_reach<kSbBins / kSbThreads>(kSbBins, need - ahead, [&](uint32_t i) { return MASS ? sh.tot[i] : (unsigned long long)sh.totc[i]; },
+                                                  [&](uint32_t i, unsigned long long before) { sh.found_bin = i; sh.found_mass = ahead + before; });
             }
-            sync();
+            tell();
             const uint32_t bin = sh.found_bin;
-            ahead = sh.found_before;
+            ahead = sh.found_mass;
             sync();
             if (bin == 0xffffffffu) return false;  // the whole range holds less than `need` (first level only)
             off += bin << shift;
             if (shift == 0) break;
             range = (1u << shift) - 1u;
-            shift = shift > 11 ? shift - 11 : 0;
+            shift = shift > kSbBits ? shift - kSbBits : 0;
         }
         *key = top - off;
         *before = ahead;
@@ -280,18 +401,18 @@ struct SampleRow {
     }
 };
 
-template <typename T, int ITEMS, bool HELD>
-__global__ void __launch_bounds__(kSbThreads) sample_batch_kernel(SampleParams p) {
-    __shared__ SbShared sh;
-    SampleRow<T, ITEMS, HELD> r(sh, p);
+template <typename T, bool HELD>
+__global__ void __launch_bounds__(kSbThreads, 2) sample_batch_kernel(SampleParams p) {
+    static_assert(sizeof(SbShared) % 16 == 0, "the logits follow it");
+    extern __shared__ __align__(16) uint8_t dyn[];
+    SbShared& sh = *reinterpret_cast<SbShared*>(dyn);
+    SampleRow<T, HELD> r(sh, reinterpret_cast<float4*>(dyn + sizeof(SbShared)), p);
     const uint32_t b = blockIdx.x / r.C;
     const float temp = p.temperature ? p.temperature[b] : 1.0f;
-    if constexpr (HELD) {
-#pragma unroll
-        for (int j = 0; j < ITEMS / 8; ++j) r.load(r.id_of(j), r.x + 8 * j);
-    }
+    if constexpr (HELD) r.hold();
     uint32_t first;
-    r.maximum(&first);
+    float least;
+    r.maximum(&first, &least);
     const bool none = r.m == -INFINITY;
     if (none || temp <= 0.0f) {
         if (r.rank == 0 && threadIdx.x == 0) {
@@ -301,51 +422,107 @@ __global__ void __launch_bounds__(kSbThreads) sample_batch_kernel(SampleParams p
         return;
     }
     r.inv = 1.0f / temp;
+    const float reach = fminf((r.m - least) * r.inv, kSbReach);
+    r.steps = reach > 0.0f ? (float)(kSbBins - 2) / reach : 0.0f;
     const float top_p = p.top_p ? p.top_p[b] : 1.0f, min_p = p.min_p ? p.min_p[b] : 0.0f;
     const int32_t top_k = p.top_k ? p.top_k[b] : 0;
     const uint32_t top = sb_key(r.m);
+    const bool cut_k = top_k > 0 && (uint32_t)top_k < p.vocab, cut_p = top_p < 1.0f;
 
-    // Kept: keys above `key`, and the first `ties` (by id) of the tokens at it.
+    // Kept: keys above `key`, and the first `ties` (by id) of the `all` tokens at it.
     // Nothing at or below -inf is kept.
-    uint32_t key = sb_key(-INFINITY);
-    unsigned long long ties = 0, before;
-    uint32_t found;
-    if (top_k > 0 && (uint32_t)top_k < p.vocab &&
-        r.template search<false>(top, sb_key(-INFINITY) + 1u, (unsigned long long)top_k, &found, &before)) {
-        key = found;
-        ties = (unsigned long long)top_k - before;
-    }
-    if (top_p < 1.0f) {
-        unsigned long long mine = 0;
-        r.each([&](float v, uint32_t) { if (sb_key(v) > key) mine += r.weight(v); });
-        unsigned long long mass = r.sum(mine);
-        const float at = __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key);
-        const unsigned long long w_at = ties ? r.weight(at) : 0ull;
-        mass += ties * w_at;
-        const double want = ceil((double)top_p * (double)mass);
-        const unsigned long long need = want < 1.0 ? 1ull : (unsigned long long)want;
-        // reached among the keys above `key`, or by some of the ties at it
-        if (key < top && r.template search<true>(top, key + 1u, need, &found, &before)) {
-            const float cut = __uint_as_float((found & 0x80000000u) ? found & 0x7fffffffu : ~found);
-            const unsigned long long w = r.weight(cut);
-            key = found;
-            ties = (need - before + w - 1) / w;
-        } else if (ties && w_at) {
-            const unsigned long long n = (need - (mass - ties * w_at) + w_at - 1) / w_at;
-            if (n < ties) ties = n;
+    uint32_t key = sb_key(-INFINITY), ties = 0, all = 0;
+    if (min_p > 1.0f) {
+        key = top; ties = 1; all = 0xffffffffu;  // the first maximum alone
+    } else if (cut_k || cut_p) {
+        r.histogram(cut_k, cut_p);
+        // rank 0 keeps what it needs between the steps in shared memory
+        bool listed = false, beyond = true;  // a step's tokens are in the list; top-k cuts nothing that weighs
+        if (cut_k) {
+            if (r.rank == 0) {
+                if (threadIdx.x == 0) sh.found_bin = kSbBins - 1;
+                r.template first_reach<kSbBins / kSbThreads>(
+                    kSbBins, (unsigned long long)top_k, [&](uint32_t i) { return (unsigned long long)sh.totc[i]; },
+                    [&](uint32_t i, unsigned long long before) { sh.found_bin = i; sh.found_mass = before; });
+            }
+            r.tell();
+            beyond = sh.found_bin == kSbBins - 1;
+            if (!beyond) {
+                const uint32_t in = (uint32_t)((unsigned long long)top_k - sh.found_mass);  // tokens of the step that are kept
+                listed = r.list_bin();
+                if (listed) {
+                    if (r.rank == 0 && threadIdx.x == 0) r.cut_at(in - 1);
+                    __syncthreads();
+                    r.tell();
+                    key = sh.found_key; ties = sh.found_ties; all = sh.found_all;
+                } else {
+                    uint32_t found;
+                    unsigned long long before;
+                    r.template search<false>(top, sb_key(-INFINITY) + 1u, (unsigned long long)top_k, &found, &before);
+                    key = found;
+                    ties = (uint32_t)((unsigned long long)top_k - before);
+                    all = 0xffffffffu;  // not counted yet
+                }
+            }
+        }
+        if (cut_p) {
+            // the weight of the top-k set, and the weight to reach
+            unsigned long long mine = 0;
+            r.each([&](float v, uint32_t) { if (sb_key(v) > key) mine += r.weight(v); });
+            const float at = __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key);
+            const unsigned long long w_at = ties ? r.weight(at) : 0ull;
+            const unsigned long long mass = r.sum(mine) + ties * w_at;
+            const double want = ceil((double)top_p * (double)mass);
+            const unsigned long long need = want < 1.0 ? 1ull : (unsigned long long)want;
+            const unsigned long long above = mass - ties * w_at;
+            if (need > above) {  // reached by some of the ties at the top-k threshold
+                const unsigned long long n = (need - above + w_at - 1) / w_at;
+                if (n < ties) ties = (uint32_t)n;
+            } else {
+                bool radix = !beyond && !listed;  // (the radix search has used the histogram's place)
+                if (!radix) {
+                    if (r.rank == 0)
+                        r.template first_reach<kSbBins / kSbThreads>(
+                            kSbBins, need, [&](uint32_t i) { return sh.tot[i]; },
+                            [&](uint32_t i, unsigned long long before) { sh.found_bin = i; sh.found_mass = before; });
+                    r.tell();
+                    const unsigned long long in = need - sh.found_mass;  // weight to reach within the step
+                    radix = !r.list_bin();
+                    if (!radix) {
+                        if (r.rank == 0)
+                            r.template first_reach<kSbList / kSbThreads>(
+                                sh.listed, in,
+                                [&](uint32_t i) {
+                                    const uint32_t k = sh.list_key[i];
+                                    return r.weight(__uint_as_float((k & 0x80000000u) ? k & 0x7fffffffu : ~k));
+                                },
+                                [&](uint32_t i, unsigned long long) { r.cut_at(i); });
+                        r.tell();
+                        key = sh.found_key; ties = sh.found_ties; all = sh.found_all;
+                    }
+                }
+                if (radix) {
+                    uint32_t found;
+                    unsigned long long before;
+                    r.template search<true>(top, key + 1u, need, &found, &before);
+                    const unsigned long long w = r.weight(__uint_as_float((found & 0x80000000u) ? found & 0x7fffffffu : ~found));
+                    key = found;
+                    ties = (uint32_t)((need - before + w - 1) / w);
+                    all = 0xffffffffu;
+                }
+            }
         }
     }
-    if (min_p > 1.0f) { key = top; ties = 1; }
 
-    // Tokens at `key` are kept by rank among them: their number before this thread's
-    // matters only where some of them are cut.
-    unsigned long long n_ties = 0;
-    if (ties) {
-        r.each([&](float v, uint32_t) { if (sb_key(v) == key) ++n_ties; });
-    }
+    // Tokens at `key` are kept by rank among them: their number before this CTA matters
+    // only where some of them are cut.
     unsigned long long ties_before = 0;
-    const unsigned long long all_ties = ties ? r.sum(n_ties, &ties_before) : 0ull;
-    if (ties && all_ties == ties) { --key; ties = 0; }  // all of them: a plain threshold
+    if (ties && ties != all) {
+        unsigned long long n = 0;
+        r.each([&](float v, uint32_t) { if (sb_key(v) == key) ++n; });
+        all = (uint32_t)r.sum(n, &ties_before);
+    }
+    if (ties && all == ties) { --key; ties = 0; }  // all of them: a plain threshold
 
     const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
     constexpr int W = kSbThreads / 32;
@@ -383,7 +560,7 @@ __global__ void __launch_bounds__(kSbThreads) sample_batch_kernel(SampleParams p
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const uint32_t k = sb_key(v[e]);
-            const bool in = k > key || (ties && k == key && tie++ < ties);
+            const bool in = k > key || (ties && k == key && tie++ < (unsigned long long)ties);
             const float x = in ? r.expo(v[e]) : 0.0f;
             w[e] = x >= min_p || k == top ? (unsigned long long)(x * kSbUnit) : 0ull;
             s += w[e];
@@ -391,10 +568,18 @@ __global__ void __launch_bounds__(kSbThreads) sample_batch_kernel(SampleParams p
         return s;
     };
     unsigned long long mine = 0, cta_before, cta_total;
-    r.each_round([&](const float* v, uint32_t) {
-        unsigned long long w[8];
-        mine += kept(v, w);
-    });
+    if (ties == 0) {
+        r.each([&](float v, uint32_t) {
+            const uint32_t k = sb_key(v);
+            const float x = k > key ? r.expo(v) : 0.0f;
+            mine += x >= min_p || k == top ? (unsigned long long)(x * kSbUnit) : 0ull;
+        });
+    } else {
+        r.each_round([&](const float* v, uint32_t) {
+            unsigned long long w[8];
+            mine += kept(v, w);
+        });
+    }
     const unsigned long long total = r.sum(mine, &cta_before, &cta_total);
     const float u = p.u[b];
     unsigned long long target = (unsigned long long)((double)(u > 0.0f ? u : 0.0f) * (double)total);
@@ -419,14 +604,26 @@ __global__ void __launch_bounds__(kSbThreads) sample_batch_kernel(SampleParams p
     });
 }
 
-template <typename T, int ITEMS, bool HELD>
+template <typename T, bool HELD>
 static cudaError_t sample_launch(SampleParams p, uint32_t rows, uint32_t cluster, cudaStream_t s) {
     p.share = (p.vocab + cluster - 1) / cluster;
     p.share = (p.share + 7) / 8 * 8;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(rows * cluster);
     cfg.blockDim = dim3(kSbThreads);
+    const uint32_t round = kSbThreads * 8;
+    cfg.dynamicSmemBytes = sizeof(SbShared) + (HELD ? (p.share + round - 1) / round * round * 4 : 0);
     cfg.stream = s;
+    static std::atomic<uint64_t> ready{0};  // devices whose attribute is set
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    if (dev >= 64 || !(ready.load(std::memory_order_relaxed) >> dev & 1)) {
+        e = cudaFuncSetAttribute(sample_batch_kernel<T, HELD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                 sizeof(SbShared) + (HELD ? kSbHeld * 4 : 0));
+        if (e != cudaSuccess) return e;
+        if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
+    }
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = cluster;
@@ -434,17 +631,17 @@ static cudaError_t sample_launch(SampleParams p, uint32_t rows, uint32_t cluster
     cfg.attrs = attr;
     cfg.numAttrs = 1;
     g_launches.fetch_add(1, std::memory_order_relaxed);
-    return cudaLaunchKernelEx(&cfg, sample_batch_kernel<T, ITEMS, HELD>, p);
+    return cudaLaunchKernelEx(&cfg, sample_batch_kernel<T, HELD>, p);
 }
 
 template <typename T>
 static cudaError_t sample_pick(const SampleParams& p, uint32_t rows, cudaStream_t s) {
-    constexpr uint32_t held = kSbThreads * 32;
     uint32_t c = 1;
-    while (c < kSbMaxCluster && p.vocab > c * held) c *= 2;
-    if (p.vocab <= c * held) return sample_launch<T, 32, true>(p, rows, c, s);
-    if (p.vocab <= 2 * c * held) return sample_launch<T, 64, true>(p, rows, c, s);
-    return sample_launch<T, 8, false>(p, rows, c, s);
+    while (c < kSbMaxCluster && p.vocab > c * kSbShare) c *= 2;
+    // few rows: smaller shares, as long as the CTAs fit the SMs side by side
+    while (c < kSbMaxCluster && (uint64_t)rows * c * 2 <= 148 && p.vocab > c * 4096) c *= 2;
+    if (p.vocab <= c * kSbHeld) return sample_launch<T, true>(p, rows, c, s);
+    return sample_launch<T, false>(p, rows, c, s);
 }
 
 }  // namespace bt
