@@ -36,9 +36,26 @@ constexpr int kSbBits = 10, kSbBins = 1 << kSbBits;
 constexpr int kSbList = 1024;
 constexpr uint32_t kSbShare = 16384;  // logits of a CTA at two CTAs an SM
 constexpr uint32_t kSbHeld = 45056;   // and at one
+constexpr uint32_t kSbSums = 192;  // (round, warp) sums kept: 12 rounds of 4096 logits
 constexpr uint32_t kSbMaxCluster = 8;
 constexpr float kSbReach = 27.8f;  // exp(-27.8) < 2^-40: tokens further below the maximum weigh nothing
 constexpr float kSbUnit = 1099511627776.0f;  // 2^40
+
+// floor(2^40 e) of 0 <= e <= 1 as hi 2^23 + lo, both still carrying the bits of 2^23
+// (kSbBias): additions rounded down leave the floors in the low mantissa bits, which
+// takes four operations of the FMA pipe where a 64-bit conversion waits for a slow one.
+constexpr uint32_t kSbBias = 0x4b000000u;
+struct SbWeight {
+    uint32_t hi, lo;
+    __device__ __forceinline__ unsigned long long value() const {
+        return ((unsigned long long)(hi - kSbBias) << 23) + (lo - kSbBias);
+    }
+};
+__device__ __forceinline__ SbWeight sb_weight(float e) {
+    const float a = __fmaf_rd(e, 131072.0f, 8388608.0f);                           // 2^23 + floor(2^17 e)
+    const float rest = __fmaf_rn(e, 131072.0f, -__fsub_rn(a, 8388608.0f));         // exact
+    return {__float_as_uint(a), __float_as_uint(__fmaf_rd(rest, 8388608.0f, 8388608.0f))};
+}
 
 struct SampleParams {
     const void* logits;
@@ -57,6 +74,7 @@ struct __align__(16) SbShared {
     unsigned long long tot[kSbBins];
     uint32_t totc[kSbBins];
     uint32_t list_key[kSbList], list_id[kSbList], listed;
+    unsigned long long sums[kSbSums];
     unsigned long long red64[32];
     unsigned long long part[kSbMaxCluster];  // one value from every CTA
     float redf[32], redm[32];
@@ -147,9 +165,7 @@ struct SampleRow {
     }
 
     __device__ __forceinline__ float expo(float v) const { return v == m ? 1.0f : expf((v - m) * inv); }
-    __device__ __forceinline__ unsigned long long weight(float v) const {
-        return (unsigned long long)(expo(v) * kSbUnit);
-    }
+    __device__ __forceinline__ unsigned long long weight(float v) const { return sb_weight(expo(v)).value(); }
 
     __device__ __forceinline__ void sync() {
         if (C > 1) cl.sync();
@@ -436,7 +452,7 @@ __global__ void __launch_bounds__(kSbThreads, 2) sample_batch_kernel(SampleParam
         key = top; ties = 1; all = 0xffffffffu;  // the first maximum alone
     } else if (cut_k || cut_p) {
         r.histogram(cut_k, cut_p);
-        // rank 0 keeps what it needs between the steps in shared memory
+        uint32_t k_bin = 0;
         bool listed = false, beyond = true;  // a step's tokens are in the list; top-k cuts nothing that weighs
         if (cut_k) {
             if (r.rank == 0) {
@@ -446,7 +462,8 @@ __global__ void __launch_bounds__(kSbThreads, 2) sample_batch_kernel(SampleParam
                     [&](uint32_t i, unsigned long long before) { sh.found_bin = i; sh.found_mass = before; });
             }
             r.tell();
-            beyond = sh.found_bin == kSbBins - 1;
+            k_bin = sh.found_bin;
+            beyond = k_bin == kSbBins - 1;
             if (!beyond) {
                 const uint32_t in = (uint32_t)((unsigned long long)top_k - sh.found_mass);  // tokens of the step that are kept
                 listed = r.list_bin();
@@ -467,11 +484,20 @@ __global__ void __launch_bounds__(kSbThreads, 2) sample_batch_kernel(SampleParam
         }
         if (cut_p) {
             // the weight of the top-k set, and the weight to reach
-            unsigned long long mine = 0;
-            r.each([&](float v, uint32_t) { if (sb_key(v) > key) mine += r.weight(v); });
             const float at = __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key);
             const unsigned long long w_at = ties ? r.weight(at) : 0ull;
-            const unsigned long long mass = r.sum(mine) + ties * w_at;
+            unsigned long long mass = 0;
+            if (beyond || listed) {  // the steps before the threshold's, and the listed tokens above it
+                const uint32_t steps = beyond ? kSbBins : k_bin;
+                if (r.rank == 0) {
+                    for (uint32_t i = threadIdx.x; i < steps; i += kSbThreads) mass += sh.tot[i];
+                    for (uint32_t i = threadIdx.x; listed && i < sh.listed && sh.list_key[i] > key; i += kSbThreads)
+                        mass += r.weight(__uint_as_float((sh.list_key[i] & 0x80000000u) ? sh.list_key[i] & 0x7fffffffu : ~sh.list_key[i]));
+                }
+            } else {
+                r.each([&](float v, uint32_t) { if (sb_key(v) > key) mass += r.weight(v); });
+            }
+            mass = r.sum(mass) + ties * w_at;
             const double want = ceil((double)top_p * (double)mass);
             const unsigned long long need = want < 1.0 ? 1ull : (unsigned long long)want;
             const unsigned long long above = mass - ties * w_at;
@@ -524,72 +550,74 @@ __global__ void __launch_bounds__(kSbThreads, 2) sample_batch_kernel(SampleParam
     }
     if (ties && all == ties) { --key; ties = 0; }  // all of them: a plain threshold
 
+    // The weights that the tokens are drawn with, summed for every (round, warp), 256
+    // consecutive ids; kSbSums of the sums are kept.
     const uint32_t lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-    constexpr int W = kSbThreads / 32;
-    // Running sums over a round's threads in order of ids: `run` on entry is what comes
-    // before the round, on return before the next one; the result is before this thread.
-    auto running = [&](unsigned long long mine, unsigned long long& run) {
-        unsigned long long inc = mine;
+    constexpr uint32_t W = kSbThreads / 32;
+    // rank of this thread's first tie of a round among the row's ties; `run`: the ties before the round
+    auto tie_rank = [&](const float* v, unsigned long long& run) {
+        uint32_t n = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) n += sb_key(v[e]) == key ? 1u : 0u;
+        uint32_t inc = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const unsigned long long t = __shfl_up_sync(0xffffffffu, inc, o);
+            const uint32_t t = __shfl_up_sync(0xffffffffu, inc, o);
             if (lane >= (uint32_t)o) inc += t;
         }
         __syncthreads();
-        if (lane == 31) sh.red64[warp] = inc;
+        if (lane == 31) sh.redi[warp] = inc;
         __syncthreads();
-        unsigned long long at = run + inc - mine;
-        for (int c = 0; c < W; ++c) {
-            const unsigned long long t = sh.red64[c];
-            if (c < (int)warp) at += t;
-            run += t;
+        unsigned long long at = run + inc - n;
+        for (uint32_t c = 0; c < W; ++c) {
+            if (c < warp) at += sh.redi[c];
+            run += sh.redi[c];
         }
         return at;
     };
-    // The weights that a round's tokens are drawn with.
-    unsigned long long tie_run = ties_before;
-    auto kept = [&](const float* v, unsigned long long (&w)[8]) {
-        unsigned long long tie = 0;
-        if (ties) {
-            unsigned long long n = 0;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) n += sb_key(v[e]) == key ? 1u : 0u;
-            tie = running(n, tie_run);
-        }
-        unsigned long long s = 0;
+    // a token's weight; `tie`: its rank, should it be a tie
+    auto kept = [&](float v, unsigned long long& tie) {
+        const uint32_t k = sb_key(v);
+        const bool in = k > key || (ties && k == key && tie++ < (unsigned long long)ties);
+        const float x = in ? r.expo(v) : 0.0f;
+        return sb_weight(x >= min_p || k == top ? x : 0.0f);
+    };
+    unsigned long long mine = 0, cta_before, cta_total, tie_run = ties_before;
+    uint32_t round = 0;
+    r.each_round([&](const float* v, uint32_t) {
+        unsigned long long tie = ties ? tie_rank(v, tie_run) : 0ull;
+        uint32_t hi = 0, lo = 0;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const uint32_t k = sb_key(v[e]);
-            const bool in = k > key || (ties && k == key && tie++ < (unsigned long long)ties);
-            const float x = in ? r.expo(v[e]) : 0.0f;
-            w[e] = x >= min_p || k == top ? (unsigned long long)(x * kSbUnit) : 0ull;
-            s += w[e];
+            const SbWeight w = kept(v[e], tie);
+            hi += w.hi - kSbBias;
+            lo += w.lo - kSbBias;
         }
-        return s;
-    };
-    unsigned long long mine = 0, cta_before, cta_total;
-    if (ties == 0) {
-        r.each([&](float v, uint32_t) {
-            const uint32_t k = sb_key(v);
-            const float x = k > key ? r.expo(v) : 0.0f;
-            mine += x >= min_p || k == top ? (unsigned long long)(x * kSbUnit) : 0ull;
-        });
-    } else {
-        r.each_round([&](const float* v, uint32_t) {
-            unsigned long long w[8];
-            mine += kept(v, w);
-        });
-    }
+        const unsigned long long s = warp_sum64(((unsigned long long)hi << 23) + lo);
+        if (lane == 0) {
+            if (round < kSbSums / W) sh.sums[round * W + warp] = s;
+            mine += s;
+        }
+        ++round;
+    });
     const unsigned long long total = r.sum(mine, &cta_before, &cta_total);
     const float u = p.u[b];
     unsigned long long target = (unsigned long long)((double)(u > 0.0f ? u : 0.0f) * (double)total);
     if (target >= total) target = total - 1;
     if (target < cta_before || target - cta_before >= cta_total) return;  // another CTA holds the token
-    unsigned long long run = cta_before;
-    tie_run = ties_before;
-    r.each_round([&](const float* v, uint32_t id) {
-        unsigned long long w[8];
-        unsigned long long at = running(kept(v, w), run);
+
+    // The part that holds it, by the sums in order; a row with more parts is summed again.
+    auto draw = [&](const float* v, uint32_t id, unsigned long long before, unsigned long long tie) {
+        unsigned long long w[8], s = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) { w[e] = kept(v[e], tie).value(); s += w[e]; }
+        unsigned long long inc = s;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const unsigned long long t = __shfl_up_sync(0xffffffffu, inc, o);
+            if (lane >= (uint32_t)o) inc += t;
+        }
+        unsigned long long at = before + inc - s;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             if (at <= target && target - at < w[e]) {
@@ -601,6 +629,31 @@ __global__ void __launch_bounds__(kSbThreads, 2) sample_batch_kernel(SampleParam
             }
             at += w[e];
         }
+    };
+    unsigned long long run = cta_before;
+    tie_run = ties_before;
+    round = 0;
+    r.each_round([&](const float* v, uint32_t id) {
+        const unsigned long long tie = ties ? tie_rank(v, tie_run) : 0ull;
+        if (round >= kSbSums / W) {  // this round's sums were not kept
+            unsigned long long t = tie, s = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s += kept(v[e], t).value();
+            s = warp_sum64(s);
+            __syncthreads();
+            if (lane == 0) sh.sums[warp] = s;
+            __syncthreads();
+        }
+        const unsigned long long* sums = sh.sums + (round < kSbSums / W ? round * W : 0);
+        unsigned long long before = run;
+        for (uint32_t c = 0; c < W; ++c) {
+            const unsigned long long s = sums[c];
+            if (c < warp) before += s;
+            run += s;
+        }
+        // the warp whose part holds the target goes through its tokens
+        if (before <= target && target - before < sums[warp]) draw(v, id, before, tie);
+        ++round;
     });
 }
 
