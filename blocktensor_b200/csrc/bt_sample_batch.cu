@@ -14,14 +14,20 @@
 // Layout.  A row is a cluster of up to 8 CTAs; each holds its share of the row in shared
 // memory, so the logits are read from memory once whatever the row's parameters ask for.
 // (Held in registers, 32 values a thread, every pass is unrolled 32 times and spills.)
-// A threshold is found in two steps: one histogram of the tokens (and weights) over
-// 1023 equal steps of (m - l) / T, added up over the cluster, gives the step it lies in; the tokens of that step, a few hundred, are
-// collected, sorted and counted through by the cluster's first CTA.  Where one step
-// holds more than kSbList tokens (many equal logits) a radix search over the
-// order-preserving keys, 10 bits a level, takes its place.  A row that does not fit
-// (more than 8 * kSbHeld logits) is read again at every pass.
+// At full batches the issue slots are the limit (14 operations a logit take as long as
+// reading it), so the passes do little for a logit that cannot be kept:
+//   top_k <= 512: every thread has the maximum of its logits; the k-th largest of these
+//     bounds the k-th largest logit from below, which leaves little more than k
+//     candidates.  The cluster's first CTA lists and sorts them, cuts, and draws.
+//   else, for top-p or a large top_k: one histogram of the tokens and weights over 1023
+//     equal steps of (m - l) / T, added up over the cluster, gives the step a threshold
+//     lies in; the tokens of that step, a few hundred, are listed, sorted and counted
+//     through.  Where one step holds more than kSbList tokens (many equal logits) a radix
+//     search over the order-preserving keys, 10 bits a level, takes its place.  Then the
+//     kept weights are summed, and the part of the row that holds the draw gone through.
+// A row that does not fit (more than 8 * kSbHeld logits) is read again at every pass.
 //
-// Bound: memory for large batches, the chain of cluster barriers for single rows.
+// Bound: issue slots for large batches, the chain of cluster barriers for single rows.
 #include <cooperative_groups.h>
 
 #include "bt_internal.h"
@@ -91,10 +97,29 @@ __device__ __forceinline__ uint32_t sb_key(float v) {
     return (b & 0x80000000u) ? ~b : (b | 0x80000000u);  // larger float, larger key
 }
 
+__device__ __forceinline__ float sb_value(uint32_t key) {
+    return __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key);
+}
+
+__device__ __forceinline__ float sb_max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ float sb_max8(const float* v) {
+    return fmaxf(sb_max3(sb_max3(v[0], v[1], v[2]), v[3], v[4]), sb_max3(v[5], v[6], v[7]));
+}
+
 __device__ __forceinline__ unsigned long long warp_sum64(unsigned long long v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
+}
+
+// Where u lies in the running sum.
+__device__ __forceinline__ unsigned long long sb_target(float u, unsigned long long total) {
+    const unsigned long long t = (unsigned long long)((double)(u > 0.0f ? u : 0.0f) * (double)total);
+    return t < total ? t : total - 1;
 }
 
 template <typename T, bool HELD>
@@ -107,6 +132,9 @@ struct SampleRow {
     uint32_t C, rank, base, end;  // this CTA's ids: [base, end)
     float4* held;                  // the CTA's logits, two float4 rows of kSbThreads a round
     float m, inv, steps;          // the row's maximum, 1 / temperature, histogram steps per unit
+    float mine, low;              // this thread's maximum, and about its smallest logit above -inf
+    bool flat = false;            // only the logits equal to flat_at count, alike
+    float flat_at = 0.0f;
 
     __device__ SampleRow(SbShared& s, float4* h, const SampleParams& pp) : cl(cg::this_cluster()), sh(s), p(pp), held(h) {
         C = cl.num_blocks();
@@ -116,7 +144,7 @@ struct SampleRow {
         end = min(p.vocab, base + p.share);
     }
 
-    // Eight logits from id i on; ids past the share's end, NaN and -inf are -inf, -0 is 0.
+    // Eight logits from id i on; ids past the share's end and NaN are -inf.
     __device__ __forceinline__ void load(uint32_t i, float* v) const {
         float f[8];
         if (i + VEC <= end) {
@@ -126,7 +154,11 @@ struct SampleRow {
             for (int e = 0; e < VEC; ++e) f[e] = i + e < end ? Act<T>::to_f(row[i + e]) : -INFINITY;
         }
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) v[e] = f[e] == f[e] ? f[e] + 0.0f : -INFINITY;
+        for (int e = 0; e < VEC; ++e) v[e] = fmaxf(f[e], -INFINITY);
+        if (!HELD && flat) {
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) v[e] = v[e] == flat_at ? 0.0f : -INFINITY;
+        }
     }
 
     __device__ __forceinline__ uint32_t id_of(uint32_t j) const { return base + (j * kSbThreads + threadIdx.x) * VEC; }
@@ -145,15 +177,39 @@ struct SampleRow {
             f(v, id_of(j));
         }
     }
-    // Brings the CTA's logits into shared memory, each thread its own.
-    __device__ __forceinline__ void hold() {
+    // The thread's maximum and (from one logit in eight) its minimum; where the logits are
+    // held, brings them into shared memory, each thread its own.
+    __device__ __forceinline__ void first_look() {
+        mine = -INFINITY;
+        low = INFINITY;
 #pragma unroll 2
         for (uint32_t j = 0, n = (end - base + kSbThreads * VEC - 1) / (kSbThreads * VEC); j < n; ++j) {
             float v[VEC];
             load(id_of(j), v);
-            held[2 * j * kSbThreads + threadIdx.x] = make_float4(v[0], v[1], v[2], v[3]);
-            held[(2 * j + 1) * kSbThreads + threadIdx.x] = make_float4(v[4], v[5], v[6], v[7]);
+            mine = fmaxf(mine, sb_max8(v));
+            if (v[0] > -INFINITY) low = fminf(low, v[0]);
+            if constexpr (HELD) {
+                held[2 * j * kSbThreads + threadIdx.x] = make_float4(v[0], v[1], v[2], v[3]);
+                held[(2 * j + 1) * kSbThreads + threadIdx.x] = make_float4(v[4], v[5], v[6], v[7]);
+            }
         }
+    }
+    // From now on only the logits equal to the maximum count, with equal weights (+inf among
+    // them, or a temperature whose inverse is infinite).
+    __device__ void flatten() {
+        flat = true;
+        flat_at = m;
+        if constexpr (HELD) {
+            for (uint32_t j = 0, n = (end - base + kSbThreads * VEC - 1) / (kSbThreads * VEC); j < 2 * n; ++j) {
+                float4 v = held[j * kSbThreads + threadIdx.x];
+                v.x = v.x == m ? 0.0f : -INFINITY; v.y = v.y == m ? 0.0f : -INFINITY;
+                v.z = v.z == m ? 0.0f : -INFINITY; v.w = v.w == m ? 0.0f : -INFINITY;
+                held[j * kSbThreads + threadIdx.x] = v;
+            }
+        }
+        mine = mine == m ? 0.0f : -INFINITY;
+        m = 0.0f;
+        inv = 1.0f;
     }
     // f(value, id) for every token of this thread, in order of ids.
     template <typename F>
@@ -164,7 +220,7 @@ struct SampleRow {
         });
     }
 
-    __device__ __forceinline__ float expo(float v) const { return v == m ? 1.0f : expf((v - m) * inv); }
+    __device__ __forceinline__ float expo(float v) const { return expf((v - m) * inv); }  // (1 at the maximum)
     __device__ __forceinline__ unsigned long long weight(float v) const { return sb_weight(expo(v)).value(); }
 
     __device__ __forceinline__ void sync() {
@@ -195,50 +251,60 @@ struct SampleRow {
         return t;
     }
 
-    // The row's maximum, its lowest id, and the smallest logit above -inf.
-    __device__ void maximum(uint32_t* arg, float* least) {
-        float best = -INFINITY, low = INFINITY;
-        uint32_t at = 0xffffffffu;
-        each([&](float v, uint32_t id) {
-            if (v > best) { best = v; at = id; }
-            low = fminf(low, v == -INFINITY ? INFINITY : v);
-        });
-        warp_argmax(best, at);
-        low = -warp_max(-low);
-        if (threadIdx.x % 32 == 0) { sh.redf[threadIdx.x / 32] = best; sh.redm[threadIdx.x / 32] = low; sh.redi[threadIdx.x / 32] = at; }
+    // The row's maximum m; returns about its smallest logit above -inf.
+    __device__ float maximum() {
+        const float best = warp_max(mine), least = -warp_max(-low);
+        if (threadIdx.x % 32 == 0) { sh.redf[threadIdx.x / 32] = best; sh.redm[threadIdx.x / 32] = least; }
         __syncthreads();
         if (threadIdx.x < 32) {
             const bool in = threadIdx.x < kSbThreads / 32;
-            best = in ? sh.redf[threadIdx.x] : -INFINITY;
-            low = -warp_max(in ? -sh.redm[threadIdx.x] : -INFINITY);
-            at = in ? sh.redi[threadIdx.x] : 0xffffffffu;
-            warp_argmax(best, at);
+            const float a = warp_max(in ? sh.redf[threadIdx.x] : -INFINITY), b = -warp_max(in ? -sh.redm[threadIdx.x] : -INFINITY);
             if (threadIdx.x < C) {
-                *cl.map_shared_rank(&sh.fpart[rank], threadIdx.x) = best;
-                *cl.map_shared_rank(&sh.mpart[rank], threadIdx.x) = low;
-                *cl.map_shared_rank(&sh.ipart[rank], threadIdx.x) = at;
+                *cl.map_shared_rank(&sh.fpart[rank], threadIdx.x) = a;
+                *cl.map_shared_rank(&sh.mpart[rank], threadIdx.x) = b;
             }
         }
         sync();
-        best = -INFINITY;
-        low = INFINITY;
-        at = 0xffffffffu;
+        m = -INFINITY;
+        float all = INFINITY;
         for (uint32_t c = 0; c < C; ++c) {
-            if (better(sh.fpart[c], sh.ipart[c], best, at)) { best = sh.fpart[c]; at = sh.ipart[c]; }
-            low = fminf(low, sh.mpart[c]);
+            m = fmaxf(m, sh.fpart[c]);
+            all = fminf(all, sh.mpart[c]);
         }
-        m = best;
-        *arg = at;
-        *least = low;
+        return all;
+    }
+    // The lowest id of a logit equal to m, in rank 0's thread 0.
+    __device__ uint32_t first_of_maximum() {
+        uint32_t at = 0xffffffffu;
+        if (mine == m) {
+            each_round([&](const float* v, uint32_t id) {
+                if (sb_max8(v) != m) return;
+#pragma unroll
+                for (int e = VEC - 1; e >= 0; --e) {
+                    if (v[e] == m) at = min(at, id + e);
+                }
+            });
+        }
+        at = __reduce_min_sync(0xffffffffu, at);
+        if (threadIdx.x % 32 == 0) sh.redi[threadIdx.x / 32] = at;
+        __syncthreads();
+        if (threadIdx.x < 32) {
+            at = __reduce_min_sync(0xffffffffu, threadIdx.x < kSbThreads / 32 ? sh.redi[threadIdx.x] : 0xffffffffu);
+            if (threadIdx.x == 0) *cl.map_shared_rank(&sh.ipart[rank], 0) = at;
+        }
         sync();
+        for (uint32_t c = 0; c < C; ++c) at = min(at, sh.ipart[c]);
+        return at;
     }
 
     // ---- the two-step search
 
-    // The step of a logit: 0 .. kSbBins - 2 evenly over the row's range, kSbBins - 1 beyond kSbReach.
+    // The step of a logit: 0 .. kSbBins - 2 evenly over about the row's range (the last one
+    // takes what lies below it), kSbBins - 1 beyond kSbReach.
     // Monotone in the logit, rounding included.
     __device__ __forceinline__ uint32_t bin_of(float v) const {
-        return v == m ? 0u : (uint32_t)fminf((m - v) * inv * steps, (float)(kSbBins - 1));
+        const float x = (m - v) * inv;
+        return x < kSbReach ? (uint32_t)fminf(x * steps, (float)(kSbBins - 2)) : kSbBins - 1;
     }
 
     // Adds up the cluster's histograms at rank 0.
@@ -319,19 +385,30 @@ struct SampleRow {
         sync();
     }
 
-    // The tokens of found_bin, sorted (largest first, equal ones by id), at rank 0; false: too many.
-    __device__ bool list_bin() {
-        const uint32_t bin = sh.found_bin;
+    // The tokens of steps `from` .. `to`, sorted (largest first, equal ones by id), at rank 0;
+    // false: too many.
+    __device__ bool list_bins(uint32_t from, uint32_t to) {
+        // no logit below this is in them (the margins cover the roundings of either side)
+        const float reach = (float)(to + 1) / steps / inv, bound = steps > 0.0f ? m - reach * 1.0001f - fabsf(m) * 1e-5f : -INFINITY;
         if (rank == 0 && threadIdx.x == 0) sh.listed = 0;
         sync();
         uint32_t* keys = cl.map_shared_rank(sh.list_key, 0);
         uint32_t* ids = cl.map_shared_rank(sh.list_id, 0);
         uint32_t* count = cl.map_shared_rank(&sh.listed, 0);
-        each([&](float v, uint32_t id) {
-            if (v == -INFINITY || bin_of(v) != bin) return;
-            const uint32_t at = atomicAdd(count, 1u);
-            if (at < kSbList) { keys[at] = sb_key(v); ids[at] = id; }
-        });
+        if (mine >= bound) {
+            each_round([&](const float* v, uint32_t id) {
+                if (!(sb_max8(v) >= bound)) return;
+#pragma unroll 1
+                for (int e = 0; e < VEC; ++e) {
+                    const float x = v[e];
+                    if (x == -INFINITY) continue;
+                    const uint32_t bin = bin_of(x);
+                    if (bin < from || bin > to) continue;
+                    const uint32_t at = atomicAdd(count, 1u);
+                    if (at < kSbList) { keys[at] = sb_key(x + 0.0f); ids[at] = id + e; }  // (-0 is 0)
+                }
+            });
+        }
         sync();
         const uint32_t n = *count;
         if (n > kSbList) return false;
@@ -369,6 +446,43 @@ struct SampleRow {
         sh.found_all = last - first + 1;
     }
 
+    // Rank 0: cuts the sorted list, which holds the `k` <= kSbThreads largest tokens, by top-k,
+    // top-p and min-p, and draws from what is left.
+    __device__ void draw_listed(uint32_t k, float top_p, float min_p, float u, uint32_t b) {
+        const uint32_t i = threadIdx.x;
+        uint32_t keep = min(k, sh.listed);
+        const float v = i < keep ? sb_value(sh.list_key[i]) : 0.0f, e = i < keep ? expo(v) : 0.0f;
+        const uint32_t id = i < keep ? sh.list_id[i] : 0xffffffffu;
+        if (top_p < 1.0f) {
+            const unsigned long long w = sb_weight(e).value();
+            unsigned long long mass = warp_sum64(w);
+            __syncthreads();
+            if (i % 32 == 0) sh.red64[i / 32] = mass;
+            __syncthreads();
+            mass = 0;
+            for (int c = 0; c < kSbThreads / 32; ++c) mass += sh.red64[c];
+            const double want = ceil((double)top_p * (double)mass);
+            first_reach<1>(keep, want < 1.0 ? 1ull : (unsigned long long)want, [&](uint32_t) { return w; },
+                           [&](uint32_t at, unsigned long long) { sh.found_ties = at + 1; });
+            keep = sh.found_ties;
+        }
+        const unsigned long long w = i < keep && (e >= min_p || i == 0) ? sb_weight(e).value() : 0ull;
+        sh.tot[i] = w;
+        __syncthreads();
+        // the weights of the kept tokens with lower ids, and of all
+        unsigned long long before = 0, total = 0;
+        for (uint32_t j = 0; j < keep; ++j) {
+            const unsigned long long x = sh.tot[j];
+            total += x;
+            if (sh.list_id[j] < id) before += x;
+        }
+        const unsigned long long target = sb_target(u, total);
+        if (w && before <= target && target - before < w) {
+            p.token[b] = (int32_t)id;
+            if (p.logprob) p.logprob[b] = (v - m) * inv - logf(__ull2float_rn(total) / kSbUnit);
+        }
+    }
+
     // Searches the keys from `top` (the largest) down for the one at which the running
     // count (MASS false) or weight (MASS true) of the tokens in decreasing order reaches
     // `need` >= 1; keys below `floor_key` are not searched.  True: *key is it and *before
@@ -389,7 +503,7 @@ struct SampleRow {
             }
             __syncthreads();
             each([&](float v, uint32_t) {
-                const uint32_t d = top - sb_key(v) - off;  // wraps (and so is far) for larger keys
+                const uint32_t d = top - sb_key(v + 0.0f) - off;  // wraps (and so is far) for larger keys
                 if (d <= range) {
                     if (MASS) add_weight(d >> shift, weight(v));
                     else atomicAdd(&sh.cnt[d >> shift], 1u);
@@ -425,25 +539,53 @@ __global__ void __launch_bounds__(kSbThreads, 2) sample_batch_kernel(SampleParam
     SampleRow<T, HELD> r(sh, reinterpret_cast<float4*>(dyn + sizeof(SbShared)), p);
     const uint32_t b = blockIdx.x / r.C;
     const float temp = p.temperature ? p.temperature[b] : 1.0f;
-    if constexpr (HELD) r.hold();
-    uint32_t first;
-    float least;
-    r.maximum(&first, &least);
-    const bool none = r.m == -INFINITY;
-    if (none || temp <= 0.0f) {
+    r.first_look();
+    const float least = r.maximum();
+    if (r.m == -INFINITY) {
         if (r.rank == 0 && threadIdx.x == 0) {
-            p.token[b] = none ? -1 : (int32_t)first;
-            if (p.logprob) p.logprob[b] = none ? -INFINITY : 0.0f;
+            p.token[b] = -1;
+            if (p.logprob) p.logprob[b] = -INFINITY;
+        }
+        return;
+    }
+    if (temp <= 0.0f) {
+        const uint32_t first = r.first_of_maximum();
+        if (r.rank == 0 && threadIdx.x == 0) {
+            p.token[b] = (int32_t)first;
+            if (p.logprob) p.logprob[b] = 0.0f;
         }
         return;
     }
     r.inv = 1.0f / temp;
+    if (r.m == INFINITY || r.inv == INFINITY) r.flatten();
     const float reach = fminf((r.m - least) * r.inv, kSbReach);
     r.steps = reach > 0.0f ? (float)(kSbBins - 2) / reach : 0.0f;
     const float top_p = p.top_p ? p.top_p[b] : 1.0f, min_p = p.min_p ? p.min_p[b] : 0.0f;
     const int32_t top_k = p.top_k ? p.top_k[b] : 0;
-    const uint32_t top = sb_key(r.m);
+    const uint32_t top = sb_key(r.m + 0.0f);
+    const float u = p.u[b];
     const bool cut_k = top_k > 0 && (uint32_t)top_k < p.vocab, cut_p = top_p < 1.0f;
+
+    // ---- a short list holds everything
+    if (cut_k && top_k <= (int32_t)kSbThreads) {
+        // step that the k-th largest of the threads' maxima lies in
+        for (uint32_t i = threadIdx.x; i < kSbBins; i += kSbThreads) sh.cnt[i] = 0;
+        __syncthreads();
+        if (r.mine > -INFINITY) atomicAdd(&sh.cnt[r.bin_of(r.mine)], 1u);
+        r.gather_bins(true, false);
+        if (r.rank == 0) {
+            if (threadIdx.x == 0) sh.found_bin = 0xffffffffu;
+            r.template first_reach<kSbBins / kSbThreads>(
+                kSbBins, (unsigned long long)top_k, [&](uint32_t i) { return (unsigned long long)sh.totc[i]; },
+                [&](uint32_t i, unsigned long long) { sh.found_bin = i; });
+        }
+        r.tell();
+        const uint32_t last = sh.found_bin;
+        if (last < kSbBins - 1 && r.list_bins(0, last)) {
+            if (r.rank == 0) r.draw_listed((uint32_t)top_k, top_p, min_p, u, b);
+            return;
+        }
+    }
 
     // Kept: keys above `key`, and the first `ties` (by id) of the `all` tokens at it.
     // Nothing at or below -inf is kept.
@@ -466,7 +608,7 @@ __global__ void __launch_bounds__(kSbThreads, 2) sample_batch_kernel(SampleParam
             beyond = k_bin == kSbBins - 1;
             if (!beyond) {
                 const uint32_t in = (uint32_t)((unsigned long long)top_k - sh.found_mass);  // tokens of the step that are kept
-                listed = r.list_bin();
+                listed = r.list_bins(k_bin, k_bin);
                 if (listed) {
                     if (r.rank == 0 && threadIdx.x == 0) r.cut_at(in - 1);
                     __syncthreads();
@@ -484,7 +626,7 @@ __global__ void __launch_bounds__(kSbThreads, 2) sample_batch_kernel(SampleParam
         }
         if (cut_p) {
             // the weight of the top-k set, and the weight to reach
-            const float at = __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key);
+            const float at = sb_value(key);
             const unsigned long long w_at = ties ? r.weight(at) : 0ull;
             unsigned long long mass = 0;
             if (beyond || listed) {  // the steps before the threshold's, and the listed tokens above it
@@ -492,10 +634,10 @@ __global__ void __launch_bounds__(kSbThreads, 2) sample_batch_kernel(SampleParam
                 if (r.rank == 0) {
                     for (uint32_t i = threadIdx.x; i < steps; i += kSbThreads) mass += sh.tot[i];
                     for (uint32_t i = threadIdx.x; listed && i < sh.listed && sh.list_key[i] > key; i += kSbThreads)
-                        mass += r.weight(__uint_as_float((sh.list_key[i] & 0x80000000u) ? sh.list_key[i] & 0x7fffffffu : ~sh.list_key[i]));
+                        mass += r.weight(sb_value(sh.list_key[i]));
                 }
             } else {
-                r.each([&](float v, uint32_t) { if (sb_key(v) > key) mass += r.weight(v); });
+                r.each([&](float v, uint32_t) { if (v > at) mass += r.weight(v); });
             }
             mass = r.sum(mass) + ties * w_at;
             const double want = ceil((double)top_p * (double)mass);
@@ -513,15 +655,12 @@ __global__ void __launch_bounds__(kSbThreads, 2) sample_batch_kernel(SampleParam
                             [&](uint32_t i, unsigned long long before) { sh.found_bin = i; sh.found_mass = before; });
                     r.tell();
                     const unsigned long long in = need - sh.found_mass;  // weight to reach within the step
-                    radix = !r.list_bin();
+                    { const uint32_t bin = sh.found_bin; radix = !r.list_bins(bin, bin); }
                     if (!radix) {
                         if (r.rank == 0)
                             r.template first_reach<kSbList / kSbThreads>(
                                 sh.listed, in,
-                                [&](uint32_t i) {
-                                    const uint32_t k = sh.list_key[i];
-                                    return r.weight(__uint_as_float((k & 0x80000000u) ? k & 0x7fffffffu : ~k));
-                                },
+                                [&](uint32_t i) { return r.weight(sb_value(sh.list_key[i])); },
                                 [&](uint32_t i, unsigned long long) { r.cut_at(i); });
                         r.tell();
                         key = sh.found_key; ties = sh.found_ties; all = sh.found_all;
@@ -531,7 +670,7 @@ __global__ void __launch_bounds__(kSbThreads, 2) sample_batch_kernel(SampleParam
                     uint32_t found;
                     unsigned long long before;
                     r.template search<true>(top, key + 1u, need, &found, &before);
-                    const unsigned long long w = r.weight(__uint_as_float((found & 0x80000000u) ? found & 0x7fffffffu : ~found));
+                    const unsigned long long w = r.weight(sb_value(found));
                     key = found;
                     ties = (uint32_t)((need - before + w - 1) / w);
                     all = 0xffffffffu;
@@ -545,10 +684,16 @@ __global__ void __launch_bounds__(kSbThreads, 2) sample_batch_kernel(SampleParam
     unsigned long long ties_before = 0;
     if (ties && ties != all) {
         unsigned long long n = 0;
-        r.each([&](float v, uint32_t) { if (sb_key(v) == key) ++n; });
+        r.each([&](float v, uint32_t) { if (v == sb_value(key)) ++n; });
         all = (uint32_t)r.sum(n, &ties_before);
     }
-    if (ties && all == ties) { --key; ties = 0; }  // all of them: a plain threshold
+    float edge = sb_value(key);  // kept: above it, and `ties` of the tokens at it
+    if (ties && all == ties) {   // all of them: above the next lower number (past -0, which equals 0)
+        edge = sb_value(edge == 0.0f ? sb_key(-0.0f) - 1u : key - 1u);
+        ties = 0;
+    }
+    // no logit below this passes min_p (the margin covers the roundings)
+    const float floor_p = min_p > 0.0f ? r.m + (logf(fminf(min_p, 1.0f)) - 1e-3f) / r.inv - fabsf(r.m) * 1e-5f : -INFINITY;
 
     // The weights that the tokens are drawn with, summed for every (round, warp), 256
     // consecutive ids; kSbSums of the sums are kept.
@@ -558,7 +703,7 @@ __global__ void __launch_bounds__(kSbThreads, 2) sample_batch_kernel(SampleParam
     auto tie_rank = [&](const float* v, unsigned long long& run) {
         uint32_t n = 0;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) n += sb_key(v[e]) == key ? 1u : 0u;
+        for (int e = 0; e < 8; ++e) n += v[e] == edge ? 1u : 0u;
         uint32_t inc = n;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -577,21 +722,23 @@ __global__ void __launch_bounds__(kSbThreads, 2) sample_batch_kernel(SampleParam
     };
     // a token's weight; `tie`: its rank, should it be a tie
     auto kept = [&](float v, unsigned long long& tie) {
-        const uint32_t k = sb_key(v);
-        const bool in = k > key || (ties && k == key && tie++ < (unsigned long long)ties);
+        const bool in = v > edge || (ties && v == edge && tie++ < (unsigned long long)ties);
         const float x = in ? r.expo(v) : 0.0f;
-        return sb_weight(x >= min_p || k == top ? x : 0.0f);
+        return sb_weight(x >= min_p || v == r.m ? x : 0.0f);
     };
     unsigned long long mine = 0, cta_before, cta_total, tie_run = ties_before;
     uint32_t round = 0;
     r.each_round([&](const float* v, uint32_t) {
         unsigned long long tie = ties ? tie_rank(v, tie_run) : 0ull;
         uint32_t hi = 0, lo = 0;
+        const float best = sb_max8(v);
+        if (best >= edge && best >= floor_p && best > -INFINITY) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const SbWeight w = kept(v[e], tie);
-            hi += w.hi - kSbBias;
-            lo += w.lo - kSbBias;
+            for (int e = 0; e < 8; ++e) {
+                const SbWeight w = kept(v[e], tie);
+                hi += w.hi - kSbBias;
+                lo += w.lo - kSbBias;
+            }
         }
         const unsigned long long s = warp_sum64(((unsigned long long)hi << 23) + lo);
         if (lane == 0) {
@@ -601,9 +748,7 @@ __global__ void __launch_bounds__(kSbThreads, 2) sample_batch_kernel(SampleParam
         ++round;
     });
     const unsigned long long total = r.sum(mine, &cta_before, &cta_total);
-    const float u = p.u[b];
-    unsigned long long target = (unsigned long long)((double)(u > 0.0f ? u : 0.0f) * (double)total);
-    if (target >= total) target = total - 1;
+    const unsigned long long target = sb_target(u, total);
     if (target < cta_before || target - cta_before >= cta_total) return;  // another CTA holds the token
 
     // The part that holds it, by the sums in order; a row with more parts is summed again.
@@ -622,10 +767,7 @@ __global__ void __launch_bounds__(kSbThreads, 2) sample_batch_kernel(SampleParam
         for (int e = 0; e < 8; ++e) {
             if (at <= target && target - at < w[e]) {
                 p.token[b] = (int32_t)(id + e);
-                if (p.logprob) {
-                    const float x = v[e] == r.m ? 0.0f : (v[e] - r.m) * r.inv;
-                    p.logprob[b] = x - logf(__ull2float_rn(total) / kSbUnit);
-                }
+                if (p.logprob) p.logprob[b] = (v[e] - r.m) * r.inv - logf(__ull2float_rn(total) / kSbUnit);
             }
             at += w[e];
         }
