@@ -10,6 +10,7 @@ followed and show in :meth:`KV4Cache.check`.
 from __future__ import annotations
 
 import ctypes as C
+from struct import Struct
 
 import torch
 
@@ -19,7 +20,16 @@ from .native import BT_BF16, BT_F16, BT_F32, KV4, KV4AttnArgs, QkArgs, SampleArg
 __all__ = ["KV4Cache", "qk_norm_rope", "rope_table", "sample_batch"]
 
 _DTYPES = {torch.float32: BT_F32, torch.float16: BT_F16, torch.bfloat16: BT_BF16}
-_NO_HEADS = (None, 0, 0)
+_NO_HEADS = (0, 0, 0)
+
+# The argument structs packed in one step: a call on one token is bound by the host, and a
+# ctypes structure takes several microseconds to fill.
+_pack_qk = Struct("<" + "Qqq" * 5 + "5Q6Iif")
+_pack_attn = Struct("<" + "Qqq" * 2 + "3Q6Iif")
+_pack_sample = Struct("<Qq7Q2IiI")
+assert (_pack_qk.size, _pack_attn.size, _pack_sample.size) == (C.sizeof(QkArgs), C.sizeof(KV4AttnArgs), C.sizeof(SampleArgs))
+
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _dtype(t) -> int:
@@ -29,38 +39,37 @@ def _dtype(t) -> int:
     return d
 
 
-def _heads(t, name, like=None, heads=None):
-    """(pointer, token stride, head stride) of a [tokens, heads, head_dim] tensor."""
+def _heads(t, name, shape=None, dtype=None, dev=None):
+    """(pointer, token stride, head stride) of a [tokens, heads, head_dim] tensor (of the given shape, type
+    and device)."""
     if t.dim() != 3 or not t.is_cuda:
         raise ValueError(f"{name}: expected a [tokens, heads, head_dim] CUDA tensor")
-    s = t.stride()
-    if s[2] != 1 and t.shape[2] > 1:
+    a, b, c = t.stride()
+    if c != 1 and t.shape[2] > 1:
         raise ValueError(f"{name}: the elements of a head must be contiguous")
-    if like is not None and (t.shape[0] != like.shape[0] or t.shape[2] != like.shape[2] or t.dtype != like.dtype
-                             or t.device != like.device or (heads is not None and t.shape[1] != heads)):
+    if shape is not None and (t.shape != shape or t.dtype is not dtype or t.get_device() != dev):
         raise ValueError(f"{name}: tokens, heads, head_dim, dtype or device do not match")
-    return t.data_ptr(), s[0], s[1]
+    return t.data_ptr(), a, b
 
 
-def _vector(t, name, n, dtype, device):
-    if t.dtype != dtype or t.device != device or t.numel() != n or not t.is_contiguous():
-        raise ValueError(f"{name}: expected {n} contiguous {dtype} values on {device}")
+def _vector(t, name, n, dtype, dev):
+    if t.dtype is not dtype or t.numel() != n or not t.is_contiguous() or not t.is_cuda or t.get_device() != dev:
+        raise ValueError(f"{name}: expected {n} contiguous {dtype} values on cuda:{dev}")
     return t.data_ptr()
 
 
-def _launch(name, device, stream, outs, *args):
+def _launch(fn, name, dev, stream, outs, *args):
     """The C call on the tensors' device; ``outs``: tensors allocated here for the call."""
-    fn = getattr(native.load(), name)
     if stream is None:
-        s = torch.cuda.current_stream(device).cuda_stream
+        s = _raw_stream(dev)
     else:
         s = stream.cuda_stream
         for t in outs:
             t.record_stream(stream)
-    if device.index == torch.cuda.current_device():
+    if dev == torch.cuda.current_device():
         rc = fn(*args, s)
     else:
-        with torch.cuda.device(device):
+        with torch.cuda.device(dev):
             rc = fn(*args, s)
     if rc:
         native.check(rc, name)
@@ -76,38 +85,41 @@ def rope_table(positions: int, rot_dim: int, theta: float = 10000.0, device="cud
     return torch.stack([angle.cos(), angle.sin()], -1).float().to(device)
 
 
-def _rope(table, device):
+def _rope(table, dev):
     if table is None:
-        return None, 0, 0
-    if table.dim() != 3 or table.shape[2] != 2 or table.dtype != torch.float32 or table.device != device or not table.is_contiguous():
+        return 0, 0, 0
+    if table.dim() != 3 or table.dtype is not torch.float32 or not table.is_contiguous() or not table.is_cuda or table.get_device() != dev:
         raise ValueError("table: expected a contiguous [positions, rot_dim / 2, 2] float32 tensor on the queries' device")
-    return table.data_ptr(), table.shape[0], 2 * table.shape[1]
+    n, half, two = table.shape
+    if two != 2:
+        raise ValueError("table: expected (cos, sin) pairs in its last dimension")
+    return table.data_ptr(), n, 2 * half
 
 
 def qk_norm_rope(q, k, q_weight, k_weight, positions, table, eps: float = 1e-5, q_out=None, k_out=None, stream=None):
     """Norms of each head of q [T, H, hd] and k [T, KVH, hd] and their rotation, one pass over both
     (bt_cuda_qk_norm_rope).  q_weight / k_weight: [hd] float32, or None for no norm; table: rope_table(),
     or None for no rotation; positions: [T] int32.  q_out / k_out may be q and k.  k may be None."""
-    hd = q.shape[-1]
     qh = _heads(q, "q")
-    dev, tokens = q.device, q.shape[0]
-    q_out = torch.empty_like(q, memory_format=torch.contiguous_format) if q_out is None else q_out
+    shape, dtype, dev = q.shape, q.dtype, q.get_device()
+    tokens, heads, hd = shape
+    q_out = q.new_empty(shape) if q_out is None else q_out
     outs = [q_out]
     kh = koh = _NO_HEADS
     kv_heads = 0
     if k is not None:
-        kh = _heads(k, "k", q)
-        kv_heads = k.shape[1]
-        k_out = torch.empty_like(k, memory_format=torch.contiguous_format) if k_out is None else k_out
-        koh = _heads(k_out, "k_out", q, kv_heads)
+        kv_heads = k.shape[1] if k.dim() == 3 else 0
+        k_shape = (tokens, kv_heads, hd)
+        kh = _heads(k, "k", k_shape, dtype, dev)
+        k_out = k.new_empty(k_shape) if k_out is None else k_out
+        koh = _heads(k_out, "k_out", k_shape, dtype, dev)
         outs.append(k_out)
-    rp, rn, rot = _rope(table, dev)
-    a = QkArgs(*qh, *kh, *_NO_HEADS, *_heads(q_out, "q_out", q, q.shape[1]), *koh,
-               None if q_weight is None else _vector(q_weight, "q_weight", hd, torch.float32, dev),
-               None if k_weight is None else _vector(k_weight, "k_weight", hd, torch.float32, dev),
-               _vector(positions, "positions", tokens, torch.int32, dev), None,
-               rp, rn, rot, tokens, q.shape[1], kv_heads, hd, _dtype(q), eps)
-    _launch("bt_cuda_qk_norm_rope", dev, stream, outs, C.byref(a))
+    a = _pack_qk.pack(*qh, *kh, *_NO_HEADS, *_heads(q_out, "q_out", shape, dtype, dev), *koh,
+                      0 if q_weight is None else _vector(q_weight, "q_weight", hd, torch.float32, dev),
+                      0 if k_weight is None else _vector(k_weight, "k_weight", hd, torch.float32, dev),
+                      _vector(positions, "positions", tokens, torch.int32, dev), 0,
+                      *_rope(table, dev), tokens, heads, kv_heads, hd, _dtype(q), eps)
+    _launch(native.load().bt_cuda_qk_norm_rope, "bt_cuda_qk_norm_rope", dev, stream, outs, a)
     return q_out, k_out
 
 
@@ -165,7 +177,8 @@ class KV4Cache:
         self._c = KV4(k_rows.data_ptr(), v_rows.data_ptr(), page_table.data_ptr() if self.paged else None,
                       self.status.data_ptr(), n_seq, max_seq, kv_heads, head_dim, self.page_tokens, self.n_pages,
                       self.max_pages, 0)
-        self._ref = C.byref(self._c)
+        self._ref = C.addressof(self._c)
+        self._index = device.index
 
     # ------------------------------------------------------------ pages
 
@@ -219,34 +232,37 @@ class KV4Cache:
         return self._append(q, k, v, q_weight, k_weight, slots, positions, table, eps, q_out, stream)
 
     def _append(self, q, k, v, q_weight, k_weight, slots, positions, table, eps, q_out, stream):
-        kh = _heads(k, "k")
-        dev, tokens, hd = k.device, k.shape[0], k.shape[2]
-        if k.shape[1] != self.kv_heads or hd != self.head_dim or dev != self.device:
-            raise ValueError("append: k must have the cache's kv_heads, head_dim and device")
+        if k.dim() != 3:
+            raise ValueError("append: expected [tokens, kv_heads, head_dim] tensors")
+        dev, hd, tokens, dtype = self._index, self.head_dim, k.shape[0], k.dtype
+        shape = (tokens, self.kv_heads, hd)  # of the cache
+        kh = _heads(k, "k", shape, dtype, dev)
         qh = qoh = _NO_HEADS
         heads, outs = 0, ()
         if q is not None:
-            qh, heads = _heads(q, "q", k), q.shape[1]
-            q_out = torch.empty_like(q, memory_format=torch.contiguous_format) if q_out is None else q_out
-            qoh, outs = _heads(q_out, "q_out", q, heads), (q_out,)
-        rp, rn, rot = _rope(table, dev)
-        a = QkArgs(*qh, *kh, *_heads(v, "v", k, self.kv_heads), *qoh, *_NO_HEADS,
-                   None if q_weight is None else _vector(q_weight, "q_weight", hd, torch.float32, dev),
-                   None if k_weight is None else _vector(k_weight, "k_weight", hd, torch.float32, dev),
-                   _vector(positions, "positions", tokens, torch.int32, dev), _vector(slots, "slots", tokens, torch.int32, dev),
-                   rp, rn, rot, tokens, heads, self.kv_heads, hd, _dtype(k), eps)
-        _launch("bt_cuda_kv4_append", dev, stream, outs, self._ref, C.byref(a))
+            heads = q.shape[1] if q.dim() == 3 else 0
+            q_shape = (tokens, heads, hd)
+            qh = _heads(q, "q", q_shape, dtype, dev)
+            q_out = q.new_empty(q_shape) if q_out is None else q_out
+            qoh, outs = _heads(q_out, "q_out", q_shape, dtype, dev), (q_out,)
+        a = _pack_qk.pack(*qh, *kh, *_heads(v, "v", shape, dtype, dev), *qoh, *_NO_HEADS,
+                          0 if q_weight is None else _vector(q_weight, "q_weight", hd, torch.float32, dev),
+                          0 if k_weight is None else _vector(k_weight, "k_weight", hd, torch.float32, dev),
+                          _vector(positions, "positions", tokens, torch.int32, dev), _vector(slots, "slots", tokens, torch.int32, dev),
+                          *_rope(table, dev), tokens, heads, self.kv_heads, hd, _dtype(k), eps)
+        _launch(native.load().bt_cuda_kv4_append, "bt_cuda_kv4_append", dev, stream, outs, self._ref, a)
         return q_out
 
     def read(self, slots, positions, dtype=torch.float16, stream=None):
         """The values that the rows at (slots[t], positions[t]) stand for: k, v [T, KVH, hd]."""
-        dev, tokens = self.device, positions.numel()
+        dev, tokens = self._index, positions.numel()
         if dtype not in _DTYPES:
             raise ValueError("read: dtype must be float32, float16 or bfloat16")
-        k = torch.empty((tokens, self.kv_heads, self.head_dim), dtype=dtype, device=dev)
+        k = torch.empty((tokens, self.kv_heads, self.head_dim), dtype=dtype, device=self.device)
         v = torch.empty_like(k)
-        _launch("bt_cuda_kv4_read", dev, stream, (k, v), self._ref, _vector(slots, "slots", tokens, torch.int32, dev),
-                _vector(positions, "positions", tokens, torch.int32, dev), tokens, _DTYPES[dtype], k.data_ptr(), v.data_ptr())
+        _launch(native.load().bt_cuda_kv4_read, "bt_cuda_kv4_read", dev, stream, (k, v), self._ref,
+                _vector(slots, "slots", tokens, torch.int32, dev), _vector(positions, "positions", tokens, torch.int32, dev),
+                tokens, _DTYPES[dtype], k.data_ptr(), v.data_ptr())
         return k, v
 
     # ------------------------------------------------------------ attention
@@ -261,24 +277,26 @@ class KV4Cache:
         slots [n] int32: the sequences' slots; None: sequence i is slot i.  max_q: no sequence has more
         queries (0: not known)."""
         qh = _heads(q, "q")
-        dev, tokens, heads, n = q.device, q.shape[0], q.shape[1], kv_len.numel()
-        if q.shape[2] != self.head_dim or dev != self.device:
+        dev, shape, n = self._index, q.shape, kv_len.numel()
+        tokens, heads, hd = shape
+        if hd != self.head_dim or q.get_device() != dev:
             raise ValueError("attention: q must have the cache's head_dim and device")
         if window < 0 or sinks < 0 or max_q < 0:
             raise ValueError("attention: window, sinks and max_q must not be negative")
-        out = torch.empty_like(q, memory_format=torch.contiguous_format) if out is None else out
-        a = KV4AttnArgs(*qh, *_heads(out, "out", q, heads), _vector(kv_len, "kv_len", n, torch.int32, dev),
-                        None if q_start is None else _vector(q_start, "q_start", n + 1, torch.int32, dev),
-                        None if slots is None else _vector(slots, "slots", n, torch.int32, dev),
-                        n, tokens, heads, max_q, window, sinks, _dtype(q), self.head_dim ** -0.5 if scale is None else scale)
-        s = (torch.cuda.current_stream(dev) if stream is None else stream).cuda_stream
+        out = q.new_empty(shape) if out is None else out
+        a = _pack_attn.pack(*qh, *_heads(out, "out", shape, q.dtype, dev), _vector(kv_len, "kv_len", n, torch.int32, dev),
+                            0 if q_start is None else _vector(q_start, "q_start", n + 1, torch.int32, dev),
+                            0 if slots is None else _vector(slots, "slots", n, torch.int32, dev),
+                            n, tokens, heads, max_q, window, sinks, _dtype(q), hd ** -0.5 if scale is None else scale)
+        s = _raw_stream(dev) if stream is None else stream.cuda_stream
         ws = self._workspaces.get(s)
         if ws is None:  # one for every stream that the calls come from
             with torch.cuda.device(dev):
                 size = native.load().bt_cuda_kv4_attention_workspace()
             with torch.cuda.stream(torch.cuda.current_stream(dev) if stream is None else stream):
-                ws = self._workspaces[s] = torch.zeros(size, dtype=torch.uint8, device=dev)
-        _launch("bt_cuda_kv4_attention", dev, stream, (out,), self._ref, C.byref(a), ws.data_ptr(), ws.numel())
+                ws = torch.zeros(size, dtype=torch.uint8, device=self.device)
+            ws = self._workspaces[s] = (ws.data_ptr(), size, ws)
+        _launch(native.load().bt_cuda_kv4_attention, "bt_cuda_kv4_attention", dev, stream, (out,), self._ref, a, ws[0], ws[1])
         return out
 
 
@@ -288,16 +306,16 @@ def sample_batch(logits, u, temperature=None, top_k=None, top_p=None, min_p=None
     None for none of that.  Returns (token [B] int32, logprob [B] float32)."""
     if logits.dim() != 2 or not logits.is_cuda or (logits.stride(1) != 1 and logits.shape[1] > 1):
         raise ValueError("sample_batch: expected a [rows, vocab] CUDA tensor with contiguous rows")
-    dev, (rows, vocab) = logits.device, logits.shape
+    dev, (rows, vocab) = logits.get_device(), logits.shape
     f32, i32 = torch.float32, torch.int32
-    token = torch.empty(rows, dtype=i32, device=dev) if token is None else token
-    logprob = torch.empty(rows, dtype=f32, device=dev) if logprob is None else logprob
-    a = SampleArgs(logits.data_ptr(), logits.stride(0), _vector(u, "u", rows, f32, dev),
-                   None if temperature is None else _vector(temperature, "temperature", rows, f32, dev),
-                   None if top_k is None else _vector(top_k, "top_k", rows, i32, dev),
-                   None if top_p is None else _vector(top_p, "top_p", rows, f32, dev),
-                   None if min_p is None else _vector(min_p, "min_p", rows, f32, dev),
-                   _vector(token, "token", rows, i32, dev), _vector(logprob, "logprob", rows, f32, dev),
-                   rows, vocab, _dtype(logits), 0)
-    _launch("bt_cuda_sample_batch", dev, stream, (token, logprob), C.byref(a))
+    token = torch.empty(rows, dtype=i32, device=logits.device) if token is None else token
+    logprob = torch.empty(rows, dtype=f32, device=logits.device) if logprob is None else logprob
+    a = _pack_sample.pack(logits.data_ptr(), logits.stride(0), _vector(u, "u", rows, f32, dev),
+                          0 if temperature is None else _vector(temperature, "temperature", rows, f32, dev),
+                          0 if top_k is None else _vector(top_k, "top_k", rows, i32, dev),
+                          0 if top_p is None else _vector(top_p, "top_p", rows, f32, dev),
+                          0 if min_p is None else _vector(min_p, "min_p", rows, f32, dev),
+                          _vector(token, "token", rows, i32, dev), _vector(logprob, "logprob", rows, f32, dev),
+                          rows, vocab, _dtype(logits), 0)
+    _launch(native.load().bt_cuda_sample_batch, "bt_cuda_sample_batch", dev, stream, (token, logprob), a)
     return token, logprob
