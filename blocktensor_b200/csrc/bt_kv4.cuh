@@ -41,19 +41,35 @@ inline bool heads_wide(const bt_heads& h, int dtype) {
     return !h.data || ((uintptr_t)h.data % 16 == 0 && (h.token_stride * b) % 16 == 0 && (h.head_stride * b) % 16 == 0);
 }
 
-// Eight consecutive elements as fp32.  `wide`: the address is 16-byte aligned.
+// Eight consecutive elements as they are.  `wide`: the address is 16-byte aligned.
+template <typename T>
+union Raw8 {
+    uint4 u[sizeof(T) / 2];
+    T t[8];
+    __device__ Raw8() {}
+    __device__ __forceinline__ void load(const T* p, bool wide) {
+        if (wide) {
+#pragma unroll
+            for (int i = 0; i < (int)(sizeof(T) / 2); ++i) u[i] = reinterpret_cast<const uint4*>(p)[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) t[i] = p[i];
+        }
+    }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < (int)(sizeof(T) / 2); ++i) u[i] = make_uint4(0, 0, 0, 0);
+    }
+    __device__ __forceinline__ void get(float (&x)[8]) const {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = Act<T>::to_f(t[i]);
+    }
+};
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, bool wide, float (&x)[8]) {
-    union { uint4 u[sizeof(T) / 2]; T t[8]; } r;
-    if (wide) {
-#pragma unroll
-        for (int i = 0; i < (int)(sizeof(T) / 2); ++i) r.u[i] = reinterpret_cast<const uint4*>(p)[i];
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) r.t[i] = p[i];
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = Act<T>::to_f(r.t[i]);
+    Raw8<T> r;
+    r.load(p, wide);
+    r.get(x);
 }
 
 template <typename T>

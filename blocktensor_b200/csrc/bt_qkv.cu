@@ -107,19 +107,30 @@ __global__ void __launch_bounds__(kQkvThreads) qkv_kernel(QkvParams p) {
     }
     if (!in_table && threadIdx.x == 0 && blockIdx.y == 0 && APPEND && slot >= 0) p.map.flag(BT_KV4_RANGE);
 
-    // whole warps loop together (the shuffles need every lane); rows past the end are idle
-    const uint32_t step = RPI * gridDim.y;
-    for (uint32_t r0 = blockIdx.y * RPI; r0 < rows; r0 += step) {
-        const uint32_t r = r0 + threadIdx.x / LPR;
-        const bool on = r < rows;
-        const bool is_q = r < n_q, is_k = !is_q && r < n_q + (p.k ? p.kv_heads : 0);
-        const uint32_t h = is_q ? r : is_k ? r - n_q : r - n_q - (p.k ? p.kv_heads : 0);
-        float x[8] = {};
-        if (on) {
-            const T* src = is_q ? (const T*)p.q + t * p.q_ts + h * p.q_hs
-                         : is_k ? (const T*)p.k + t * p.k_ts + h * p.k_hs : (const T*)p.v + t * p.v_ts + h * p.v_hs;
-            load8(src + 8 * l, p.wide, x);
-        }
+    // Whole warps loop together (the shuffles need every lane); rows past the end are idle.
+    // The next kAhead sets of rows are on their way while one is worked on: 36 warps an SM
+    // with one 16-byte load a lane each are 18 KB in flight, less than half of what the
+    // memory's latency takes.
+    constexpr int kAhead = 2;
+    const uint32_t step = RPI * gridDim.y, n_qk = n_q + (p.k ? p.kv_heads : 0);
+    auto load = [&](uint32_t r, Raw8<T>& x) {
+        if (r >= rows) { x.zero(); return; }
+        const T* src = r < n_q ? (const T*)p.q + t * p.q_ts + r * p.q_hs
+                     : r < n_qk ? (const T*)p.k + t * p.k_ts + (r - n_q) * p.k_hs : (const T*)p.v + t * p.v_ts + (r - n_qk) * p.v_hs;
+        x.load(src + 8 * l, p.wide);
+    };
+    const uint32_t r_first = blockIdx.y * RPI + threadIdx.x / LPR;
+    Raw8<T> ahead[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) load(r_first + i * step, ahead[i]);
+    for (uint32_t r0 = blockIdx.y * RPI, r = r_first; r0 < rows; r0 += step, r += step) {
+        float x[8];
+        ahead[0].get(x);
+#pragma unroll
+        for (int i = 0; i + 1 < kAhead; ++i) ahead[i] = ahead[i + 1];
+        load(r + kAhead * step, ahead[kAhead - 1]);
+        const bool on = r < rows, is_q = r < n_q, is_k = !is_q && r < n_qk;
+        const uint32_t h = is_q ? r : is_k ? r - n_q : r - n_qk;
         const float* w = is_q ? p.qw : is_k ? p.kw : nullptr;
         float ss = 0.0f;
 #pragma unroll
@@ -148,7 +159,8 @@ __global__ void __launch_bounds__(kQkvThreads) qkv_kernel(QkvParams p) {
         } else if (!APPEND && on) {
             store8((T*)p.k_out + t * p.ko_ts + h * p.ko_hs + 8 * l, p.wide, x);
         }
-        if (APPEND) {
+        // (the warp's last row: a warp of queries alone has nothing to store in the cache)
+        if (APPEND && r0 + (threadIdx.x | 31) / LPR >= n_q) {
             uint32_t pair;
             const uint32_t code = quantise8(x, &pair);
             if (on && !is_q && row0 >= 0 && in_table) {
