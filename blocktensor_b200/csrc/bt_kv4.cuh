@@ -41,49 +41,68 @@ inline bool heads_wide(const bt_heads& h, int dtype) {
     return !h.data || ((uintptr_t)h.data % 16 == 0 && (h.token_stride * b) % 16 == 0 && (h.head_stride * b) % 16 == 0);
 }
 
-// Eight consecutive elements as they are.  `wide`: the address is 16-byte aligned.
-template <typename T>
-union Raw8 {
-    uint4 u[sizeof(T) / 2];
-    T t[8];
-    __device__ Raw8() {}
+// N consecutive elements as they are.  `wide`: the address allows accesses of all N
+// (at most 16 bytes at a time).
+template <typename T, int N>
+union RawN {
+    static constexpr int WORDS = N * (int)sizeof(T) / 4, PIECE = WORDS >= 4 ? 4 : 2;
+    uint32_t w[WORDS];
+    T t[N];
+    __device__ RawN() {}
     __device__ __forceinline__ void load(const T* p, bool wide) {
         if (wide) {
 #pragma unroll
-            for (int i = 0; i < (int)(sizeof(T) / 2); ++i) u[i] = reinterpret_cast<const uint4*>(p)[i];
+            for (int i = 0; i < WORDS / PIECE; ++i) {
+                if (PIECE == 4) {
+                    const uint4 v = reinterpret_cast<const uint4*>(p)[i];
+                    w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+                } else {
+                    const uint2 v = reinterpret_cast<const uint2*>(p)[i];
+                    w[2 * i] = v.x; w[2 * i + 1] = v.y;
+                }
+            }
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) t[i] = p[i];
+            for (int i = 0; i < N; ++i) t[i] = p[i];
+        }
+    }
+    __device__ __forceinline__ void store(T* p, bool wide) const {
+        if (wide) {
+#pragma unroll
+            for (int i = 0; i < WORDS / PIECE; ++i) {
+                if (PIECE == 4) reinterpret_cast<uint4*>(p)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+                else reinterpret_cast<uint2*>(p)[i] = make_uint2(w[2 * i], w[2 * i + 1]);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) p[i] = t[i];
         }
     }
     __device__ __forceinline__ void zero() {
 #pragma unroll
-        for (int i = 0; i < (int)(sizeof(T) / 2); ++i) u[i] = make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < WORDS; ++i) w[i] = 0;
     }
-    __device__ __forceinline__ void get(float (&x)[8]) const {
+    __device__ __forceinline__ void get(float (&x)[N]) const {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = Act<T>::to_f(t[i]);
+        for (int i = 0; i < N; ++i) x[i] = Act<T>::to_f(t[i]);
+    }
+    __device__ __forceinline__ void set(const float (&x)[N]) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) t[i] = Act<T>::from_f(x[i]);
     }
 };
 template <typename T>
 __device__ __forceinline__ void load8(const T* p, bool wide, float (&x)[8]) {
-    Raw8<T> r;
+    RawN<T, 8> r;
     r.load(p, wide);
     r.get(x);
 }
 
 template <typename T>
 __device__ __forceinline__ void store8(T* p, bool wide, const float (&x)[8]) {
-    union { uint4 u[sizeof(T) / 2]; T t[8]; } r;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) r.t[i] = Act<T>::from_f(x[i]);
-    if (wide) {
-#pragma unroll
-        for (int i = 0; i < (int)(sizeof(T) / 2); ++i) reinterpret_cast<uint4*>(p)[i] = r.u[i];
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) p[i] = r.t[i];
-    }
+    RawN<T, 8> r;
+    r.set(x);
+    r.store(p, wide);
 }
 
 // ---------------------------------------------------------------- the cache

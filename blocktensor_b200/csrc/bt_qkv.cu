@@ -7,13 +7,17 @@
 //   (y_i, y_{i + rot/2}) <- (y_i cos - y_{i + rot/2} sin, y_i sin + y_{i + rot/2} cos)
 // and for the cache, per 64 elements, scale and min in fp16 and 4-bit codes.
 //
-// Bound: memory (7 operations for the 4 to 8 bytes an element moves).  Layout: a
-// lane holds 8 consecutive elements of a row (one or two 16-byte loads), a row is
-// head_dim / 8 lanes, so sums and the rotation's partner are a few shuffles and a
-// group of 64 is 8 lanes whose codes are one 32-bit word each.  A CTA works on one
-// token: a lane keeps its cos/sin and weights in registers and takes the token's
-// head rows in turn, so the table's row is read once per token and not once per
-// head.  With few tokens the heads of a token are spread over blockIdx.y.
+// Bound: memory (7 operations for the 4 to 8 bytes an element moves), with the issue
+// slots close behind.  Layout: a row is head_dim / 8 lanes, a lane holds the four
+// elements from 4l and the four that they are rotated with, from rot / 2 + 4l, so the
+// rotation needs no exchange (with 8 consecutive elements a lane, 8 shuffles and as many
+// selects of about 110 instructions); sums are 3 to 5 shuffles.  Rows that go to the
+// cache take 8 consecutive elements a lane instead: a group of 64 is 8 lanes then, whose
+// codes are one 32-bit word each.  A CTA works on one token: a lane keeps its rotation
+// and weights, multiplied, in registers and takes the token's head rows in turn, queries,
+// keys and values each in a loop of their own (one loop over all of them spends a third of
+// its instructions on addresses), so the table's row is read once per token and not once
+// per head.  With few tokens the rows of a token are spread over blockIdx.y.
 #include "bt_kv4.cuh"
 
 namespace bt {
@@ -70,105 +74,173 @@ __device__ __forceinline__ uint32_t quantise8(const float (&y)[8], uint32_t* pai
     return w;
 }
 
-template <typename T, int HD, bool APPEND>
-__global__ void __launch_bounds__(kQkvThreads) qkv_kernel(QkvParams p) {
-    constexpr int LPR = HD / 8, RPI = kQkvThreads / LPR;  // lanes of a row, rows of a CTA at a time
-    const uint32_t t = blockIdx.x, l = threadIdx.x % LPR;
-    const uint32_t rows = (p.q ? p.heads : 0) + (p.k ? p.kv_heads : 0) + (APPEND ? p.kv_heads : 0);
-    const uint32_t n_q = p.q ? p.heads : 0;
+template <typename T, int HD, bool APPEND, bool WIDE>
+__global__ void __launch_bounds__(kQkvThreads, 8) qkv_kernel(const __grid_constant__ QkvParams p) {
+    constexpr int LPR = HD / 8, RPI = kQkvThreads / LPR;  // lanes of a row, rows of a set
+    const uint32_t t = blockIdx.x, l = threadIdx.x % LPR, in_set = threadIdx.x / LPR;
+    const uint32_t n_q = p.q ? p.heads : 0, n_k = p.k ? p.kv_heads : 0;
+    const uint32_t q_sets = (n_q + RPI - 1) / RPI, k_sets = (n_k + RPI - 1) / RPI;
     const int32_t pos = p.positions[t];
-
-    // this lane's rotation: elements 8l .. 8l+7 pair with those of lane l +- rot / 16
-    const uint32_t half_lanes = p.rot / 16;
-    const bool turned = p.rope && l < 2 * half_lanes;
-    const bool second = l >= half_lanes;
     const bool in_table = !p.rope || (uint32_t)pos < p.rope_positions;
-    const int partner = (int)(threadIdx.x & 31) + (turned ? (second ? -(int)half_lanes : (int)half_lanes) : 0);
-    float2 cs[8];
-    if (turned && in_table) {
-        const float4* src = reinterpret_cast<const float4*>(p.rope + (size_t)pos * (p.rot / 2) + 8 * (second ? l - half_lanes : l));
+    int64_t row0 = -1;  // the cache row of KV head 0
+    if (APPEND) {
+        const int32_t slot = p.slots[t];
+        row0 = p.map.row(slot, 0, pos);
+        if (slot >= 0 && (row0 < 0 || !in_table) && threadIdx.x == 0 && blockIdx.y == 0) p.map.flag(BT_KV4_RANGE);
+        if (!in_table) row0 = -1;
+    }
+
+    // This lane's elements in the paired layout, and what multiplies them.
+    const uint32_t half = p.rot / 2;
+    const bool turned = l < p.rot / 8;
+    const uint32_t at_a = turned ? 4 * l : 8 * l, at_b = turned ? half + 4 * l : 8 * l + 4;
+    float ac[4], as[4], bc[4], bs[4];  // weights times cos and sin
+    auto weights = [&](const float* w) {
+        float wa[4] = {1, 1, 1, 1}, wb[4] = {1, 1, 1, 1};
+        if (w) {
+            const float4 a = __ldg(reinterpret_cast<const float4*>(w + at_a)), b = __ldg(reinterpret_cast<const float4*>(w + at_b));
+            wa[0] = a.x; wa[1] = a.y; wa[2] = a.z; wa[3] = a.w;
+            wb[0] = b.x; wb[1] = b.y; wb[2] = b.z; wb[3] = b.w;
+        }
+        float2 cs[4] = {make_float2(1, 0), make_float2(1, 0), make_float2(1, 0), make_float2(1, 0)};
+        if (!in_table) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) cs[i] = make_float2(NAN, NAN);
+        } else if (turned) {
+            const float4* src = reinterpret_cast<const float4*>(p.rope + (size_t)pos * half + 4 * l);
+            const float4 x = __ldg(src), y = __ldg(src + 1);
+            cs[0] = make_float2(x.x, x.y); cs[1] = make_float2(x.z, x.w); cs[2] = make_float2(y.x, y.y); cs[3] = make_float2(y.z, y.w);
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float4 f = __ldg(src + i);
-            cs[2 * i] = make_float2(f.x, f.y);
-            cs[2 * i + 1] = make_float2(f.z, f.w);
+            ac[i] = wa[i] * cs[i].x; as[i] = wa[i] * cs[i].y;
+            bc[i] = wb[i] * cs[i].x; bs[i] = wb[i] * cs[i].y;
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) cs[i] = make_float2(1.0f, 0.0f);
-    }
-    const float sign = second ? 1.0f : -1.0f;
-    int32_t slot = 0;
-    int64_t row0 = -1;
-    if (APPEND) {
-        slot = p.slots[t];
-        row0 = p.map.row(slot, 0, pos);
-        if (row0 < 0 && slot >= 0 && threadIdx.x == 0 && blockIdx.y == 0) p.map.flag(BT_KV4_RANGE);
-    }
-    if (!in_table && threadIdx.x == 0 && blockIdx.y == 0 && APPEND && slot >= 0) p.map.flag(BT_KV4_RANGE);
-
-    // Whole warps loop together (the shuffles need every lane); rows past the end are idle.
-    // The next kAhead sets of rows are on their way while one is worked on: 36 warps an SM
-    // with one 16-byte load a lane each are 18 KB in flight, less than half of what the
-    // memory's latency takes.
-    constexpr int kAhead = 2;
-    const uint32_t step = RPI * gridDim.y, n_qk = n_q + (p.k ? p.kv_heads : 0);
-    auto load = [&](uint32_t r, Raw8<T>& x) {
-        if (r >= rows) { x.zero(); return; }
-        const T* src = r < n_q ? (const T*)p.q + t * p.q_ts + r * p.q_hs
-                     : r < n_qk ? (const T*)p.k + t * p.k_ts + (r - n_q) * p.k_hs : (const T*)p.v + t * p.v_ts + (r - n_qk) * p.v_hs;
-        x.load(src + 8 * l, p.wide);
     };
-    const uint32_t r_first = blockIdx.y * RPI + threadIdx.x / LPR;
-    Raw8<T> ahead[kAhead];
+
+    // A set is RPI rows, one for each LPR lanes; this CTA takes every gridDim.y-th of a part's
+    // sets, kTogether of them loaded before the first is worked on.
+    const uint32_t gap = RPI * gridDim.y;
+    auto turned_rows = [&](const void* from, int64_t hs, void* to, int64_t ths, uint32_t n, const float* w, uint32_t first) {
+        constexpr int kTogether = 2;
+        uint32_t h = first * RPI;
+        bool ready = false;
+        const T* src = (const T*)from + (int64_t)(h + in_set) * hs;
+        T* dst = (T*)to + (int64_t)(h + in_set) * ths;
+        const int64_t step = (int64_t)gap * hs, to_step = (int64_t)gap * ths;
+        for (; h < n; h += kTogether * gap) {
+            RawN<T, 4> xa[kTogether], xb[kTogether];
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i) load(r_first + i * step, ahead[i]);
-    for (uint32_t r0 = blockIdx.y * RPI, r = r_first; r0 < rows; r0 += step, r += step) {
-        float x[8];
-        ahead[0].get(x);
-#pragma unroll
-        for (int i = 0; i + 1 < kAhead; ++i) ahead[i] = ahead[i + 1];
-        load(r + kAhead * step, ahead[kAhead - 1]);
-        const bool on = r < rows, is_q = r < n_q, is_k = !is_q && r < n_qk;
-        const uint32_t h = is_q ? r : is_k ? r - n_q : r - n_qk;
-        const float* w = is_q ? p.qw : is_k ? p.kw : nullptr;
-        float ss = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
-        ss = row_sum<LPR>(ss);
-        if (w) {
-            const float inv = rsqrtf(ss * (1.0f / HD) + p.eps);
-            const float4 w0 = __ldg(reinterpret_cast<const float4*>(w + 8 * l)), w1 = __ldg(reinterpret_cast<const float4*>(w + 8 * l) + 1);
-            x[0] *= inv * w0.x; x[1] *= inv * w0.y; x[2] *= inv * w0.z; x[3] *= inv * w0.w;
-            x[4] *= inv * w1.x; x[5] *= inv * w1.y; x[6] *= inv * w1.z; x[7] *= inv * w1.w;
-        }
-        if (p.rope) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float o = __shfl_sync(0xffffffffu, x[i], partner);
-                // first half: a cos - b sin; second half: b cos + a sin
-                if (turned && (is_q || is_k)) x[i] = in_table ? x[i] * cs[i].x + sign * o * cs[i].y : NAN;
+            for (int k = 0; k < kTogether; ++k) {
+                if (h + k * gap + in_set < n) {
+                    xa[k].load(src + k * step + at_a, WIDE);
+                    xb[k].load(src + k * step + at_b, WIDE);
+                } else {
+                    xa[k].zero();
+                    xb[k].zero();
+                }
             }
-            if (!in_table && !turned) {
+            if (!ready) { weights(w); ready = true; }  // (while the rows are on their way)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = NAN;
+            for (int k = 0; k < kTogether; ++k) {
+                if (h + k * gap >= n) break;  // (the whole CTA's set)
+                float a[4], b[4], inv = 1.0f;
+                xa[k].get(a);
+                xb[k].get(b);
+                if (w) {
+                    float ss = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) ss = fmaf(a[i], a[i], fmaf(b[i], b[i], ss));
+                    inv = rsqrtf(row_sum<LPR>(ss) * (1.0f / HD) + p.eps);
+                }
+                float ya[4], yb[4];
+                if (turned) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        ya[i] = (a[i] * ac[i] - b[i] * bs[i]) * inv;
+                        yb[i] = (a[i] * as[i] + b[i] * bc[i]) * inv;
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) { ya[i] = a[i] * ac[i] * inv; yb[i] = b[i] * bc[i] * inv; }
+                }
+                if (h + k * gap + in_set < n) {
+                    RawN<T, 4> r;
+                    r.set(ya);
+                    r.store(dst + k * to_step + at_a, WIDE);
+                    r.set(yb);
+                    r.store(dst + k * to_step + at_b, WIDE);
+                }
+            }
+            src += kTogether * step;
+            dst += kTogether * to_step;
+        }
+    };
+    // Keys (normed and rotated) or values into the cache.
+    auto cached_rows = [&](const void* from, int64_t hs, uint8_t* rows, const float* w, bool keys, uint32_t first) {
+        constexpr int kTogether = 2;
+        uint32_t h = first * RPI;
+        const uint32_t n = n_k;
+        const T* src = (const T*)from + (int64_t)(h + in_set) * hs + 8 * l;
+        const int64_t step = (int64_t)gap * hs;
+        for (; h < n; h += kTogether * gap, src += kTogether * step) {
+            RawN<T, 8> raw[kTogether];
+#pragma unroll
+            for (int k = 0; k < kTogether; ++k) {
+                if (h + k * gap + in_set < n) raw[k].load(src + k * step, WIDE);
+                else raw[k].zero();
+            }
+#pragma unroll
+            for (int k = 0; k < kTogether; ++k) {
+                if (h + k * gap >= n) break;
+                float x[8];
+                raw[k].get(x);
+                if (w) {
+                    float ss = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
+                    const float inv = rsqrtf(row_sum<LPR>(ss) * (1.0f / HD) + p.eps);
+                    const float4 w0 = __ldg(reinterpret_cast<const float4*>(w + 8 * l)), w1 = __ldg(reinterpret_cast<const float4*>(w + 8 * l) + 1);
+                    x[0] *= inv * w0.x; x[1] *= inv * w0.y; x[2] *= inv * w0.z; x[3] *= inv * w0.w;
+                    x[4] *= inv * w1.x; x[5] *= inv * w1.y; x[6] *= inv * w1.z; x[7] *= inv * w1.w;
+                }
+                if (keys && p.rope && in_table) {
+                    // elements 8l .. 8l + 7 pair with those of lane l +- rot / 16
+                    const uint32_t lanes = p.rot / 16;
+                    const bool turn = l < 2 * lanes, second = l >= lanes;
+                    const int partner = (int)(threadIdx.x & 31) + (turn ? (second ? -(int)lanes : (int)lanes) : 0);
+                    const float4* cs = reinterpret_cast<const float4*>(p.rope + (size_t)pos * half + 8 * (turn ? (second ? l - lanes : l) : 0));
+#pragma unroll
+                    for (int i = 0; i < 8; i += 2) {
+                        const float4 c = __ldg(cs + i / 2);
+                        const float o0 = __shfl_sync(0xffffffffu, x[i], partner), o1 = __shfl_sync(0xffffffffu, x[i + 1], partner);
+                        // first half: a cos - b sin; second half: b cos + a sin
+                        if (turn) {
+                            x[i] = x[i] * c.x + (second ? o0 : -o0) * c.y;
+                            x[i + 1] = x[i + 1] * c.z + (second ? o1 : -o1) * c.w;
+                        }
+                    }
+                }
+                uint32_t pair;
+                const uint32_t code = quantise8(x, &pair);
+                const uint32_t row_h = h + k * gap + in_set;
+                if (row_h < n && row0 >= 0) {
+                    uint8_t* dst = rows + (size_t)(row0 + (int64_t)row_h * p.map.page_tokens) * kv4_row_bytes(HD);
+                    reinterpret_cast<uint32_t*>(dst)[l] = code;
+                    if (l % 8 == 0) reinterpret_cast<uint32_t*>(dst + HD / 2)[l / 8] = pair;
+                }
             }
         }
-        if (is_q && on) {
-            store8((T*)p.q_out + t * p.qo_ts + h * p.qo_hs + 8 * l, p.wide, x);
-        } else if (!APPEND && on) {
-            store8((T*)p.k_out + t * p.ko_ts + h * p.ko_hs + 8 * l, p.wide, x);
-        }
-        // (the warp's last row: a warp of queries alone has nothing to store in the cache)
-        if (APPEND && r0 + (threadIdx.x | 31) / LPR >= n_q) {
-            uint32_t pair;
-            const uint32_t code = quantise8(x, &pair);
-            if (on && !is_q && row0 >= 0 && in_table) {
-                uint8_t* dst = (is_k ? p.map.k : p.map.v) + (size_t)(row0 + (int64_t)h * p.map.page_tokens) * kv4_row_bytes(HD);
-                reinterpret_cast<uint32_t*>(dst)[l] = code;
-                if (l % 8 == 0) reinterpret_cast<uint32_t*>(dst + HD / 2)[l / 8] = pair;
-            }
-        }
+    };
+    // the sets of all parts go round the CTAs of the token in order
+    const uint32_t y = blockIdx.y, gy = gridDim.y;
+    auto first_set = [&](uint32_t before) { return (y + gy - before % gy) % gy; };
+    if (p.q) turned_rows((const T*)p.q + t * p.q_ts, p.q_hs, (T*)p.q_out + t * p.qo_ts, p.qo_hs, n_q, p.qw, y);
+    if (APPEND) {
+        cached_rows((const T*)p.k + t * p.k_ts, p.k_hs, p.map.k, p.kw, true, first_set(q_sets));
+        cached_rows((const T*)p.v + t * p.v_ts, p.v_hs, p.map.v, nullptr, false, first_set(q_sets + k_sets));
+    } else if (p.k) {
+        turned_rows((const T*)p.k + t * p.k_ts, p.k_hs, (T*)p.k_out + t * p.ko_ts, p.ko_hs, n_k, p.kw, first_set(q_sets));
     }
 }
 
@@ -264,19 +336,21 @@ static int qkv_launch(const bt_qk_args* a, const bt_kv4* cache, const char* who,
     p.heads = a->heads; p.kv_heads = a->kv_heads; p.eps = a->eps;
     p.wide = heads_wide(a->q, a->dtype) && heads_wide(a->k, a->dtype) && heads_wide(a->q_out, a->dtype) &&
              (append ? heads_wide(a->v, a->dtype) : heads_wide(a->k_out, a->dtype));
-    const uint32_t rows = (p.q ? p.heads : 0) + (p.k ? p.kv_heads : 0) + (append ? p.kv_heads : 0);
-    const uint32_t per = kQkvThreads / (a->head_dim / 8), passes = (rows + per - 1) / per;
+    const uint32_t per = kQkvThreads / (a->head_dim / 8);
+    const uint32_t sets = (p.q ? (p.heads + per - 1) / per : 0) + (p.k ? (append ? 2 : 1) * ((p.kv_heads + per - 1) / per) : 0);
     // about four CTAs per SM before a CTA takes more than one set of rows
     uint32_t gy = a->tokens >= 592 ? 1 : (592 + a->tokens - 1) / a->tokens;
-    if (gy > passes) gy = passes;
+    if (gy > sets) gy = sets;
     const dim3 grid(a->tokens, gy);
     const cudaStream_t s = as_stream(stream);
     g_launches.fetch_add(1, std::memory_order_relaxed);
     auto go = [&](auto type, auto hd) {
         using T = decltype(type);
         constexpr int HD = decltype(hd)::value;
-        if (append) qkv_kernel<T, HD, true><<<grid, kQkvThreads, 0, s>>>(p);
-        else qkv_kernel<T, HD, false><<<grid, kQkvThreads, 0, s>>>(p);
+        if (append && p.wide) qkv_kernel<T, HD, true, true><<<grid, kQkvThreads, 0, s>>>(p);
+        else if (append) qkv_kernel<T, HD, true, false><<<grid, kQkvThreads, 0, s>>>(p);
+        else if (p.wide) qkv_kernel<T, HD, false, true><<<grid, kQkvThreads, 0, s>>>(p);
+        else qkv_kernel<T, HD, false, false><<<grid, kQkvThreads, 0, s>>>(p);
     };
     auto by_hd = [&](auto type) {
         if (a->head_dim == 64) go(type, std::integral_constant<int, 64>());
