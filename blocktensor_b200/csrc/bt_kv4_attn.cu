@@ -321,10 +321,12 @@ __global__ void __launch_bounds__(AttnCfg<HD, TERMS>::NW * 32, 1) kv4_attn_kerne
                 const uint32_t d = lane * E + e, n = d % 8;
                 const uint32_t step_k = d / 64 * 4 + d / 8 % 2 * 2 + (n >> 1 & 1);
                 const uint32_t to = ((step_k * 32 + c * 4 + d / 16 % 4) * 2 + (n & 1)) * 4 + (n >> 2) * 2;
-                const float v = n & 1 ? x[e] * 0.0625f : x[e];  // codes of odd places weigh 16 times as much
-                const __half hi = __float2half_rn(v);
-                *reinterpret_cast<__half*>(qfrag + to) = hi;
-                if (TERMS == 2) *reinterpret_cast<__half*>(qfrag + NG * 4 * 256 + to) = __float2half_rn(v - __half2float(hi));
+                const float odd = n & 1 ? 0.0625f : 1.0f;  // codes of odd places weigh 16 times as much
+                // Two terms: whole multiples of 2^3 and of 2^-9 (11 bits each), so that an MMA's sums
+                // are exact whatever bits it drops when it aligns them.
+                const float hi = TERMS == 2 ? rintf(x[e] * 0x1p-3f) * 0x1p3f : x[e];
+                *reinterpret_cast<__half*>(qfrag + to) = __float2half_rn(hi * odd);
+                if (TERMS == 2) *reinterpret_cast<__half*>(qfrag + NG * 4 * 256 + to) = __float2half_rn(rintf((x[e] - hi) * 0x1p9f) * 0x1p-9f * odd);
             }
 #pragma unroll
             for (int o = 1; o < 64 / E; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -360,6 +362,7 @@ __global__ void __launch_bounds__(AttnCfg<HD, TERMS>::NW * 32, 1) kv4_attn_kerne
         int v_exp = 0;              // p s is multiplied by 2^v_exp
         float v_mul = 1.0f;
 
+        constexpr float kLazy = TERMS == 2 ? 0.0f : kLazyMax;
         const uint32_t r0 = key_of(g), r1 = r0 + 2;                  // keys of MMA rows g and g + 8
         const uint32_t ra = key_of(2 * t), rb = key_of(2 * t + 1);   // and of rows 2t, 2t + 1 (+ 8: + 2)
         const uint32_t k_at = r0 * C::RB + 8 * t, e_at = r0 * C::RB + HD / 2;
@@ -396,22 +399,30 @@ __global__ void __launch_bounds__(AttnCfg<HD, TERMS>::NW * 32, 1) kv4_attn_kerne
                     const uint2 va = *reinterpret_cast<const uint2*>(pa), vb = *reinterpret_cast<const uint2*>(pb);
                     a[0] = va.x; a[1] = va.y; b[0] = vb.x; b[1] = vb.y;
                 }
-                float c[4] = {};
+                float c[4] = {}, low[4] = {};
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const uint32_t a8 = a[h] >> 8, b8 = b[h] >> 8;
-                    const uint32_t f0[4] = {a[h] & 0x000f000fu, b[h] & 0x000f000fu, a[h] & 0x00f000f0u, b[h] & 0x00f000f0u};
-                    const uint32_t f1[4] = {a8 & 0x000f000fu, b8 & 0x000f000fu, a8 & 0x00f000f0u, b8 & 0x00f000f0u};
+                    const uint32_t f0[4] = {codes<TERMS, 0>(a[h]), codes<TERMS, 0>(b[h]), codes<TERMS, 1>(a[h]), codes<TERMS, 1>(b[h])};
+                    const uint32_t f1[4] = {codes<TERMS, 0>(a8), codes<TERMS, 0>(b8), codes<TERMS, 1>(a8), codes<TERMS, 1>(b8)};
                     const int k = 4 * j + 2 * h;
                     mma_f16(c, f0[0], f0[1], f0[2], f0[3], qf[k][0], qf[k][1]);
                     mma_f16(c, f1[0], f1[1], f1[2], f1[3], qf[k + 1][0], qf[k + 1][1]);
                     if (TERMS == 2) {
-                        mma_f16(c, f0[0], f0[1], f0[2], f0[3], ql[k][0], ql[k][1]);
-                        mma_f16(c, f1[0], f1[1], f1[2], f1[3], ql[k + 1][0], ql[k + 1][1]);
+                        mma_f16(low, f0[0], f0[1], f0[2], f0[3], ql[k][0], ql[k][1]);
+                        mma_f16(low, f1[0], f1[1], f1[2], f1[3], ql[k + 1][0], ql[k + 1][1]);
                     }
                 }
-                const float2 e0 = unpack_half2(*reinterpret_cast<const uint32_t*>(kt + e_at + 4 * j));
-                const float2 e1 = unpack_half2(*reinterpret_cast<const uint32_t*>(kt + e_at + 2 * C::RB + 4 * j));
+                if (TERMS == 2) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) c[i] += low[i];
+                }
+                float2 e0 = unpack_half2(*reinterpret_cast<const uint32_t*>(kt + e_at + 4 * j));
+                float2 e1 = unpack_half2(*reinterpret_cast<const uint32_t*>(kt + e_at + 2 * C::RB + 4 * j));
+                if (TERMS == 2) {  // (of codes less 8)
+                    e0.y = fmaf(8.0f, e0.x, e0.y);
+                    e1.y = fmaf(8.0f, e1.x, e1.y);
+                }
                 s[0] = fmaf(e0.x, c[0], fmaf(e0.y, qsum[j][0], s[0]));
                 s[1] = fmaf(e0.x, c[1], fmaf(e0.y, qsum[j][1], s[1]));
                 s[2] = fmaf(e1.x, c[2], fmaf(e1.y, qsum[j][0], s[2]));
@@ -437,7 +448,7 @@ __global__ void __launch_bounds__(AttnCfg<HD, TERMS>::NW * 32, 1) kv4_attn_kerne
             }
             uint32_t big = big2 & 0xffffu;
             const float top0 = fmaxf(s[0], s[2]), top1 = fmaxf(s[1], s[3]);
-            if (__any_sync(0xffffffffu, top0 > m[0] + kLazyMax || top1 > m[1] + kLazyMax || big > v_bound)) {
+            if (__any_sync(0xffffffffu, top0 > m[0] + kLazy || top1 > m[1] + kLazy || big > v_bound)) {
                 float a = top0, b = top1;
 #pragma unroll
                 for (int x = 4; x < 32; x <<= 1) {
@@ -452,8 +463,8 @@ __global__ void __launch_bounds__(AttnCfg<HD, TERMS>::NW * 32, 1) kv4_attn_kerne
                 big = __reduce_max_sync(0xffffffffu, big);
                 float fv = 1.0f;
                 if (big > v_bound) {
-                    // s < 2^(x + 1): p s 2^v_exp stays below 2^15 with p <= 2^8
-                    const int x = max((int)(big >> 10), 1) - 15, e = 6 - x;
+                    // s < 2^(x + 1): p s 2^v_exp stays below 2^15 with p <= 2^kLazy
+                    const int x = max((int)(big >> 10), 1) - 15, e = 14 - (int)kLazy - x;
                     fv = v_bound ? __int_as_float((127 + e - v_exp) << 23) : 0.0f;
                     v_exp = e;
                     v_mul = __int_as_float((127 + e) << 23);
@@ -476,29 +487,49 @@ __global__ void __launch_bounds__(AttnCfg<HD, TERMS>::NW * 32, 1) kv4_attn_kerne
 #pragma unroll
             for (int j = 0; j < NG; ++j) {
                 const float2 x0 = unpack_half2(ev[0][j]), x1 = unpack_half2(ev[1][j]);
-                mo[j][0] = fmaf(s[0], x0.y, fmaf(s[2], x1.y, mo[j][0]));
-                mo[j][1] = fmaf(s[1], x0.y, fmaf(s[3], x1.y, mo[j][1]));
+                const float mid0 = fmaf(8.0f, x0.x, x0.y), mid1 = fmaf(8.0f, x1.x, x1.y);  // what code 8 stands for
+                mo[j][0] = fmaf(s[0], mid0, fmaf(s[2], mid1, mo[j][0]));
+                mo[j][1] = fmaf(s[1], mid0, fmaf(s[3], mid1, mo[j][1]));
                 const float s0 = x0.x * v_mul, s1 = x1.x * v_mul;
-                const uint32_t h0 = pack_half2(s[0] * s0, s[1] * s0), h1 = pack_half2(s[2] * s1, s[3] * s1);
-                const uint32_t b0 = transpose8(h0), b1 = transpose8(h1);
+                float w[4] = {s[0] * s0, s[1] * s0, s[2] * s1, s[3] * s1};
                 uint32_t b2 = 0, b3 = 0;
-                if (TERMS == 2) {
-                    const float2 y0 = unpack_half2(h0), y1 = unpack_half2(h1);
-                    b2 = transpose8(pack_half2(fmaf(s[0], s0, -y0.x), fmaf(s[1], s0, -y0.y)));
-                    b3 = transpose8(pack_half2(fmaf(s[2], s1, -y1.x), fmaf(s[3], s1, -y1.y)));
+                if (TERMS == 2) {  // whole multiples of 2^4 and 2^-8, as the queries (by additions that round there)
+                    float r[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float hi = __fsub_rn(__fadd_rn(w[i], 0x1.8p27f), 0x1.8p27f);
+                        r[i] = __fsub_rn(__fadd_rn(w[i] - hi, 0x1.8p15f), 0x1.8p15f);
+                        w[i] = hi;
+                    }
+                    b2 = transpose8(pack_half2(r[0], r[1]));
+                    b3 = transpose8(pack_half2(r[2], r[3]));
                 }
+                const uint32_t b0 = transpose8(pack_half2(w[0], w[1])), b1 = transpose8(pack_half2(w[2], w[3]));
                 const uint32_t va = *reinterpret_cast<const uint32_t*>(kt + va_at + 32 * j), vb = *reinterpret_cast<const uint32_t*>(kt + vb_at + 32 * j);
                 const uint32_t vc = *reinterpret_cast<const uint32_t*>(kt + va_at + 32 * j + 2 * C::RB), vd = *reinterpret_cast<const uint32_t*>(kt + vb_at + 32 * j + 2 * C::RB);
                 uint32_t f[4] = {__byte_perm(va, vb, 0x5410), __byte_perm(va, vb, 0x7632), __byte_perm(vc, vd, 0x5410), __byte_perm(vc, vd, 0x7632)};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {  // dims 8g + i (rows g) and 8g + i + 4 (rows g + 8) of the group
-                    const uint32_t mask = i & 1 ? 0x00f000f0u : 0x000f000fu;
                     if (i == 2) {
 #pragma unroll
                         for (int k = 0; k < 4; ++k) f[k] >>= 8;
                     }
-                    mma_f16(o[4 * j + i], f[0] & mask, f[1] & mask, f[2] & mask, f[3] & mask, b0, b1);
-                    if (TERMS == 2) mma_f16(o[4 * j + i], f[0] & mask, f[1] & mask, f[2] & mask, f[3] & mask, b2, b3);
+                    uint32_t a[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) a[k] = i & 1 ? codes<TERMS, 1>(f[k]) : codes<TERMS, 0>(f[k]);
+                    if (TERMS == 1) {
+                        const uint32_t eight = i & 1 ? 0x80808080u : 0x80088008u;  // minus code 8
+                        mma_f16(o[4 * j + i], eight, eight, eight, eight, b0, b1);
+                    }
+                    if (TERMS == 1) {
+                        mma_f16(o[4 * j + i], a[0], a[1], a[2], a[3], b0, b1);
+                    } else {
+                        float t[4] = {}, low[4] = {};
+                        mma_f16(t, a[0], a[1], a[2], a[3], b0, b1);
+                        mma_f16(low, a[0], a[1], a[2], a[3], b2, b3);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) o[4 * j + i][k] += t[k] + low[k];
+                    }
                 }
             }
         };

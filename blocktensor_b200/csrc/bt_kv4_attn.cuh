@@ -4,13 +4,21 @@
 // Mathematics.  Eight (query, head) columns that share a KV head go over 16-key
 // tiles.  With codes c, and (s, m) the pair of a key's 64-element group j,
 //   score[key][col] = sum_j s_j (sum_{i in j} c_i q_i) + m_j (sum_{i in j} q_i)
-//   out[col][d]     = sum_key (p s_j) c_d + sum_key p m_j,     d in group j
+//   out[col][d]     = sum_key (p s_j) (c_d - 8) + sum_key p (m_j + 8 s_j),   d in group j
 // so the tensor cores only ever see codes, which are exact in fp16: a code's four
 // bits masked into the low mantissa bits of a half are the subnormal c 2^-24 (or
 // c 2^-20 from the next nibble up), one logical operation for two codes and no
 // conversion.  s and m stay in fp32.  The queries (scaled by a power of two per
 // column so that both terms stay normal) are exact for fp16 and bf16 inputs and two
-// fp16 terms (22 bits) for fp32; p s_j likewise is one or two terms.
+// fp16 terms (22 bits) for fp32; p s_j likewise is one or two terms.  The 8 is there
+// because the sums of c and of m are many times their difference, which makes p's
+// rounding and the tensor cores' truncated accumulation come out as much larger.  For
+// 16-bit types an MMA with a constant operand takes it off O (the tensor pipe is a sixth
+// busy; fp16 error 3.8e-4 -> 2.7e-4, of which 2.1e-4 are the result's own rounding).  For
+// fp32 the codes themselves are lowered, of K too: between two MMAs the sum would still
+// be large (550 keys: error 3e-5 with c, 1.4e-5 with two MMAs, 5.5e-6 so).  And both
+// terms of fp32 queries and of p s_j are whole multiples of a step each, so that an MMA's
+// sums are exact: the tensor cores drop low bits when they align products (1.1e-6).
 //
 // mma.sync m16n8k16: scores have the 16 keys as M, the 8 columns as N; out has 16
 // dims as M and the tile's 16 keys as K.  tcgen05 has no use here: M is the cache's
@@ -55,6 +63,17 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Two codes of a word (bits 0-3 or, ODD, 4-7 of its halves) as fp16: c 2^-24 or c 2^-20;
+// with two terms (c - 8) instead of c.
+template <int TERMS, int ODD>
+__device__ __forceinline__ uint32_t codes(uint32_t w) {
+    const uint32_t c = w & (ODD ? 0x00f000f0u : 0x000f000fu);
+    if (TERMS == 1) return c;
+    const uint32_t eight = ODD ? 0x80808080u : 0x80088008u;
+    const __half2 r = __hadd2(*reinterpret_cast<const __half2*>(&c), *reinterpret_cast<const __half2*>(&eight));
+    return *reinterpret_cast<const uint32_t*>(&r);
 }
 
 // 8x8 transpose of halves over the warp: lane (g, t) gives row g, columns 2t, 2t+1
