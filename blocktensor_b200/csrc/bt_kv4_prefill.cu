@@ -49,6 +49,7 @@ struct PfCfg {
     static constexpr uint32_t IDESC_O = (1u << 4) | ((HD >> 3) << 17) | ((128u >> 4) << 24);
 };
 
+constexpr uint32_t kPfSeqs = 64;
 struct PfShared {
     uint64_t raw_full[2][kPfRaw], raw_empty[2][kPfRaw];        // of K, of V
     uint64_t full[2][kPfStages], empty[2][kPfStages];
@@ -56,6 +57,7 @@ struct PfShared {
     uint32_t pieces[16];  // of a tile: which of its 16-key pieces hold keys
     uint32_t tmem;
     volatile uint32_t dead;  // a wait gave up: everybody leaves
+    SeqWork seq[kPfSeqs];    // the first sequences, so that finding a block waits for no memory
 };
 
 // MMAs issued by one elected lane of a converged warp: A and B in shared memory, or A in
@@ -138,15 +140,19 @@ __device__ __forceinline__ int32_t window_start(const AttnParams& p, int32_t pos
     return p.window && pos >= 0 && (uint32_t)pos >= p.window ? pos - (int32_t)p.window : -1;
 }
 
+__device__ __forceinline__ SeqWork pf_seq(const AttnParams& p, const PfShared& sh, uint32_t i) {
+    return i < kPfSeqs ? sh.seq[i] : seq_work(p, i, false);
+}
+
 // Walks all blocks in order; every lane of a warp calls it alike.
 struct PfWalk {
     uint32_t s0;     // first sequence of the 32 that the lanes look at
     uint64_t base;   // blocks before them
-    __device__ __forceinline__ bool find(const AttnParams& p, uint64_t b, uint32_t lane, PfItem* it) {
+    __device__ __forceinline__ bool find(const AttnParams& p, const PfShared& sh, uint64_t b, uint32_t lane, PfItem* it) {
         for (; s0 < p.n; s0 += 32) {
             uint32_t own = 0;
             if (s0 + lane < p.n) {
-                const SeqWork w = seq_work(p, s0 + lane, false);
+                const SeqWork w = pf_seq(p, sh, s0 + lane);
                 const uint32_t rows = (uint32_t)w.count * p.group;
                 own = rows > p.few_rows ? (rows + 255) / 256 * p.map.kv_heads : 0;
             }
@@ -160,7 +166,7 @@ struct PfWalk {
             if (b < base + all) {
                 const uint32_t hit = __ffs(__ballot_sync(0xffffffffu, b < base + inc)) - 1;
                 const uint32_t at = (uint32_t)(b - base - __shfl_sync(0xffffffffu, inc - own, hit));
-                it->w = seq_work(p, s0 + hit, false);
+                it->w = pf_seq(p, sh, s0 + hit);
                 const uint32_t total = (uint32_t)it->w.count * p.group, blocks = (total + 255) / 256;
                 const uint32_t block = blocks - 1 - at / p.map.kv_heads;  // longest first
                 it->head = at % p.map.kv_heads;
@@ -228,6 +234,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
         sh.dead = 0;
         fence_mbar_init();
     }
+    if (tid < kPfSeqs && tid < p.n) sh.seq[tid] = seq_work(p, tid, false);
     tcgen05_fence_before();
     __syncthreads();
     tcgen05_fence_after();
@@ -263,7 +270,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
         const uint32_t lanes = tmem + ((warp & 3) * 32u << 16), o_at = lanes + 256 + r * 128;
         const float sign = p.scale_log2 < 0.0f ? -1.0f : 1.0f;
         uint32_t done = 0, o_phase = 0;  // tiles this half has done
-        for (uint32_t turn = 0; walk.find(p, block_of(turn), lane, &it); ++turn) {
+        for (uint32_t turn = 0; walk.find(p, sh, block_of(turn), lane, &it); ++turn) {
             if (it.rows <= r * 128) { tile_no += it.tiles; continue; }
             const bool there = r * 128 + row < it.rows;
             const uint32_t c = it.row0 + r * 128 + (there ? row : 0);
@@ -276,10 +283,13 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
                 // the row as fp16, scaled so that its largest element is in [2^13, 2^14)
                 const T* src = (const T*)p.q + token * p.q_ts + head * p.q_hs;
                 float big = 0.0f;
-#pragma unroll 4
+                RawN<T, 8> raw[CH];
+#pragma unroll
+                for (int k = 0; k < CH; ++k) raw[k].load(src + 8 * k, p.wide);
+#pragma unroll
                 for (int k = 0; k < CH; ++k) {
                     float x[8];
-                    load8(src + 8 * k, p.wide, x);
+                    raw[k].get(x);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(x[e]));
                 }
@@ -288,10 +298,10 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
                 const bool flat = p.scale_log2 == 0.0f;  // all scores equal: f stays positive
                 const float mul = there && !flat ? sign * __int_as_float((127 + up) << 23) : 0.0f;
                 f = flat ? 1.0f : fabsf(p.scale_log2) * __int_as_float((127 - up) << 23);
-#pragma unroll 4
+#pragma unroll
                 for (int k = 0; k < CH; ++k) {
                     float x[8];
-                    load8(src + 8 * k, p.wide, x);
+                    raw[k].get(x);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) x[e] = there ? x[e] * mul : 0.0f;
                     uint4 v;
@@ -403,7 +413,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
         uint8_t* raw = raws + side * kPfRaw * C::RAW;
         uint8_t* to = kvs + side * kPfStages * C::KV;
         uint32_t raw_at = 0, raw_phase = 0, st = 0, st_phase = 1;
-        for (uint32_t turn = 0; walk.find(p, block_of(turn), lane, &it); ++turn) {
+        for (uint32_t turn = 0; walk.find(p, sh, block_of(turn), lane, &it); ++turn) {
             bool ok = true;
             for (uint32_t i = 0; i < it.tiles; ++i) {
                 if (!(ok = warp_wait(&sh.raw_full[side][raw_at], raw_phase) && warp_wait(&sh.empty[side][st], st_phase))) break;
@@ -476,7 +486,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
         if (blockIdx.x == 0) {
             for (uint32_t i = lane; i < p.n; i += 32) seq_work(p, i, true);  // reports what is out of range
         }
-        for (uint32_t turn = 0; walk.find(p, block_of(turn), lane, &it); ++turn) {
+        for (uint32_t turn = 0; walk.find(p, sh, block_of(turn), lane, &it); ++turn) {
             bool ok = true;
             for (uint32_t i = 0; i < it.tiles; ++i) {
                 const int32_t key = it.key0(i) + 16 * (int32_t)lane;
@@ -531,7 +541,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
             ++made;
             return true;
         };
-        for (uint32_t turn = 0; walk.find(p, block_of(turn), lane, &it); ++turn) {
+        for (uint32_t turn = 0; walk.find(p, sh, block_of(turn), lane, &it); ++turn) {
             bool ok = true;
             if (it.rows <= r * 128) {  // nothing in this half: the tiles pass by
                 for (uint32_t i = 0; i < it.tiles; ++i) {

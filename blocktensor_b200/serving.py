@@ -42,14 +42,22 @@ def _dtype(t) -> int:
 def _heads(t, name, shape=None, dtype=None, dev=None):
     """(pointer, token stride, head stride) of a [tokens, heads, head_dim] tensor (of the given shape, type
     and device)."""
-    if t.dim() != 3 or not t.is_cuda:
+    strides = t.stride()
+    if len(strides) != 3 or not t.is_cuda:
         raise ValueError(f"{name}: expected a [tokens, heads, head_dim] CUDA tensor")
-    a, b, c = t.stride()
-    if c != 1 and t.shape[2] > 1:
+    if strides[2] != 1 and t.shape[2] > 1:
         raise ValueError(f"{name}: the elements of a head must be contiguous")
     if shape is not None and (t.shape != shape or t.dtype is not dtype or t.get_device() != dev):
         raise ValueError(f"{name}: tokens, heads, head_dim, dtype or device do not match")
-    return t.data_ptr(), a, b
+    return t.data_ptr(), strides[0], strides[1]
+
+
+def _out(t, name, shape, like, dev):
+    """(tensor, (pointer, strides)): the caller's output, checked, or a new one."""
+    if t is None:
+        t = like.new_empty(shape)
+        return t, (t.data_ptr(), shape[1] * shape[2], shape[2])
+    return t, _heads(t, name, shape, like.dtype, dev)
 
 
 def _vector(t, name, n, dtype, dev):
@@ -103,7 +111,7 @@ def qk_norm_rope(q, k, q_weight, k_weight, positions, table, eps: float = 1e-5, 
     qh = _heads(q, "q")
     shape, dtype, dev = q.shape, q.dtype, q.get_device()
     tokens, heads, hd = shape
-    q_out = q.new_empty(shape) if q_out is None else q_out
+    q_out, qoh = _out(q_out, "q_out", shape, q, dev)
     outs = [q_out]
     kh = koh = _NO_HEADS
     kv_heads = 0
@@ -111,10 +119,9 @@ def qk_norm_rope(q, k, q_weight, k_weight, positions, table, eps: float = 1e-5, 
         kv_heads = k.shape[1] if k.dim() == 3 else 0
         k_shape = (tokens, kv_heads, hd)
         kh = _heads(k, "k", k_shape, dtype, dev)
-        k_out = k.new_empty(k_shape) if k_out is None else k_out
-        koh = _heads(k_out, "k_out", k_shape, dtype, dev)
+        k_out, koh = _out(k_out, "k_out", k_shape, k, dev)
         outs.append(k_out)
-    a = _pack_qk.pack(*qh, *kh, *_NO_HEADS, *_heads(q_out, "q_out", shape, dtype, dev), *koh,
+    a = _pack_qk.pack(*qh, *kh, *_NO_HEADS, *qoh, *koh,
                       0 if q_weight is None else _vector(q_weight, "q_weight", hd, torch.float32, dev),
                       0 if k_weight is None else _vector(k_weight, "k_weight", hd, torch.float32, dev),
                       _vector(positions, "positions", tokens, torch.int32, dev), 0,
@@ -243,8 +250,8 @@ class KV4Cache:
             heads = q.shape[1] if q.dim() == 3 else 0
             q_shape = (tokens, heads, hd)
             qh = _heads(q, "q", q_shape, dtype, dev)
-            q_out = q.new_empty(q_shape) if q_out is None else q_out
-            qoh, outs = _heads(q_out, "q_out", q_shape, dtype, dev), (q_out,)
+            q_out, qoh = _out(q_out, "q_out", q_shape, q, dev)
+            outs = (q_out,)
         a = _pack_qk.pack(*qh, *kh, *_heads(v, "v", shape, dtype, dev), *qoh, *_NO_HEADS,
                           0 if q_weight is None else _vector(q_weight, "q_weight", hd, torch.float32, dev),
                           0 if k_weight is None else _vector(k_weight, "k_weight", hd, torch.float32, dev),
@@ -283,8 +290,8 @@ class KV4Cache:
             raise ValueError("attention: q must have the cache's head_dim and device")
         if window < 0 or sinks < 0 or max_q < 0:
             raise ValueError("attention: window, sinks and max_q must not be negative")
-        out = q.new_empty(shape) if out is None else out
-        a = _pack_attn.pack(*qh, *_heads(out, "out", shape, q.dtype, dev), _vector(kv_len, "kv_len", n, torch.int32, dev),
+        out, oh = _out(out, "out", shape, q, dev)
+        a = _pack_attn.pack(*qh, *oh, _vector(kv_len, "kv_len", n, torch.int32, dev),
                             0 if q_start is None else _vector(q_start, "q_start", n + 1, torch.int32, dev),
                             0 if slots is None else _vector(slots, "slots", n, torch.int32, dev),
                             n, tokens, heads, max_q, window, sinks, _dtype(q), hd ** -0.5 if scale is None else scale)
