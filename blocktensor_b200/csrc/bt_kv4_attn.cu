@@ -741,12 +741,15 @@ static cudaError_t attn_launch(const AttnParams& p, int sms, cudaStream_t s) {
 
 using namespace bt;
 
-// tickets of every range, then two pieces for each
+// Tickets, then partial results: two pieces for every range of the few-row kernel, or the
+// prefill kernel's parts (the two run one after the other).
 static uint64_t ticket_bytes(int sms) { return ((uint64_t)sms * kMaxGroups * 4 + 255) / 256 * 256; }
 
 extern "C" uint64_t bt_cuda_kv4_attention_workspace(void) {
     const int sms = device_sms();
-    return sms > 0 ? ticket_bytes(sms) + (uint64_t)sms * kMaxGroups * 2 * kPieceFloats * 4 : 0;
+    if (sms <= 0) return 0;
+    const uint64_t few = (uint64_t)sms * kMaxGroups * 2 * kPieceFloats * 4, many = prefill_workspace(sms);
+    return ticket_bytes(sms) + (few > many ? few : many);
 }
 
 extern "C" int bt_cuda_kv4_attention(const bt_kv4* cache, const bt_kv4_attn_args* a, void* workspace,
@@ -776,10 +779,15 @@ extern "C" int bt_cuda_kv4_attention(const bt_kv4* cache, const bt_kv4_attn_args
     p.partial = (float*)((uint8_t*)workspace + ticket_bytes(sms));
     const cudaStream_t s = as_stream(stream);
     // Sequences with many rows go to the tcgen05 kernel, which unpacks a tile once for 256 rows
-    // instead of once for 8 but takes a whole tile's time for any number of them.
+    // instead of once for 8 but takes a whole tile's time for any number of them.  Measured, us,
+    // few-row kernel / tcgen05: 1 sequence, 8 KV heads of 128, 8192 keys: 32 rows 24 / 41, 64 rows
+    // 35 / 42, 128 rows 60 / 42; 512 keys: 64 rows 13 / 21, 256 rows 25 / 29, 512 rows 31 / 29.
+    // 8 sequences, 4 KV heads of 64, 8192 keys: 16 rows 26 / 42, 32 rows 44 / 42, 64 rows 70 / 42;
+    // 512 keys: 32 rows 15 / 16, 64 rows 20 / 16.
+    const uint32_t few_rows = (uint64_t)a->n * cache->kv_heads >= 16 ? 32 : 64;
     const uint64_t most = (uint64_t)(!a->q_start ? 1 : a->max_q ? a->max_q : a->tokens) * p.group;
-    const bool many = prefill_takes(a->dtype, cache->head_dim) && most > kFewRows;
-    p.few_rows = !many ? 0xffffffffu : a->n == 1 ? 0 : kFewRows;
+    const bool many = prefill_takes(a->dtype, cache->head_dim) && most > few_rows;
+    p.few_rows = !many ? 0xffffffffu : a->n == 1 ? 0 : few_rows;
     if (many) BT_CUDA_CHECK(launch_kv4_prefill(p, a->dtype, cache->head_dim, sms, s));
     if (p.few_rows == 0) return BT_OK;
     auto by_hd = [&](auto type, auto terms) {

@@ -50,9 +50,9 @@ struct AttnParams {
 // The many-row kernel (bt_kv4_prefill.cu): whether it takes a type and head_dim, and its
 // launch over the sequences with more than few_rows rows.
 bool prefill_takes(int dtype, uint32_t head_dim);
+uint64_t prefill_workspace(int sms);  // bytes of its partial results
 cudaError_t launch_kv4_prefill(const AttnParams& p, int dtype, uint32_t head_dim, int sms, cudaStream_t s);
 
-constexpr uint32_t kFewRows = 64;     // see bt_cuda_kv4_attention
 constexpr float kLazyMax = 8.0f;     // a row's reference maximum may be exceeded by 2^8 before it moves
 constexpr float kNothing = -1e30f;   // a row's maximum before it sees a key (finite: differences stay defined)
 

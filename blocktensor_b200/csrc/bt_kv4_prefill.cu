@@ -24,7 +24,10 @@
 // buffers of the halves in columns 0 and 128, O in 256 and 384.
 //
 // A CTA is resident on an SM and takes blocks of rows in turn, those with the
-// longest keys first.  V's rows (the N of P V) are stored in the order e, chunk of
+// longest keys first.  Where there are less than half as many blocks as SMs, the tiles of
+// a block are cut into up to sqrt(tiles) equal parts, one a CTA; the parts' O, m and l go to the workspace,
+// and the CTA that finds itself last (an atomic ticket) adds them in order (8 blocks over
+// 8192 keys: 120 -> 41 us).  V's rows (the N of P V) are stored in the order e, chunk of
 // d = 8 chunk + e, so that the unpackers' 16-byte stores of neighbouring lanes are
 // contiguous; K's and Q's elements of 8 are in the order 0 4 1 5 2 6 3 7, in which a
 // word's codes come out two at a time.
@@ -39,6 +42,9 @@ constexpr int kPfSoftmax = 128, kPfUnpack = 80, kPfRest = 56;
 static_assert(2 * kPfSoftmax + 2 * kPfUnpack + kPfRest <= 5 * 96, "no more than the block is launched with");
 constexpr uint32_t kPfRaw = 3;     // packed K (and V) tiles in flight
 constexpr uint32_t kPfStages = 4;  // unpacked K (and V) tiles
+
+// Floats of a part in the workspace: O of 256 rows, and their m and l.
+template <int HD> constexpr size_t kPfPiece = 256 * HD + 512;
 
 template <int HD>
 struct PfCfg {
@@ -57,6 +63,7 @@ struct PfShared {
     uint32_t pieces[16];  // of a tile: which of its 16-key pieces hold keys
     uint32_t tmem;
     volatile uint32_t dead;  // a wait gave up: everybody leaves
+    uint32_t last;           // this CTA's part of a block is the last to be done
     SeqWork seq[kPfSeqs];    // the first sequences, so that finding a block waits for no memory
 };
 
@@ -126,9 +133,11 @@ struct PfItem {
     SeqWork w;
     uint32_t head, row0, rows;  // rows row0 .. of the sequence's count * group
     int32_t top, above;         // positions seen: (above, top] and [0, sinks)
-    uint32_t tiles, sink_tiles;
+    uint32_t tiles, sink_tiles; // of this part
     int32_t lo;
-    __device__ __forceinline__ int32_t key0(uint32_t t) const {
+    uint32_t tile0, parts;      // the part's first tile; parts of the block
+    __device__ __forceinline__ int32_t key0(uint32_t i) const {
+        const uint32_t t = tile0 + i;
         return (int32_t)t * kPfKeys + (t < sink_tiles ? 0 : lo - (int32_t)sink_tiles * kPfKeys);
     }
     __device__ __forceinline__ bool any(int32_t k, int32_t n, uint32_t sinks) const {
@@ -148,14 +157,26 @@ __device__ __forceinline__ SeqWork pf_seq(const AttnParams& p, const PfShared& s
 struct PfWalk {
     uint32_t s0;     // first sequence of the 32 that the lanes look at
     uint64_t base;   // blocks before them
-    __device__ __forceinline__ bool find(const AttnParams& p, const PfShared& sh, uint64_t b, uint32_t lane, PfItem* it) {
+    uint32_t parts;  // of every block
+    // blocks of sequence i
+    __device__ __forceinline__ uint32_t blocks_of(const AttnParams& p, const PfShared& sh, uint32_t i) const {
+        if (i >= p.n) return 0;
+        const uint32_t rows = (uint32_t)pf_seq(p, sh, i).count * p.group;
+        return rows > p.few_rows ? (rows + 255) / 256 * p.map.kv_heads : 0;
+    }
+    __device__ __forceinline__ void start(const AttnParams& p, const PfShared& sh, uint32_t lane) {
+        s0 = 0;
+        base = 0;
+        uint64_t all = 0;
+        for (uint32_t i = lane; i < p.n; i += 32) all += blocks_of(p, sh, i);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) all += __shfl_xor_sync(0xffffffffu, all, o);
+        parts = all > 0 && all * 2 <= gridDim.x ? gridDim.x / (uint32_t)all : 1;
+    }
+    __device__ __forceinline__ bool find(const AttnParams& p, const PfShared& sh, uint64_t unit, uint32_t lane, PfItem* it) {
+        const uint64_t b = parts > 1 ? (uint32_t)unit / parts : unit;
         for (; s0 < p.n; s0 += 32) {
-            uint32_t own = 0;
-            if (s0 + lane < p.n) {
-                const SeqWork w = pf_seq(p, sh, s0 + lane);
-                const uint32_t rows = (uint32_t)w.count * p.group;
-                own = rows > p.few_rows ? (rows + 255) / 256 * p.map.kv_heads : 0;
-            }
+            const uint32_t own = blocks_of(p, sh, s0 + lane);
             uint64_t inc = own;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -178,6 +199,15 @@ struct PfWalk {
                 it->lo = (it->above + 1) & ~(kPfKeys - 1);
                 it->sink_tiles = p.window ? min((min(p.sinks, 0x7fffff00u) + kPfKeys - 1) / kPfKeys, (uint32_t)it->lo / kPfKeys) : 0;
                 it->tiles = it->top < 0 ? 0 : it->sink_tiles + (uint32_t)(it->top - it->lo) / kPfKeys + 1;
+                it->tile0 = 0;
+                it->parts = 1;
+                if (parts > 1) {
+                    // adding up a part costs about as much as a tile: sqrt(tiles) parts are best
+                    const uint32_t n = it->parts = min(parts, max(1u, (uint32_t)sqrtf((float)it->tiles))), part = (uint32_t)unit % parts;
+                    it->tile0 = it->tiles * part / n;
+                    it->tiles = it->tiles * (part + 1) / n - it->tile0;
+                    if (part >= n) it->rows = it->tiles = 0;  // nothing left for this CTA
+                }
                 return true;
             }
             base += all;
@@ -259,8 +289,9 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
     auto block_of = [&](uint32_t turn) {
         return (uint64_t)turn * gridDim.x + (turn & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
     };
-    PfItem it;
-    PfWalk walk = {0, 0};
+    PfItem it = {};
+    PfWalk walk;
+    walk.start(p, sh, lane);
     uint32_t tile_no = 0;  // tiles before the item, over all of this CTA's items
 
     if (warp < 8) {
@@ -270,6 +301,17 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
         const uint32_t lanes = tmem + ((warp & 3) * 32u << 16), o_at = lanes + 256 + r * 128;
         const float sign = p.scale_log2 < 0.0f ? -1.0f : 1.0f;
         uint32_t done = 0, o_phase = 0;  // tiles this half has done
+        auto meet = [&](uint32_t block_no) {  // both halves have written their part: sh.last, whether the block is complete
+            const uint32_t threads = it.rows > 128 ? 256 : 128;
+            asm volatile("bar.sync 2, %0;" ::"r"(threads) : "memory");
+            if (tid == 0) {
+                __threadfence();
+                sh.last = atomicAdd(p.tickets + block_no, 1u) == it.parts - 1;
+                if (sh.last) p.tickets[block_no] = 0;  // ready for the next call
+                __threadfence();
+            }
+            asm volatile("bar.sync 2, %0;" ::"r"(threads) : "memory");
+        };
         for (uint32_t turn = 0; walk.find(p, sh, block_of(turn), lane, &it); ++turn) {
             if (it.rows <= r * 128) { tile_no += it.tiles; continue; }
             const bool there = r * 128 + row < it.rows;
@@ -382,25 +424,80 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
                 if (lane == 0) mbar_arrive(&sh.p_full[r][buf]);
                 ++done;
             }
-            if (!ok) break;
             tile_no += it.tiles;
-            if (it.tiles) {
-                if (!warp_wait(&sh.o_full[r], o_phase)) break;
+            if (ok && it.tiles) {
+                ok = warp_wait(&sh.o_full[r], o_phase);
                 o_phase ^= 1;
                 tcgen05_fence_after();
             }
-            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            if (!ok) {
+                if (it.parts > 1) meet((uint32_t)block_of(turn) / walk.parts);  // the other half may be waiting here
+                break;
+            }
+            const uint32_t parts = it.parts, at = r * 128 + row, unit = (uint32_t)block_of(turn), block_no = unit / walk.parts;
+            // a part: O as [HD / 4][256] float4 (columns as in tensor memory), then (m, l) of the rows
+            auto part_o = [&](uint32_t k) { return reinterpret_cast<float4*>(p.partial + (size_t)(block_no * walk.parts + k) * kPfPiece<HD>); };
+            auto part_ml = [&](uint32_t k) { return reinterpret_cast<float2*>(part_o(k) + HD / 4 * 256); };
+            float scale = l == 0.0f ? 0.0f : 1.0f / l;
+            if (parts > 1) {
+                __stcg(part_ml(unit % walk.parts) + at, make_float2(m, l));
+                if (it.tiles) {
+#pragma unroll 1
+                    for (int h = 0; h < HD / 16; ++h) {
+                        uint32_t o[16];
+                        tmem_ld16(o_at + 16 * h, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            __stcg(part_o(unit % walk.parts) + (4 * h + k) * 256 + at, make_float4(__uint_as_float(o[4 * k]), __uint_as_float(o[4 * k + 1]),
+                                                                                      __uint_as_float(o[4 * k + 2]), __uint_as_float(o[4 * k + 3])));
+                    }
+                }
+                meet(block_no);
+                if (!sh.last) continue;
+                m = kNothing;
+                for (uint32_t k = 0; k < parts; ++k) m = fmaxf(m, __ldcg(part_ml(k) + at).x);
+                l = 0.0f;
+                for (uint32_t k = 0; k < parts; ++k) {
+                    const float2 ml = __ldcg(part_ml(k) + at);
+                    l += ml.y == 0.0f ? 0.0f : ml.y * exp2_fast(ml.x - m);
+                }
+                scale = l == 0.0f ? 0.0f : 1.0f / l;
+            }
 #pragma unroll 1
             for (int h = 0; h < CH / 8; ++h) {  // column e CH + chunk is element 8 chunk + e
-                uint32_t o[8][8];
+                float o[8][8];
+                if (parts > 1) {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) tmem_ld8(o_at + e * CH + 8 * h, o[e]);
-                tmem_wait_ld();
+                    for (int e = 0; e < 8; ++e) {
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) o[e][k] = 0.0f;
+                    }
+#pragma unroll 1
+                    for (uint32_t k = 0; k < parts; ++k) {
+                        const float2 ml = __ldcg(part_ml(k) + at);
+                        if (ml.y == 0.0f) continue;  // saw nothing (a part without tiles has no O)
+                        const float f = exp2_fast(ml.x - m);
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) {
+#pragma unroll
+                            for (int q = 0; q < 2; ++q) {
+                                const float4 v = __ldcg(part_o(k) + (e * (CH / 4) + 2 * h + q) * 256 + at);
+                                o[e][4 * q] = fmaf(v.x, f, o[e][4 * q]); o[e][4 * q + 1] = fmaf(v.y, f, o[e][4 * q + 1]);
+                                o[e][4 * q + 2] = fmaf(v.z, f, o[e][4 * q + 2]); o[e][4 * q + 3] = fmaf(v.w, f, o[e][4 * q + 3]);
+                            }
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) tmem_ld8(o_at + e * CH + 8 * h, reinterpret_cast<uint32_t(&)[8]>(o[e]));
+                    tmem_wait_ld();
+                }
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
                     float x[8];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] = it.tiles ? __uint_as_float(o[e][k]) * inv : 0.0f;
+                    for (int e = 0; e < 8; ++e) x[e] = l == 0.0f ? 0.0f : o[e][k] * scale;
                     if (there) store8(out + 8 * (8 * h + k), p.wide, x);
                 }
             }
@@ -604,6 +701,8 @@ static cudaError_t prefill_go(const AttnParams& p, int sms, cudaStream_t s) {
     kv4_prefill_kernel<T, HD><<<sms, kPfThreads, PfCfg<HD>::SMEM, s>>>(p);
     return cudaGetLastError();
 }
+
+uint64_t prefill_workspace(int sms) { return (uint64_t)sms * kPfPiece<128> * 4; }
 
 bool prefill_takes(int dtype, uint32_t head_dim) { return dtype != BT_F32 && head_dim <= 128; }
 

@@ -31,6 +31,10 @@ assert (_pack_qk.size, _pack_attn.size, _pack_sample.size) == (C.sizeof(QkArgs),
 
 _raw_stream = torch._C._cuda_getCurrentRawStream
 
+# (device, stream) -> (pointer, bytes, tensor): the attention's scratch, kept as calls of one
+# stream follow one another
+_workspaces = {}
+
 
 def _dtype(t) -> int:
     d = _DTYPES.get(t.dtype)
@@ -180,7 +184,6 @@ class KV4Cache:
             raise ValueError("KV4Cache: a page_table needs page_tokens")
         self.page_table = page_table
         self.status = torch.zeros(1, dtype=torch.int32, device=device)
-        self._workspaces = {}
         self._c = KV4(k_rows.data_ptr(), v_rows.data_ptr(), page_table.data_ptr() if self.paged else None,
                       self.status.data_ptr(), n_seq, max_seq, kv_heads, head_dim, self.page_tokens, self.n_pages,
                       self.max_pages, 0)
@@ -296,13 +299,13 @@ class KV4Cache:
                             0 if slots is None else _vector(slots, "slots", n, torch.int32, dev),
                             n, tokens, heads, max_q, window, sinks, _dtype(q), hd ** -0.5 if scale is None else scale)
         s = _raw_stream(dev) if stream is None else stream.cuda_stream
-        ws = self._workspaces.get(s)
-        if ws is None:  # one for every stream that the calls come from
+        ws = _workspaces.get((dev, s))
+        if ws is None:  # one for every stream that calls come from, for all caches
             with torch.cuda.device(dev):
                 size = native.load().bt_cuda_kv4_attention_workspace()
             with torch.cuda.stream(torch.cuda.current_stream(dev) if stream is None else stream):
                 ws = torch.zeros(size, dtype=torch.uint8, device=self.device)
-            ws = self._workspaces[s] = (ws.data_ptr(), size, ws)
+            ws = _workspaces[dev, s] = (ws.data_ptr(), size, ws)
         _launch(native.load().bt_cuda_kv4_attention, "bt_cuda_kv4_attention", dev, stream, (out,), self._ref, a, ws[0], ws[1])
         return out
 

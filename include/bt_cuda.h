@@ -575,7 +575,8 @@ typedef struct bt_kv4_attn_args {
  * in the table.  workspace: device memory of
  * bt_cuda_kv4_attention_workspace() bytes, zeroed once before its first call
  * (calls leave it ready for the next); calls that may overlap on the GPU need
- * one each.  Deterministic: the same inputs give the same bits. */
+ * one each; after BT_KV4_TIMEOUT it is zeroed again.  Deterministic: the same
+ * inputs give the same bits. */
 BT_API int bt_cuda_kv4_attention(const bt_kv4* cache, const bt_kv4_attn_args* a, void* workspace,
                                  uint64_t workspace_bytes, void* stream);
 /* Bytes of workspace that a call needs on the current device, whatever its sizes. */
