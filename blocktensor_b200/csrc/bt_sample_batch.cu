@@ -228,6 +228,16 @@ struct SampleRow {
         else __syncthreads();
     }
 
+    // No CTA touches another's shared memory before it runs or after it has ended: arrived() at
+    // the start and running() before the first access; arrived() after a CTA's last access and
+    // running() before the one that is read ends.
+    __device__ __forceinline__ void arrived() {
+        if (C > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    }
+    __device__ __forceinline__ void running() {
+        if (C > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
+
     // Sum of v over the row's threads, in every thread; `before`: over the CTAs of lower
     // rank only; `own`: over this CTA.
     __device__ unsigned long long sum(unsigned long long v, unsigned long long* before = nullptr,
@@ -256,6 +266,7 @@ struct SampleRow {
         const float best = warp_max(mine), least = -warp_max(-low);
         if (threadIdx.x % 32 == 0) { sh.redf[threadIdx.x / 32] = best; sh.redm[threadIdx.x / 32] = least; }
         __syncthreads();
+        running();
         if (threadIdx.x < 32) {
             const bool in = threadIdx.x < kSbThreads / 32;
             const float a = warp_max(in ? sh.redf[threadIdx.x] : -INFINITY), b = -warp_max(in ? -sh.redm[threadIdx.x] : -INFINITY);
@@ -541,6 +552,7 @@ __global__ void __launch_bounds__(kSbThreads, 2) sample_batch_kernel(SampleParam
     SampleRow<T, HELD> r(sh, reinterpret_cast<float4*>(dyn + sizeof(SbShared)), p);
     const uint32_t b = blockIdx.x / r.C;
     const float temp = p.temperature ? p.temperature[b] : 1.0f;
+    r.arrived();
     r.first_look();
     const float least = r.maximum();
     if (r.m == -INFINITY) {
@@ -584,7 +596,11 @@ __global__ void __launch_bounds__(kSbThreads, 2) sample_batch_kernel(SampleParam
         r.tell();
         const uint32_t last = sh.found_bin;
         if (last < kSbBins - 1 && r.list_bins(0, last)) {
-            if (r.rank == 0) r.draw_listed((uint32_t)top_k, top_p, min_p, u, b);
+            r.arrived();  // the list's length is read: the first CTA's shared memory may go
+            if (r.rank == 0) {
+                r.draw_listed((uint32_t)top_k, top_p, min_p, u, b);
+                r.running();
+            }
             return;
         }
     }
