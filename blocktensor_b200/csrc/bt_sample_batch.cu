@@ -325,9 +325,8 @@ struct SampleRow {
         for (uint32_t i = rank * mine + threadIdx.x; i < (rank + 1) * mine; i += kSbThreads) {
             unsigned long long w = 0;
             uint32_t n = 0;
-#pragma unroll
-            for (uint32_t c = 0; c < kSbMaxCluster; ++c) {  // (unrolled: the remote loads overlap)
-                if (c >= C) break;
+#pragma unroll 2
+            for (uint32_t c = 0; c < C; ++c) {  // (unrolled: remote loads overlap)
                 if (weights) w += ((unsigned long long)*cl.map_shared_rank(&sh.hi[i], c) << 32) + *cl.map_shared_rank(&sh.lo[i], c);
                 if (counts) n += *cl.map_shared_rank(&sh.cnt[i], c);
             }
