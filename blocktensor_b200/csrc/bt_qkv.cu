@@ -46,6 +46,44 @@ __device__ __forceinline__ float row_sum(float v) {
     return v;
 }
 
+// Mean of the squares of a row, 8 consecutive elements a lane, each square and sum rounded,
+// added in the order of PyTorch's row mean (by measurement): 32 partial sums, of 4
+// consecutive elements (head_dim 128), of 4 and the 4 that lie 128 further (256), or of
+// elements 32 apart (64), then halves on halves.  A key that goes to the cache is normed
+// so, because a code at the edge between two steps falls to one or the other with the
+// last bit of the norm: this way the cached codes are those of a plain fp32 computation.
+template <int HD>
+__device__ __forceinline__ float plain_mean_square(const float (&x)[8]) {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __fmul_rn(x[i], x[i]);
+    auto add_lane = [](float a, int o) { return __fadd_rn(a, __shfl_xor_sync(0xffffffffu, a, o)); };
+    if (HD == 64) {
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = add_lane(v[i], o);
+        }
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) {
+#pragma unroll
+            for (int i = 0; i < o; ++i) v[i] = __fadd_rn(v[i], v[i + o]);
+        }
+        return v[0] * (1.0f / HD);
+    }
+    if (HD == 256) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = add_lane(v[i], 16);
+    }
+    float a = __fadd_rn(__fadd_rn(__fadd_rn(v[0], v[1]), v[2]), v[3]), b = __fadd_rn(__fadd_rn(__fadd_rn(v[4], v[5]), v[6]), v[7]);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) {
+        a = add_lane(a, o);
+        b = add_lane(b, o);
+    }
+    return __fadd_rn(a, b) * (1.0f / HD);
+}
+
 // Quantises the 64 elements of 8 neighbouring lanes; the lane's 8 codes, and the
 // group's pair as (scale, min) halves.
 __device__ __forceinline__ uint32_t quantise8(const float (&y)[8], uint32_t* pair) {
@@ -61,8 +99,8 @@ __device__ __forceinline__ uint32_t quantise8(const float (&y)[8], uint32_t* pai
         lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
         hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
     }
-    // (max - min) / 15 and 1 / scale as IEEE divisions: the codes are part of the format
-    const __half s = __float2half_rn(__fdiv_rn(__fsub_rn(hi, lo), 15.0f)), m = __float2half_rn(lo);
+    // the roundings are part of the format: a product with fp32's 1 / 15, and an IEEE 1 / scale
+    const __half s = __float2half_rn(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f)), m = __float2half_rn(lo);
     const float sf = __half2float(s), mf = __half2float(m), inv = sf > 0.0f ? __fdiv_rn(1.0f, sf) : 0.0f;
     uint32_t w = 0;
 #pragma unroll
@@ -196,13 +234,11 @@ __global__ void __launch_bounds__(kQkvThreads, 8) qkv_kernel(const __grid_consta
                 float x[8];
                 raw[k].get(x);
                 if (w) {
-                    float ss = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
-                    const float inv = rsqrtf(row_sum<LPR>(ss) * (1.0f / HD) + p.eps);
+                    const float inv = rsqrtf(__fadd_rn(plain_mean_square<HD>(x), p.eps));
                     const float4 w0 = __ldg(reinterpret_cast<const float4*>(w + 8 * l)), w1 = __ldg(reinterpret_cast<const float4*>(w + 8 * l) + 1);
-                    x[0] *= inv * w0.x; x[1] *= inv * w0.y; x[2] *= inv * w0.z; x[3] *= inv * w0.w;
-                    x[4] *= inv * w1.x; x[5] *= inv * w1.y; x[6] *= inv * w1.z; x[7] *= inv * w1.w;
+                    const float wv[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(__fmul_rn(x[i], inv), wv[i]);
                 }
                 if (keys && p.rope && in_table) {
                     // elements 8l .. 8l + 7 pair with those of lane l +- rot / 16
@@ -216,8 +252,8 @@ __global__ void __launch_bounds__(kQkvThreads, 8) qkv_kernel(const __grid_consta
                         const float o0 = __shfl_sync(0xffffffffu, x[i], partner), o1 = __shfl_sync(0xffffffffu, x[i + 1], partner);
                         // first half: a cos - b sin; second half: b cos + a sin
                         if (turn) {
-                            x[i] = x[i] * c.x + (second ? o0 : -o0) * c.y;
-                            x[i + 1] = x[i + 1] * c.z + (second ? o1 : -o1) * c.w;
+                            x[i] = __fadd_rn(__fmul_rn(x[i], c.x), __fmul_rn(second ? o0 : -o0, c.y));
+                            x[i + 1] = __fadd_rn(__fmul_rn(x[i + 1], c.z), __fmul_rn(second ? o1 : -o1, c.w));
                         }
                     }
                 }

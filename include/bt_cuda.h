@@ -539,7 +539,7 @@ BT_API int bt_cuda_qk_norm_rope(const bt_qk_args* a, void* stream);
 /* The same with the keys and the (unchanged) values of token t stored in 4 bits
  * at position positions[t] of slot slots[t] of the cache, one launch.  Values
  * are held to +-57344 and NaN becomes 0 (four bits hold neither).  Per 64
- * elements: min and scale = (max - min) / 15 are rounded to fp16, code =
+ * elements: min and scale = (max - min) * (1 / 15) are rounded to fp16, code =
  * clamp(round((x - min) * (1 / scale)), 0, 15).  slots[t] < 0: the token is
  * padding and stores nothing.  q.data NULL: keys and values only. */
 BT_API int bt_cuda_kv4_append(const bt_kv4* cache, const bt_qk_args* a, void* stream);

@@ -135,7 +135,7 @@ def ref_rows(x):
     s = x.shape
     x = x.reshape(*s[:-1], s[-1] // 64, 64)
     lo, hi = x.min(-1), x.max(-1)
-    scale, low = ((hi - lo) / np.float32(15)).astype(np.float16), lo.astype(np.float16)
+    scale, low = ((hi - lo) * (np.float32(1) / np.float32(15))).astype(np.float16), lo.astype(np.float16)
     sf = scale.astype(np.float32)
     inv = np.where(sf > 0, np.float32(1) / np.where(sf > 0, sf, np.float32(1)), np.float32(0)).astype(np.float32)
     code = np.rint((x - low.astype(np.float32)[..., None]) * inv[..., None]).clip(0, 15).astype(np.uint8).reshape(s)
@@ -249,6 +249,29 @@ def test_append_normed(cuda, dt):
     only = cuda.KV4Cache(2, 40, kv, hd)
     assert only._append(None, k, v, None, w[1], slots, pos, table, 1e-5, None, None) is None
     assert torch.equal(only.k_rows, cache.k_rows)
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_append_normed_plain_codes(cuda, dt, hd):
+    """The cached rows are those of keys that plain fp32 PyTorch norms and rotates, bit for bit (a code at the
+    edge between two steps would fall either way with the last bit of the norm)."""
+    torch = T()
+    g = gen(hd)
+    dtype = getattr(torch, dt)
+    tokens, kv = 3001, 4
+    k, v = ((randn(g, tokens, kv, hd) * (1 + 2 * torch.rand(hd, generator=g, device="cuda"))).to(dtype) for _ in range(2))
+    w = 1 + 0.3 * randn(g, hd)
+    table = cuda.rope_table(tokens, hd, 500000.0)
+    pos = torch.arange(tokens, dtype=torch.int32, device="cuda")
+    cache = cuda.KV4Cache(1, tokens, kv, hd)
+    cache._append(None, k, v, None, w, torch.zeros_like(pos), pos, table, 1e-5, None, None)
+    x = k.float()
+    x = x * torch.rsqrt((x * x).mean(-1, keepdim=True) + 1e-5) * w
+    c, s = table[:, None, :, 0], table[:, None, :, 1]
+    a, b = x[..., :hd // 2], x[..., hd // 2:]
+    want = ref_rows(torch.cat([a * c - b * s, a * s + b * c], -1))
+    assert np.array_equal(cache.k_rows[0, :, :tokens].transpose(0, 1).cpu().numpy(), want)
 
 
 # ---------------------------------------------------------------- attention
