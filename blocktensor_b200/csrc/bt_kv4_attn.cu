@@ -360,7 +360,7 @@ __global__ void __launch_bounds__(AttnCfg<HD, TERMS>::NW * 32, 1) kv4_attn_kerne
         float o[NG * 4][4] = {}, mo[NG][2] = {}, m[2] = {kNothing, kNothing}, l[2] = {};
         uint32_t v_bound = 0;       // no V scale so far is larger (as fp16 bits)
         int v_exp = 0;              // p s is multiplied by 2^v_exp
-        float v_mul = 1.0f;
+        float v_mul = 1.0f, v_eight = -8.0f;  // 2^v_exp, -8 2^-v_exp
 
         constexpr float kLazy = TERMS == 2 ? 0.0f : kLazyMax;
         const uint32_t r0 = key_of(g), r1 = r0 + 2;                  // keys of MMA rows g and g + 8
@@ -468,6 +468,7 @@ __global__ void __launch_bounds__(AttnCfg<HD, TERMS>::NW * 32, 1) kv4_attn_kerne
                     fv = v_bound ? __int_as_float((127 + e - v_exp) << 23) : 0.0f;
                     v_exp = e;
                     v_mul = __int_as_float((127 + e) << 23);
+                    v_eight = -__int_as_float((130 - e) << 23);
                     v_bound = big | 0x3ffu;
                 }
                 l[0] *= fa;
@@ -504,7 +505,13 @@ __global__ void __launch_bounds__(AttnCfg<HD, TERMS>::NW * 32, 1) kv4_attn_kerne
                     b2 = transpose8(pack_half2(r[0], r[1]));
                     b3 = transpose8(pack_half2(r[2], r[3]));
                 }
-                const uint32_t b0 = transpose8(pack_half2(w[0], w[1])), b1 = transpose8(pack_half2(w[2], w[3]));
+                const uint32_t h0 = pack_half2(w[0], w[1]), h1 = pack_half2(w[2], w[3]);
+                if (TERMS == 1) {  // the 8 taken off, by what p s was rounded to
+                    const float2 y0 = unpack_half2(h0), y1 = unpack_half2(h1);
+                    mo[j][0] = fmaf(y0.x, v_eight, fmaf(y1.x, v_eight, mo[j][0]));
+                    mo[j][1] = fmaf(y0.y, v_eight, fmaf(y1.y, v_eight, mo[j][1]));
+                }
+                const uint32_t b0 = transpose8(h0), b1 = transpose8(h1);
                 const uint32_t va = *reinterpret_cast<const uint32_t*>(kt + va_at + 32 * j), vb = *reinterpret_cast<const uint32_t*>(kt + vb_at + 32 * j);
                 const uint32_t vc = *reinterpret_cast<const uint32_t*>(kt + va_at + 32 * j + 2 * C::RB), vd = *reinterpret_cast<const uint32_t*>(kt + vb_at + 32 * j + 2 * C::RB);
                 uint32_t f[4] = {__byte_perm(va, vb, 0x5410), __byte_perm(va, vb, 0x7632), __byte_perm(vc, vd, 0x5410), __byte_perm(vc, vd, 0x7632)};
@@ -517,10 +524,6 @@ __global__ void __launch_bounds__(AttnCfg<HD, TERMS>::NW * 32, 1) kv4_attn_kerne
                     uint32_t a[4];
 #pragma unroll
                     for (int k = 0; k < 4; ++k) a[k] = i & 1 ? codes<TERMS, 1>(f[k]) : codes<TERMS, 0>(f[k]);
-                    if (TERMS == 1) {
-                        const uint32_t eight = i & 1 ? 0x80808080u : 0x80088008u;  // minus code 8
-                        mma_f16(o[4 * j + i], eight, eight, eight, eight, b0, b1);
-                    }
                     if (TERMS == 1) {
                         mma_f16(o[4 * j + i], a[0], a[1], a[2], a[3], b0, b1);
                     } else {

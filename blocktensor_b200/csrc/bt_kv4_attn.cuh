@@ -13,10 +13,11 @@
 // fp16 terms (22 bits) for fp32; p s_j likewise is one or two terms.  The 8 is there
 // because the sums of c and of m are many times their difference, which makes p's
 // rounding and the tensor cores' truncated accumulation come out as much larger.  For
-// 16-bit types an MMA with a constant operand takes it off O (the tensor pipe is a sixth
-// busy; fp16 error 3.8e-4 -> 2.7e-4, of which 2.1e-4 are the result's own rounding).  For
-// fp32 the codes themselves are lowered, of K too: between two MMAs the sum would still
-// be large (550 keys: error 3e-5 with c, 1.4e-5 with two MMAs, 5.5e-6 so).  And both
+// 16-bit types the MMAs still add c, and 8 times what p s was rounded to is taken off in
+// fp32 (fp16 error 3.8e-4 -> 2.7e-4, of which 2.1e-4 are the result's own rounding; an
+// MMA with a constant operand for it costs a seventh of the time).  For fp32 the codes
+// themselves are lowered, of K too: the truncated sums would be large otherwise (550 keys:
+// error 3e-5 with c, 1.4e-5 with two MMAs, 5.5e-6 so).  And both
 // terms of fp32 queries and of p s_j are whole multiples of a step each, so that an MMA's
 // sums are exact: the tensor cores drop low bits when they align products (1.1e-6).
 //
