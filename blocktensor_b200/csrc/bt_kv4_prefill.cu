@@ -325,30 +325,41 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
                 // the row as fp16, scaled so that its largest element is in [2^13, 2^14)
                 const T* src = (const T*)p.q + token * p.q_ts + head * p.q_hs;
                 float big = 0.0f;
-                RawN<T, 8> raw[CH];
+                constexpr int N = CH < 8 ? CH : 8;  // chunks at a time (all of a long row would spill)
+                RawN<T, 8> raw[N];
+                auto load_chunks = [&](int first) {
 #pragma unroll
-                for (int k = 0; k < CH; ++k) raw[k].load(src + 8 * k, p.wide);
+                    for (int k = 0; k < N; ++k) raw[k].load(src + 8 * (first + k), p.wide);
+                };
+#pragma unroll 1
+                for (int first = CH - N; first >= 0; first -= N) {  // (ends with the chunks that are stored first)
+                    load_chunks(first);
 #pragma unroll
-                for (int k = 0; k < CH; ++k) {
-                    float x[8];
-                    raw[k].get(x);
+                    for (int k = 0; k < N; ++k) {
+                        float x[8];
+                        raw[k].get(x);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(x[e]));
+                        for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(x[e]));
+                    }
                 }
                 const int be = (int)(__float_as_uint(big) >> 23);
                 const int up = be > 0 && be < 255 ? min(13 - (be - 127), 126) : 0;
                 const bool flat = p.scale_log2 == 0.0f;  // all scores equal: f stays positive
                 const float mul = there && !flat ? sign * __int_as_float((127 + up) << 23) : 0.0f;
                 f = flat ? 1.0f : fabsf(p.scale_log2) * __int_as_float((127 - up) << 23);
+#pragma unroll 1
+                for (int first = 0; first < CH; first += N) {
+                    if (first > 0) load_chunks(first);
 #pragma unroll
-                for (int k = 0; k < CH; ++k) {
-                    float x[8];
-                    raw[k].get(x);
+                    for (int k = 0; k < N; ++k) {
+                        float x[8];
+                        raw[k].get(x);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] = there ? x[e] * mul : 0.0f;
-                    uint4 v;
-                    v.x = pack_half2(x[0], x[4]); v.y = pack_half2(x[1], x[5]); v.z = pack_half2(x[2], x[6]); v.w = pack_half2(x[3], x[7]);
-                    *reinterpret_cast<uint4*>(qs + r * C::Q + (k * 128 + row) * 16) = v;
+                        for (int e = 0; e < 8; ++e) x[e] = there ? x[e] * mul : 0.0f;
+                        uint4 v;
+                        v.x = pack_half2(x[0], x[4]); v.y = pack_half2(x[1], x[5]); v.z = pack_half2(x[2], x[6]); v.w = pack_half2(x[3], x[7]);
+                        *reinterpret_cast<uint4*>(qs + r * C::Q + ((first + k) * 128 + row) * 16) = v;
+                    }
                 }
                 fence_proxy_async();
                 __syncwarp();
