@@ -3,9 +3,9 @@
 //
 // Dealing out the work.  An item is (sequence, KV head, block of 8 columns); its units
 // are 32 keys.  A range of units goes to a group of warps:
-//   few items (no more than half the SMs): a group is a whole CTA, and every item is cut
-//     into pieces of its own, of about equal length over all items, so that a CTA has
-//     one piece of one item;
+//   few items (less than SMs, and lengths that allow it): a group is a whole CTA, and every
+//     item is cut into pieces of its own, of about equal length over all items, so that a
+//     CTA has one piece of one item;
 //   many items: a group is 4 warps, and the units of all items in order (kItemCost more
 //     for an item's own cost) are cut into equal ranges, so that a group works on whole
 //     items but for its first and its last.
@@ -38,7 +38,8 @@ struct AttnCfg {
 constexpr int kMaxGroups = 4;                        // of a CTA
 constexpr uint32_t kPieceFloats = 8 * 256 + 16;      // sums, maxima and sums of probabilities of 8 columns
 
-constexpr uint32_t kItemCost = 4;
+constexpr uint32_t kItemCost = 4;    // units (256 items of 64 to 1500 keys of 64: 50 us, 67 with 1)
+constexpr uint32_t kPieceCost = 48;  // units
 
 // floor(a / b); 32 bits wide wherever that does (64-bit divisions are long)
 __device__ __forceinline__ uint64_t div64(uint64_t a, uint32_t b) {
@@ -124,7 +125,7 @@ struct AttnShared {
     uint32_t halves[16][4];  // which 16-key halves of a stage hold keys
     float m[16][8], l[16][8];
     uint64_t warp_units[16];
-    uint32_t warp_items[16];
+    uint32_t warp_items[16], warp_longest[16];
     uint64_t start_at[kMaxGroups];
     uint32_t start_seq[kMaxGroups], last[kMaxGroups];
     float qsum[kMaxGroups][8][4], factor[kMaxGroups][8];
@@ -135,7 +136,8 @@ __device__ __forceinline__ void group_sync(uint32_t group, uint32_t threads) {
     asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "r"(threads) : "memory");
 }
 
-template <typename T, int HD, int TERMS>
+// MAY_BE_FEW: without it the work is dealt out in equal ranges whatever it is.
+template <typename T, int HD, int TERMS, bool MAY_BE_FEW>
 __global__ void __launch_bounds__(AttnCfg<HD, TERMS>::NW * 32, 1) kv4_attn_kernel(const __grid_constant__ AttnParams p) {
     using C = AttnCfg<HD, TERMS>;
     constexpr int NG = C::NG, NW = C::NW, S = C::STAGES;
@@ -149,39 +151,49 @@ __global__ void __launch_bounds__(AttnCfg<HD, TERMS>::NW * 32, 1) kv4_attn_kerne
     if (lane < S) mbar_init(&sh.bar[warp][lane], 1);
     fence_mbar_init();
     uint64_t total = 0;
-    uint32_t items = 0;
+    uint32_t items = 0, longest = 0;
     SeqWork mine = {};  // the sequence this thread looked at last
     for (uint32_t i = tid; i < p.n; i += NW * 32) {
         mine = few_row_work(p, i, blockIdx.x == 0);
         const uint32_t it = mine.blocks * p.map.kv_heads;
         total += (uint64_t)it * mine.tiles;
         items += it;
+        if (MAY_BE_FEW && it) longest = max(longest, mine.tiles);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
         total += __shfl_xor_sync(0xffffffffu, total, o);
         items += __shfl_xor_sync(0xffffffffu, items, o);
     }
-    if (lane == 0) { sh.warp_units[warp] = total; sh.warp_items[warp] = items; }
+    if (MAY_BE_FEW) longest = __reduce_max_sync(0xffffffffu, longest);
+    if (lane == 0) { sh.warp_units[warp] = total; sh.warp_items[warp] = items; sh.warp_longest[warp] = longest; }
     __syncthreads();
     total = sh.warp_units[lane % NW];
     items = sh.warp_items[lane % NW];
+    if (MAY_BE_FEW) longest = __reduce_max_sync(0xffffffffu, sh.warp_longest[lane % NW]);
 #pragma unroll
     for (int o = NW / 2; o > 0; o >>= 1) {
         total += __shfl_xor_sync(0xffffffffu, total, o);
         items += __shfl_xor_sync(0xffffffffu, items, o);
     }
     if (total == 0) return;
-    const bool few = items <= gridDim.x / 2;
+    // Units of a range.  Pieces: as sum ceil(t / step) <= total / step + items, no more of
+    // them than CTAs; and half a unit at least for each warp.  The longest item's may be
+    // kPieceCost units longer than an equal range would be: that is what the ends of several
+    // items a group cost.  8 KV heads of 128, pieces / ranges: 1 sequence of 4096 keys 14 / 24
+    // us, 9 of them 23 / 30, 12 of them 30 / 31, 16 of them 31 / 38; 16 sequences of 600 to
+    // 24000 keys 132 / 74 (to the ranges by this rule).
+    uint64_t step = 0;
+    bool few = false;
+    if (MAY_BE_FEW && items < gridDim.x) {
+        step = max(div64(total + gridDim.x - items - 1, gridDim.x - items), (uint64_t)(NW / 2));
+        step = min(step, (uint64_t)longest);
+        few = longest <= div64(longest + step - 1, (uint32_t)step) * (div64(total, gridDim.x) + kPieceCost);
+    }
     const uint32_t WG = few ? NW : 4;  // warps of a group
     const uint32_t per_cta = NW / WG, group = warp / WG, gw = warp % WG;
     const uint32_t range = group * gridDim.x + blockIdx.x;  // this group's
-    // units of a range.  Few items: as sum ceil(t / step) <= total / step + items, no more
-    // pieces than CTAs; and half a unit at least for each warp.
-    uint64_t step;
-    if (few) {
-        step = max(div64(total + gridDim.x - items - 1, gridDim.x - items), (uint64_t)(NW / 2));
-    } else {
+    if (!few) {
         total += (uint64_t)items * kItemCost;
         step = div64(total + gridDim.x * per_cta - 1, gridDim.x * per_cta);
     }
@@ -724,19 +736,22 @@ static int device_sms() {
 }
 
 template <typename T, int HD, int TERMS>
-static cudaError_t attn_launch(const AttnParams& p, int sms, cudaStream_t s) {
+static cudaError_t attn_launch(const AttnParams& p, bool may_be_few, int sms, cudaStream_t s) {
     using C = AttnCfg<HD, TERMS>;
-    static std::atomic<uint64_t> ready{0};  // devices whose attribute is set
+    static std::atomic<uint64_t> ready{0};  // devices whose attributes are set
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (dev >= 64 || !(ready.load(std::memory_order_relaxed) >> dev & 1)) {
-        e = cudaFuncSetAttribute(kv4_attn_kernel<T, HD, TERMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+        e = cudaFuncSetAttribute(kv4_attn_kernel<T, HD, TERMS, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+        if (e == cudaSuccess)
+            e = cudaFuncSetAttribute(kv4_attn_kernel<T, HD, TERMS, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
         if (e != cudaSuccess) return e;
         if (dev < 64) ready.fetch_or(1ull << dev, std::memory_order_relaxed);
     }
     g_launches.fetch_add(1, std::memory_order_relaxed);
-    kv4_attn_kernel<T, HD, TERMS><<<sms, C::NW * 32, C::SMEM, s>>>(p);
+    if (may_be_few) kv4_attn_kernel<T, HD, TERMS, true><<<sms, C::NW * 32, C::SMEM, s>>>(p);
+    else kv4_attn_kernel<T, HD, TERMS, false><<<sms, C::NW * 32, C::SMEM, s>>>(p);
     return cudaGetLastError();
 }
 
@@ -793,12 +808,16 @@ extern "C" int bt_cuda_kv4_attention(const bt_kv4* cache, const bt_kv4_attn_args
     p.few_rows = !many ? 0xffffffffu : a->n == 1 ? 0 : few_rows;
     if (many) BT_CUDA_CHECK(launch_kv4_prefill(p, a->dtype, cache->head_dim, sms, s));
     if (p.few_rows == 0) return BT_OK;
+    // An instance that deals out nothing but equal ranges is 3 to 5 % faster at that; it takes
+    // calls whose items (as far as the host can tell: empty sequences have none) reach the SMs.
+    const uint64_t blocks = a->q_start ? (uint64_t)a->tokens * p.group / 8 + a->n : (uint64_t)a->n * ((p.group + 7) / 8);
+    const bool may_be_few = blocks * cache->kv_heads < (uint64_t)sms;
     auto by_hd = [&](auto type, auto terms) {
         using T = decltype(type);
         constexpr int N = decltype(terms)::value;
-        if (cache->head_dim == 64) return attn_launch<T, 64, N>(p, sms, s);
-        if (cache->head_dim == 128) return attn_launch<T, 128, N>(p, sms, s);
-        return attn_launch<T, 256, N>(p, sms, s);
+        if (cache->head_dim == 64) return attn_launch<T, 64, N>(p, may_be_few, sms, s);
+        if (cache->head_dim == 128) return attn_launch<T, 128, N>(p, may_be_few, sms, s);
+        return attn_launch<T, 256, N>(p, may_be_few, sms, s);
     };
     if (a->dtype == BT_F32) BT_CUDA_CHECK(by_hd(float(), std::integral_constant<int, 2>()));
     else if (a->dtype == BT_F16) BT_CUDA_CHECK(by_hd(__half(), std::integral_constant<int, 1>()));

@@ -417,6 +417,25 @@ def test_attention_single(cuda, dt, hd, i):
          layout=["plain", "fused", "off"][i % 3]).check()
 
 
+DEALT = [  # items around the numbers of SMs and of half of them, even and ragged
+    ([900] * 9, 8, 8),
+    ([129] * 16, 8, 3),
+    ([60, 4000, 31, 1, 0, 700, 33, 32, 64, 65], 12, 1),
+    ([2500] + [3] * 72, 2, 4),
+    ([33] * 147, 1, 1),
+    ([70, 1] * 74, 1, 2),
+    ([40] * 149, 1, 2),
+    ([0] * 200 + [500, 20], 4, 1),
+]
+
+
+@pytest.mark.parametrize("dt,hd", [("float32", 64), ("float16", 128), ("bfloat16", 256)])
+@pytest.mark.parametrize("i", range(len(DEALT)))
+def test_attention_dealing(cuda, dt, hd, i):
+    lens, kv, group = DEALT[i]
+    Case(cuda, 300 + i, dt, hd, kv, group, lens, [1] * len(lens), page=16 * (i % 2)).check()
+
+
 CHUNKS = [
     # lens, counts, kv, group, page, window, sinks
     ([2], [2], 1, 1, 0, 0, 0),
