@@ -31,6 +31,10 @@
 // d = 8 chunk + e, so that the unpackers' 16-byte stores of neighbouring lanes are
 // contiguous; K's and Q's elements of 8 are in the order 0 4 1 5 2 6 3 7, in which a
 // word's codes come out two at a time.
+//
+// Measured, bf16, 64 heads over 8 of 128: 2048 queries ending 8192 keys 575 us, 837 TFLOP/s
+// of 1642 (tensor pipe 45 to 50 % busy, exponential unit 45 %, issue slots 58 %).  128-key
+// tiles with one S buffer a half took 715 us; one warp issuing for both halves 756.
 #include "bt_kv4_attn.cuh"
 
 namespace bt {
