@@ -30,6 +30,7 @@ _pack_sample = Struct("<Qq7Q2IiI")
 assert (_pack_qk.size, _pack_attn.size, _pack_sample.size) == (C.sizeof(QkArgs), C.sizeof(KV4AttnArgs), C.sizeof(SampleArgs))
 
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
 
 # (device, stream) -> (pointer, bytes, tensor): the attention's scratch, kept as calls of one
 # stream follow one another
@@ -59,13 +60,14 @@ def _heads(t, name, shape=None, dtype=None, dev=None):
 def _out(t, name, shape, like, dev):
     """(tensor, (pointer, strides)): the caller's output, checked, or a new one."""
     if t is None:
-        t = like.new_empty(shape)
+        # (empty_like keeps strides, so it only serves contiguous tensors; 0.5 us less than new_empty)
+        t = torch.empty_like(like) if like.is_contiguous() else like.new_empty(shape)
         return t, (t.data_ptr(), shape[1] * shape[2], shape[2])
     return t, _heads(t, name, shape, like.dtype, dev)
 
 
 def _vector(t, name, n, dtype, dev):
-    if t.dtype is not dtype or t.numel() != n or not t.is_contiguous() or not t.is_cuda or t.get_device() != dev:
+    if t.dtype is not dtype or t.numel() != n or not t.is_contiguous() or t.get_device() != dev:
         raise ValueError(f"{name}: expected {n} contiguous {dtype} values on cuda:{dev}")
     return t.data_ptr()
 
@@ -78,7 +80,7 @@ def _launch(fn, name, dev, stream, outs, *args):
         s = stream.cuda_stream
         for t in outs:
             t.record_stream(stream)
-    if dev == torch.cuda.current_device():
+    if dev == _current_device():
         rc = fn(*args, s)
     else:
         with torch.cuda.device(dev):
@@ -100,7 +102,7 @@ def rope_table(positions: int, rot_dim: int, theta: float = 10000.0, device="cud
 def _rope(table, dev):
     if table is None:
         return 0, 0, 0
-    if table.dim() != 3 or table.dtype is not torch.float32 or not table.is_contiguous() or not table.is_cuda or table.get_device() != dev:
+    if table.dim() != 3 or table.dtype is not torch.float32 or not table.is_contiguous() or table.get_device() != dev:
         raise ValueError("table: expected a contiguous [positions, rot_dim / 2, 2] float32 tensor on the queries' device")
     n, half, two = table.shape
     if two != 2:
