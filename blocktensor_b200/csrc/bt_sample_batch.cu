@@ -428,7 +428,21 @@ struct SampleRow {
         sync();
         const uint32_t n = *count;
         if (n > kSbList) return false;
-        if (rank == 0) {
+        if (rank == 0 && n <= kSbThreads / 4) {
+            // every entry's place is the number of entries before it: four threads count for one
+            const uint32_t i = threadIdx.x / 4;
+            const uint32_t key = i < n ? sh.list_key[i] : 0, id = i < n ? sh.list_id[i] : 0;
+            uint32_t place = 0;
+            for (uint32_t j = threadIdx.x % 4; j < n; j += 4) {
+                const uint32_t kj = sh.list_key[j], ij = sh.list_id[j];
+                place += kj > key || (kj == key && ij < id) ? 1u : 0u;
+            }
+            place += __shfl_xor_sync(0xffffffffu, place, 1);
+            place += __shfl_xor_sync(0xffffffffu, place, 2);
+            __syncthreads();
+            if (i < n && threadIdx.x % 4 == 0) { sh.list_key[place] = key; sh.list_id[place] = id; }
+            __syncthreads();
+        } else if (rank == 0) {
             uint32_t size = 2;
             while (size < n) size <<= 1;
             for (uint32_t i = n + threadIdx.x; i < size; i += kSbThreads) { sh.list_key[i] = 0; sh.list_id[i] = 0xffffffffu; }
