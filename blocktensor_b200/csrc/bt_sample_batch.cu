@@ -29,9 +29,9 @@
 //
 // Bound: issue slots and cluster barriers for large batches, the chain of cluster barriers
 // for single rows.  Measured, fp32, temperature 0.7: 256 rows of 128256 with top-k 50 and
-// top-p 0.9 144 us (0.9 TB/s), with top-p alone 220 us; one row of 32000 12.7 us.  The short
-// list against the histogram, 256 rows of 128256: top-k 50 144 / 273 us, 200 185 / 299,
-// 512 (the list's limit) 248 / 320.
+// top-p 0.9 135 us (1.0 TB/s), with top-p alone 220 us; one row of 32000 11.2 us.  The short
+// list against the histogram, 256 rows of 128256: top-k 50 135 / 275 us, 200 186 / 296,
+// 512 (the list's limit) 249 / 312.
 #include <cooperative_groups.h>
 
 #include "bt_internal.h"
@@ -430,6 +430,7 @@ struct SampleRow {
         if (n > kSbList) return false;
         if (rank == 0 && n <= kSbThreads / 4) {
             // every entry's place is the number of entries before it: four threads count for one
+            // (up to 128 entries this takes 1.2 us less than the sort's 28 barriers; at 256 the same)
             const uint32_t i = threadIdx.x / 4;
             const uint32_t key = i < n ? sh.list_key[i] : 0, id = i < n ? sh.list_id[i] : 0;
             uint32_t place = 0;
@@ -867,12 +868,12 @@ static cudaError_t sample_launch(SampleParams p, uint32_t rows, uint32_t cluster
 template <typename T>
 static cudaError_t sample_pick(const SampleParams& p, uint32_t rows, cudaStream_t s) {
     // A row that one CTA can hold has no use for cluster barriers (256 rows, one CTA / two or
-    // four: 32000 logits 34 / 41 us, 45000 logits 39 / 64); a longer one gains by two CTAs an
-    // SM (256 rows of 128256: 144 us, with one 151).
+    // four: 32000 logits 31 / 38 us, 45000 logits 36 / 59); a longer one gains by two CTAs an
+    // SM (256 rows of 128256: 135 us, with one 143).
     uint32_t c = 1;
     while (p.vocab > kSbHeld && c < kSbMaxCluster && p.vocab > c * kSbShare) c *= 2;
     // few rows: smaller shares, as long as the CTAs fit the SMs side by side (1 row of 32000:
-    // 12.7 us, 17.1 without; 16 rows 15.0 and 17.4)
+    // 11.2 us, 16.1 without; 16 rows 13.4 and 16.0)
     while (c < kSbMaxCluster && (uint64_t)rows * c * 2 <= 148 && p.vocab > c * 4096) c *= 2;
     if (p.vocab <= c * kSbHeld) return sample_launch<T, true>(p, rows, c, s);
     return sample_launch<T, false>(p, rows, c, s);
