@@ -404,8 +404,10 @@ struct SampleRow {
     // The tokens of steps `from` .. `to`, sorted (largest first, equal ones by id), at rank 0;
     // false: too many.
     __device__ bool list_bins(uint32_t from, uint32_t to) {
-        // no logit below this is in them (the margins cover the roundings of either side)
-        const float reach = (float)(to + 1) / steps / inv, bound = steps > 0.0f ? m - reach * 1.0001f - fabsf(m) * 1e-5f : -INFINITY;
+        // no logit below this is in them (the margins cover the roundings of either side); the last
+        // step but one takes all that lies below it, down to kSbReach
+        const float reach = (to < kSbBins - 2 ? (float)(to + 1) / steps : kSbReach) / inv;
+        const float bound = steps > 0.0f ? m - reach * 1.0001f - fabsf(m) * 1e-5f : -INFINITY;
         if (rank == 0 && threadIdx.x == 0) sh.listed = 0;
         sync();
         uint32_t* keys = cl.map_shared_rank(sh.list_key, 0);

@@ -1,0 +1,51 @@
+"""GPU: cases at which the serving operators once answered wrongly or could have, against the plain 64-bit
+references of test_gpu_serving.py (its tolerances, unless a test derives its own)."""
+import numpy as np
+import pytest
+
+from test_gpu_serving import DT, T, check_rows, gen, ints, randn
+
+pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------- sampling
+
+def masked_rows(g, rows, vocab, allowed, barred):
+    """Logits of constrained rows: all but `allowed` tokens are barred, one of the allowed ones stands well above
+    the rest, and of every eight neighbours the first is barred unless it is one of the two largest."""
+    torch = T()
+    x = torch.full((rows, vocab), barred, device="cuda")
+    for b in range(rows):
+        ids = torch.randperm(vocab, generator=g, device="cuda")
+        ids = ids[ids % 8 != 0][:allowed]
+        x[b, ids] = randn(g, len(ids)) * 0.3
+        first = torch.randperm((vocab + 7) // 8, generator=g, device="cuda")[:2] * 8
+        x[b, first] = torch.tensor([2.5, 2.4], device="cuda")[:len(first)]
+    return x
+
+
+@pytest.mark.parametrize("barred", [float("-inf"), float("nan")])
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("vocab", [64, 5000, 32000, 128256, 400000])
+def test_sample_masked_rows(cuda, dt, vocab, barred):
+    """Rows that allow a few tokens: none of them is lost on the way to a threshold, whichever path takes the
+    row (short list, histogram, both cuts; one CTA to a cluster; rows that are read again at every pass)."""
+    torch = T()
+    g, rng = gen(vocab), np.random.default_rng(vocab)
+    rows, allowed = 24, min(vocab // 3, 3000)
+    x = masked_rows(g, rows, vocab, allowed, barred).to(getattr(torch, dt))
+    k = [[3, 0, 40, 600, 512, 0, 2, 2000][i % 8] for i in range(rows)]
+    p = [[1.0, 0.9, 0.9, 1.0, 0.5, 0.99, 1.0, 0.8][i % 8] for i in range(rows)]
+    t = [[1.0, 0.3, 3.0][i % 3] for i in range(rows)]
+    u = rng.random(rows).astype(np.float32).tolist()
+    assert check_rows(cuda, x, u, t, k, p, [0.0] * rows) <= 3
+
+
+def test_sample_few_tokens(cuda):
+    """Four tokens of 32000: all of the kept ones can be drawn."""
+    torch = T()
+    x = torch.full((64, 32000), -float("inf"), device="cuda")
+    x[:, [8, 16, 25, 33]] = torch.tensor([2.0, 1.9, 1.7, 1.7], device="cuda")
+    u = [(i + 0.5) / 64 for i in range(64)]
+    for k, p in ((3, 1.0), (0, 0.9), (4, 0.9), (600, 0.95)):
+        assert check_rows(cuda, x, u, [1.0] * 64, [k] * 64, [p] * 64, [0.0] * 64) == 0
