@@ -148,7 +148,7 @@ __global__ void __launch_bounds__(AttnCfg<HD, TERMS>::NW * 32, 1) kv4_attn_kerne
     float* slots = reinterpret_cast<float*>(dyn + NW * (S * C::STAGE));
 
     // ---- how much work there is
-    if (lane < S) mbar_init(&sh.bar[warp][lane], 1);
+    if (lane < S) mbar_init(&sh.bar[warp][lane], 1 + p.stalled);
     fence_mbar_init();
     uint64_t total = 0;
     uint32_t items = 0, longest = 0;
@@ -236,7 +236,8 @@ __global__ void __launch_bounds__(AttnCfg<HD, TERMS>::NW * 32, 1) kv4_attn_kerne
 
     // ---- the ring of this warp: lane 0 walks ahead and copies
     Walk& next = sh.copy[warp];
-    uint32_t put = 0, got = 0, got_phase = 0, ahead = 0;  // stages: next to fill, next to read, filled and not read
+    uint32_t put = 0, got = 0, got_phase = 0;  // stages: next to fill, next to read
+    uint32_t ahead = 0;                        // (lane 0) stages filled and not read
     bool dead = false;                                     // a wait gave up
     auto issue = [&] {  // copies the next unit that some column sees, if there is one
         if (lane == 0) {
@@ -554,7 +555,7 @@ __global__ void __launch_bounds__(AttnCfg<HD, TERMS>::NW * 32, 1) kv4_attn_kerne
             const int32_t key0 = w.key0(tile0 + x);
             if (!seen.any(key0, kUnit, p.sinks)) continue;
             if (!dead) {
-                const bool in_time = mbar_wait(&sh.bar[warp][got], got_phase, nullptr);
+                const bool in_time = mbar_wait(&sh.bar[warp][got], got_phase, nullptr, p.wait_ns);
                 if (!__all_sync(0xffffffffu, in_time)) {
                     dead = true;
                     if (lane == 0) p.map.flag(BT_KV4_TIMEOUT);
@@ -570,7 +571,7 @@ __global__ void __launch_bounds__(AttnCfg<HD, TERMS>::NW * 32, 1) kv4_attn_kerne
                 __syncwarp();  // every lane is done with the stage
                 got_phase ^= got + 1 == S ? 1u : 0u;
                 got = got + 1 == S ? 0 : got + 1;
-                --ahead;
+                if (lane == 0) --ahead;
                 issue();
                 __syncwarp();
             }
@@ -718,8 +719,8 @@ __global__ void __launch_bounds__(AttnCfg<HD, TERMS>::NW * 32, 1) kv4_attn_kerne
         group_sync(group, threads);  // the slots and the queries' place are free again
     }
     // after an expired wait copies may still be on their way to this CTA's shared memory
-    for (; dead && ahead > 0; --ahead) {
-        mbar_wait(&sh.bar[warp][got], got_phase, nullptr);
+    for (; dead && lane == 0 && ahead > 0; --ahead) {
+        mbar_wait(&sh.bar[warp][got], got_phase, nullptr, p.wait_ns);
         got_phase ^= got + 1 == S ? 1u : 0u;
         got = got + 1 == S ? 0 : got + 1;
     }
@@ -763,6 +764,14 @@ using namespace bt;
 // prefill kernel's parts (the two run one after the other).
 static uint64_t ticket_bytes(int sms) { return ((uint64_t)sms * kMaxGroups * 4 + 255) / 256 * 256; }
 
+static std::atomic<uint32_t> g_stall_ms{0};
+
+extern "C" int bt_cuda_kv4_inject_stall(uint32_t wait_ms) {
+    BT_CHECK_ARG(wait_ms <= 2000, "kv4_inject_stall: at most 2000 ms");
+    g_stall_ms.store(wait_ms, std::memory_order_relaxed);
+    return BT_OK;
+}
+
 extern "C" uint64_t bt_cuda_kv4_attention_workspace(void) {
     const int sms = device_sms();
     if (sms <= 0) return 0;
@@ -795,6 +804,9 @@ extern "C" int bt_cuda_kv4_attention(const bt_kv4* cache, const bt_kv4_attn_args
     p.wide = heads_wide(a->q, a->dtype) && heads_wide(a->out, a->dtype);
     p.tickets = (uint32_t*)workspace;
     p.partial = (float*)((uint8_t*)workspace + ticket_bytes(sms));
+    const uint32_t stall_ms = g_stall_ms.load(std::memory_order_relaxed);
+    p.stalled = stall_ms ? 1 : 0;
+    p.wait_ns = stall_ms ? stall_ms * 1000000u : kWaitNs;
     const cudaStream_t s = as_stream(stream);
     // Sequences with many rows go to the tcgen05 kernel, which unpacks a tile once for 256 rows
     // instead of once for 8 but takes a whole tile's time for any number of them.  Measured, us,

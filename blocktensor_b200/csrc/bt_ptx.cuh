@@ -70,12 +70,12 @@ __device__ __forceinline__ uint64_t global_ns_after(float dep) {
 }
 
 // Bounded wait for the phase with parity `parity`; false (and *err set) on timeout.
-__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, uint32_t* err) {
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, uint32_t* err, uint32_t limit_ns = kWaitNs) {
     if (mbar_try_wait(bar, parity)) return true;
     const uint64_t t0 = global_ns();
     while (true) {
         if (mbar_try_wait_sleep(bar, parity, 100000u)) return true;
-        if (global_ns() - t0 > kWaitNs) {
+        if (global_ns() - t0 > limit_ns) {
             if (err) atomicExch(err, 1u);
             return false;
         }

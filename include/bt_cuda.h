@@ -581,6 +581,11 @@ BT_API int bt_cuda_kv4_attention(const bt_kv4* cache, const bt_kv4_attn_args* a,
                                  uint64_t workspace_bytes, void* stream);
 /* Bytes of workspace that a call needs on the current device, whatever its sizes. */
 BT_API uint64_t bt_cuda_kv4_attention_workspace(void);
+/* Fault injection on the host, for tests of BT_KV4_TIMEOUT: the device waits of
+ * this process's later bt_cuda_kv4_attention calls for their copies cannot end
+ * and give up after wait_ms (at most 2000); 0: as usual again.  No GPU fault, no
+ * hang. */
+BT_API int bt_cuda_kv4_inject_stall(uint32_t wait_ms);
 
 typedef struct bt_sample_args {
     const void*    logits;       /* [rows][vocab], rows row_stride elements apart */

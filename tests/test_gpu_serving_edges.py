@@ -1,9 +1,11 @@
 """GPU: cases at which the serving operators once answered wrongly or could have, against the plain 64-bit
 references of test_gpu_serving.py (its tolerances, unless a test derives its own)."""
+import time
+
 import numpy as np
 import pytest
 
-from test_gpu_serving import DT, T, check_rows, gen, ints, randn
+from test_gpu_serving import DT, T, Case, check_rows, gen, ints, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -49,3 +51,34 @@ def test_sample_few_tokens(cuda):
     u = [(i + 0.5) / 64 for i in range(64)]
     for k, p in ((3, 1.0), (0, 0.9), (4, 0.9), (600, 0.95)):
         assert check_rows(cuda, x, u, [1.0] * 64, [k] * 64, [p] * 64, [0.0] * 64) == 0
+
+
+# ---------------------------------------------------------------- attention
+
+def expire(c):
+    """One call of the case with device waits that run out after 5 ms: seconds until the host knows."""
+    from blocktensor_b200 import native
+    torch = T()
+    torch.cuda.synchronize()
+    native.call("bt_cuda_kv4_inject_stall", 5)
+    try:
+        t0 = time.time()
+        with pytest.raises(native.CudaBackendError) as e:
+            c.run()
+        took = time.time() - t0
+    finally:
+        native.call("bt_cuda_kv4_inject_stall", 0)
+    assert e.value.code == native.BT_ERR_DEVICE_TIMEOUT
+    return took
+
+
+@pytest.mark.parametrize("dt,hd", [("float32", 64), ("float16", 128), ("bfloat16", 256)])
+@pytest.mark.parametrize("lens", [[40], [5000], [900] * 9, [700, 3, 0, 64, 200] * 40])
+def test_attention_waits_run_out(cuda, dt, hd, lens):
+    """Waits for copies that give up end the kernel at once (a warp waits five times at most, for its unit
+    and for the four copies it has in flight: 25 ms), and the next call is right."""
+    torch = T()
+    c = Case(cuda, 400 + len(lens), dt, hd, 2, 4, lens, [1] * len(lens), 16)
+    good = c.check()
+    assert expire(c) < 1.0
+    assert torch.equal(c.run(), good)
