@@ -63,6 +63,7 @@ constexpr uint32_t kPfSeqs = 64;
 struct PfShared {
     uint64_t raw_full[2][kPfRaw], raw_empty[2][kPfRaw];        // of K, of V
     uint64_t full[2][kPfStages], empty[2][kPfStages];
+    uint64_t cleared;                                          // pairs of V rows that no row sees
     uint64_t q_full[2], s_full[2][2], p_full[2][2], pv_done[2], o_full[2], drain[2];  // of the halves
     uint32_t pieces[16];  // of a tile: which of its 16-key pieces hold keys
     uint32_t tmem;
@@ -260,11 +261,12 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
     }
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
-            for (uint32_t k = 0; k < kPfRaw; ++k) { mbar_init(&sh.raw_full[i][k], 1); mbar_init(&sh.raw_empty[i][k], 4); }
+            for (uint32_t k = 0; k < kPfRaw; ++k) { mbar_init(&sh.raw_full[i][k], 1 + p.stalled); mbar_init(&sh.raw_empty[i][k], 4); }
             for (uint32_t k = 0; k < kPfStages; ++k) { mbar_init(&sh.full[i][k], 4); mbar_init(&sh.empty[i][k], 2); }
             for (int k = 0; k < 2; ++k) { mbar_init(&sh.s_full[i][k], 1); mbar_init(&sh.p_full[i][k], 4); }
             mbar_init(&sh.q_full[i], 4); mbar_init(&sh.pv_done[i], 1); mbar_init(&sh.o_full[i], 1); mbar_init(&sh.drain[i], 1);
         }
+        mbar_init(&sh.cleared, 4);
         sh.dead = 0;
         fence_mbar_init();
     }
@@ -280,7 +282,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
         const uint64_t t0 = global_ns();
         while (!sh.dead) {
             if (mbar_try_wait_sleep(bar, parity, 20000u)) return true;
-            if (global_ns() - t0 > kWaitNs) {
+            if (global_ns() - t0 > p.wait_ns) {
                 sh.dead = 1;
                 p.map.flag(BT_KV4_TIMEOUT);
             }
@@ -524,7 +526,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
         const uint32_t u = tid & 127, side = warp < 12 ? 0 : 1;
         uint8_t* raw = raws + side * kPfRaw * C::RAW;
         uint8_t* to = kvs + side * kPfStages * C::KV;
-        uint32_t raw_at = 0, raw_phase = 0, st = 0, st_phase = 1;
+        uint32_t raw_at = 0, raw_phase = 0, st = 0, st_phase = 1, cleared = 0;
         for (uint32_t turn = 0; walk.find(p, sh, block_of(turn), lane, &it); ++turn) {
             bool ok = true;
             for (uint32_t i = 0; i < it.tiles; ++i) {
@@ -556,7 +558,11 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
 #pragma unroll
                             for (int j = 0; j < HD / 64; ++j) e[j] = 0;
                         }
-                        asm volatile("bar.sync 1, 128;" ::: "memory");
+                        // (an mbarrier: a warp that gave up does not come, and this wait ends with it)
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&sh.cleared);
+                        if (!(ok = warp_wait(&sh.cleared, cleared))) break;
+                        cleared ^= 1;
                     }
                     // a thread 8 keys x 8 elements
                     const uint32_t oct = u / CH, chunk = u % CH;
@@ -629,8 +635,8 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
         }
         // every copy has arrived before the CTA may end (a wait may have given up on one)
         for (uint32_t k = sent > kPfRaw ? sent - kPfRaw : 0; k < sent; ++k) {
-            mbar_wait(&sh.raw_full[0][k % kPfRaw], k / kPfRaw & 1, nullptr);
-            mbar_wait(&sh.raw_full[1][k % kPfRaw], k / kPfRaw & 1, nullptr);
+            mbar_wait(&sh.raw_full[0][k % kPfRaw], k / kPfRaw & 1, nullptr, p.wait_ns);
+            mbar_wait(&sh.raw_full[1][k % kPfRaw], k / kPfRaw & 1, nullptr, p.wait_ns);
         }
     } else if (warp < 19) {
         // ------------------------------------------------ MMAs of a half

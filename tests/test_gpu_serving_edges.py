@@ -82,3 +82,15 @@ def test_attention_waits_run_out(cuda, dt, hd, lens):
     good = c.check()
     assert expire(c) < 1.0
     assert torch.equal(c.run(), good)
+
+
+@pytest.mark.parametrize("dt,hd", [("float16", 64), ("bfloat16", 128)])
+@pytest.mark.parametrize("lens,counts,window", [([2000], [300], 0), ([900, 40], [900, 40], 0), ([800] * 40, [200] * 40, 300)])
+def test_attention_chunk_waits_run_out(cuda, dt, hd, lens, counts, window):
+    """The same in the many-row kernel, with parts of a block on several SMs, masked tiles and several blocks
+    a CTA: every warp leaves (seven waits of 5 ms at most)."""
+    torch = T()
+    c = Case(cuda, 500 + len(lens), dt, hd, 2, 8, lens, counts, 64, window, 4 if window else 0)
+    good = c.check()
+    assert expire(c) < 1.0
+    assert torch.equal(c.run(), good)
