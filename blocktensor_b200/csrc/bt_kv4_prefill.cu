@@ -7,7 +7,9 @@
 // A tile's keys and values are unpacked once into fp16 operands in shared memory
 // (scale * code + min, one rounding of 2^-12 rms) and serve both 128-row halves.
 // Queries enter scaled by a power of two per row, exact for bf16 and fp16; P is
-// rounded to fp16 (2^-12 rms); sums, maxima and O are fp32.
+// rounded to fp16 (2^-12 rms); sums, maxima and O are fp32.  m is held 7 below the
+// running maximum, so that P reaches 2^15 and a key counts down to 2^-32 of the largest
+// (fp16 ends at 2^-25: 131071 keys of 2^-25.5 beside one of 1 would lose their 0.3 %).
 //
 // Bound: at head_dim 128, 128 keys are 2048 tensor cycles (both halves' S and P V),
 // 2048 cycles of the exponential unit (256 x 128) and about 1500 issue slots a scheduler
@@ -44,6 +46,7 @@ constexpr int kPfThreads = 5 * 128;
 // Registers a thread of each warpgroup, of the 96 at launch.
 constexpr int kPfSoftmax = 128, kPfUnpack = 80, kPfRest = 56;
 static_assert(2 * kPfSoftmax + 2 * kPfUnpack + kPfRest <= 5 * 96, "no more than the block is launched with");
+constexpr float kPfAbove = 7.0f;   // a row's maximum is above its reference m by this, and by kLazyMax more at most
 constexpr uint32_t kPfRaw = 3;     // packed K (and V) tiles in flight
 constexpr uint32_t kPfStages = 4;  // unpacked K (and V) tiles
 
@@ -401,8 +404,8 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
                     for (int k = 0; k < 4; ++k) top4[k] = max3(top4[k], s[e + 2 * k], s[e + 2 * k + 1]);
                 }
                 const float top = max3(fmaxf(top4[0], top4[1]), top4[2], top4[3]) * f;
-                if (__any_sync(0xffffffffu, top > m + kLazyMax)) {
-                    const float now = fmaxf(m, top), fix = exp2_fast(m - now);
+                if (__any_sync(0xffffffffu, top > m + (kPfAbove + kLazyMax))) {
+                    const float now = fmaxf(m, top - kPfAbove), fix = exp2_fast(m - now);
                     m = now;
                     l *= fix;
                     if (i > 0) {  // once the products of the tiles so far are complete

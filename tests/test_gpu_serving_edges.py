@@ -5,7 +5,7 @@ import time
 import numpy as np
 import pytest
 
-from test_gpu_serving import DT, T, Case, check_rows, gen, ints, randn
+from test_gpu_serving import DT, HALF_ULP, T, Case, check_rows, gen, ints, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -94,3 +94,30 @@ def test_attention_chunk_waits_run_out(cuda, dt, hd, lens, counts, window):
     good = c.check()
     assert expire(c) < 1.0
     assert torch.equal(c.run(), good)
+
+
+@pytest.mark.parametrize("dt,hd", [("float16", 64), ("bfloat16", 128)])
+@pytest.mark.parametrize("tokens,n_keys", [(40, 131072), (320, 131072), (1, 131072)])
+@pytest.mark.parametrize("first", [True, False])
+@pytest.mark.parametrize("bits", [12.5, 24.5, 25.5, 28.5])
+def test_attention_peak_over_a_long_tail(cuda, dt, hd, tokens, n_keys, first, bits):
+    """One key whose value is 0 stands `bits` powers of two above all others, whose values are 1: the tail's
+    share of a row is N / (N + 2^bits).  Of a probability 2^-12 of itself may be lost where it is rounded to
+    fp16, or 2^-32 of the row's largest (half a unit of fp16's smallest, 2^-24, with the largest at 2^7 or
+    more); of the rest 2^-18; and the result's own rounding."""
+    torch = T()
+    kv, group = 8, 8
+    cache = cuda.KV4Cache(1, n_keys, kv, hd)
+    pair = np.array([0, 1], np.float16).view(np.uint8)  # scale 0, min 1
+    groups = torch.from_numpy(np.tile(pair, hd // 64)).cuda()
+    cache.v_rows[..., hd // 2:] = groups                # ones; keys are zeros
+    peak = 0 if first else n_keys - tokens
+    cache.k_rows[0, :, peak, hd // 2:] = groups
+    cache.v_rows[0, :, peak] = 0
+    q = torch.ones(tokens, kv * group, hd, dtype=getattr(torch, dt), device="cuda")
+    out = cache.attention(q, ints([n_keys]), q_start=ints([0, tokens]), max_q=tokens, scale=bits * np.log(2.0) / hd)
+    cache.check()
+    tail = torch.arange(n_keys - tokens, n_keys, device="cuda").double()  # keys that a row sees beside the peak
+    want = (tail / (tail + 2.0 ** bits))[:, None, None]
+    tol = tail[:, None, None] * 2.0 ** -32 + (2.0 ** -12 + HALF_ULP[dt]) * want + 2.0 ** -18
+    assert float(((out.double() - want).abs() / tol).max()) <= 1
