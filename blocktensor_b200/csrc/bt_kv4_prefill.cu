@@ -66,7 +66,6 @@ constexpr uint32_t kPfSeqs = 64;
 struct PfShared {
     uint64_t raw_full[2][kPfRaw], raw_empty[2][kPfRaw];        // of K, of V
     uint64_t full[2][kPfStages], empty[2][kPfStages];
-    uint64_t cleared;                                          // pairs of V rows that no row sees
     uint64_t q_full[2], s_full[2][2], p_full[2][2], pv_done[2], o_full[2], drain[2];  // of the halves
     uint32_t pieces[16];  // of a tile: which of its 16-key pieces hold keys
     uint32_t tmem;
@@ -269,7 +268,6 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
             for (int k = 0; k < 2; ++k) { mbar_init(&sh.s_full[i][k], 1); mbar_init(&sh.p_full[i][k], 4); }
             mbar_init(&sh.q_full[i], 4); mbar_init(&sh.pv_done[i], 1); mbar_init(&sh.o_full[i], 1); mbar_init(&sh.drain[i], 1);
         }
-        mbar_init(&sh.cleared, 4);
         sh.dead = 0;
         fence_mbar_init();
     }
@@ -529,7 +527,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
         const uint32_t u = tid & 127, side = warp < 12 ? 0 : 1;
         uint8_t* raw = raws + side * kPfRaw * C::RAW;
         uint8_t* to = kvs + side * kPfStages * C::KV;
-        uint32_t raw_at = 0, raw_phase = 0, st = 0, st_phase = 1, cleared = 0;
+        uint32_t raw_at = 0, raw_phase = 0, st = 0, st_phase = 1;
         for (uint32_t turn = 0; walk.find(p, sh, block_of(turn), lane, &it); ++turn) {
             bool ok = true;
             for (uint32_t i = 0; i < it.tiles; ++i) {
@@ -552,20 +550,18 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
                         *reinterpret_cast<uint4*>(dst + k * (kPfKeys * 16)) = v;
                     }
                 } else {
-                    // what no row sees may hold anything: its pairs become zero
+                    // what no row sees may hold anything: its pairs become zero, by the warp that reads them
                     const int32_t k0 = it.key0(i);
                     const uint32_t pieces = sh.pieces[(tile_no + i) & 15];
                     if (pieces != 0xfu || k0 + kPfKeys - 1 > it.top || (k0 <= it.above && (uint32_t)(k0 + kPfKeys) > p.sinks)) {
-                        if (u < kPfKeys && (!(pieces >> (u >> 4) & 1) || !it.any(k0 + (int32_t)u, 1, p.sinks))) {
-                            uint32_t* e = reinterpret_cast<uint32_t*>(raw + raw_at * C::RAW + u * C::RB + HD / 2);
+                        constexpr uint32_t OWN = 256 / CH;  // keys of a warp
+                        const uint32_t key = u / 32 * OWN + lane;
+                        if (lane < OWN && key < kPfKeys && (!(pieces >> (key >> 4) & 1) || !it.any(k0 + (int32_t)key, 1, p.sinks))) {
+                            uint32_t* e = reinterpret_cast<uint32_t*>(raw + raw_at * C::RAW + key * C::RB + HD / 2);
 #pragma unroll
                             for (int j = 0; j < HD / 64; ++j) e[j] = 0;
                         }
-                        // (an mbarrier: a warp that gave up does not come, and this wait ends with it)
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(&sh.cleared);
-                        if (!(ok = warp_wait(&sh.cleared, cleared))) break;
-                        cleared ^= 1;
                     }
                     // a thread 8 keys x 8 elements
                     const uint32_t oct = u / CH, chunk = u % CH;
