@@ -3,7 +3,10 @@ attention over them, batched sampling (bt_cuda_qk_norm_rope, bt_cuda_kv4_*, bt_c
 include/bt_cuda.h, which states their mathematics).
 
 Activations are fp32, fp16 or bf16 tensors whose last dimension is contiguous; every call checks its
-arguments (ValueError), launches on ``stream`` or torch's current stream, and does not synchronise.
+arguments (ValueError), launches on torch's current stream or on ``stream``, and does not synchronise.
+With ``stream`` the call is as if made under ``torch.cuda.stream(stream)``: the caller orders the two
+streams; what the call allocates is that stream's, and no tensor that it was given or returns is reused
+before both streams are done with it.
 Index tensors (positions, slots, lengths) are int32 on the device; values out of range are never
 followed and show in :meth:`KV4Cache.check`.
 """
@@ -72,14 +75,30 @@ def _vector(t, name, n, dtype, dev):
     return t.data_ptr()
 
 
-def _launch(fn, name, dev, stream, outs, *args):
-    """The C call on the tensors' device; ``outs``: tensors allocated here for the call."""
-    if stream is None:
-        s = _raw_stream(dev)
-    else:
-        s = stream.cuda_stream
-        for t in outs:
-            t.record_stream(stream)
+def _elsewhere(stream):
+    """Whether a call has to change streams."""
+    return stream is not None and stream.cuda_stream != _raw_stream(stream.device_index)
+
+
+def _on_stream(stream, keep, f, *args):
+    """f(*args) on ``stream``; ``keep``: tensors that it uses beside its arguments."""
+    here = torch.cuda.current_stream(stream.device)
+    given = [t for t in (*args, *keep) if isinstance(t, torch.Tensor) and t.is_cuda]
+    if any(t.get_device() != stream.device_index for t in given):
+        raise ValueError("stream: of another device than the tensors")
+    with torch.cuda.stream(stream):
+        out = f(*args)
+    for t in given:
+        t.record_stream(stream)
+    for t in out if isinstance(out, tuple) else (out,):
+        if t is not None and not any(t is g for g in given):
+            t.record_stream(here)
+    return out
+
+
+def _launch(fn, name, dev, *args):
+    """The C call on the tensors' device and its current stream."""
+    s = _raw_stream(dev)
     if dev == _current_device():
         rc = fn(*args, s)
     else:
@@ -114,11 +133,12 @@ def qk_norm_rope(q, k, q_weight, k_weight, positions, table, eps: float = 1e-5, 
     """Norms of each head of q [T, H, hd] and k [T, KVH, hd] and their rotation, one pass over both
     (bt_cuda_qk_norm_rope).  q_weight / k_weight: [hd] float32, or None for no norm; table: rope_table(),
     or None for no rotation; positions: [T] int32.  q_out / k_out may be q and k.  k may be None."""
+    if _elsewhere(stream):
+        return _on_stream(stream, (), qk_norm_rope, q, k, q_weight, k_weight, positions, table, eps, q_out, k_out)
     qh = _heads(q, "q")
     shape, dtype, dev = q.shape, q.dtype, q.get_device()
     tokens, heads, hd = shape
     q_out, qoh = _out(q_out, "q_out", shape, q, dev)
-    outs = [q_out]
     kh = koh = _NO_HEADS
     kv_heads = 0
     if k is not None:
@@ -126,13 +146,12 @@ def qk_norm_rope(q, k, q_weight, k_weight, positions, table, eps: float = 1e-5, 
         k_shape = (tokens, kv_heads, hd)
         kh = _heads(k, "k", k_shape, dtype, dev)
         k_out, koh = _out(k_out, "k_out", k_shape, k, dev)
-        outs.append(k_out)
     a = _pack_qk.pack(*qh, *kh, *_NO_HEADS, *qoh, *koh,
                       0 if q_weight is None else _vector(q_weight, "q_weight", hd, torch.float32, dev),
                       0 if k_weight is None else _vector(k_weight, "k_weight", hd, torch.float32, dev),
                       _vector(positions, "positions", tokens, torch.int32, dev), 0,
                       *_rope(table, dev), tokens, heads, kv_heads, hd, _dtype(q), eps)
-    _launch(native.load().bt_cuda_qk_norm_rope, "bt_cuda_qk_norm_rope", dev, stream, outs, a)
+    _launch(native.load().bt_cuda_qk_norm_rope, "bt_cuda_qk_norm_rope", dev, a)
     return q_out, k_out
 
 
@@ -232,6 +251,9 @@ class KV4Cache:
         if status & native.BT_KV4_RANGE:
             raise IndexError("KV4Cache: a slot, position, length or page was out of range")
 
+    def _tensors(self):
+        return (self.k_rows, self.v_rows, self.status) + (() if self.page_table is None else (self.page_table,))
+
     # ------------------------------------------------------------ rows
 
     def append(self, k, v, slots, positions, stream=None):
@@ -244,35 +266,39 @@ class KV4Cache:
         return self._append(q, k, v, q_weight, k_weight, slots, positions, table, eps, q_out, stream)
 
     def _append(self, q, k, v, q_weight, k_weight, slots, positions, table, eps, q_out, stream):
+        if _elsewhere(stream):
+            return _on_stream(stream, self._tensors(), self._append, q, k, v, q_weight, k_weight, slots, positions, table, eps,
+                              q_out, None)
         if k.dim() != 3:
             raise ValueError("append: expected [tokens, kv_heads, head_dim] tensors")
         dev, hd, tokens, dtype = self._index, self.head_dim, k.shape[0], k.dtype
         shape = (tokens, self.kv_heads, hd)  # of the cache
         kh = _heads(k, "k", shape, dtype, dev)
         qh = qoh = _NO_HEADS
-        heads, outs = 0, ()
+        heads = 0
         if q is not None:
             heads = q.shape[1] if q.dim() == 3 else 0
             q_shape = (tokens, heads, hd)
             qh = _heads(q, "q", q_shape, dtype, dev)
             q_out, qoh = _out(q_out, "q_out", q_shape, q, dev)
-            outs = (q_out,)
         a = _pack_qk.pack(*qh, *kh, *_heads(v, "v", shape, dtype, dev), *qoh, *_NO_HEADS,
                           0 if q_weight is None else _vector(q_weight, "q_weight", hd, torch.float32, dev),
                           0 if k_weight is None else _vector(k_weight, "k_weight", hd, torch.float32, dev),
                           _vector(positions, "positions", tokens, torch.int32, dev), _vector(slots, "slots", tokens, torch.int32, dev),
                           *_rope(table, dev), tokens, heads, self.kv_heads, hd, _dtype(k), eps)
-        _launch(native.load().bt_cuda_kv4_append, "bt_cuda_kv4_append", dev, stream, outs, self._ref, a)
+        _launch(native.load().bt_cuda_kv4_append, "bt_cuda_kv4_append", dev, self._ref, a)
         return q_out
 
     def read(self, slots, positions, dtype=torch.float16, stream=None):
         """The values that the rows at (slots[t], positions[t]) stand for: k, v [T, KVH, hd]."""
+        if _elsewhere(stream):
+            return _on_stream(stream, self._tensors(), self.read, slots, positions, dtype)
         dev, tokens = self._index, positions.numel()
         if dtype not in _DTYPES:
             raise ValueError("read: dtype must be float32, float16 or bfloat16")
         k = torch.empty((tokens, self.kv_heads, self.head_dim), dtype=dtype, device=self.device)
         v = torch.empty_like(k)
-        _launch(native.load().bt_cuda_kv4_read, "bt_cuda_kv4_read", dev, stream, (k, v), self._ref,
+        _launch(native.load().bt_cuda_kv4_read, "bt_cuda_kv4_read", dev, self._ref,
                 _vector(slots, "slots", tokens, torch.int32, dev), _vector(positions, "positions", tokens, torch.int32, dev),
                 tokens, _DTYPES[dtype], k.data_ptr(), v.data_ptr())
         return k, v
@@ -288,6 +314,8 @@ class KV4Cache:
         [n + 1] int32: sequence i's queries are rows q_start[i] .. q_start[i + 1] - 1 of q; None: one each.
         slots [n] int32: the sequences' slots; None: sequence i is slot i.  max_q: no sequence has more
         queries (0: not known)."""
+        if _elsewhere(stream):
+            return _on_stream(stream, self._tensors(), self.attention, q, kv_len, q_start, slots, max_q, window, sinks, scale, out)
         qh = _heads(q, "q")
         dev, shape, n = self._index, q.shape, kv_len.numel()
         tokens, heads, hd = shape
@@ -300,15 +328,14 @@ class KV4Cache:
                             0 if q_start is None else _vector(q_start, "q_start", n + 1, torch.int32, dev),
                             0 if slots is None else _vector(slots, "slots", n, torch.int32, dev),
                             n, tokens, heads, max_q, window, sinks, _dtype(q), hd ** -0.5 if scale is None else scale)
-        s = _raw_stream(dev) if stream is None else stream.cuda_stream
+        s = _raw_stream(dev)
         ws = _workspaces.get((dev, s))
         if ws is None:  # one for every stream that calls come from, for all caches
             with torch.cuda.device(dev):
                 size = native.load().bt_cuda_kv4_attention_workspace()
-            with torch.cuda.stream(torch.cuda.current_stream(dev) if stream is None else stream):
-                ws = torch.zeros(size, dtype=torch.uint8, device=self.device)
+            ws = torch.zeros(size, dtype=torch.uint8, device=self.device)
             ws = _workspaces[dev, s] = (ws.data_ptr(), size, ws)
-        _launch(native.load().bt_cuda_kv4_attention, "bt_cuda_kv4_attention", dev, stream, (out,), self._ref, a, ws[0], ws[1])
+        _launch(native.load().bt_cuda_kv4_attention, "bt_cuda_kv4_attention", dev, self._ref, a, ws[0], ws[1])
         return out
 
 
@@ -316,6 +343,8 @@ def sample_batch(logits, u, temperature=None, top_k=None, top_p=None, min_p=None
     """A token for every row of logits [B, V] from the given random numbers u [B] in [0, 1)
     (bt_cuda_sample_batch).  temperature, top_p, min_p [B] float32 and top_k [B] int32 on the device, or
     None for none of that.  Returns (token [B] int32, logprob [B] float32)."""
+    if _elsewhere(stream):
+        return _on_stream(stream, (), sample_batch, logits, u, temperature, top_k, top_p, min_p, token, logprob)
     if logits.dim() != 2 or not logits.is_cuda or (logits.stride(1) != 1 and logits.shape[1] > 1):
         raise ValueError("sample_batch: expected a [rows, vocab] CUDA tensor with contiguous rows")
     dev, (rows, vocab) = logits.get_device(), logits.shape
@@ -329,5 +358,5 @@ def sample_batch(logits, u, temperature=None, top_k=None, top_p=None, min_p=None
                           0 if min_p is None else _vector(min_p, "min_p", rows, f32, dev),
                           _vector(token, "token", rows, i32, dev), _vector(logprob, "logprob", rows, f32, dev),
                           rows, vocab, _dtype(logits), 0)
-    _launch(native.load().bt_cuda_sample_batch, "bt_cuda_sample_batch", dev, stream, (token, logprob), a)
+    _launch(native.load().bt_cuda_sample_batch, "bt_cuda_sample_batch", dev, a)
     return token, logprob

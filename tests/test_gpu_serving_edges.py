@@ -121,3 +121,78 @@ def test_attention_peak_over_a_long_tail(cuda, dt, hd, tokens, n_keys, first, bi
     want = (tail / (tail + 2.0 ** bits))[:, None, None]
     tol = tail[:, None, None] * 2.0 ** -32 + (2.0 ** -12 + HALF_ULP[dt]) * want + 2.0 ** -18
     assert float(((out.double() - want).abs() / tol).max()) <= 1
+
+
+# ---------------------------------------------------------------- streams
+
+def operators(cuda, g):
+    """Every operator as f(inputs, stream) -> outputs, on inputs (a list of tensors) of its own, at sizes that the
+    caching allocator keeps in blocks of their own."""
+    torch = T()
+    n, kv, hd = 512, 8, 128
+    cache = cuda.KV4Cache(n, 64, kv, hd)
+    table, w = cuda.rope_table(64, hd), torch.ones(hd, device="cuda")
+    slots = torch.arange(n, device="cuda").int()
+    pos = torch.arange(n, device="cuda").int() % 64
+    lens, u = pos + 1, torch.rand(64, generator=g, device="cuda")
+    x = lambda h: randn(g, n, h, hd)  # noqa: E731
+    cache.append(x(kv), x(kv), slots, torch.zeros_like(pos))
+    return {
+        "norms": ([x(16), x(kv)], lambda i, s: cuda.qk_norm_rope(i[0], i[1], w, w, pos, table, stream=s)),
+        "append": ([x(16), x(kv), x(kv)],
+                   lambda i, s: (cache.append_normed(i[0], i[1], i[2], w, w, slots, pos, table, stream=s),)),
+        "read": ([pos.clone()], lambda i, s: cache.read(slots, i[0], torch.float32, stream=s)),
+        "attention": ([x(16)], lambda i, s: (cache.attention(i[0], lens, stream=s),)),
+        "sample": ([randn(g, 64, 65536)], lambda i, s: cuda.sample_batch(i[0], u, stream=s)),
+    }
+
+
+@pytest.mark.parametrize("name", ["norms", "append", "read", "attention", "sample"])
+def test_streams_and_freed_memory(cuda, name):
+    """Outputs do not take memory that the current stream still has work on; inputs that the caller drops after
+    the call are not reused while it runs; outputs that the caller drops are not while the current stream reads."""
+    torch = T()
+    inputs, f = operators(cuda, gen(81))[name]
+    want = [t.clone() for t in f(inputs, None)]
+    side, here = torch.cuda.Stream(), torch.cuda.current_stream()
+    torch.cuda.synchronize()
+    f(inputs, side)
+    torch.cuda.synchronize()
+
+    # freed on the current stream, with a read of it pending there
+    old = [torch.full_like(t, 3) for t in want]
+    places = {t.data_ptr() for t in old}
+    torch.cuda._sleep(100_000_000)
+    kept = [t.clone() for t in old]
+    del old
+    out = f(inputs, side)
+    assert not places & {t.data_ptr() for t in out}
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(out, want))
+    torch.cuda.synchronize()
+    assert all(bool((t == 3).all()) for t in kept)
+
+    # inputs that are dropped while the call has not begun
+    mine = [t.clone() for t in inputs]
+    places = {t.data_ptr() for t in mine}
+    side.wait_stream(here)
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(100_000_000)
+    out = f(mine, side)
+    del mine
+    again = [torch.zeros_like(t) for t in inputs]
+    assert not places & {t.data_ptr() for t in again}
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+    # outputs that are dropped while the current stream has not read them
+    places = {t.data_ptr() for t in out}
+    here.wait_stream(side)
+    torch.cuda._sleep(100_000_000)
+    kept = [t.clone() for t in out]
+    del out
+    with torch.cuda.stream(side):
+        again = [torch.zeros_like(t) for t in want]
+    assert not places & {t.data_ptr() for t in again}
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(kept, want))
