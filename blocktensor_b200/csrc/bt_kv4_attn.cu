@@ -762,7 +762,17 @@ using namespace bt;
 
 // Tickets, then partial results: two pieces for every range of the few-row kernel, or the
 // prefill kernel's parts (the two run one after the other).
-static uint64_t ticket_bytes(int sms) { return ((uint64_t)sms * kMaxGroups * 4 + 255) / 256 * 256; }
+static bool tickets_fit(int sms) { return (uint64_t)sms * kMaxGroups * 4 <= BT_KV4_WORKSPACE_ZERO; }
+
+extern "C" uint64_t bt_cuda_capture_id(void* stream) {
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    if (cudaStreamGetCaptureInfo(as_stream(stream), &status, &id) != cudaSuccess) {
+        cudaGetLastError();  // (the legacy stream beside a capture: it is in none)
+        return 0;
+    }
+    return status == cudaStreamCaptureStatusNone ? 0 : id;
+}
 
 static std::atomic<uint32_t> g_stall_ms{0};
 
@@ -774,9 +784,9 @@ extern "C" int bt_cuda_kv4_inject_stall(uint32_t wait_ms) {
 
 extern "C" uint64_t bt_cuda_kv4_attention_workspace(void) {
     const int sms = device_sms();
-    if (sms <= 0) return 0;
+    if (sms <= 0 || !tickets_fit(sms)) return 0;
     const uint64_t few = (uint64_t)sms * kMaxGroups * 2 * kPieceFloats * 4, many = prefill_workspace(sms);
-    return ticket_bytes(sms) + (few > many ? few : many);
+    return BT_KV4_WORKSPACE_ZERO + (few > many ? few : many);
 }
 
 extern "C" int bt_cuda_kv4_attention(const bt_kv4* cache, const bt_kv4_attn_args* a, void* workspace,
@@ -794,7 +804,7 @@ extern "C" int bt_cuda_kv4_attention(const bt_kv4* cache, const bt_kv4_attn_args
     BT_CHECK_ARG(a->q.data && a->out.data && a->kv_len, "kv4_attention: null q, out or kv_len");
     BT_CHECK_ARG(((uintptr_t)a->q.data | (uintptr_t)a->out.data) % act_bytes(a->dtype) == 0, "kv4_attention: a tensor is not aligned to its elements");
     const int sms = device_sms();
-    if (sms <= 0) return fail(BT_ERR_CUDA, "kv4_attention: no device");
+    if (sms <= 0 || !tickets_fit(sms)) return fail(BT_ERR_CUDA, "kv4_attention: no device, or one of more than 1024 SMs");
     BT_CHECK_ARG(workspace && (uintptr_t)workspace % 256 == 0 && workspace_bytes >= bt_cuda_kv4_attention_workspace(),
                  "kv4_attention: the workspace is null, not 256-byte aligned or too small");
     p.q = a->q.data; p.out = a->out.data; p.q_ts = a->q.token_stride; p.q_hs = a->q.head_stride;
@@ -803,7 +813,7 @@ extern "C" int bt_cuda_kv4_attention(const bt_kv4* cache, const bt_kv4_attn_args
     p.window = a->window; p.sinks = a->window ? a->sinks : 0; p.scale_log2 = a->scale * 1.4426950408889634f;
     p.wide = heads_wide(a->q, a->dtype) && heads_wide(a->out, a->dtype);
     p.tickets = (uint32_t*)workspace;
-    p.partial = (float*)((uint8_t*)workspace + ticket_bytes(sms));
+    p.partial = (float*)((uint8_t*)workspace + BT_KV4_WORKSPACE_ZERO);
     const uint32_t stall_ms = g_stall_ms.load(std::memory_order_relaxed);
     p.stalled = stall_ms ? 1 : 0;
     p.wait_ns = stall_ms ? stall_ms * 1000000u : kWaitNs;

@@ -29,6 +29,7 @@ BT_BF16 = 2
 
 BT_KV4_RANGE = 1
 BT_KV4_TIMEOUT = 2
+BT_KV4_WORKSPACE_ZERO = 16384
 
 
 class CudaBackendError(RuntimeError):
@@ -152,6 +153,7 @@ SIGNATURES = {
     "bt_cuda_kv4_attention": (_i32, [_vp, _vp, _vp, _u64, _vp]),
     "bt_cuda_kv4_attention_workspace": (_u64, []),
     "bt_cuda_kv4_inject_stall": (_i32, [_u32]),
+    "bt_cuda_capture_id": (_u64, [_vp]),
     "bt_cuda_sample_batch": (_i32, [_vp, _vp]),
     "bt_engine_create": (_i32, [_i32, C.POINTER(ModelConfig), C.POINTER(EngineOptions), C.POINTER(_vp)]),
     "bt_engine_destroy": (_i32, [_vp]),

@@ -36,8 +36,29 @@ _raw_stream = torch._C._cuda_getCurrentRawStream
 _current_device = torch._C._cuda_getDevice
 
 # (device, stream) -> (pointer, bytes, tensor): the attention's scratch, kept as calls of one
-# stream follow one another
+# stream follow one another.  Calls that are captured take one of their capture's own (the
+# fourth member is its number), which the graph clears at every replay: graphs may be replayed
+# in any order and beside one another and calls.
 _workspaces = {}
+_captured = {}
+_is_capturing = torch._C._cuda_isCurrentStreamCapturing
+
+
+def _workspace(dev):
+    """(pointer, bytes) of the attention's scratch for a call on a device's current stream."""
+    s = _raw_stream(dev)
+    capture = 0
+    if dev != _current_device() or _is_capturing():
+        capture = native.load().bt_cuda_capture_id(s)
+    cache = _captured if capture else _workspaces
+    ws = cache.get((dev, s))
+    if ws is None or ws[3] != capture:
+        with torch.cuda.device(dev):
+            size = native.load().bt_cuda_kv4_attention_workspace()
+            mem = torch.empty(size, dtype=torch.uint8, device="cuda")
+            mem[:native.BT_KV4_WORKSPACE_ZERO].zero_()
+        ws = cache[dev, s] = (mem.data_ptr(), size, mem, capture)
+    return ws[0], ws[1]
 
 
 def _dtype(t) -> int:
@@ -328,14 +349,7 @@ class KV4Cache:
                             0 if q_start is None else _vector(q_start, "q_start", n + 1, torch.int32, dev),
                             0 if slots is None else _vector(slots, "slots", n, torch.int32, dev),
                             n, tokens, heads, max_q, window, sinks, _dtype(q), hd ** -0.5 if scale is None else scale)
-        s = _raw_stream(dev)
-        ws = _workspaces.get((dev, s))
-        if ws is None:  # one for every stream that calls come from, for all caches
-            with torch.cuda.device(dev):
-                size = native.load().bt_cuda_kv4_attention_workspace()
-            ws = torch.zeros(size, dtype=torch.uint8, device=self.device)
-            ws = _workspaces[dev, s] = (ws.data_ptr(), size, ws)
-        _launch(native.load().bt_cuda_kv4_attention, "bt_cuda_kv4_attention", dev, self._ref, a, ws[0], ws[1])
+        _launch(native.load().bt_cuda_kv4_attention, "bt_cuda_kv4_attention", dev, self._ref, a, *_workspace(dev))
         return out
 
 

@@ -573,14 +573,19 @@ typedef struct bt_kv4_attn_args {
  * share a KV head, in order.  A row that sees nothing becomes 0.  Positions that
  * no row of their sequence sees may hold anything, and their pages need not be
  * in the table.  workspace: device memory of
- * bt_cuda_kv4_attention_workspace() bytes, zeroed once before its first call
- * (calls leave it ready for the next); calls that may overlap on the GPU need
- * one each; after BT_KV4_TIMEOUT it is zeroed again.  Deterministic: the same
- * inputs give the same bits. */
+ * bt_cuda_kv4_attention_workspace() bytes, whose first BT_KV4_WORKSPACE_ZERO are
+ * zeroed once before its first call (calls leave it ready for the next); calls
+ * that may overlap on the GPU need one each, and so do captured graphs whose
+ * replays may; after BT_KV4_TIMEOUT they are zeroed again.  Deterministic: the
+ * same inputs give the same bits. */
+#define BT_KV4_WORKSPACE_ZERO 16384u
 BT_API int bt_cuda_kv4_attention(const bt_kv4* cache, const bt_kv4_attn_args* a, void* workspace,
                                  uint64_t workspace_bytes, void* stream);
 /* Bytes of workspace that a call needs on the current device, whatever its sizes. */
 BT_API uint64_t bt_cuda_kv4_attention_workspace(void);
+/* A number for the capture that a stream is in, another one for every capture;
+ * 0: none. */
+BT_API uint64_t bt_cuda_capture_id(void* stream);
 /* Fault injection on the host, for tests of BT_KV4_TIMEOUT: the device waits of
  * this process's later bt_cuda_kv4_attention calls for their copies cannot end
  * and give up after wait_ms (at most 2000); 0: as usual again.  No GPU fault, no

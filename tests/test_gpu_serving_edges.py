@@ -196,3 +196,80 @@ def test_streams_and_freed_memory(cuda, name):
     assert not places & {t.data_ptr() for t in again}
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(kept, want))
+
+
+# ---------------------------------------------------------------- graphs
+
+def capture(c, lens, out, starts):
+    """A graph of two calls, made as a program would that has not called before: no stream given, no call first."""
+    torch = T()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for o in out:
+            c.cache.attention(c.q, lens, q_start=starts, max_q=max(c.counts), out=o)
+    return graph
+
+
+@pytest.mark.parametrize("lens,counts", [([3000, 300], [1, 1]), ([1500], [200])])
+def test_attention_graphs_are_independent(cuda, lens, counts):
+    """Graphs captured on one stream, without a call before: the later one replayed first, whatever their
+    scratch held; eager calls on the capture stream between them; both at a time on two streams."""
+    from blocktensor_b200 import serving
+    torch = T()
+    c = Case(cuda, 600 + len(lens), "float16", 128, 2, 8, lens, counts, 64)
+    starts = None if max(counts) == 1 else c.starts
+    want = c.check()
+    at = ints(lens)
+    outs = [[torch.zeros_like(c.q) for _ in range(2)] for _ in range(2)]
+    torch.cuda.synchronize()
+    known = set(serving._workspaces)
+    graphs = [capture(c, at, o, starts) for o in outs]
+    assert set(serving._workspaces) == known  # nothing of a capture serves eager calls
+    for kept in (serving._workspaces, serving._captured):
+        for key, ws in kept.items():
+            if key not in known:
+                ws[2].fill_(255)
+    for g in (1, 0):
+        graphs[g].replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, want) for o in outs[g])
+    side = [torch.cuda.Stream(), torch.cuda.Stream()]
+    with torch.cuda.stream(torch.cuda.graph.default_capture_stream):
+        eager = c.cache.attention(c.q, at, q_start=starts, max_q=max(counts))
+    torch.cuda.synchronize()
+    assert torch.equal(eager, want)
+    for _ in range(20):
+        for g in range(2):
+            for o in outs[g]:
+                o.zero_()
+        for g in range(2):
+            side[g].wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side[g]):
+                for _ in range(10):
+                    graphs[g].replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, want) for g in range(2) for o in outs[g])
+    c.cache.check()
+
+
+def test_attention_graph_with_branches(cuda):
+    """Calls on two streams of one capture do not share scratch."""
+    torch = T()
+    c = Case(cuda, 620, "bfloat16", 64, 2, 4, [5000], [1], 16)
+    want, at = c.check(), ints([5000])
+    outs = [torch.zeros_like(c.q) for _ in range(8)]
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        here = torch.cuda.current_stream()
+        side.wait_stream(here)
+        for i, o in enumerate(outs):
+            c.cache.attention(c.q, at, out=o, stream=side if i % 2 else None)
+        here.wait_stream(side)
+    for _ in range(20):
+        for o in outs:
+            o.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, want) for o in outs)

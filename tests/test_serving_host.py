@@ -161,3 +161,12 @@ def test_cache_object_refusals(kw):
     args.update(kw)
     with pytest.raises(ValueError):
         bt.KV4Cache(**args)
+
+
+def test_workspace_constants(nat):
+    """The bindings' constants are the header's; a library without a device reports no workspace and no capture."""
+    src = open(f"{ROOT}/include/bt_cuda.h").read()
+    assert int(re.search(r"#define BT_KV4_WORKSPACE_ZERO (\d+)u", src).group(1)) == nat.BT_KV4_WORKSPACE_ZERO
+    assert nat.load().bt_cuda_capture_id(None) == 0
+    refused(nat, "bt_cuda_kv4_inject_stall", 2001, match="2000")
+    nat.call("bt_cuda_kv4_inject_stall", 0)
