@@ -268,6 +268,8 @@ class KV4Cache:
         status = int(self.status.item())
         self.status.zero_()
         if status & native.BT_KV4_TIMEOUT:
+            for key in [k for k in _workspaces if k[0] == self._index]:  # (to be cleared before its next call)
+                del _workspaces[key]
             raise native.CudaBackendError(native.BT_ERR_DEVICE_TIMEOUT, "KV4Cache: a device wait gave up")
         if status & native.BT_KV4_RANGE:
             raise IndexError("KV4Cache: a slot, position, length or page was out of range")

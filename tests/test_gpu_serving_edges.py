@@ -273,3 +273,18 @@ def test_attention_graph_with_branches(cuda):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(o, want) for o in outs)
+
+
+@pytest.mark.parametrize("counts", [[1], [200]])
+def test_attention_after_a_timeout(cuda, counts):
+    """Whatever an expired wait left in the scratch, the next call begins with cleared tickets."""
+    from blocktensor_b200 import native, serving
+    torch = T()
+    c = Case(cuda, 630, "float16", 64, 2, 4, [3000], counts, 16)
+    good = c.check()
+    for ws in serving._workspaces.values():
+        ws[2].fill_(255)
+    c.cache.status.fill_(native.BT_KV4_TIMEOUT)
+    with pytest.raises(native.CudaBackendError):
+        c.cache.check()
+    assert torch.equal(c.run(), good)

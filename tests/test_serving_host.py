@@ -170,3 +170,27 @@ def test_workspace_constants(nat):
     assert nat.load().bt_cuda_capture_id(None) == 0
     refused(nat, "bt_cuda_kv4_inject_stall", 2001, match="2000")
     nat.call("bt_cuda_kv4_inject_stall", 0)
+
+
+def test_timeout_drops_the_scratch():
+    """What a call whose wait gave up leaves in the attention's scratch serves no later call of that device."""
+    import blocktensor_b200 as bt
+    from blocktensor_b200 import native, serving
+    c = bt.KV4Cache(1, 16, 1, 64, device="cpu")
+    keys = [(c._index, 7), (c._index, 9), ("another device", 7)]
+    for k in keys:
+        serving._workspaces[k] = (0, 0, None, 0)
+    try:
+        c.status.fill_(native.BT_KV4_RANGE)
+        with pytest.raises(IndexError):
+            c.check()
+        assert all(k in serving._workspaces for k in keys)
+        c.status.fill_(native.BT_KV4_TIMEOUT)
+        with pytest.raises(native.CudaBackendError) as e:
+            c.check()
+        assert e.value.code == native.BT_ERR_DEVICE_TIMEOUT
+        assert [k in serving._workspaces for k in keys] == [False, False, True]
+        c.check()
+    finally:
+        for k in keys:
+            serving._workspaces.pop(k, None)
