@@ -582,7 +582,7 @@ __global__ void __launch_bounds__(kSbThreads, 2) sample_batch_kernel(SampleParam
         }
         return;
     }
-    if (temp <= 0.0f) {
+    if (!(temp > 0.0f)) {
         const uint32_t first = r.first_of_maximum();
         if (r.rank == 0 && threadIdx.x == 0) {
             p.token[b] = (int32_t)first;
@@ -594,7 +594,7 @@ __global__ void __launch_bounds__(kSbThreads, 2) sample_batch_kernel(SampleParam
     if (r.m == INFINITY || r.inv == INFINITY) r.flatten();
     const float reach = fminf((r.m - least) * r.inv, kSbReach);
     r.steps = reach > 0.0f ? (float)(kSbBins - 2) / reach : 0.0f;
-    const float top_p = p.top_p ? p.top_p[b] : 1.0f, min_p = p.min_p ? p.min_p[b] : 0.0f;
+    const float top_p = p.top_p ? p.top_p[b] : 1.0f, min_p = p.min_p ? fmaxf(p.min_p[b], 0.0f) : 0.0f;  // (0 for NaN)
     const int32_t top_k = p.top_k ? p.top_k[b] : 0;
     const uint32_t top = sb_key(r.m + 0.0f);
     const float u = p.u[b];

@@ -596,10 +596,10 @@ typedef struct bt_sample_args {
     const void*    logits;       /* [rows][vocab], rows row_stride elements apart */
     int64_t        row_stride;
     const float*   u;            /* [rows] device: random numbers in [0, 1) */
-    const float*   temperature;  /* [rows] device, or NULL: 1; <= 0: greedy */
+    const float*   temperature;  /* [rows] device, or NULL: 1; <= 0 or NaN: greedy */
     const int32_t* top_k;        /* [rows] device, or NULL; <= 0: no cut */
-    const float*   top_p;        /* [rows] device, or NULL; >= 1: no cut */
-    const float*   min_p;        /* [rows] device, or NULL; <= 0: no cut */
+    const float*   top_p;        /* [rows] device, or NULL; >= 1 or NaN: no cut */
+    const float*   min_p;        /* [rows] device, or NULL; <= 0 or NaN: no cut */
     int32_t*       token;        /* [rows] device */
     float*         logprob;      /* [rows] device, or NULL */
     uint32_t       rows, vocab;  /* vocab <= 4194304 */

@@ -288,3 +288,20 @@ def test_attention_after_a_timeout(cuda, counts):
     with pytest.raises(native.CudaBackendError):
         c.cache.check()
     assert torch.equal(c.run(), good)
+
+
+@pytest.mark.parametrize("vocab", [100, 60000, 400000])
+def test_sample_nan_parameters(cuda, vocab):
+    """A NaN temperature is greedy, a NaN top-p or min-p cuts nothing, and a NaN u draws as 0 does."""
+    torch = T()
+    g, rows = gen(vocab), 8
+    x = randn(g, rows, vocab)
+    x[1::2, vocab // 2:vocab // 2 + 5] = 9.0  # equal maxima
+    f = lambda v: torch.full((rows,), v, device="cuda")  # noqa: E731
+    u, nan = torch.linspace(0, 0.99, rows, device="cuda"), f(float("nan"))
+    for k in (None, torch.full((rows,), 40, dtype=torch.int32, device="cuda")):
+        same = lambda a, b: all(torch.equal(s, t) for s, t in zip(a, b))  # noqa: E731
+        assert same(cuda.sample_batch(x, u, nan, k), cuda.sample_batch(x, u, f(0.0), k))
+        assert same(cuda.sample_batch(x, u, None, k, nan, None), cuda.sample_batch(x, u, None, k))
+        assert same(cuda.sample_batch(x, u, None, k, None, nan), cuda.sample_batch(x, u, None, k))
+        assert same(cuda.sample_batch(x, nan, None, k), cuda.sample_batch(x, f(0.0), None, k))
