@@ -21,6 +21,8 @@
 // step): a call on short caches spends its time fetching it.
 #include "bt_kv4_attn.cuh"
 
+#include <cmath>
+
 namespace bt {
 
 template <int HD, int TERMS>
@@ -344,8 +346,10 @@ __global__ void __launch_bounds__(AttnCfg<HD, TERMS>::NW * 32, 1) kv4_attn_kerne
 #pragma unroll
             for (int o = 1; o < 64 / E; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
             if (lane % (64 / E) == 0) sh.qsum[group][c][lane / (64 / E)] = sum * 0x1p-24f;
-            // scores come in units of 2^-24 2^up
-            if (lane == 0) sh.factor[group][c] = p.scale_log2 * __int_as_float((127 - up) << 23) * 0x1p24f;
+            // scores come in units of 2^-24 2^up (queries from 2^117 on would overflow the factor but not a
+            // score: a smaller one leaves such scores in their order, and one of them takes all)
+            const float factor = p.scale_log2 * __int_as_float((127 - up) << 23) * 0x1p24f;
+            if (lane == 0) sh.factor[group][c] = fminf(fmaxf(factor, -kLargest), kLargest);
         }
         group_sync(group, WG * 32);
         uint32_t qf[NG * 4][2], ql[TERMS == 2 ? NG * 4 : 1][2];
@@ -800,6 +804,8 @@ extern "C" int bt_cuda_kv4_attention(const bt_kv4* cache, const bt_kv4_attn_args
     BT_CHECK_ARG((uint64_t)a->tokens * a->heads <= 0x7fffffffu && a->n <= 0x7fffffffu, "kv4_attention: too many rows or sequences");
     BT_CHECK_ARG(a->q_start || a->tokens == a->n, "kv4_attention: without q_start there is one query per sequence");
     BT_CHECK_ARG(a->slots || a->n <= cache->n_seq, "kv4_attention: more sequences than slots");
+    p.scale_log2 = a->scale * 1.4426950408889634f;
+    BT_CHECK_ARG(std::isfinite(p.scale_log2), "kv4_attention: scale is not finite");
     if (a->tokens == 0 || a->n == 0) return BT_OK;
     BT_CHECK_ARG(a->q.data && a->out.data && a->kv_len, "kv4_attention: null q, out or kv_len");
     BT_CHECK_ARG(((uintptr_t)a->q.data | (uintptr_t)a->out.data) % act_bytes(a->dtype) == 0, "kv4_attention: a tensor is not aligned to its elements");
@@ -810,7 +816,7 @@ extern "C" int bt_cuda_kv4_attention(const bt_kv4* cache, const bt_kv4_attn_args
     p.q = a->q.data; p.out = a->out.data; p.q_ts = a->q.token_stride; p.q_hs = a->q.head_stride;
     p.o_ts = a->out.token_stride; p.o_hs = a->out.head_stride; p.kv_len = a->kv_len; p.q_start = a->q_start; p.slots = a->slots;
     p.n = a->n; p.tokens = a->tokens; p.heads = a->heads; p.group = a->heads / cache->kv_heads;
-    p.window = a->window; p.sinks = a->window ? a->sinks : 0; p.scale_log2 = a->scale * 1.4426950408889634f;
+    p.window = a->window; p.sinks = a->window ? a->sinks : 0;
     p.wide = heads_wide(a->q, a->dtype) && heads_wide(a->out, a->dtype);
     p.tickets = (uint32_t*)workspace;
     p.partial = (float*)((uint8_t*)workspace + BT_KV4_WORKSPACE_ZERO);

@@ -59,7 +59,8 @@ uint64_t prefill_workspace(int sms);  // bytes of its partial results
 cudaError_t launch_kv4_prefill(const AttnParams& p, int dtype, uint32_t head_dim, int sms, cudaStream_t s);
 
 constexpr float kLazyMax = 8.0f;     // a row's reference maximum may be exceeded by 2^8 before it moves
-constexpr float kNothing = -1e30f;   // a row's maximum before it sees a key (finite: differences stay defined)
+constexpr float kLargest = 3.402823466e38f;
+constexpr float kNothing = -kLargest;  // a row's maximum before it sees a key (finite: differences stay defined)
 
 // ---------------------------------------------------------------- mma helpers
 

@@ -47,6 +47,10 @@ constexpr int kPfThreads = 5 * 128;
 constexpr int kPfSoftmax = 128, kPfUnpack = 80, kPfRest = 56;
 static_assert(2 * kPfSoftmax + 2 * kPfUnpack + kPfRest <= 5 * 96, "no more than the block is launched with");
 constexpr float kPfAbove = 7.0f;   // a row's maximum is above its reference m by this, and by kLazyMax more at most
+// A row whose reference would pass this goes on with a smaller factor f of its scores: in
+// f S - m the product is not rounded and m is, and from 2^27 on that alone can leave fp16's
+// range.  Operands of 11 bits tell no scores apart there that this brings together.
+constexpr float kPfFar = 4194304.0f;
 constexpr uint32_t kPfRaw = 3;     // packed K (and V) tiles in flight
 constexpr uint32_t kPfStages = 4;  // unpacked K (and V) tiles
 
@@ -70,6 +74,7 @@ struct PfShared {
     uint32_t pieces[16];  // of a tile: which of its 16-key pieces hold keys
     uint32_t tmem;
     volatile uint32_t dead;  // a wait gave up: everybody leaves
+    float factor[256];       // f of the rows at their start
     uint32_t last;           // this CTA's part of a block is the last to be done
     SeqWork seq[kPfSeqs];    // the first sequences, so that finding a block waits for no memory
 };
@@ -354,6 +359,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
                 const bool flat = p.scale_log2 == 0.0f;  // all scores equal: f stays positive
                 const float mul = there && !flat ? sign * __int_as_float((127 + up) << 23) : 0.0f;
                 f = flat ? 1.0f : fabsf(p.scale_log2) * __int_as_float((127 - up) << 23);
+                sh.factor[r * 128 + row] = f;
 #pragma unroll 1
                 for (int first = 0; first < CH; first += N) {
                     if (first > 0) load_chunks(first);
@@ -406,6 +412,11 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
                     const float now = fmaxf(m, top - kPfAbove), fix = exp2_fast(m - now);
                     m = now;
                     l *= fix;
+                    if (fabsf(now) > kPfFar && now != kNothing) {
+                        const float less = kPfFar / fabsf(now);
+                        m *= less;
+                        f *= less;
+                    }
                     if (i > 0) {  // once the products of the tiles so far are complete
                         if (!(ok = warp_wait(&sh.pv_done[r], (done - 1) & 1))) break;
                         tcgen05_fence_after();
@@ -458,6 +469,8 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
             auto part_ml = [&](uint32_t k) { return reinterpret_cast<float2*>(part_o(k) + HD / 4 * 256); };
             float scale = l == 0.0f ? 0.0f : 1.0f / l;
             if (parts > 1) {
+                // (in the row's own scale; a row of a part without tiles has no f)
+                if (it.tiles && f != sh.factor[at]) m *= sh.factor[at] / f;
                 __stcg(part_ml(unit % walk.parts) + at, make_float2(m, l));
                 if (it.tiles) {
 #pragma unroll 1

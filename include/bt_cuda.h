@@ -564,7 +564,7 @@ typedef struct bt_kv4_attn_args {
     uint32_t       window;    /* 0: none; else a query at position p sees positions > p - window ... */
     uint32_t       sinks;     /* ... and positions < sinks (with a window only) */
     int32_t        dtype;     /* BT_F32, BT_F16 or BT_BF16: q and out */
-    float          scale;     /* of the scores, e.g. 1 / sqrt(head_dim) */
+    float          scale;     /* of the scores, e.g. 1 / sqrt(head_dim); finite */
 } bt_kv4_attn_args;
 
 /* Causal attention over a 4-bit cache.  Sequence i's queries are its last

@@ -305,3 +305,30 @@ def test_sample_nan_parameters(cuda, vocab):
         assert same(cuda.sample_batch(x, u, None, k, nan, None), cuda.sample_batch(x, u, None, k))
         assert same(cuda.sample_batch(x, u, None, k, None, nan), cuda.sample_batch(x, u, None, k))
         assert same(cuda.sample_batch(x, nan, None, k), cuda.sample_batch(x, f(0.0), None, k))
+
+
+@pytest.mark.parametrize("dt,hd", [("float32", 64), ("bfloat16", 64), ("bfloat16", 128), ("bfloat16", 256), ("float32", 256)])
+@pytest.mark.parametrize("lens,counts", [([1], [1]), ([300, 2, 1], [1, 1, 1]), ([40], [40]), ([700], [120])])
+@pytest.mark.parametrize("size", [1e25, 1e31, 1e35, 1e36])
+def test_attention_huge_queries(cuda, dt, hd, lens, counts, size):
+    """Queries so large that one key takes all: scores of either sign up to what fp32 holds.  Rows whose best two
+    scores lie within 2 % of the largest are not judged (the order of such may turn with fp16 operands)."""
+    torch = T()
+    c = Case(cuda, 640, dt, hd, 2, 4, lens, counts)
+    c.q.copy_((c.q.float() * (size / 10)).to(c.q.dtype))
+    got, (want, _) = c.run().double(), c.want()
+    row = judged = 0
+    for i, (length, count) in enumerate(zip(lens, counts)):
+        q_at = torch.arange(length - count, length, device="cuda")
+        for h in range(8):
+            k, v = c.k[i][:, h // 4], c.v[i][:, h // 4]
+            s = (c.q[row:row + count, h].double() @ k.T).masked_fill(torch.arange(length, device="cuda") > q_at[:, None], -np.inf)
+            best = s.topk(min(2, length), -1).values
+            second = best[:, 1] if length > 1 else torch.full_like(best[:, 0], -np.inf)
+            clear = best[:, 0] - second > 0.02 * s.masked_fill(s == -np.inf, 0).abs().amax(-1)
+            tol = (2.0 ** -18 if dt == "float32" else 2.0 ** -11) * v.abs().max() + HALF_ULP[dt] * want[row:row + count, h].abs()
+            err = (got[row:row + count, h] - want[row:row + count, h]).abs()
+            assert bool((err <= tol)[clear].all())
+            judged += int(clear.sum())
+        row += count
+    assert judged >= 4 * sum(counts) and bool(got.isfinite().all())

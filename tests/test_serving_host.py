@@ -194,3 +194,11 @@ def test_timeout_drops_the_scratch():
     finally:
         for k in keys:
             serving._workspaces.pop(k, None)
+
+
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), -float("inf"), 3e38])
+def test_attention_scale_refusals(nat, scale):
+    """(3e38 passes fp32's range on its way to powers of two)"""
+    a = nat.KV4AttnArgs(q=4096, q_token_stride=512, q_head_stride=128, out=4096, out_token_stride=512, out_head_stride=128,
+                        kv_len=4096, n=2, tokens=2, heads=4, scale=scale)
+    refused(nat, "bt_cuda_kv4_attention", C.byref(kv4(nat)), C.byref(a), 4096, 1 << 40, None, match="finite")
