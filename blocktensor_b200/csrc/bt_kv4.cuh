@@ -134,6 +134,9 @@ struct Kv4Map {
     }
 };
 
+// SMs of the current device (asked once); 0: none.
+int device_sms();
+
 // Checks a cache descriptor; BT_OK or an error with its message set.
 int kv4_map(const bt_kv4* c, const char* who, Kv4Map* out);
 

@@ -730,16 +730,6 @@ __global__ void __launch_bounds__(AttnCfg<HD, TERMS>::NW * 32, 1) kv4_attn_kerne
     }
 }
 
-static int device_sms() {
-    static std::atomic<int> known[64];
-    int dev = 0, sms = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess) return 0;
-    if (dev < 64 && (sms = known[dev].load(std::memory_order_relaxed)) > 0) return sms;
-    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
-    if (dev < 64) known[dev].store(sms, std::memory_order_relaxed);
-    return sms;
-}
-
 template <typename T, int HD, int TERMS>
 static cudaError_t attn_launch(const AttnParams& p, bool may_be_few, int sms, cudaStream_t s) {
     using C = AttnCfg<HD, TERMS>;

@@ -310,6 +310,16 @@ __global__ void __launch_bounds__(kQkvThreads) kv4_read_kernel(Kv4Map map, const
     }
 }
 
+int device_sms() {
+    static std::atomic<int> known[64];
+    int dev = 0, sms = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+    if (dev < 64 && (sms = known[dev].load(std::memory_order_relaxed)) > 0) return sms;
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+    if (dev < 64) known[dev].store(sms, std::memory_order_relaxed);
+    return sms;
+}
+
 int kv4_map(const bt_kv4* c, const char* who, Kv4Map* m) {
     const std::string w(who);
     BT_CHECK_ARG(c, w + ": null cache");
@@ -380,7 +390,10 @@ static int qkv_launch(const bt_qk_args* a, const bt_kv4* cache, const char* who,
     const uint32_t sets = (p.q ? (p.heads + per - 1) / per : 0) + (p.k ? (append ? 2 : 1) * ((p.kv_heads + per - 1) / per) : 0);
     // about four CTAs per SM before a CTA takes more than one set of rows (append, 64 + 8 + 8
     // heads: 1 token 3.2 us, in one CTA 6.1; 592 tokens 8.2 us, a CTA a set 12.3)
-    uint32_t gy = a->tokens >= 592 ? 1 : (592 + a->tokens - 1) / a->tokens;
+    const int sms = device_sms();
+    if (sms <= 0) return fail(BT_ERR_CUDA, w + ": no device");
+    const uint32_t ctas = 4 * (uint32_t)sms;
+    uint32_t gy = a->tokens >= ctas ? 1 : (ctas + a->tokens - 1) / a->tokens;
     if (gy > sets) gy = sets;
     const dim3 grid(a->tokens, gy);
     const cudaStream_t s = as_stream(stream);

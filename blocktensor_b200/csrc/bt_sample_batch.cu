@@ -876,7 +876,9 @@ static cudaError_t sample_pick(const SampleParams& p, uint32_t rows, cudaStream_
     while (p.vocab > kSbHeld && c < kSbMaxCluster && p.vocab > c * kSbShare) c *= 2;
     // few rows: smaller shares, as long as the CTAs fit the SMs side by side (1 row of 32000:
     // 11.2 us, 16.1 without; 16 rows 13.4 and 16.0)
-    while (c < kSbMaxCluster && (uint64_t)rows * c * 2 <= 148 && p.vocab > c * 4096) c *= 2;
+    const int sms = device_sms();
+    if (sms <= 0) return cudaErrorNoDevice;
+    while (c < kSbMaxCluster && (uint64_t)rows * c * 2 <= (uint64_t)sms && p.vocab > c * 4096) c *= 2;
     if (p.vocab <= c * kSbHeld) return sample_launch<T, true>(p, rows, c, s);
     return sample_launch<T, false>(p, rows, c, s);
 }
