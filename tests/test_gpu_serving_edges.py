@@ -5,7 +5,7 @@ import time
 import numpy as np
 import pytest
 
-from test_gpu_serving import DT, HALF_ULP, T, Case, check_rows, gen, ints, randn
+from test_gpu_serving import DT, HALF_ULP, T, Case, check_rows, gen, ints, randn, ref_values
 
 pytestmark = pytest.mark.gpu
 
@@ -332,3 +332,190 @@ def test_attention_huge_queries(cuda, dt, hd, lens, counts, size):
             judged += int(clear.sum())
         row += count
     assert judged >= 4 * sum(counts) and bool(got.isfinite().all())
+
+
+# ---------------------------------------------------------------- attention, every key counted
+
+ROUND = {"float16": 2.0 ** -12, "bfloat16": 2.0 ** -9}  # rms of the result's own rounding, relative
+
+
+def deviations(c, got):
+    """The errors of 16-bit attention in standard deviations of what its roundings add up to: keys, values and
+    probabilities held to 2^-12 rms each (a key moves a score by 2^-12 sqrt(sum (q k)^2), and that score's share
+    of the result by p (v - o)), independent of one another, and the result's rounding.  A key left out or
+    counted twice among n alike moves a row by |v - o| / n, some 2^11 / sqrt(n) of these."""
+    torch = T()
+    out, row = [], 0
+    for i, (length, count) in enumerate(zip(c.lens, c.counts)):
+        if length == 0 or count == 0:
+            assert bool((got[row:row + count] == 0).all())
+            row += count
+            continue
+        at, q_at = torch.arange(length, device="cuda"), torch.arange(length - count, length, device="cuda")[:, None]
+        seen = at <= q_at
+        if c.window:
+            seen &= (at > q_at - c.window) | (at < c.sinks)
+        for h in range(c.kv * c.group):
+            k, v = c.k[i][:, h // c.group], c.v[i][:, h // c.group]
+            q = c.q[row:row + count, h].double() * c.scale
+            p = torch.nan_to_num(torch.softmax((q @ k.T).masked_fill(~seen, -np.inf), -1))
+            o = p @ v
+            p2 = p.pow(2)
+            w = p2 * (q.pow(2) @ k.pow(2).T)
+            var = 2 * p2 @ v.pow(2) + w @ v.pow(2) - 2 * o * (w @ v) + o.pow(2) * w.sum(-1, keepdim=True)
+            dev = (2.0 ** -24 * var + (ROUND[c.dt] * o).pow(2) + 2.0 ** -46 * v.abs().max() ** 2).sqrt()
+            out.append((got[row:row + count, h].double() - o) / dev)
+        row += count
+    return torch.cat([x.flatten() for x in out])
+
+
+def check_rms(c, **kw):
+    """Within 1.25 of these deviations (upper bounds) in the root mean square over thousands of elements."""
+    d = float(deviations(c, c.run(**kw)).pow(2).mean().sqrt())
+    assert d <= 1.25, d
+
+
+CALLS = [
+    # lens, counts, kv, group, page, window, sinks
+    ([700, 33, 129, 64, 255], [1] * 5, 2, 4, 64, 0, 0),
+    ([4097], [1], 2, 8, 16, 0, 0),
+    ([900, 3, 400, 40, 0], [1] * 5, 2, 8, 16, 100, 4),
+    ([1023, 1025, 65, 63, 1], [1] * 5, 4, 1, 16, 0, 0),
+    ([700], [100], 1, 8, 0, 0, 0),
+    ([129, 700, 128, 31], [128, 200, 127, 31], 2, 3, 32, 0, 0),
+    ([2049], [130], 2, 4, 16, 0, 0),
+    ([1100], [600], 4, 8, 256, 400, 1),
+    ([260, 20, 400], [260, 20, 5], 2, 8, 16, 33, 70),
+]
+
+
+@pytest.mark.parametrize("dt", ["float16", "bfloat16"])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("i", range(len(CALLS)))
+def test_attention_rms(cuda, dt, hd, i):
+    lens, counts, kv, group, page, window, sinks = CALLS[i]
+    check_rms(Case(cuda, 700 + i, dt, hd, kv, group, lens, counts, page, window, sinks, shuffle=i % 2 == 0))
+
+
+def count_keys(cuda, seed, dt, hd, kv, group, lens, counts, page=0, window=0, sinks=0, flagged=None):
+    """Queries of zeros give every key that a row sees the same weight, and key j's value is 1 in element j % hd
+    and 0 elsewhere (zeros too unless j is in `flagged`): times their number, a row of the result counts the keys.
+    Probabilities, their sums and the products are powers of two and small whole numbers, so that what is left is
+    the result's rounding and an fp32 reciprocal's.  What no row sees is NaN, pages of it are not in the table."""
+    torch = T()
+    g, n, max_seq = gen(seed), len(lens), max(lens) + 3
+    cache = cuda.KV4Cache(n, max_seq, kv, hd, page_tokens=page, n_pages=n * -(-max_seq // page) if page else 0)
+    if page:
+        cache.page_table[:] = torch.randperm(cache.n_pages, generator=g, device="cuda").int().view(n, -1)
+    k = torch.randint(0, 256, (kv, hd // 2 + hd // 16), generator=g, device="cuda", dtype=torch.uint8)
+    k[:, hd // 2:] = torch.tensor([0.3, -2.0], device="cuda").half().view(torch.uint8).repeat(hd // 64)
+    cache.k_rows.fill_(0xFF)
+    cache.v_rows.fill_(0xFF)
+    one = torch.tensor([1.0, 0.0], device="cuda").half().view(torch.uint8).repeat(hd // 64)
+    want = []
+    for i, (length, count) in enumerate(zip(lens, counts)):
+        at, q_at = torch.arange(length, device="cuda"), torch.arange(length - count, length, device="cuda")[:, None]
+        seen = at <= q_at
+        if window:
+            seen &= (at > q_at - window) | (at < sinks)
+        live = at[seen.any(0)]
+        rows = torch.zeros(length, hd // 2 + hd // 16, dtype=torch.uint8, device="cuda")
+        flag = torch.ones_like(at, dtype=torch.bool) if flagged is None else (at >= flagged[0]) & (at < flagged[1])
+        rows[at, at % hd // 2] = torch.where(flag, 1 << 4 * (at % 2), 0).to(torch.uint8)
+        rows[:, hd // 2:] = one
+        p = cache.page_table[i, live // page].long() if page else torch.full_like(live, i)
+        cache.v_rows[p, :, live % cache.page_tokens] = rows[live][:, None]
+        cache.k_rows[p, :, live % cache.page_tokens] = k
+        if page:
+            gone = torch.ones(cache.max_pages, dtype=torch.bool, device="cuda")
+            gone[live // page] = False
+            cache.page_table[i][gone] = -1
+        onehot = torch.zeros(length, hd, dtype=torch.float64, device="cuda")
+        onehot[at, at % hd] = flag.double()
+        want.append(seen.double() @ onehot / seen.sum(1, keepdim=True).clamp(min=1))
+    q = torch.zeros(sum(counts), kv * group, hd, dtype=getattr(torch, dt), device="cuda")
+    starts = None if all(c == 1 for c in counts) else ints(np.concatenate([[0], np.cumsum(counts)]).tolist())
+    out = cache.attention(q, ints(lens), q_start=starts, max_q=max(counts), window=window, sinks=sinks)
+    cache.check()
+    want = torch.cat(want)[:, None]
+    assert bool(((out.double() - want).abs() <= (HALF_ULP[dt] + 2.0 ** -22) * want).all())
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("i", range(len(CALLS)))
+def test_attention_counts_every_key(cuda, dt, hd, i):
+    lens, counts, kv, group, page, window, sinks = CALLS[i]
+    count_keys(cuda, 750 + i, dt, hd, kv, group, lens, counts, page, window, sinks)
+
+
+@pytest.mark.parametrize("dt,hd,group,count", [("float16", 64, 8, 1), ("float32", 128, 4, 1), ("float16", 128, 8, 20),
+                                               ("bfloat16", 64, 8, 130)])
+def test_attention_counts_every_key_of_many(cuda, dt, hd, group, count):
+    """100003 keys, 32 an element at a time."""
+    for lo in range(0, 100003, 32 * hd):
+        count_keys(cuda, 770, dt, hd, 1, group, [100003], [count], flagged=(lo, lo + 32 * hd))
+
+
+@pytest.mark.parametrize("dt,hd", [("float16", 64), ("bfloat16", 128)])
+@pytest.mark.parametrize("n", [33, 64, 65, 150])
+def test_attention_many_prompts(cuda, dt, hd, n):
+    """More sequences with many rows than a warp has lanes and than the kernel keeps at hand, short ones and
+    empty ones among them."""
+    lens = [[90, 1, 40, 0, 130, 7][i % 6] + i % 5 for i in range(n)]
+    counts = [[40, 1, 33, 0, 130, 7][i % 6] for i in range(n)]
+    check_rms(Case(cuda, 720 + n, dt, hd, 2, 4, lens, counts, 16, shuffle=True))
+    count_keys(cuda, 720 + n, dt, hd, 2, 4, lens, counts, 16)
+
+
+@pytest.mark.parametrize("dt,hd", [("float32", 64), ("float16", 128), ("bfloat16", 256)])
+@pytest.mark.parametrize("n", [257, 513, 1100])
+def test_attention_many_sequences(cuda, dt, hd, n):
+    """More sequences than a CTA of the few-row kernel has threads."""
+    lens = [[1, 17, 40, 0, 33][i % 5] for i in range(n - 1)] + [300]
+    Case(cuda, 730 + n, dt, hd, 2, 4, lens, [1] * n, 16).check()
+    count_keys(cuda, 730 + n, dt, hd, 2, 4, lens, [1] * n, 16)
+
+
+def test_attention_chunk_past_4gb(cuda):
+    """The many-row kernel on rows beyond the first 4 GB of the pool."""
+    torch = T()
+    if torch.cuda.mem_get_info()[0] < 16 << 30:
+        pytest.skip("needs 16 GB")
+    g, kv, group, hd, max_seq = gen(62), 4, 4, 128, 2_200_000  # 72 B * 4 * 2.2 M = 0.63 GB a slot, 8 slots a side
+    cache = cuda.KV4Cache(8, max_seq, kv, hd)
+    length, window, count = 2_100_000, 300, 100
+    first = length - count + 1 - window
+    pos = torch.arange(first, length, device="cuda").int()
+    for lo in range(0, len(pos), 128):
+        p = pos[lo:lo + 128]
+        cache.append(randn(g, len(p), kv, hd), randn(g, len(p), kv, hd), torch.full_like(p, 7), p)
+    q = randn(g, count, kv * group, hd).half()
+    out = cache.attention(q, ints([length]), q_start=ints([0, count]), slots=ints([7]), max_q=count, window=window)
+    cache.check()
+    # the same rows at the start of a small cache, with the window's edge as it lies
+    small = cuda.KV4Cache(1, len(pos), kv, hd)
+    small.k_rows[0, :, :len(pos)] = cache.k_rows[7, :, first:length]
+    small.v_rows[0, :, :len(pos)] = cache.v_rows[7, :, first:length]
+    kk, vv = (ref_values(r[0, :, :len(pos)], hd) for r in (small.k_rows, small.v_rows))
+    at, q_at = torch.arange(first, length, device="cuda"), torch.arange(length - count, length, device="cuda")[:, None]
+    seen = (at <= q_at) & (at > q_at - window)
+    for h in range(kv * group):
+        k, v = kk[h // group], vv[h // group]
+        p = torch.softmax((q[:, h].double() @ k.T * hd ** -0.5).masked_fill(~seen, -np.inf), -1)
+        # (the tolerance of test_attention_past_4gb, which these sizes keep to alike)
+        assert float((out[:, h].double() - p @ v).abs().max()) <= (6 * 1.0 + 4) * 2.0 ** -11 * float(v.abs().max())
+
+
+@pytest.mark.parametrize("dt,hd", [("float16", 64), ("bfloat16", 128)])
+def test_attention_rows_of_no_sequence(cuda, dt, hd):
+    """Rows of q before the first sequence's, between none and after the last one's are not written."""
+    torch = T()
+    c = Case(cuda, 740, dt, hd, 2, 4, [50, 300], [1, 60])
+    want = c.run(out=torch.full_like(c.q, 5))
+    pad = torch.zeros(7, *c.q.shape[1:], dtype=c.q.dtype, device="cuda")
+    q = torch.cat([pad[:3], c.q, pad])
+    out = torch.full_like(q, 5)
+    c.cache.attention(q, ints(c.lens), q_start=c.starts + 3, max_q=60, out=out)
+    c.cache.check()
+    assert torch.equal(out[3:-7], want) and bool((out[:3] == 5).all()) and bool((out[-7:] == 5).all())
