@@ -9,8 +9,9 @@
 // bits masked into the low mantissa bits of a half are the subnormal c 2^-24 (or
 // c 2^-20 from the next nibble up), one logical operation for two codes and no
 // conversion.  s and m stay in fp32.  The queries (scaled by a power of two per
-// column so that both terms stay normal) are exact for fp16 and bf16 inputs and two
-// fp16 terms (22 bits) for fp32; p s_j likewise is one or two terms.  The 8 is there
+// column, its largest element to 2^13) are exact for fp16 and bf16 inputs down to 2^-23
+// of that element, and off by 2^-34 of it at most below, where fp16's steps end; for
+// fp32 they are two fp16 terms (22 bits); p s_j likewise is one or two terms.  The 8 is there
 // because the sums of c and of m are many times their difference, which makes p's
 // rounding and the tensor cores' truncated accumulation come out as much larger.  For
 // 16-bit types the MMAs still add c, and 8 times what p s was rounded to is taken off in

@@ -6,7 +6,8 @@
 //   S = Q K^T,  P = exp2(f S - m),  O += P V,  l += sum P,  out = O / l.
 // A tile's keys and values are unpacked once into fp16 operands in shared memory
 // (scale * code + min, one rounding of 2^-12 rms) and serve both 128-row halves.
-// Queries enter scaled by a power of two per row, exact for bf16 and fp16; P is
+// Queries enter scaled by a power of two per row, exact for bf16 and fp16 (below 2^-27 of
+// the row's largest element off by 2^-38 of it at most); P is
 // rounded to fp16 (2^-12 rms); sums, maxima and O are fp32.  m is held 7 below the
 // running maximum, so that P reaches 2^15 and a key counts down to 2^-32 of the largest
 // (fp16 ends at 2^-25: 131071 keys of 2^-25.5 beside one of 1 would lose their 0.3 %).

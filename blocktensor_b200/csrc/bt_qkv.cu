@@ -51,11 +51,11 @@ __device__ __forceinline__ float row_sum(float v) {
 }
 
 // Mean of the squares of a row, 8 consecutive elements a lane, each square and sum rounded,
-// added in the order of PyTorch's row mean (by measurement): 32 partial sums, of 4
-// consecutive elements (head_dim 128), of 4 and the 4 that lie 128 further (256), or of
-// elements 32 apart (64), then halves on halves.  A key that goes to the cache is normed
-// so, because a code at the edge between two steps falls to one or the other with the
-// last bit of the norm: this way the cached codes are those of a plain fp32 computation.
+// added in the order that bt_cuda.h defines (where PyTorch 2.11's row mean has it too): 32
+// partial sums, of 4 consecutive elements (head_dim 128), of 4 and the 4 that lie 128
+// further (256), or of elements 32 apart (64), then halves on halves.  A code at the edge
+// between two steps falls to one or the other with the last bit of the norm: with every
+// rounding defined, a plain fp32 computation gives the cached codes bit for bit.
 template <int HD>
 __device__ __forceinline__ float plain_mean_square(const float (&x)[8]) {
     float v[8];

@@ -336,7 +336,8 @@ class KV4Cache:
         kv_len [n] int32: cached positions of each sequence; its queries are the last ones.  q_start
         [n + 1] int32: sequence i's queries are rows q_start[i] .. q_start[i + 1] - 1 of q; None: one each.
         slots [n] int32: the sequences' slots; None: sequence i is slot i.  max_q: no sequence has more
-        queries (0: not known)."""
+        queries (0: not known).  Rows of q that belong to no sequence are not written (in a new output they
+        hold anything)."""
         if _elsewhere(stream):
             return _on_stream(stream, self._tensors(), self.attention, q, kv_len, q_start, slots, max_q, window, sinks, scale, out)
         qh = _heads(q, "q")

@@ -461,8 +461,9 @@ BT_API int bt_batch_pages(bt_batch* b, uint32_t* free_pages, uint32_t* total_pag
 /* batched sampling (no counterpart in the reference)                   */
 /* ------------------------------------------------------------------ */
 
-/* Element types of the activations these operators take and give.  All
- * arithmetic is fp32 (or wider); results are rounded once, to the type. */
+/* Element types of the activations these operators take and give.  Results are
+ * rounded once, to the type; sums, norms, maxima and probabilities are fp32 or
+ * wider.  What is held in fewer bits on the way is stated at the operator. */
 #define BT_F32  0
 #define BT_F16  1
 #define BT_BF16 2
@@ -473,7 +474,8 @@ BT_API int bt_batch_pages(bt_batch* b, uint32_t* free_pages, uint32_t* total_pag
  *     A row of bt_kv4_row_bytes(head_dim) = head_dim / 2 + head_dim / 16 bytes
  *     holds head_dim / 2 bytes of codes (element 2i in the low nibble of byte i),
  *     then for every 64 elements a pair (scale, min) of fp16; code c stands for
- *     scale * c + min.
+ *     scale * c + min.  Scales are finite and not negative (append writes no
+ *     others).
  *   page_table: device int32 [n_seq][max_pages], the page of positions
  *     [i page_tokens, (i + 1) page_tokens) of a slot; page_tokens is then a power
  *     of two >= 16.  NULL: slot s owns page s, n_pages = n_seq, and page_tokens
@@ -537,7 +539,18 @@ typedef struct bt_qk_args {
 BT_API int bt_cuda_qk_norm_rope(const bt_qk_args* a, void* stream);
 
 /* The same with the keys and the (unchanged) values of token t stored in 4 bits
- * at position positions[t] of slot slots[t] of the cache, one launch.  Values
+ * at position positions[t] of slot slots[t] of the cache, one launch.  A key is
+ * normed and rotated by separate fp32 operations, each rounded, so that its codes
+ * can be told exactly (qk_norm_rope fuses some and may differ in the last bits: a
+ * key that it returns, quantised, may differ from the cached one by a step):
+ * squares; their sum in the order below; mean = sum * (1 / head_dim); x *
+ * rsqrtf(mean + eps), * weight; a cos - b sin and b cos + a sin of rounded
+ * products.  The order of the sum:
+ *   head_dim 128: partial sum i of 32 adds squares 4i .. 4i + 3 one by one;
+ *   head_dim 256: the same of square[4i + k] + square[4i + k + 128];
+ *   head_dim 64: partial sum i of 32 is square[i] + square[i + 32];
+ * then halves on halves: s[i] + s[i + 16], of these s[i] + s[i + 8], and so on.
+ * Values
  * are held to +-57344 and NaN becomes 0 (four bits hold neither).  Per 64
  * elements: min and scale = (max - min) * (1 / 15) are rounded to fp16, code =
  * clamp(round((x - min) * (1 / scale)), 0, 15).  slots[t] < 0: the token is
@@ -577,7 +590,15 @@ typedef struct bt_kv4_attn_args {
  * zeroed once before its first call (calls leave it ready for the next); calls
  * that may overlap on the GPU need one each, and so do captured graphs whose
  * replays may; after BT_KV4_TIMEOUT they are zeroed again.  Deterministic: the
- * same inputs give the same bits. */
+ * same inputs give the same bits.  Rows of q that belong to no sequence are
+ * neither read nor written.
+ * Precision.  fp32: queries, and probabilities times scales, are held to 2^-23 of
+ * the largest (error about 4e-7 of the values' size).  16-bit types: queries are
+ * exact, or held to 2^-34 of their row's largest element; with up to 32 or 64
+ * (query, head) rows a KV head probabilities times scales are rounded to fp16,
+ * with more rows (head_dim 64 and 128) keys, values and probabilities are, 2^-12
+ * rms each (fp16 results are off by 2.7e-4 and 4.9e-4, of which 2.1e-4 are their
+ * own rounding; bf16 ones by 1.8e-3, of which 1.7e-3). */
 #define BT_KV4_WORKSPACE_ZERO 16384u
 BT_API int bt_cuda_kv4_attention(const bt_kv4* cache, const bt_kv4_attn_args* a, void* workspace,
                                  uint64_t workspace_bytes, void* stream);

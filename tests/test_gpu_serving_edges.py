@@ -5,7 +5,7 @@ import time
 import numpy as np
 import pytest
 
-from test_gpu_serving import DT, HALF_ULP, T, Case, check_rows, gen, ints, randn, ref_values
+from test_gpu_serving import DT, HALF_ULP, T, Case, check_rows, gen, ints, randn, ref_rows, ref_values
 
 pytestmark = pytest.mark.gpu
 
@@ -519,3 +519,43 @@ def test_attention_rows_of_no_sequence(cuda, dt, hd):
     c.cache.attention(q, ints(c.lens), q_start=c.starts + 3, max_q=60, out=out)
     c.cache.check()
     assert torch.equal(out[3:-7], want) and bool((out[:3] == 5).all()) and bool((out[-7:] == 5).all())
+
+
+# ---------------------------------------------------------------- cached keys, as bt_cuda.h defines them
+
+def defined_key(x, w, eps, cos, sin):
+    """The norm and rotation of bt_cuda_kv4_append in numpy fp32, operation by operation (rsqrtf by the device)."""
+    torch = T()
+    s = x * x
+    hd = x.shape[-1]
+    if hd == 256:
+        s = s[..., :128] + s[..., 128:]
+    if hd == 64:
+        s = s[..., :32] + s[..., 32:]
+    else:
+        four = s.reshape(*s.shape[:-1], 32, 4)
+        s = ((four[..., 0] + four[..., 1]) + four[..., 2]) + four[..., 3]
+    while s.shape[-1] > 1:
+        half = s.shape[-1] // 2
+        s = s[..., :half] + s[..., half:]
+    mean = s * np.float32(1 / hd) + np.float32(eps)
+    x = x * torch.rsqrt(torch.from_numpy(mean).cuda()).cpu().numpy() * w
+    h = cos.shape[-1]
+    a, b = x[..., :h], x[..., h:2 * h]
+    return np.concatenate([a * cos - b * sin, b * cos + a * sin, x[..., 2 * h:]], -1)
+
+
+@pytest.mark.parametrize("dt", DT)
+@pytest.mark.parametrize("hd,rot", [(64, 64), (64, 16), (128, 128), (128, 96), (256, 256), (256, 64)])
+def test_append_codes_as_defined(cuda, dt, hd, rot):
+    torch = T()
+    g, tokens, kv = gen(hd + rot), 700, 3
+    k, v = ((randn(g, tokens, kv, hd) * (1 + 2 * torch.rand(hd, generator=g, device="cuda"))).to(getattr(torch, dt)) for _ in range(2))
+    w, table = 1 + 0.3 * randn(g, hd), cuda.rope_table(tokens, rot, 500000.0)
+    pos = torch.arange(tokens, dtype=torch.int32, device="cuda")
+    cache = cuda.KV4Cache(1, tokens, kv, hd)
+    cache.append_normed(torch.zeros_like(k), k, v, None, w, torch.zeros_like(pos), pos, table, 1e-5)
+    cos, sin = (table[:, None, :, i].cpu().numpy() for i in (0, 1))
+    want = defined_key(k.float().cpu().numpy(), w.cpu().numpy(), 1e-5, cos, sin)
+    assert want.dtype == np.float32
+    assert np.array_equal(cache.k_rows[0, :, :tokens].transpose(0, 1).cpu().numpy(), ref_rows(torch.from_numpy(want)))
