@@ -80,6 +80,8 @@ class Decoder4:
     def forward(self, tokens, slots: Sequence[int], counts: Sequence[int]):
         """Logits [sum(counts), vocab] of ``counts[i]`` more tokens of each slot, which enter its caches."""
         s = self.shape
+        if len(set(slots)) != len(slots) or len(counts) != len(slots) or min(counts, default=0) < 1 or len(tokens) != sum(counts):
+            raise ValueError("forward: expected different slots, and one token or more for each")
         for slot, c in zip(slots, counts):
             self.caches[0].reserve(slot, self.lens[slot] + c)
         positions = [self.lens[slot] + j for slot, c in zip(slots, counts) for j in range(c)]

@@ -559,3 +559,21 @@ def test_append_codes_as_defined(cuda, dt, hd, rot):
     want = defined_key(k.float().cpu().numpy(), w.cpu().numpy(), 1e-5, cos, sin)
     assert want.dtype == np.float32
     assert np.array_equal(cache.k_rows[0, :, :tokens].transpose(0, 1).cpu().numpy(), ref_rows(torch.from_numpy(want)))
+
+
+# ---------------------------------------------------------------- the decoder
+
+def test_decoder_refusals(cuda):
+    """A slot named twice, a slot without tokens, tokens that do not add up: refused before anything is kept."""
+    from blocktensor_b200.serve4 import Decoder4, Shape
+    torch = T()
+    m = Decoder4(Shape(vocab=256, dim=128, hidden=256, layers=1, heads=2, kv_heads=1, head_dim=64), 2, 64, page_tokens=16)
+    free, u = m.caches[0].pages(), torch.full((2,), 0.5, device="cuda")
+    for prompts, slots in (([[1, 2], []], [0, 1]), ([[1], [2]], [0, 0]), ([], []), ([[1]], [0, 1])):
+        with pytest.raises(ValueError):
+            m.prefill(prompts, slots, u)
+    with pytest.raises(ValueError):
+        m.forward(torch.ones(3, dtype=torch.int64, device="cuda"), [0, 1], [1, 1])
+    assert m.caches[0].pages() == free and m.lens == [0, 0]
+    assert m.prefill([[1, 2], [3]], [0, 1], u).shape == (2,)
+    m.check()
