@@ -238,7 +238,7 @@ class KV4Cache:
         """Pages for positions 0 .. positions - 1 of a slot; MemoryError (and none taken) when too few are free."""
         if self._free is None:
             raise ValueError("reserve: this cache does not hand out its pages")
-        if not 0 <= slot < self.n_seq or positions > self.max_seq:
+        if not 0 <= slot < self.n_seq or not 0 <= positions <= self.max_seq:
             raise IndexError("reserve: slot or positions out of range")
         held = self._held[slot]
         more = -(-positions // self.page_tokens) - len(held)
@@ -254,6 +254,8 @@ class KV4Cache:
         """A slot's pages back to the pool.  Work that reads them has to be on the same stream, or done."""
         if self._free is None:
             raise ValueError("release: this cache does not hand out its pages")
+        if not 0 <= slot < self.n_seq:
+            raise IndexError("release: slot out of range")
         self._free += reversed(self._held[slot])
         self._held[slot] = []
         self.page_table[slot] = -1

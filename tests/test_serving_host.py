@@ -202,3 +202,18 @@ def test_attention_scale_refusals(nat, scale):
     a = nat.KV4AttnArgs(q=4096, q_token_stride=512, q_head_stride=128, out=4096, out_token_stride=512, out_head_stride=128,
                         kv_len=4096, n=2, tokens=2, heads=4, scale=scale)
     refused(nat, "bt_cuda_kv4_attention", C.byref(kv4(nat)), C.byref(a), 4096, 1 << 40, None, match="finite")
+
+
+def test_page_slots_out_of_range():
+    """A slot that is not the cache's is refused, a negative one too (it names none, not the last)."""
+    import blocktensor_b200 as bt
+    c = bt.KV4Cache(3, 100, 2, 64, page_tokens=16, n_pages=8, device="cpu")
+    c.reserve(2, 33)
+    for slot in (-1, 3):
+        with pytest.raises(IndexError):
+            c.release(slot)
+        with pytest.raises(IndexError):
+            c.reserve(slot, 1)
+    with pytest.raises(IndexError):
+        c.reserve(1, -1)
+    assert c.pages() == (5, 8) and int((c.page_table[2] >= 0).sum()) == 3
