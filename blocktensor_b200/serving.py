@@ -347,13 +347,16 @@ class KV4Cache:
         tokens, heads, hd = shape
         if hd != self.head_dim or q.get_device() != dev:
             raise ValueError("attention: q must have the cache's head_dim and device")
-        if window < 0 or sinks < 0 or max_q < 0:
-            raise ValueError("attention: window, sinks and max_q must not be negative")
+        if min(window, sinks, max_q) < 0 or max(window, sinks, max_q) > 0xffffffff:
+            raise ValueError("attention: window, sinks and max_q must be in 0 .. 2^32 - 1")
+        scale = hd ** -0.5 if scale is None else scale
+        if not abs(scale) < 2e38:
+            raise ValueError("attention: scale is not finite")
         out, oh = _out(out, "out", shape, q, dev)
         a = _pack_attn.pack(*qh, *oh, _vector(kv_len, "kv_len", n, torch.int32, dev),
                             0 if q_start is None else _vector(q_start, "q_start", n + 1, torch.int32, dev),
                             0 if slots is None else _vector(slots, "slots", n, torch.int32, dev),
-                            n, tokens, heads, max_q, window, sinks, _dtype(q), hd ** -0.5 if scale is None else scale)
+                            n, tokens, heads, max_q, window, sinks, _dtype(q), scale)
         _launch(native.load().bt_cuda_kv4_attention, "bt_cuda_kv4_attention", dev, self._ref, a, *_workspace(dev))
         return out
 

@@ -577,3 +577,30 @@ def test_decoder_refusals(cuda):
     assert m.caches[0].pages() == free and m.lens == [0, 0]
     assert m.prefill([[1, 2], [3]], [0, 1], u).shape == (2,)
     m.check()
+
+
+def test_attention_integer_refusals(cuda):
+    """Numbers past 32 bits are refused as other arguments are."""
+    torch = T()
+    c, q = cuda.KV4Cache(1, 16, 1, 64), torch.zeros(1, 1, 64, device="cuda")
+    for kw in (dict(window=1 << 32), dict(window=9, sinks=1 << 32), dict(max_q=1 << 32), dict(sinks=-1), dict(scale=float("nan")),
+               dict(scale=1e39)):
+        with pytest.raises(ValueError):
+            c.attention(q, ints([1]), **kw)
+
+
+@pytest.mark.parametrize("dt,hd", [("float32", 64), ("float16", 128), ("bfloat16", 64), ("bfloat16", 256)])
+@pytest.mark.parametrize("counts", [[1, 1], [90, 40]])
+def test_attention_nan_and_infinite_queries(cuda, dt, hd, counts):
+    """A NaN or infinite element makes its own (query, head) row NaN and no other one."""
+    torch = T()
+    c = Case(cuda, 760, dt, hd, 2, 4, [500, 77], counts, 16)
+    want = c.check()
+    bad = [(0, 0, float("nan")), (sum(counts) // 2, 3, float("inf")), (sum(counts) - 1, 7, -float("inf"))]
+    for row, head, v in bad:
+        c.q[row, head, 5] = v
+    got = c.run()
+    for row, head, _ in bad:
+        assert bool(got[row, head].isnan().all())
+        got[row, head] = want[row, head]
+    assert torch.equal(got, want)
