@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(AttnCfg<HD, TERMS>::NW * 32, 1) kv4_attn_kerne
     float* slots = reinterpret_cast<float*>(dyn + NW * (S * C::STAGE));
 
     // ---- how much work there is
-    if (lane < S) mbar_init(&sh.bar[warp][lane], 1 + p.stalled);
+    if (lane < S) mbar_init(&sh.bar[warp][lane], p.arrivals);
     fence_mbar_init();
     uint64_t total = 0;
     uint32_t items = 0, longest = 0;
@@ -559,7 +559,7 @@ __global__ void __launch_bounds__(AttnCfg<HD, TERMS>::NW * 32, 1) kv4_attn_kerne
             const int32_t key0 = w.key0(tile0 + x);
             if (!seen.any(key0, kUnit, p.sinks)) continue;
             if (!dead) {
-                const bool in_time = mbar_wait(&sh.bar[warp][got], got_phase, nullptr, p.wait_ns);
+                const bool in_time = mbar_wait(&sh.bar[warp][got], got_phase, nullptr, p.wait_ns());
                 if (!__all_sync(0xffffffffu, in_time)) {
                     dead = true;
                     if (lane == 0) p.map.flag(BT_KV4_TIMEOUT);
@@ -575,7 +575,7 @@ __global__ void __launch_bounds__(AttnCfg<HD, TERMS>::NW * 32, 1) kv4_attn_kerne
                 __syncwarp();  // every lane is done with the stage
                 got_phase ^= got + 1 == S ? 1u : 0u;
                 got = got + 1 == S ? 0 : got + 1;
-                if (lane == 0) --ahead;
+                --ahead;  // (of no meaning in the other lanes)
                 issue();
                 __syncwarp();
             }
@@ -724,7 +724,7 @@ __global__ void __launch_bounds__(AttnCfg<HD, TERMS>::NW * 32, 1) kv4_attn_kerne
     }
     // after an expired wait copies may still be on their way to this CTA's shared memory
     for (; dead && lane == 0 && ahead > 0; --ahead) {
-        mbar_wait(&sh.bar[warp][got], got_phase, nullptr, p.wait_ns);
+        mbar_wait(&sh.bar[warp][got], got_phase, nullptr, p.wait_ns());
         got_phase ^= got + 1 == S ? 1u : 0u;
         got = got + 1 == S ? 0 : got + 1;
     }
@@ -768,11 +768,11 @@ extern "C" uint64_t bt_cuda_capture_id(void* stream) {
     return status == cudaStreamCaptureStatusNone ? 0 : id;
 }
 
-static std::atomic<uint32_t> g_stall_ms{0};
+static std::atomic<uint8_t> g_stall_ms{0};
 
 extern "C" int bt_cuda_kv4_inject_stall(uint32_t wait_ms) {
-    BT_CHECK_ARG(wait_ms <= 2000, "kv4_inject_stall: at most 2000 ms");
-    g_stall_ms.store(wait_ms, std::memory_order_relaxed);
+    BT_CHECK_ARG(wait_ms <= 255, "kv4_inject_stall: at most 255 ms");
+    g_stall_ms.store((uint8_t)wait_ms, std::memory_order_relaxed);
     return BT_OK;
 }
 
@@ -810,9 +810,8 @@ extern "C" int bt_cuda_kv4_attention(const bt_kv4* cache, const bt_kv4_attn_args
     p.wide = heads_wide(a->q, a->dtype) && heads_wide(a->out, a->dtype);
     p.tickets = (uint32_t*)workspace;
     p.partial = (float*)((uint8_t*)workspace + BT_KV4_WORKSPACE_ZERO);
-    const uint32_t stall_ms = g_stall_ms.load(std::memory_order_relaxed);
-    p.stalled = stall_ms ? 1 : 0;
-    p.wait_ns = stall_ms ? stall_ms * 1000000u : kWaitNs;
+    p.stall_ms = g_stall_ms.load(std::memory_order_relaxed);
+    p.arrivals = p.stall_ms ? 2 : 1;
     const cudaStream_t s = as_stream(stream);
     // Sequences with many rows go to the tcgen05 kernel, which unpacks a tile once for 256 rows
     // instead of once for 8 but takes a whole tile's time for any number of them.  Measured, us,

@@ -45,12 +45,13 @@ struct AttnParams {
     uint32_t window, sinks;
     float scale_log2;                  // scale * log2(e)
     uint32_t few_rows;                 // sequences with more (query, head) rows a KV head go to the prefill kernel
-    uint32_t wait_ns;                  // limit of a wait for copies
-    uint32_t stalled;                  // 1: such waits cannot end (bt_cuda_kv4_inject_stall)
     bool wide;
+    uint8_t arrivals;                  // of a copy's barrier: 1, or 2 where waits are not to end (bt_cuda_kv4_inject_stall)
+    uint8_t stall_ms;                  // not 0: their limit then
     Kv4Map map;
     float* partial;                    // workspace: partial results and their tickets
     uint32_t* tickets;
+    __device__ __forceinline__ uint32_t wait_ns() const { return stall_ms ? stall_ms * 1000000u : kWaitNs; }
 };
 
 // The many-row kernel (bt_kv4_prefill.cu): whether it takes a type and head_dim, and its

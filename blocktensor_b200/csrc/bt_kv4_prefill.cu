@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
     }
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
-            for (uint32_t k = 0; k < kPfRaw; ++k) { mbar_init(&sh.raw_full[i][k], 1 + p.stalled); mbar_init(&sh.raw_empty[i][k], 4); }
+            for (uint32_t k = 0; k < kPfRaw; ++k) { mbar_init(&sh.raw_full[i][k], p.arrivals); mbar_init(&sh.raw_empty[i][k], 4); }
             for (uint32_t k = 0; k < kPfStages; ++k) { mbar_init(&sh.full[i][k], 4); mbar_init(&sh.empty[i][k], 2); }
             for (int k = 0; k < 2; ++k) { mbar_init(&sh.s_full[i][k], 1); mbar_init(&sh.p_full[i][k], 4); }
             mbar_init(&sh.q_full[i], 4); mbar_init(&sh.pv_done[i], 1); mbar_init(&sh.o_full[i], 1); mbar_init(&sh.drain[i], 1);
@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
         const uint64_t t0 = global_ns();
         while (!sh.dead) {
             if (mbar_try_wait_sleep(bar, parity, 20000u)) return true;
-            if (global_ns() - t0 > p.wait_ns) {
+            if (global_ns() - t0 > p.wait_ns()) {
                 sh.dead = 1;
                 p.map.flag(BT_KV4_TIMEOUT);
             }
@@ -648,8 +648,8 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(const __grid
         }
         // every copy has arrived before the CTA may end (a wait may have given up on one)
         for (uint32_t k = sent > kPfRaw ? sent - kPfRaw : 0; k < sent; ++k) {
-            mbar_wait(&sh.raw_full[0][k % kPfRaw], k / kPfRaw & 1, nullptr, p.wait_ns);
-            mbar_wait(&sh.raw_full[1][k % kPfRaw], k / kPfRaw & 1, nullptr, p.wait_ns);
+            mbar_wait(&sh.raw_full[0][k % kPfRaw], k / kPfRaw & 1, nullptr, p.wait_ns());
+            mbar_wait(&sh.raw_full[1][k % kPfRaw], k / kPfRaw & 1, nullptr, p.wait_ns());
         }
     } else if (warp < 19) {
         // ------------------------------------------------ MMAs of a half

@@ -44,21 +44,13 @@ _captured = {}
 _is_capturing = torch._C._cuda_isCurrentStreamCapturing
 
 
-def _workspace(dev):
-    """(pointer, bytes) of the attention's scratch for a call on a device's current stream."""
-    s = _raw_stream(dev)
-    capture = 0
-    if dev != _current_device() or _is_capturing():
-        capture = native.load().bt_cuda_capture_id(s)
-    cache = _captured if capture else _workspaces
-    ws = cache.get((dev, s))
-    if ws is None or ws[3] != capture:
-        with torch.cuda.device(dev):
-            size = native.load().bt_cuda_kv4_attention_workspace()
-            mem = torch.empty(size, dtype=torch.uint8, device="cuda")
-            mem[:native.BT_KV4_WORKSPACE_ZERO].zero_()
-        ws = cache[dev, s] = (mem.data_ptr(), size, mem, capture)
-    return ws[0], ws[1]
+def _new_workspace(cache, dev, s, capture):
+    with torch.cuda.device(dev):
+        size = native.load().bt_cuda_kv4_attention_workspace()
+        mem = torch.empty(size, dtype=torch.uint8, device="cuda")
+        mem[:native.BT_KV4_WORKSPACE_ZERO].zero_()
+    ws = cache[dev, s] = (mem.data_ptr(), size, mem, capture)
+    return ws
 
 
 def _dtype(t) -> int:
@@ -98,7 +90,7 @@ def _vector(t, name, n, dtype, dev):
 
 def _elsewhere(stream):
     """Whether a call has to change streams."""
-    return stream is not None and stream.cuda_stream != _raw_stream(stream.device_index)
+    return stream.cuda_stream != _raw_stream(stream.device_index)
 
 
 def _on_stream(stream, keep, f, *args):
@@ -154,7 +146,7 @@ def qk_norm_rope(q, k, q_weight, k_weight, positions, table, eps: float = 1e-5, 
     """Norms of each head of q [T, H, hd] and k [T, KVH, hd] and their rotation, one pass over both
     (bt_cuda_qk_norm_rope).  q_weight / k_weight: [hd] float32, or None for no norm; table: rope_table(),
     or None for no rotation; positions: [T] int32.  q_out / k_out may be q and k.  k may be None."""
-    if _elsewhere(stream):
+    if stream is not None and _elsewhere(stream):
         return _on_stream(stream, (), qk_norm_rope, q, k, q_weight, k_weight, positions, table, eps, q_out, k_out)
     qh = _heads(q, "q")
     shape, dtype, dev = q.shape, q.dtype, q.get_device()
@@ -291,7 +283,7 @@ class KV4Cache:
         return self._append(q, k, v, q_weight, k_weight, slots, positions, table, eps, q_out, stream)
 
     def _append(self, q, k, v, q_weight, k_weight, slots, positions, table, eps, q_out, stream):
-        if _elsewhere(stream):
+        if stream is not None and _elsewhere(stream):
             return _on_stream(stream, self._tensors(), self._append, q, k, v, q_weight, k_weight, slots, positions, table, eps,
                               q_out, None)
         if k.dim() != 3:
@@ -316,7 +308,7 @@ class KV4Cache:
 
     def read(self, slots, positions, dtype=torch.float16, stream=None):
         """The values that the rows at (slots[t], positions[t]) stand for: k, v [T, KVH, hd]."""
-        if _elsewhere(stream):
+        if stream is not None and _elsewhere(stream):
             return _on_stream(stream, self._tensors(), self.read, slots, positions, dtype)
         dev, tokens = self._index, positions.numel()
         if dtype not in _DTYPES:
@@ -340,7 +332,7 @@ class KV4Cache:
         slots [n] int32: the sequences' slots; None: sequence i is slot i.  max_q: no sequence has more
         queries (0: not known).  Rows of q that belong to no sequence are not written (in a new output they
         hold anything)."""
-        if _elsewhere(stream):
+        if stream is not None and _elsewhere(stream):
             return _on_stream(stream, self._tensors(), self.attention, q, kv_len, q_start, slots, max_q, window, sinks, scale, out)
         qh = _heads(q, "q")
         dev, shape, n = self._index, q.shape, kv_len.numel()
@@ -349,15 +341,30 @@ class KV4Cache:
             raise ValueError("attention: q must have the cache's head_dim and device")
         if min(window, sinks, max_q) < 0 or max(window, sinks, max_q) > 0xffffffff:
             raise ValueError("attention: window, sinks and max_q must be in 0 .. 2^32 - 1")
-        scale = hd ** -0.5 if scale is None else scale
-        if not abs(scale) < 2e38:
+        if scale is None:
+            scale = hd ** -0.5
+        elif not abs(scale) < 2e38:
             raise ValueError("attention: scale is not finite")
         out, oh = _out(out, "out", shape, q, dev)
         a = _pack_attn.pack(*qh, *oh, _vector(kv_len, "kv_len", n, torch.int32, dev),
                             0 if q_start is None else _vector(q_start, "q_start", n + 1, torch.int32, dev),
                             0 if slots is None else _vector(slots, "slots", n, torch.int32, dev),
                             n, tokens, heads, max_q, window, sinks, _dtype(q), scale)
-        _launch(native.load().bt_cuda_kv4_attention, "bt_cuda_kv4_attention", dev, self._ref, a, *_workspace(dev))
+        lib, s, here = native.load(), _raw_stream(dev), dev == _current_device()
+        capture, cache = 0, _workspaces
+        if not here or _is_capturing():
+            capture = lib.bt_cuda_capture_id(s)
+            cache = _captured if capture else _workspaces
+        ws = cache.get((dev, s))
+        if ws is None or ws[3] != capture:
+            ws = _new_workspace(cache, dev, s, capture)
+        if here:
+            rc = lib.bt_cuda_kv4_attention(self._ref, a, ws[0], ws[1], s)
+        else:
+            with torch.cuda.device(dev):
+                rc = lib.bt_cuda_kv4_attention(self._ref, a, ws[0], ws[1], s)
+        if rc:
+            native.check(rc, "bt_cuda_kv4_attention")
         return out
 
 
@@ -365,7 +372,7 @@ def sample_batch(logits, u, temperature=None, top_k=None, top_p=None, min_p=None
     """A token for every row of logits [B, V] from the given random numbers u [B] in [0, 1)
     (bt_cuda_sample_batch).  temperature, top_p, min_p [B] float32 and top_k [B] int32 on the device, or
     None for none of that.  Returns (token [B] int32, logprob [B] float32)."""
-    if _elsewhere(stream):
+    if stream is not None and _elsewhere(stream):
         return _on_stream(stream, (), sample_batch, logits, u, temperature, top_k, top_p, min_p, token, logprob)
     if logits.dim() != 2 or not logits.is_cuda or (logits.stride(1) != 1 and logits.shape[1] > 1):
         raise ValueError("sample_batch: expected a [rows, vocab] CUDA tensor with contiguous rows")

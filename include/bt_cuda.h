@@ -609,7 +609,7 @@ BT_API uint64_t bt_cuda_kv4_attention_workspace(void);
 BT_API uint64_t bt_cuda_capture_id(void* stream);
 /* Fault injection on the host, for tests of BT_KV4_TIMEOUT: the device waits of
  * this process's later bt_cuda_kv4_attention calls for their copies cannot end
- * and give up after wait_ms (at most 2000); 0: as usual again.  No GPU fault, no
+ * and give up after wait_ms (at most 255); 0: as usual again.  No GPU fault, no
  * hang. */
 BT_API int bt_cuda_kv4_inject_stall(uint32_t wait_ms);
 

@@ -168,7 +168,7 @@ def test_workspace_constants(nat):
     src = open(f"{ROOT}/include/bt_cuda.h").read()
     assert int(re.search(r"#define BT_KV4_WORKSPACE_ZERO (\d+)u", src).group(1)) == nat.BT_KV4_WORKSPACE_ZERO
     assert nat.load().bt_cuda_capture_id(None) == 0
-    refused(nat, "bt_cuda_kv4_inject_stall", 2001, match="2000")
+    refused(nat, "bt_cuda_kv4_inject_stall", 256, match="255")
     nat.call("bt_cuda_kv4_inject_stall", 0)
 
 
