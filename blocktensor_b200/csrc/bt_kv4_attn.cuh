@@ -24,11 +24,17 @@
 //
 // mma.sync m16n8k16: scores have the 16 keys as M, the 8 columns as N; out has 16
 // dims as M and the tile's 16 keys as K.  tcgen05 has no use here: M is the cache's
-// side at 16 rows a warp, the operands come from registers after unpacking, and
-// at 4.5 bits an element the kernel is bound by issue slots before memory: about 420 a
-// 16-key tile of head_dim 128 (4608 bytes of K and V), half of them unpacking.  Measured,
-// bf16, 64 heads over 8: one sequence of 131071 keys 55 us (2.8 TB/s of 6.5; 3.6 TB/s
-// without the fixed 12 us); 8 keys to 32, 8.5 us; 16 sequences of 4096, 31 us.
+// side at 16 rows a warp, and the operands come from registers after unpacking.
+//
+// Bound: latency.  A 16-key tile of head_dim 128 (2304 bytes of K and V) takes about 420
+// issue slots, half of them unpacking, which at every slot would carry 6.4 TB/s, the
+// memory's own rate; with four warps a scheduler, each a chain of shared-memory loads,
+// logic, MMA, vote, exponential, transpose and MMA, 55 % of the slots are used over one
+// sequence of 131071 keys and 48 % over 24 windows (of 7.3 cycles between a warp's
+// instructions 1.9 are fixed latencies, 1.1 another warp's turn, 0.7 each barriers and
+// pipes, 0.6 shared memory).  Measured, bf16, 64 heads over 8: one sequence of 131071 keys
+// 56 us (2.7 TB/s of 6.5; 3.5 TB/s without the fixed 12 us); 8 keys to 32, 8.7 us; 16
+// sequences of 4096, 31 us.
 #pragma once
 
 #include "bt_kv4.cuh"

@@ -14,8 +14,9 @@
 //
 // Bound: at head_dim 128, 128 keys are 2048 tensor cycles (both halves' S and P V),
 // 2048 cycles of the exponential unit (256 x 128) and about 1500 issue slots a scheduler
-// for softmax and unpacking, so the three run side by side in warpgroups of their own,
-// which trade registers (setmaxnreg):
+// for softmax and unpacking.  None is full (below): what a tile waits for is a softmax
+// warp's own chain, loading S from tensor memory, votes, exponentials, P back.  The three
+// run side by side in warpgroups of their own, which trade registers (setmaxnreg):
 //   0, 1   softmax of a row half each, a thread a row: S from tensor memory, P back into
 //          the same columns (half as wide, behind the reader)
 //   2, 3   unpack the K and the V tiles, into four stages each
@@ -35,8 +36,10 @@
 // contiguous; K's and Q's elements of 8 are in the order 0 4 1 5 2 6 3 7, in which a
 // word's codes come out two at a time.
 //
-// Measured, bf16, 64 heads over 8 of 128: 2048 queries ending 8192 keys 575 us, 837 TFLOP/s
-// of 1642 (tensor pipe 45 to 50 % busy, exponential unit 45 %, issue slots 58 %).  128-key
+// Measured, bf16, 64 heads over 8 of 128: 2048 queries ending 8192 keys 585 us, 822 TFLOP/s
+// of 1642 (tensor pipe 47 % busy, exponential unit 47 %, issue slots 61 %; of 8.2 cycles
+// between a warp's instructions 2.0 wait for tensor memory).  Blocks of few tiles leave all
+// units idle between blocks (8 prompts through a window of 512: 13, 28 and 41 %).  128-key
 // tiles with one S buffer a half took 715 us; one warp issuing for both halves 756.
 #include "bt_kv4_attn.cuh"
 

@@ -7,8 +7,9 @@
 //   (y_i, y_{i + rot/2}) <- (y_i cos - y_{i + rot/2} sin, y_i sin + y_{i + rot/2} cos)
 // and for the cache, per 64 elements, scale and min in fp16 and 4-bit codes.
 //
-// Bound: memory (7 operations for the 4 to 8 bytes an element moves), with the issue
-// slots close behind.  Layout: a row is head_dim / 8 lanes, a lane holds the four
+// Bound: memory latency (7 operations for the 4 to 8 bytes an element moves): at 33 (norms)
+// and 28 (append) warps an SM half of a warp's time is waiting for loads, with 64 % of the
+// issue slots used.  Layout: a row is head_dim / 8 lanes, a lane holds the four
 // elements from 4l and the four that they are rotated with, from rot / 2 + 4l, so the
 // rotation needs no exchange (with 8 consecutive elements a lane, 8 shuffles and as many
 // selects of about 110 instructions); sums are 3 to 5 shuffles.  Rows that go to the

@@ -14,8 +14,8 @@
 // Layout.  A row is a cluster of up to 8 CTAs; each holds its share of the row in shared
 // memory, so the logits are read from memory once whatever the row's parameters ask for.
 // (Held in registers, 32 values a thread, every pass is unrolled 32 times and spills.)
-// At full batches the issue slots are the limit (14 operations a logit take as long as
-// reading it), so the passes do little for a logit that cannot be kept:
+// The passes do little for a logit that cannot be kept (14 operations a logit would take
+// two thirds of the time of reading it):
 //   top_k <= 512: every thread has the maximum of its logits; the k-th largest of these
 //     bounds the k-th largest logit from below, which leaves little more than k
 //     candidates.  The cluster's first CTA lists and sorts them, cuts, and draws.
@@ -27,9 +27,13 @@
 //     kept weights are summed, and the part of the row that holds the draw gone through.
 // A row that does not fit (more than 8 * kSbHeld logits) is read again at every pass.
 //
-// Bound: issue slots and cluster barriers for large batches, the chain of cluster barriers
-// for single rows.  Measured, fp32, temperature 0.7: 256 rows of 128256 with top-k 50 and
-// top-p 0.9 135 us (1.0 TB/s), with top-p alone 220 us; one row of 32000 11.2 us.  The short
+// Bound: the chain of block and cluster barriers, for single rows and, as a CTA loads
+// nothing while it works, for batches too: of 23 cycles between a warp's instructions 8.3 go
+// to barriers, 3.5 to loads, 3.4 to the barriers' fences, and 30 % of the issue slots are used
+// (256 rows of requests of all kinds).  Measured, fp32, 256 rows of 128256 (reading them takes 20
+// us): greedy 51 us, no filter 117, top-k 50 and top-p 0.9 135 (1.0 TB/s; 138 at temperature
+// 1.7), top-p 0.9 alone 220 at temperature 0.7 and 400 at 1.7, where thousands of tokens are
+// kept and weighed; one row of 32000, 11.3 us.  The short
 // list against the histogram, 256 rows of 128256: top-k 50 135 / 275 us, 200 186 / 296,
 // 512 (the list's limit) 249 / 312.
 #include <cooperative_groups.h>

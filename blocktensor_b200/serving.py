@@ -331,7 +331,8 @@ class KV4Cache:
         [n + 1] int32: sequence i's queries are rows q_start[i] .. q_start[i + 1] - 1 of q; None: one each.
         slots [n] int32: the sequences' slots; None: sequence i is slot i.  max_q: no sequence has more
         queries (0: not known).  Rows of q that belong to no sequence are not written (in a new output they
-        hold anything)."""
+        hold anything).  16-bit queries are answered with fp16 operands inside (errors in bt_cuda.h), fp32 ones
+        to fp32's precision, at several times the cost where rows are many."""
         if stream is not None and _elsewhere(stream):
             return _on_stream(stream, self._tensors(), self.attention, q, kv_len, q_start, slots, max_q, window, sinks, scale, out)
         qh = _heads(q, "q")

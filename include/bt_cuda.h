@@ -598,7 +598,8 @@ typedef struct bt_kv4_attn_args {
  * (query, head) rows a KV head probabilities times scales are rounded to fp16,
  * with more rows (head_dim 64 and 128) keys, values and probabilities are, 2^-12
  * rms each (fp16 results are off by 2.7e-4 and 4.9e-4, of which 2.1e-4 are their
- * own rounding; bf16 ones by 1.8e-3, of which 1.7e-3). */
+ * own rounding; bf16 ones by 1.8e-3, of which 1.7e-3).  A caller who wants more
+ * passes fp32 queries, which take the first form at any number of rows. */
 #define BT_KV4_WORKSPACE_ZERO 16384u
 BT_API int bt_cuda_kv4_attention(const bt_kv4* cache, const bt_kv4_attn_args* a, void* workspace,
                                  uint64_t workspace_bytes, void* stream);
