@@ -257,8 +257,10 @@ class KV4Cache:
         return (len(self._free) if self._free is not None else 0), self.n_pages
 
     def check(self):
-        """Waits for the device and raises IndexError if a call met a slot, position, length or page out of
-        range since the last check, CudaBackendError if a device wait gave up."""
+        """Waits for the device (all of its streams) and raises IndexError if a call met a slot, position, length
+        or page out of range since the last check, CudaBackendError if a device wait gave up."""
+        if self.device.type == "cuda":
+            torch.cuda.synchronize(self.device)
         status = int(self.status.item())
         self.status.zero_()
         if status & native.BT_KV4_TIMEOUT:

@@ -604,3 +604,19 @@ def test_attention_nan_and_infinite_queries(cuda, dt, hd, counts):
         assert bool(got[row, head].isnan().all())
         got[row, head] = want[row, head]
     assert torch.equal(got, want)
+
+
+def test_check_waits_for_every_stream(cuda):
+    """check() sees what a call on another stream, not yet begun, will report."""
+    torch = T()
+    c, x = cuda.KV4Cache(2, 40, 1, 64), torch.ones(1, 1, 64, device="cuda")
+    slots, pos, side = ints([5]), ints([0]), torch.cuda.Stream()
+    c.append(x, x, pos, pos, stream=side)  # (a kernel's first launch waits for the device)
+    c.check()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(100_000_000)
+    c.append(x, x, slots, pos, stream=side)
+    with pytest.raises(IndexError):
+        c.check()
+    c.check()
