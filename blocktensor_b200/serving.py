@@ -79,7 +79,10 @@ def _out(t, name, shape, like, dev):
         # (empty_like keeps strides, so it only serves contiguous tensors; 0.5 us less than new_empty)
         t = torch.empty_like(like) if like.is_contiguous() else like.new_empty(shape)
         return t, (t.data_ptr(), shape[1] * shape[2], shape[2])
-    return t, _heads(t, name, shape, like.dtype, dev)
+    h = _heads(t, name, shape, like.dtype, dev)
+    if (h[1] == 0 and shape[0] > 1) or (h[2] == 0 and shape[1] > 1):
+        raise ValueError(f"{name}: rows of an output must not share memory")
+    return t, h
 
 
 def _vector(t, name, n, dtype, dev):

@@ -620,3 +620,22 @@ def test_check_waits_for_every_stream(cuda):
     with pytest.raises(IndexError):
         c.check()
     c.check()
+
+
+def test_broadcast_outputs_are_refused(cuda):
+    """An output whose rows share memory would be written by several threads at a time."""
+    torch = T()
+    q, w, pos, table = torch.zeros(2, 4, 128, device="cuda"), torch.ones(128, device="cuda"), ints([0, 1]), cuda.rope_table(4, 128)
+    c = cuda.KV4Cache(2, 32, 2, 128)
+    for shared in (torch.zeros(1, 4, 128, device="cuda").expand(2, 4, 128), torch.zeros(2, 1, 128, device="cuda").expand(2, 4, 128)):
+        with pytest.raises(ValueError):
+            cuda.qk_norm_rope(q, None, w, None, pos, table, q_out=shared)
+        with pytest.raises(ValueError):
+            c.attention(q, pos, out=shared)
+        with pytest.raises(ValueError):
+            c.append_normed(q, q[:, :2], q[:, 2:], w, w, pos, pos, table, q_out=shared)
+        # as an input it is read as any other
+        a, _ = cuda.qk_norm_rope(shared, None, w, None, pos, table)
+        assert torch.equal(a, torch.zeros_like(q))
+    one = torch.zeros(1, 4, 128, device="cuda").as_strided((1, 4, 128), (0, 128, 1))
+    cuda.qk_norm_rope(q[:1], None, w, None, pos[:1], table, q_out=one)
